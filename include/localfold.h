@@ -471,6 +471,192 @@ typedef struct {
  * pair transition). */
 int lf_msa_module_block(lf_context* ctx, const lf_msa_block_args* args);
 
+/* ---- training: LayerNorm and its gradient, activations kept in 8 bits, 8-bit products ---- */
+
+/* No counterpart in the reference, which runs inference only.  These entry points train a layer
+ * of the stack: the forward pass keeps its activations in 8 bits, multiplies them in 8 bits, and
+ * the backward pass multiplies what was kept.
+ *
+ * A checkpoint holds a [rows, cols] matrix as e4m3 codes (4 exponent and 3 mantissa bits, largest
+ * 448, no infinity) with one scale per row and group of 128 columns.  The scale is a power of two,
+ * 2^(b - 127) with b in 1..254 as stored, the smallest that puts the group's largest finite
+ * magnitude within 448 (b = 1 for a group of zeros): the division by it is exact, so the code's
+ * rounding (to nearest, ties to even, 2^-4 relative at most above 2^-6 of the scale) is the only
+ * one.  An infinity or a NaN becomes the NaN code and leaves its neighbours' scale alone.  A value
+ * within 2^-5 of the largest of its type may round up to a power of two beyond it, which reads
+ * back as an infinity of that type.
+ *
+ *   codes   [rows][LF_CHECKPOINT_PITCH(cols)], columns from cols to the pitch hold zeros
+ *   scales  [LF_CHECKPOINT_GROUPS(cols)][LF_CHECKPOINT_SCALE_PITCH(rows)], one byte b each; bytes
+ *           of rows >= rows may hold anything
+ *
+ * codes and scales are 16-byte aligned.  An lf_fp8_weight holds an [outputs, inputs] matrix the
+ * same way with one scale per tile of 128 x 128: codes [outputs][LF_CHECKPOINT_PITCH(inputs)],
+ * scales [LF_CHECKPOINT_GROUPS(outputs)][LF_CHECKPOINT_GROUPS(inputs)].
+ *
+ * Products of two kept matrices: their values are exact in bfloat16, and with f32 outputs they are
+ * multiplied in it, products exact and sums in f32.  16-bit and 8-bit outputs of lf_fp8_linear
+ * take the 8-bit matrix instruction, whose sums are f32 too but which drops, of 8 products added
+ * at a time, what lies 2^-13 below the largest: about 2e-5 of the result for inputs of like size,
+ * far under the output's own rounding.
+ *
+ * Matrices are row-major and contiguous.  Inputs and outputs do not overlap except where it says
+ * so.  Sums over rows (gradients of weights, biases, scales and offsets) are added in a fixed
+ * order: the same call gives the same bits.
+ *
+ * scratch (lf_layer_norm_backward, lf_fp8_weight_grad, lf_transition_train and _backward): memory
+ * for the call's partial sums, at least what the entry point's _scratch function says, 16-byte
+ * aligned.  NULL: the context's workspace, which another call may replace: a call that is captured
+ * into a HIP graph has to bring its own (LF_ERR_INVALID otherwise), one for each graph that may
+ * run at the same time. */
+typedef struct {
+  int rows, cols;
+  void* codes;
+  void* scales;
+} lf_checkpoint;
+#define LF_CHECKPOINT_PITCH(cols) (((size_t)(cols) + 63) / 64 * 64)
+#define LF_CHECKPOINT_GROUPS(cols) (((size_t)(cols) + 127) / 128)
+#define LF_CHECKPOINT_SCALE_PITCH(rows) (((size_t)(rows) + 15) / 16 * 16)
+
+typedef struct {
+  int outputs, inputs;
+  void* codes;
+  void* scales;
+} lf_fp8_weight;
+
+typedef struct {
+  int act_dtype;
+  void* act;                   /* [rows, cols] of `kept`: read by pack, written by unpack */
+  const lf_checkpoint* kept;
+} lf_checkpoint_args;
+
+/* Activations to a checkpoint, and back to the values that it stands for (rounded to act_dtype;
+ * exact in f32, and in bf16 and f16 where those have the range). */
+int lf_checkpoint_pack(lf_context* ctx, const lf_checkpoint_args* args);
+int lf_checkpoint_unpack(lf_context* ctx, const lf_checkpoint_args* args);
+
+typedef struct {
+  int rows, channels;          /* channels 1..4096 */
+  int act_dtype;
+  const void* act;             /* [rows, channels] */
+  const float *scale, *offset; /* [channels] */
+  float epsilon;
+  int fast_variance;           /* AF3: E[x^2] - E[x]^2 */
+  void* out;                   /* [rows, channels], act_dtype, may alias act; or NULL */
+  float *mean, *rstd;          /* [rows], for the backward pass; or both NULL */
+  const lf_checkpoint* act_kept;  /* act, or NULL */
+  const lf_checkpoint* out_kept;  /* the normalised rows (from f32, not from out), or NULL */
+} lf_layer_norm_args;
+
+/* out = (act - mean) * rstd * scale + offset; at least one of the outputs is given. */
+int lf_layer_norm(lf_context* ctx, const lf_layer_norm_args* args);
+
+typedef struct {
+  int rows, channels;          /* channels 1..4096 */
+  int act_dtype;               /* of grad, act, residual and out */
+  const void* grad;            /* [rows, channels], the gradient of lf_layer_norm's out */
+  const void* act;             /* [rows, channels] as in the forward call, or NULL: act_kept */
+  const lf_checkpoint* act_kept;
+  const float *mean, *rstd;    /* [rows], from the forward call */
+  const float* scale;          /* [channels] */
+  const void* residual;        /* added to the gradient, or NULL */
+  void* out;                   /* [rows, channels], may alias grad, act or residual; or NULL */
+  int grad_dtype;              /* of grad_scale and grad_offset */
+  void *grad_scale, *grad_offset; /* [channels], or both NULL */
+  void* scratch;
+  size_t scratch_bytes;
+} lf_layer_norm_backward_args;
+
+/* With h = (act - mean) * rstd and g = grad * scale: out = residual + rstd * (g - E[g] - h E[g h]),
+ * grad_scale = sum over rows of grad * h, grad_offset = sum over rows of grad. */
+int lf_layer_norm_backward(lf_context* ctx, const lf_layer_norm_backward_args* args);
+size_t lf_layer_norm_backward_scratch(int rows, int channels);
+
+typedef struct {
+  lf_weight w;                 /* LF_F32, LF_F16 or LF_BF16, either layout */
+  int backward;                /* 0: out = [outputs of w, inputs of w]; 1: transposed, the operand
+                                  of the input's gradient */
+  const lf_fp8_weight* out;
+} lf_fp8_weight_args;
+
+int lf_fp8_pack_weight(lf_context* ctx, const lf_fp8_weight_args* args);
+
+typedef struct {
+  const lf_checkpoint* act;    /* [rows, inputs] */
+  const lf_fp8_weight* w;      /* [outputs, inputs] */
+  const float* bias;           /* [outputs] or NULL */
+  int relu;                    /* values below zero become zero, after the bias */
+  const lf_checkpoint* relu_of;   /* [rows, outputs] or NULL: zero where its code is zero or
+                                     negative, the gradient of a ReLU whose output was kept */
+  int out_dtype;
+  const void* residual;        /* [rows, outputs], out_dtype, added last; NULL, or with `out` */
+  void* out;                   /* [rows, outputs], may alias residual; or NULL: out_kept */
+  const lf_checkpoint* out_kept;
+} lf_fp8_linear_args;
+
+int lf_fp8_linear(lf_context* ctx, const lf_fp8_linear_args* args);
+
+typedef struct {
+  const lf_checkpoint* grad;   /* [rows, outputs]: the gradient of the linear's out */
+  const lf_checkpoint* act;    /* [rows, inputs]: what the forward call multiplied */
+  int layout;                  /* of out: LF_OUT_IN or LF_IN_OUT */
+  int grad_dtype;              /* of out and bias */
+  void* out;                   /* [outputs, inputs] or [inputs, outputs] */
+  void* bias;                  /* [outputs]: the sum of grad's rows, or NULL */
+  void* scratch;
+  size_t scratch_bytes;
+} lf_fp8_weight_grad_args;
+
+int lf_fp8_weight_grad(lf_context* ctx, const lf_fp8_weight_grad_args* args);
+size_t lf_fp8_weight_grad_scratch(int rows, int outputs, int inputs);
+
+/* What the training forward pass of a transition keeps: (rows (2 channels + hidden)) codes. */
+typedef struct {
+  lf_checkpoint act, normed;   /* [rows, channels] */
+  lf_checkpoint hidden;        /* [rows, hidden] */
+  float *mean, *rstd;          /* [rows] */
+} lf_transition_saved;
+
+/* The AF2 transition of lf_transition (LF_TRANSITION_RELU) as a training step runs it: matrices in
+ * w are LF_F32, LF_F16 or LF_BF16, vectors f32, all read at the time of the call. */
+typedef struct {
+  int rows, channels, hidden;  /* channels 1..4096 */
+  int act_dtype;
+  const void* act;
+  void* out;                   /* may alias act */
+  int accumulate;              /* 1: out = act + update */
+  int fast_variance;
+  float epsilon;
+  const lf_transition_weights* w;
+  const lf_transition_saved* saved;   /* written */
+  void* scratch;
+  size_t scratch_bytes;
+} lf_transition_train_args;
+
+int lf_transition_train(lf_context* ctx, const lf_transition_train_args* args);
+size_t lf_transition_train_scratch(int rows, int channels, int hidden);
+
+typedef struct {
+  int rows, channels, hidden;
+  int act_dtype;
+  const void* grad;            /* [rows, channels]: of lf_transition_train's out */
+  void* out;                   /* [rows, channels]: the gradient of its act, may alias grad */
+  int accumulate;              /* as in the forward call: 1 adds grad, the residual's gradient */
+  const lf_transition_weights* w;     /* as in the forward call */
+  const lf_transition_saved* saved;   /* of the forward call */
+  int grad_dtype;              /* of the gradients below */
+  void *grad_norm_scale, *grad_norm_offset;   /* [channels] */
+  void *grad_w1, *grad_b1;     /* in the layout of w->w1; [hidden] */
+  void *grad_w2, *grad_b2;     /* in the layout of w->w2; [channels] */
+  void* scratch;
+  size_t scratch_bytes;
+} lf_transition_backward_args;
+
+/* Every gradient pointer is given, but grad_b1 or grad_b2 may be NULL (a transition without that
+ * bias has it NULL in w too). */
+int lf_transition_backward(lf_context* ctx, const lf_transition_backward_args* args);
+size_t lf_transition_backward_scratch(int rows, int channels, int hidden);
+
 #ifdef __cplusplus
 }
 #endif

@@ -190,6 +190,67 @@ class lf_msa_block_args(C.Structure):
 
 
 # (name, restype, argtypes) for every function include/localfold.h declares.
+class lf_checkpoint(C.Structure):
+    _fields_ = [("rows", C.c_int), ("cols", C.c_int), ("codes", P), ("scales", P)]
+
+
+class lf_fp8_weight(C.Structure):
+    _fields_ = [("outputs", C.c_int), ("inputs", C.c_int), ("codes", P), ("scales", P)]
+
+
+KEPT = C.POINTER(lf_checkpoint)
+
+
+class lf_checkpoint_args(C.Structure):
+    _fields_ = [("act_dtype", C.c_int), ("act", P), ("kept", KEPT)]
+
+
+class lf_layer_norm_args(C.Structure):
+    _fields_ = [("rows", C.c_int), ("channels", C.c_int), ("act_dtype", C.c_int), ("act", P), ("scale", P),
+                ("offset", P), ("epsilon", C.c_float), ("fast_variance", C.c_int), ("out", P), ("mean", P),
+                ("rstd", P), ("act_kept", KEPT), ("out_kept", KEPT)]
+
+
+class lf_layer_norm_backward_args(C.Structure):
+    _fields_ = [("rows", C.c_int), ("channels", C.c_int), ("act_dtype", C.c_int), ("grad", P), ("act", P),
+                ("act_kept", KEPT), ("mean", P), ("rstd", P), ("scale", P), ("residual", P), ("out", P),
+                ("grad_dtype", C.c_int), ("grad_scale", P), ("grad_offset", P), ("scratch", P),
+                ("scratch_bytes", C.c_size_t)]
+
+
+class lf_fp8_weight_args(C.Structure):
+    _fields_ = [("w", lf_weight), ("backward", C.c_int), ("out", C.POINTER(lf_fp8_weight))]
+
+
+class lf_fp8_linear_args(C.Structure):
+    _fields_ = [("act", KEPT), ("w", C.POINTER(lf_fp8_weight)), ("bias", P), ("relu", C.c_int), ("relu_of", KEPT),
+                ("out_dtype", C.c_int), ("residual", P), ("out", P), ("out_kept", KEPT)]
+
+
+class lf_fp8_weight_grad_args(C.Structure):
+    _fields_ = [("grad", KEPT), ("act", KEPT), ("layout", C.c_int), ("grad_dtype", C.c_int), ("out", P), ("bias", P),
+                ("scratch", P), ("scratch_bytes", C.c_size_t)]
+
+
+class lf_transition_saved(C.Structure):
+    _fields_ = [("act", lf_checkpoint), ("normed", lf_checkpoint), ("hidden", lf_checkpoint), ("mean", P), ("rstd", P)]
+
+
+class lf_transition_train_args(C.Structure):
+    _fields_ = [("rows", C.c_int), ("channels", C.c_int), ("hidden", C.c_int), ("act_dtype", C.c_int), ("act", P),
+                ("out", P), ("accumulate", C.c_int), ("fast_variance", C.c_int), ("epsilon", C.c_float),
+                ("w", C.POINTER(lf_transition_weights)), ("saved", C.POINTER(lf_transition_saved)), ("scratch", P),
+                ("scratch_bytes", C.c_size_t)]
+
+
+class lf_transition_backward_args(C.Structure):
+    _fields_ = [("rows", C.c_int), ("channels", C.c_int), ("hidden", C.c_int), ("act_dtype", C.c_int), ("grad", P),
+                ("out", P), ("accumulate", C.c_int), ("w", C.POINTER(lf_transition_weights)),
+                ("saved", C.POINTER(lf_transition_saved)), ("grad_dtype", C.c_int), ("grad_norm_scale", P),
+                ("grad_norm_offset", P), ("grad_w1", P), ("grad_b1", P), ("grad_w2", P), ("grad_b2", P),
+                ("scratch", P), ("scratch_bytes", C.c_size_t)]
+
+
 PROTOTYPES = [
     ("lf_context_create", P, [C.c_int]),
     ("lf_context_destroy", None, [P]),
@@ -221,6 +282,19 @@ PROTOTYPES = [
     ("lf_af2_recycle", C.c_int, [P, C.POINTER(lf_af2_recycle_args)]),
     ("lf_msa_pair_weighted_averaging", C.c_int, [P, C.POINTER(lf_pair_averaging_args)]),
     ("lf_msa_module_block", C.c_int, [P, C.POINTER(lf_msa_block_args)]),
+    ("lf_checkpoint_pack", C.c_int, [P, C.POINTER(lf_checkpoint_args)]),
+    ("lf_checkpoint_unpack", C.c_int, [P, C.POINTER(lf_checkpoint_args)]),
+    ("lf_layer_norm", C.c_int, [P, C.POINTER(lf_layer_norm_args)]),
+    ("lf_layer_norm_backward", C.c_int, [P, C.POINTER(lf_layer_norm_backward_args)]),
+    ("lf_layer_norm_backward_scratch", C.c_size_t, [C.c_int, C.c_int]),
+    ("lf_fp8_pack_weight", C.c_int, [P, C.POINTER(lf_fp8_weight_args)]),
+    ("lf_fp8_linear", C.c_int, [P, C.POINTER(lf_fp8_linear_args)]),
+    ("lf_fp8_weight_grad", C.c_int, [P, C.POINTER(lf_fp8_weight_grad_args)]),
+    ("lf_fp8_weight_grad_scratch", C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    ("lf_transition_train", C.c_int, [P, C.POINTER(lf_transition_train_args)]),
+    ("lf_transition_train_scratch", C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    ("lf_transition_backward", C.c_int, [P, C.POINTER(lf_transition_backward_args)]),
+    ("lf_transition_backward_scratch", C.c_size_t, [C.c_int, C.c_int, C.c_int]),
 ]
 
 _lib = None

@@ -1,0 +1,128 @@
+// Activations kept in 8 bits (pack, unpack) and weights packed for 8-bit products.  Bound by memory.
+#include <algorithm>
+
+#include "lf_train.h"
+
+namespace lf {
+
+// A team of L lanes (16; 8 for rows of one half group) packs one group of one row.
+template <int ACT, int L>
+__global__ __launch_bounds__(256) void checkpoint_pack_kernel(const typename Act<ACT>::T* x, Kept k, int groups) {
+  const long long item = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
+  const long long total = (long long)k.rows * groups;
+  const bool valid = item < total;
+  const long long i = valid ? item : total - 1;
+  const size_t row = (size_t)(i / groups);
+  const int c0 = (int)(i % groups) * GROUP + (threadIdx.x % L) * 8;
+  float v[8];
+  load8<ACT>(x + row * (size_t)k.cols + c0, k.cols - c0, v);
+  keep8<L>(k, row, c0, v, valid);
+}
+
+template <int ACT>
+__global__ __launch_bounds__(256) void checkpoint_unpack_kernel(typename Act<ACT>::T* x, Kept k, int chunks) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (long long)k.rows * chunks) return;
+  const size_t row = (size_t)(i / chunks);
+  const int c0 = (int)(i % chunks) * 8;
+  const uint2 w = *reinterpret_cast<const uint2*>(k.codes + row * (size_t)k.pitch + c0);
+  const float s = scale_value(k.scales[(size_t)(c0 / GROUP) * k.sp + row]);
+  float v[8];
+  decode4(w.x, s, v);
+  decode4(w.y, s, v + 4);
+  store8<ACT>(x + row * (size_t)k.cols + c0, k.cols - c0, v);
+}
+
+constexpr int PACK_MOST = 4;
+struct PackBatch {
+  PackWeight w[PACK_MOST];
+  int first[PACK_MOST + 1];     // first block of each matrix
+  int count;
+};
+
+// One block packs one tile of 128 x 128 of the stored matrix: read once (coalesced along the stored
+// rows) into LDS, its largest magnitude, then the codes, written along the packed rows.
+__global__ __launch_bounds__(256) void pack_weight_kernel(PackBatch b) {
+  __shared__ float tile[GROUP][GROUP + 1];
+  __shared__ float sm[4];
+  int m = 0;
+  while (m + 1 < b.count && (int)blockIdx.x >= b.first[m + 1]) ++m;
+  const PackWeight& w = b.w[m];
+  const int tc = (w.cols + GROUP - 1) / GROUP;
+  const int t = blockIdx.x - b.first[m], tr = t / tc, r0 = tr * GROUP, c0 = (t % tc) * GROUP;
+  float top = 0.f;
+  for (int e = threadIdx.x; e < GROUP * GROUP; e += 256) {
+    const int r = e / GROUP, c = e % GROUP;
+    float v = 0.f;
+    if (r0 + r < w.rows && c0 + c < w.cols) v = load_act(w.data, w.dtype, (size_t)(r0 + r) * w.cols + c0 + c);
+    tile[r][c] = v;
+    top = fmaxf(top, fabsf(v) < __builtin_inff() ? fabsf(v) : 0.f);
+  }
+  top = team_reduce<64, OpMax>(top);
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = top;
+  __syncthreads();
+  const int byte = scale_byte(fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])));
+  const float inv = scale_inverse(byte);
+  const int rows = w.transpose ? w.cols : w.rows, cols = w.transpose ? w.rows : w.cols;   // of the packed matrix
+  const int p0 = w.transpose ? c0 : r0, q0 = w.transpose ? r0 : c0;
+  const int pitch = (int)LF_CHECKPOINT_PITCH(cols);
+  for (int e = threadIdx.x; e < GROUP * GROUP / 8; e += 256) {
+    const int r = e / (GROUP / 8), c = e % (GROUP / 8) * 8;
+    if (p0 + r >= rows || q0 + c >= pitch) continue;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = w.transpose ? tile[c + k][r] : tile[r][c + k];
+    *reinterpret_cast<uint2*>(w.codes + (size_t)(p0 + r) * pitch + q0 + c) = encode8(v, inv);
+  }
+  if (threadIdx.x == 0) w.scales[(size_t)(p0 / GROUP) * ((cols + GROUP - 1) / GROUP) + q0 / GROUP] = (uint8_t)byte;
+}
+
+namespace {
+template <int ACT>
+void go_pack(const void* act, const Kept& k, hipStream_t s) {
+  typedef typename Act<ACT>::T T;
+  const int groups = (k.cols + GROUP - 1) / GROUP, team = k.cols <= 64 ? 8 : 16, per = 256 / team;
+  const dim3 grid((unsigned)(((long long)k.rows * groups + per - 1) / per));
+  if (team == 8)
+    hipLaunchKernelGGL((checkpoint_pack_kernel<ACT, 8>), grid, dim3(256), 0, s, static_cast<const T*>(act), k, groups);
+  else
+    hipLaunchKernelGGL((checkpoint_pack_kernel<ACT, 16>), grid, dim3(256), 0, s, static_cast<const T*>(act), k, groups);
+}
+template <int ACT>
+void go_unpack(void* act, const Kept& k, hipStream_t s) {
+  const int chunks = (k.cols + 7) / 8;
+  const dim3 grid((unsigned)(((long long)k.rows * chunks + 255) / 256));
+  hipLaunchKernelGGL((checkpoint_unpack_kernel<ACT>), grid, dim3(256), 0, s, static_cast<typename Act<ACT>::T*>(act), k,
+                     chunks);
+}
+}  // namespace
+
+int run_checkpoint_pack(lf_context* ctx, const void* act, int dt, const Kept& k) {
+  LaunchScope ls(ctx, "checkpoint.pack");
+  if (dt == LF_F32) go_pack<DT_F32>(act, k, ctx->stream);
+  else if (dt == LF_F16) go_pack<DT_F16>(act, k, ctx->stream);
+  else go_pack<DT_BF16>(act, k, ctx->stream);
+  return check_hip(hipGetLastError(), "checkpoint pack launch");
+}
+
+int run_checkpoint_unpack(lf_context* ctx, void* act, int dt, const Kept& k) {
+  LaunchScope ls(ctx, "checkpoint.unpack");
+  if (dt == LF_F32) go_unpack<DT_F32>(act, k, ctx->stream);
+  else if (dt == LF_F16) go_unpack<DT_F16>(act, k, ctx->stream);
+  else go_unpack<DT_BF16>(act, k, ctx->stream);
+  return check_hip(hipGetLastError(), "checkpoint unpack launch");
+}
+
+int run_pack_weights(lf_context* ctx, const PackWeight* w, int count) {
+  PackBatch b{};
+  b.count = count;
+  for (int i = 0; i < count; ++i) {
+    b.w[i] = w[i];
+    b.first[i + 1] = b.first[i] + (int)(LF_CHECKPOINT_GROUPS(w[i].rows) * LF_CHECKPOINT_GROUPS(w[i].cols));
+  }
+  LaunchScope ls(ctx, "fp8.pack_weight");
+  hipLaunchKernelGGL(pack_weight_kernel, dim3(b.first[count]), dim3(256), 0, ctx->stream, b);
+  return check_hip(hipGetLastError(), "fp8 weight pack launch");
+}
+
+}  // namespace lf

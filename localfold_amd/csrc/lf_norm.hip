@@ -1,0 +1,342 @@
+// LayerNorm forward and backward.
+//
+//   m = E[x], v = E[(x - m)^2] (or E[x^2] - m^2), r = 1 / sqrt(v + eps), y = (x - m) r s + o
+//   h = (x - m) r, g = dy s:  dx = r (g - E[g] - h E[g h]),  ds = sum dy h,  do = sum dy
+//
+// Both are bound by memory: a row is read once into registers, 8 consecutive channels a lane and
+// vector, and its sums go over a team of L lanes (L * NV * 8 >= channels) by permutes.  The team is
+// the smallest that leaves a lane at most 3 vectors, so narrow rows share a wave; rows past 1024
+// channels take the whole block, whose four waves join their sums in LDS.
+#include <algorithm>
+
+#include "lf_train.h"
+
+namespace lf {
+
+struct NormParams {
+  const void* x;
+  const float *scale, *offset;
+  void* out;
+  float *mean, *rstd;
+  Kept xk, yk;                  // codes null: not wanted
+  int rows, C;
+  float eps;
+  int fast_var;
+};
+
+struct NormGradParams {
+  const void *dy, *x, *resid;
+  Kept xk;                      // read where x is null
+  const float *mean, *rstd, *scale;
+  void* out;
+  float* partial;               // [blocks][2][C], or null
+  int rows, C;
+};
+
+// Sum over a row's lanes: a team within a wave, or the whole block (L = 256), which takes a slot of
+// `sm` (4 floats) that no other sum of the same barrier interval uses.
+template <int L>
+__device__ __forceinline__ float row_sum(float v, float* sm) {
+  if constexpr (L <= 64) {
+    return team_reduce<L, OpSum>(v);
+  } else {
+    v = team_reduce<64, OpSum>(v);
+    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (sm[0] + sm[1]) + (sm[2] + sm[3]);
+  }
+}
+
+template <int ACT, int L, int NV>
+__global__ __launch_bounds__(256) void norm_kernel(NormParams p) {
+  typedef typename Act<ACT>::T T;
+  __shared__ float sm[8];
+  constexpr int SLOTS = 256 / L;
+  const int lr = threadIdx.x % L;
+  const long long row0 = (long long)blockIdx.x * SLOTS + threadIdx.x / L;
+  const bool valid = row0 < p.rows;
+  const size_t row = valid ? (size_t)row0 : (size_t)p.rows - 1;
+  const int C = p.C;
+  const T* src = static_cast<const T*>(p.x) + row * (size_t)C;
+  float x[NV][8];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c0 = (v * L + lr) * 8;
+    load8<ACT>(src + c0, C - c0, x[v]);
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += x[v][k];
+  const float n = (float)C;
+  const float mean = row_sum<L>(s, sm) / n;
+  float q = 0.f;
+  if (p.fast_var) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) q += x[v][k] * x[v][k];
+    q = row_sum<L>(q, sm + 4) / n - mean * mean;
+    q = q < 0.f ? 0.f : q;      // the difference of two roundings
+  } else {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c0 = (v * L + lr) * 8;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float d = c0 + k < C ? x[v][k] - mean : 0.f;
+        q += d * d;
+      }
+    }
+    q = row_sum<L>(q, sm + 4) / n;
+  }
+  const float r = 1.0f / sqrtf(q + p.eps);
+  if (valid && lr == 0 && p.mean) {
+    p.mean[row] = mean;
+    p.rstd[row] = r;
+  }
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c0 = (v * L + lr) * 8;
+    if (p.xk.codes) keep8<(L < 16 ? L : 16)>(p.xk, row, c0, x[v], valid);
+    if (p.out || p.yk.codes) {
+      float g[8], o[8], y[8];
+      load8<DT_F32>(p.scale + c0, C - c0, g);
+      load8<DT_F32>(p.offset + c0, C - c0, o);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y[k] = c0 + k < C ? (x[v][k] - mean) * r * g[k] + o[k] : 0.f;
+      if (p.yk.codes) keep8<(L < 16 ? L : 16)>(p.yk, row, c0, y, valid);
+      if (p.out && valid) store8<ACT>(static_cast<T*>(p.out) + row * (size_t)C + c0, C - c0, y);
+    }
+  }
+}
+
+// Rows are dealt out to a fixed number of blocks, whose lanes add up their columns' ds and do in
+// registers; a block joins its teams in LDS and writes one row of partial sums.
+template <int ACT, int L, int NV>
+__global__ __launch_bounds__(256) void norm_grad_kernel(NormGradParams p) {
+  typedef typename Act<ACT>::T T;
+  constexpr int SLOTS = 256 / L;
+  __shared__ float sm[16];
+  __shared__ float cols[L <= 64 ? SLOTS * L * 8 : 8];
+  const int lr = threadIdx.x % L, slot = threadIdx.x / L;
+  const int C = p.C;
+  const float n = (float)C;
+  float ds[NV][8] = {}, dof[NV][8] = {};
+  int parity = 0;
+  for (long long base = (long long)blockIdx.x * SLOTS; base < p.rows; base += (long long)gridDim.x * SLOTS) {
+    const bool valid = base + slot < p.rows;
+    const size_t row = valid ? (size_t)(base + slot) : (size_t)p.rows - 1;
+    const float mean = p.mean[row], r = p.rstd[row];
+    float dy[NV][8], h[NV][8], a = 0.f, b = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c0 = (v * L + lr) * 8;
+      load8<ACT>(static_cast<const T*>(p.dy) + row * (size_t)C + c0, C - c0, dy[v]);
+      if (p.x) {
+        load8<ACT>(static_cast<const T*>(p.x) + row * (size_t)C + c0, C - c0, h[v]);
+      } else {
+        uint2 w = make_uint2(0, 0);
+        float sc = 1.f;
+        if (c0 < p.xk.pitch) {
+          w = *reinterpret_cast<const uint2*>(p.xk.codes + row * (size_t)p.xk.pitch + c0);
+          sc = scale_value(p.xk.scales[(size_t)(c0 / GROUP) * p.xk.sp + row]);
+        }
+        decode4(w.x, sc, h[v]);
+        decode4(w.y, sc, h[v] + 4);
+      }
+    }
+    float g[NV][8];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c0 = (v * L + lr) * 8;
+      load8<DT_F32>(p.scale + c0, C - c0, g[v]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        h[v][k] = c0 + k < C ? (h[v][k] - mean) * r : 0.f;
+        if (valid) {
+          ds[v][k] += dy[v][k] * h[v][k];
+          dof[v][k] += dy[v][k];
+        }
+        g[v][k] *= dy[v][k];
+        a += g[v][k];
+        b += g[v][k] * h[v][k];
+      }
+    }
+    if (!p.out) continue;       // uniform
+    // the block's sums alternate between two sets of slots: a wave may still read the last row's
+    a = row_sum<L>(a, sm + 8 * parity) / n;
+    b = row_sum<L>(b, sm + 8 * parity + 4) / n;
+    parity ^= 1;
+    if (valid) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int c0 = (v * L + lr) * 8;
+        float o[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] = 0.f;
+        if (p.resid) load8<ACT>(static_cast<const T*>(p.resid) + row * (size_t)C + c0, C - c0, o);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] += r * (g[v][k] - a - h[v][k] * b);
+        store8<ACT>(static_cast<T*>(p.out) + row * (size_t)C + c0, C - c0, o);
+      }
+    }
+  }
+  if (!p.partial) return;
+  float* dst = p.partial + (size_t)blockIdx.x * 2 * C;
+  if constexpr (L > 64) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c0 = (v * L + lr) * 8;
+      store8<DT_F32>(dst + c0, C - c0, ds[v]);
+      store8<DT_F32>(dst + C + c0, C - c0, dof[v]);
+    }
+  } else {
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) cols[(slot * L + lr) * 8 + k] = half ? dof[v][k] : ds[v][k];
+        __syncthreads();
+        for (int c = threadIdx.x; c < L * 8; c += 256) {
+          const int col = v * L * 8 + c;
+          float t = 0.f;
+          for (int i = 0; i < SLOTS; ++i) t += cols[i * L * 8 + c];
+          if (col < C) dst[half * C + col] = t;
+        }
+      }
+  }
+}
+
+// Columns of [blocks][cols] partial sums added in order of the blocks, 16 runs of them at a time.
+template <int OUT>
+__global__ __launch_bounds__(1024) void norm_join_kernel(const float* partial, int blocks, int C, void* ds, void* dof) {
+  __shared__ float sm[16][64];
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
+  const int per = (blocks + 15) / 16, b0 = part * per, b1 = min(blocks, b0 + per);
+  float t = 0.f;
+  if (c < 2 * C)
+    for (int b = b0; b < b1; ++b) t += partial[(size_t)b * 2 * C + c];
+  sm[part][threadIdx.x & 63] = t;
+  __syncthreads();
+  if (part == 0 && c < 2 * C) {
+    t = 0.f;
+    for (int i = 0; i < 16; ++i) t += sm[i][threadIdx.x];
+    typedef typename Act<OUT>::T T;
+    if (c < C) Act<OUT>::st(static_cast<T*>(ds) + c, t);
+    else Act<OUT>::st(static_cast<T*>(dof) + c - C, t);
+  }
+}
+
+namespace {
+
+// A team and vectors a lane for a width: see the head of this file.
+struct Team {
+  int lanes, vectors;
+};
+Team team_of(int C) {
+  if (C <= 64) return {8, 1};
+  if (C <= 128) return {16, 1};
+  if (C <= 256) return {16, 2};
+  if (C <= 384) return {16, 3};
+  if (C <= 512) return {32, 2};
+  if (C <= 1024) return {64, 2};
+  if (C <= 2048) return {256, 1};
+  return {256, 2};
+}
+
+constexpr int GRAD_BLOCKS = 1024;   // at most; four a CU
+
+int grad_blocks(int rows, int C) {
+  const int slots = 256 / team_of(C).lanes;
+  return (int)std::min<long long>(((long long)rows + slots - 1) / slots, GRAD_BLOCKS);
+}
+
+template <template <int, int, int> class F, int ACT, class P>
+void by_team(const Team& t, const P& p, dim3 grid, hipStream_t s) {
+  if (t.lanes == 8) F<ACT, 8, 1>::go(p, grid, s);
+  else if (t.lanes == 16 && t.vectors == 1) F<ACT, 16, 1>::go(p, grid, s);
+  else if (t.lanes == 16 && t.vectors == 2) F<ACT, 16, 2>::go(p, grid, s);
+  else if (t.lanes == 16) F<ACT, 16, 3>::go(p, grid, s);
+  else if (t.lanes == 32) F<ACT, 32, 2>::go(p, grid, s);
+  else if (t.lanes == 64) F<ACT, 64, 2>::go(p, grid, s);
+  else if (t.vectors == 1) F<ACT, 256, 1>::go(p, grid, s);
+  else F<ACT, 256, 2>::go(p, grid, s);
+}
+template <template <int, int, int> class F, class P>
+void by_type(int dt, const Team& t, const P& p, dim3 grid, hipStream_t s) {
+  if (dt == LF_F32) by_team<F, DT_F32>(t, p, grid, s);
+  else if (dt == LF_F16) by_team<F, DT_F16>(t, p, grid, s);
+  else by_team<F, DT_BF16>(t, p, grid, s);
+}
+template <int ACT, int L, int NV>
+struct GoNorm {
+  static void go(const NormParams& p, dim3 grid, hipStream_t s) {
+    hipLaunchKernelGGL((norm_kernel<ACT, L, NV>), grid, dim3(256), 0, s, p);
+  }
+};
+template <int ACT, int L, int NV>
+struct GoNormGrad {
+  static void go(const NormGradParams& p, dim3 grid, hipStream_t s) {
+    hipLaunchKernelGGL((norm_grad_kernel<ACT, L, NV>), grid, dim3(256), 0, s, p);
+  }
+};
+
+}  // namespace
+
+int run_layer_norm(lf_context* ctx, const lf_layer_norm_args& a) {
+  NormParams p{};
+  p.x = a.act;
+  p.scale = a.scale;
+  p.offset = a.offset;
+  p.out = a.out;
+  p.mean = a.mean;
+  p.rstd = a.rstd;
+  if (a.act_kept) p.xk = kept_view(*a.act_kept);
+  if (a.out_kept) p.yk = kept_view(*a.out_kept);
+  p.rows = a.rows;
+  p.C = a.channels;
+  p.eps = a.epsilon;
+  p.fast_var = a.fast_variance;
+  const Team t = team_of(a.channels);
+  const int slots = 256 / t.lanes;
+  LaunchScope ls(ctx, "layer_norm");
+  by_type<GoNorm>(a.act_dtype, t, p, dim3((unsigned)(((long long)a.rows + slots - 1) / slots)), ctx->stream);
+  return check_hip(hipGetLastError(), "layer_norm launch");
+}
+
+size_t layer_norm_partials(int rows, int channels) {
+  return (size_t)grad_blocks(rows, channels) * 2 * channels * sizeof(float);
+}
+
+int run_layer_norm_backward(lf_context* ctx, const lf_layer_norm_backward_args& a, void* scratch) {
+  NormGradParams p{};
+  p.dy = a.grad;
+  p.x = a.act;
+  p.resid = a.residual;
+  if (a.act_kept) p.xk = kept_view(*a.act_kept);
+  p.mean = a.mean;
+  p.rstd = a.rstd;
+  p.scale = a.scale;
+  p.out = a.out;
+  p.partial = a.grad_scale ? static_cast<float*>(scratch) : nullptr;
+  p.rows = a.rows;
+  p.C = a.channels;
+  const int blocks = grad_blocks(a.rows, a.channels);
+  {
+    LaunchScope ls(ctx, "layer_norm.backward");
+    by_type<GoNormGrad>(a.act_dtype, team_of(a.channels), p, dim3(blocks), ctx->stream);
+  }
+  LF_TRY(check_hip(hipGetLastError(), "layer_norm backward launch"));
+  if (!a.grad_scale) return LF_OK;
+  LaunchScope ls(ctx, "layer_norm.join");
+  const dim3 grid((2 * a.channels + 63) / 64);
+  auto k = a.grad_dtype == LF_F32 ? norm_join_kernel<DT_F32> : a.grad_dtype == LF_F16 ? norm_join_kernel<DT_F16>
+                                                                                      : norm_join_kernel<DT_BF16>;
+  hipLaunchKernelGGL(k, grid, dim3(1024), 0, ctx->stream, p.partial, blocks, a.channels, a.grad_scale, a.grad_offset);
+  return check_hip(hipGetLastError(), "layer_norm join launch");
+}
+
+}  // namespace lf

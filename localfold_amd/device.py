@@ -733,3 +733,326 @@ def af2_recycle(ctx: Context, f: dict, state: dict, masks: dict, embed_ws, extra
         a.main.msa, a.main.pair = ptr(msa), ptr(pair)
     check(ctx.lib.lf_af2_recycle(ctx.handle, C.byref(a)))
     return state
+
+
+# ---------------------------------------------------------------------------------------
+# Training: LayerNorm and its gradient, activations kept in 8 bits, 8-bit products, the
+# transition's training step.  Tensors are contiguous and on the context's device.
+# ---------------------------------------------------------------------------------------
+
+def _tensor(ctx: Context, name: str, t: torch.Tensor, shape=None, dtype=None) -> int:
+    """Address of a tensor argument after its checks (None for None)."""
+    if t is None:
+        return None
+    if t.device != ctx.device:
+        raise ValueError(f"{name} is on {t.device}; the context is on {ctx.device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous, got strides {t.stride()}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}; expected {tuple(shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} is {t.dtype}; expected {dtype}")
+    return t.data_ptr()
+
+
+def _scratch(ctx: Context, a, scratch: torch.Tensor):
+    if scratch is not None:
+        a.scratch = _tensor(ctx, "scratch", scratch)
+        a.scratch_bytes = scratch.numel() * scratch.element_size()
+
+
+def _rows(t: torch.Tensor):
+    if t.dim() < 1 or t.shape[-1] == 0:
+        raise ValueError(f"activations need a last dimension, got shape {tuple(t.shape)}")
+    return t.numel() // t.shape[-1], t.shape[-1]
+
+
+class Checkpoint:
+    """A [rows, cols] matrix kept in 8 bits: `codes` uint8 [rows, cols rounded up to 64] (e4m3),
+    `scales` uint8 [groups of 128 columns, rows rounded up to 16], a byte b standing for 2^(b - 127)."""
+
+    def __init__(self, rows: int, cols: int, codes: torch.Tensor, scales: torch.Tensor):
+        want = (rows, -(-cols // 64) * 64), (-(-cols // 128), -(-rows // 16) * 16)
+        for name, t, shape in (("codes", codes, want[0]), ("scales", scales, want[1])):
+            if tuple(t.shape) != shape or t.dtype != torch.uint8 or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous uint8 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+        self.rows, self.cols, self.codes, self.scales = rows, cols, codes, scales
+        self.struct = capi.lf_checkpoint(rows, cols, codes.data_ptr(), scales.data_ptr())
+
+    def _ref(self, ctx: Context, name: str, shape=None):
+        if self.codes.device != ctx.device or self.scales.device != ctx.device:
+            raise ValueError(f"{name} is on {self.codes.device}; the context is on {ctx.device}")
+        if shape is not None and (self.rows, self.cols) != tuple(shape):
+            raise ValueError(f"{name} is {self.rows} x {self.cols}; expected {shape[0]} x {shape[1]}")
+        return C.pointer(self.struct)
+
+
+def checkpoint_empty(rows: int, cols: int, device) -> Checkpoint:
+    codes = torch.empty((rows, -(-cols // 64) * 64), dtype=torch.uint8, device=device)
+    scales = torch.empty((-(-cols // 128), -(-rows // 16) * 16), dtype=torch.uint8, device=device)
+    return Checkpoint(rows, cols, codes, scales)
+
+
+def checkpoint_pack(ctx: Context, x: torch.Tensor, out: Checkpoint = None) -> Checkpoint:
+    """x [..., cols] kept in 8 bits (lf_checkpoint_pack)."""
+    rows, cols = _rows(x)
+    if out is None:
+        out = checkpoint_empty(rows, cols, ctx.device)
+    a = capi.lf_checkpoint_args(act_code(x), _tensor(ctx, "x", x), out._ref(ctx, "out", (rows, cols)))
+    check(ctx.lib.lf_checkpoint_pack(ctx.handle, C.byref(a)))
+    return out
+
+
+def checkpoint_unpack(ctx: Context, kept: Checkpoint, dtype=torch.float32, out: torch.Tensor = None) -> torch.Tensor:
+    """The values that a checkpoint stands for (lf_checkpoint_unpack)."""
+    if out is None:
+        out = torch.empty((kept.rows, kept.cols), dtype=dtype, device=ctx.device)
+    if _rows(out) != (kept.rows, kept.cols):
+        raise ValueError(f"out has shape {tuple(out.shape)}; expected {kept.rows} x {kept.cols}")
+    a = capi.lf_checkpoint_args(act_code(out), _tensor(ctx, "out", out), kept._ref(ctx, "kept"))
+    check(ctx.lib.lf_checkpoint_unpack(ctx.handle, C.byref(a)))
+    return out
+
+
+def layer_norm(ctx: Context, x: torch.Tensor, scale: torch.Tensor, offset: torch.Tensor, epsilon: float = 1e-5,
+               fast_variance: bool = False, out: torch.Tensor = None, stats: torch.Tensor = None,
+               x_saved: Checkpoint = None, y_saved: Checkpoint = None) -> torch.Tensor:
+    """LayerNorm over the last dimension (lf_layer_norm).  Writes whichever of `out`, `stats` (float32
+    [2, rows]: mean, 1/std), `x_saved` and `y_saved` are given; `out` is made when none of `out`,
+    `x_saved`, `y_saved` is."""
+    rows, c = _rows(x)
+    if out is None and x_saved is None and y_saved is None:
+        out = torch.empty_like(x)
+    a = capi.lf_layer_norm_args()
+    a.rows, a.channels, a.act_dtype, a.act = rows, c, act_code(x), _tensor(ctx, "x", x)
+    a.scale = _tensor(ctx, "scale", scale, (c,), torch.float32)
+    a.offset = _tensor(ctx, "offset", offset, (c,), torch.float32)
+    a.epsilon, a.fast_variance = epsilon, int(fast_variance)
+    a.out = _tensor(ctx, "out", out, x.shape, x.dtype)
+    if stats is not None:
+        a.mean = _tensor(ctx, "stats", stats, (2, rows), torch.float32)
+        a.rstd = a.mean + 4 * rows
+    if x_saved is not None:
+        a.act_kept = x_saved._ref(ctx, "x_saved", (rows, c))
+    if y_saved is not None:
+        a.out_kept = y_saved._ref(ctx, "y_saved", (rows, c))
+    check(ctx.lib.lf_layer_norm(ctx.handle, C.byref(a)))
+    return out
+
+
+def layer_norm_backward(ctx: Context, grad: torch.Tensor, x, scale: torch.Tensor, stats: torch.Tensor,
+                        residual: torch.Tensor = None, out: torch.Tensor = None, grad_scale: torch.Tensor = None,
+                        grad_offset: torch.Tensor = None, grad_dtype=torch.float32, scratch: torch.Tensor = None):
+    """Gradients of layer_norm (lf_layer_norm_backward): (of x, of scale, of offset).  x: the
+    forward's activations, or the Checkpoint kept of them; `residual` is added to x's gradient."""
+    rows, c = _rows(grad)
+    if out is None:
+        out = torch.empty_like(grad)
+    if grad_scale is None:
+        grad_scale = torch.empty(c, dtype=grad_dtype, device=ctx.device)
+    if grad_offset is None:
+        grad_offset = torch.empty(c, dtype=grad_scale.dtype, device=ctx.device)
+    a = capi.lf_layer_norm_backward_args()
+    a.rows, a.channels, a.act_dtype, a.grad = rows, c, act_code(grad), _tensor(ctx, "grad", grad)
+    if isinstance(x, Checkpoint):
+        a.act_kept = x._ref(ctx, "x", (rows, c))
+    else:
+        a.act = _tensor(ctx, "x", x, grad.shape, grad.dtype)
+    a.mean = _tensor(ctx, "stats", stats, (2, rows), torch.float32)
+    a.rstd = a.mean + 4 * rows
+    a.scale = _tensor(ctx, "scale", scale, (c,), torch.float32)
+    a.residual = _tensor(ctx, "residual", residual, grad.shape, grad.dtype)
+    a.out = _tensor(ctx, "out", out, grad.shape, grad.dtype)
+    a.grad_dtype = act_code(grad_scale)
+    a.grad_scale = _tensor(ctx, "grad_scale", grad_scale, (c,))
+    a.grad_offset = _tensor(ctx, "grad_offset", grad_offset, (c,), grad_scale.dtype)
+    _scratch(ctx, a, scratch)
+    check(ctx.lib.lf_layer_norm_backward(ctx.handle, C.byref(a)))
+    return out, grad_scale, grad_offset
+
+
+class Fp8Weight:
+    """An [outputs, inputs] matrix packed for 8-bit products: `codes` uint8 [outputs, inputs rounded
+    up to 64] (e4m3), `scales` uint8 [tiles of outputs, tiles of inputs], one per 128 x 128."""
+
+    def __init__(self, outputs: int, inputs: int, codes: torch.Tensor, scales: torch.Tensor):
+        want = (outputs, -(-inputs // 64) * 64), (-(-outputs // 128), -(-inputs // 128))
+        for name, t, shape in (("codes", codes, want[0]), ("scales", scales, want[1])):
+            if tuple(t.shape) != shape or t.dtype != torch.uint8 or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous uint8 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+        self.outputs, self.inputs, self.codes, self.scales = outputs, inputs, codes, scales
+        self.struct = capi.lf_fp8_weight(outputs, inputs, codes.data_ptr(), scales.data_ptr())
+
+    def _ref(self, ctx: Context, name: str):
+        if self.codes.device != ctx.device or self.scales.device != ctx.device:
+            raise ValueError(f"{name} is on {self.codes.device}; the context is on {ctx.device}")
+        return C.pointer(self.struct)
+
+
+def _live_weight(name: str, t: torch.Tensor, layout: int) -> capi.lf_weight:
+    """lf_weight over a CUDA tensor as it is (read at the time of each call)."""
+    if t.dim() != 2 or not t.is_contiguous() or not t.is_cuda:
+        raise ValueError(f"{name} must be a contiguous 2-D CUDA tensor, got shape {tuple(t.shape)} on {t.device}")
+    return capi.lf_weight(act_code(t), layout, t.shape[0], t.shape[1], 0, t.data_ptr(), None, None)
+
+
+def fp8_weight(ctx: Context, w: torch.Tensor, layout: int = capi.LF_IN_OUT, backward: bool = False,
+               out: Fp8Weight = None) -> Fp8Weight:
+    """w (stored [inputs, outputs], or [outputs, inputs] with LF_OUT_IN) packed as [outputs, inputs],
+    or with `backward` as [inputs, outputs], the operand of the input's gradient (lf_fp8_pack_weight)."""
+    a = capi.lf_fp8_weight_args()
+    _tensor(ctx, "w", w)
+    a.w = _live_weight("w", w, layout)
+    a.backward = int(backward)
+    n, k = w.shape if (layout == capi.LF_IN_OUT) == bool(backward) else (w.shape[1], w.shape[0])
+    if out is None:
+        out = Fp8Weight(n, k, torch.empty((n, -(-k // 64) * 64), dtype=torch.uint8, device=ctx.device),
+                        torch.empty((-(-n // 128), -(-k // 128)), dtype=torch.uint8, device=ctx.device))
+    a.out = out._ref(ctx, "out")
+    check(ctx.lib.lf_fp8_pack_weight(ctx.handle, C.byref(a)))
+    return out
+
+
+def fp8_linear(ctx: Context, x: Checkpoint, w: Fp8Weight, bias: torch.Tensor = None, relu: bool = False,
+               relu_of: Checkpoint = None, residual: torch.Tensor = None, out=None, dtype=torch.bfloat16):
+    """x w^T + bias (lf_fp8_linear) into `out`: a tensor [..., outputs] or a Checkpoint.  `relu_of`: the
+    kept output of a ReLU, whose gradient this is; `residual` is added last and may be `out`."""
+    if out is None:
+        out = torch.empty((x.rows, w.outputs), dtype=dtype, device=ctx.device)
+    a = capi.lf_fp8_linear_args()
+    a.act, a.w = x._ref(ctx, "x", (x.rows, w.inputs)), w._ref(ctx, "w")
+    a.bias = _tensor(ctx, "bias", bias, (w.outputs,), torch.float32)
+    a.relu = int(relu)
+    if relu_of is not None:
+        a.relu_of = relu_of._ref(ctx, "relu_of", (x.rows, w.outputs))
+    if isinstance(out, Checkpoint):
+        if residual is not None:
+            raise ValueError("a residual needs a tensor as out")
+        a.out_kept = out._ref(ctx, "out", (x.rows, w.outputs))
+    else:
+        if _rows(out) != (x.rows, w.outputs):
+            raise ValueError(f"out has shape {tuple(out.shape)}; expected {x.rows} x {w.outputs}")
+        a.out_dtype, a.out = act_code(out), _tensor(ctx, "out", out)
+        if residual is not None:
+            a.residual = _tensor(ctx, "residual", residual, out.shape, out.dtype)
+    check(ctx.lib.lf_fp8_linear(ctx.handle, C.byref(a)))
+    return out
+
+
+def fp8_weight_grad(ctx: Context, grad: Checkpoint, x: Checkpoint, layout: int = capi.LF_OUT_IN,
+                    out: torch.Tensor = None, bias_out: torch.Tensor = None, grad_dtype=torch.float32,
+                    scratch: torch.Tensor = None):
+    """The weight's gradient grad^T x, [outputs, inputs] or with LF_IN_OUT its transpose
+    (lf_fp8_weight_grad); `bias_out` [outputs] receives the sum of grad's rows."""
+    shape = (grad.cols, x.cols) if layout == capi.LF_OUT_IN else (x.cols, grad.cols)
+    if out is None:
+        out = torch.empty(shape, dtype=grad_dtype, device=ctx.device)
+    a = capi.lf_fp8_weight_grad_args()
+    a.grad, a.act = grad._ref(ctx, "grad"), x._ref(ctx, "x", (grad.rows, x.cols))
+    a.layout, a.grad_dtype = layout, act_code(out)
+    a.out = _tensor(ctx, "out", out, shape)
+    a.bias = _tensor(ctx, "bias_out", bias_out, (grad.cols,), out.dtype)
+    _scratch(ctx, a, scratch)
+    check(ctx.lib.lf_fp8_weight_grad(ctx.handle, C.byref(a)))
+    return out
+
+
+def transition_train_weights(w: dict) -> capi.lf_transition_weights:
+    """Struct over the trainer's own CUDA tensors (not copied: a call reads what they hold then), the
+    names of transition_weights: layerNormScale/Offset, firstWeight [C, H], firstBias, secondWeight
+    [H, C], secondBias; vectors float32, matrices float32, float16 or bfloat16, biases optional."""
+    s = capi.lf_transition_weights()
+
+    def vec(name, n):
+        t = w.get(name)
+        if t is None:
+            return None
+        if tuple(t.shape) != (n,) or t.dtype != torch.float32 or not t.is_contiguous() or not t.is_cuda:
+            raise ValueError(f"{name} must be a contiguous float32 CUDA tensor of shape ({n},)")
+        return t.data_ptr()
+
+    s.w1 = _live_weight("firstWeight", w["firstWeight"], capi.LF_IN_OUT)
+    s.w2 = _live_weight("secondWeight", w["secondWeight"], capi.LF_IN_OUT)
+    c, h = w["firstWeight"].shape
+    if tuple(w["secondWeight"].shape) != (h, c):
+        raise ValueError(f"secondWeight has shape {tuple(w['secondWeight'].shape)}; expected {(h, c)}")
+    s.norm_scale, s.norm_offset = vec("layerNormScale", c), vec("layerNormOffset", c)
+    s.b1, s.b2 = vec("firstBias", h), vec("secondBias", c)
+    s._owner = dict(w)
+    return s
+
+
+class TransitionSaved:
+    """What a training forward pass of a transition keeps for its backward pass."""
+
+    def __init__(self, rows: int, channels: int, hidden: int, device):
+        self.rows, self.channels, self.hidden_size = rows, channels, hidden
+        self.act, self.normed = (checkpoint_empty(rows, channels, device) for _ in range(2))
+        self.hidden = checkpoint_empty(rows, hidden, device)
+        self.stats = torch.empty((2, rows), dtype=torch.float32, device=device)
+        self.struct = capi.lf_transition_saved(self.act.struct, self.normed.struct, self.hidden.struct,
+                                               self.stats.data_ptr(), self.stats.data_ptr() + 4 * rows)
+
+
+def transition_saved(rows: int, channels: int, hidden: int, device) -> TransitionSaved:
+    return TransitionSaved(rows, channels, hidden, device)
+
+
+def _transition_args(ctx: Context, a, x: torch.Tensor, out: torch.Tensor, wstruct, saved: TransitionSaved,
+                     accumulate: bool, scratch):
+    rows, c = _rows(x)
+    if saved.stats.device != ctx.device or (saved.rows, saved.channels) != (rows, c):
+        raise ValueError(f"saved is for {saved.rows} x {saved.channels} on {saved.stats.device}; expected {rows} x {c} "
+                         f"on {ctx.device}")
+    a.rows, a.channels, a.hidden, a.act_dtype = rows, c, saved.hidden_size, act_code(x)
+    a.out = _tensor(ctx, "out", out, x.shape, x.dtype)
+    a.accumulate = int(accumulate)
+    a.w, a.saved = C.pointer(wstruct), C.pointer(saved.struct)
+    _scratch(ctx, a, scratch)
+
+
+def transition_train(ctx: Context, x: torch.Tensor, wstruct: capi.lf_transition_weights, saved: TransitionSaved,
+                     out: torch.Tensor = None, accumulate: bool = False, fast_variance: bool = False,
+                     epsilon: float = 1e-5, scratch: torch.Tensor = None) -> torch.Tensor:
+    """The ReLU transition's training forward pass (lf_transition_train): the update, or with
+    `accumulate` x + update; `saved` receives what the backward pass needs."""
+    if out is None:
+        out = torch.empty_like(x)
+    a = capi.lf_transition_train_args()
+    a.act = _tensor(ctx, "x", x)
+    _transition_args(ctx, a, x, out, wstruct, saved, accumulate, scratch)
+    a.fast_variance, a.epsilon = int(fast_variance), epsilon
+    check(ctx.lib.lf_transition_train(ctx.handle, C.byref(a)))
+    return out
+
+
+def transition_backward(ctx: Context, grad: torch.Tensor, wstruct: capi.lf_transition_weights, saved: TransitionSaved,
+                        out: torch.Tensor = None, accumulate: bool = False, grad_dtype=torch.float32,
+                        grads: dict = None, scratch: torch.Tensor = None):
+    """Gradients of transition_train (lf_transition_backward): (of x, {name: of weight}).  `accumulate`
+    as in the forward call; `grads` may bring the buffers, all of grad_dtype."""
+    if out is None:
+        out = torch.empty_like(grad)
+    c, h = saved.channels, saved.hidden_size
+    shapes = {"layerNormScale": (c,), "layerNormOffset": (c,), "firstWeight": (c, h), "firstBias": (h,),
+              "secondWeight": (h, c), "secondBias": (c,)}
+    if wstruct.w1.layout != capi.LF_IN_OUT:
+        shapes["firstWeight"] = (h, c)
+    if wstruct.w2.layout != capi.LF_IN_OUT:
+        shapes["secondWeight"] = (c, h)
+    if not wstruct.b1:
+        del shapes["firstBias"]
+    if not wstruct.b2:
+        del shapes["secondBias"]
+    if grads is None:
+        grads = {k: torch.empty(s, dtype=grad_dtype, device=ctx.device) for k, s in shapes.items()}
+    at = {k: _tensor(ctx, f"grads[{k!r}]", grads[k], s, grad_dtype) for k, s in shapes.items()}
+    a = capi.lf_transition_backward_args()
+    a.grad = _tensor(ctx, "grad", grad)
+    _transition_args(ctx, a, grad, out, wstruct, saved, accumulate, scratch)
+    a.grad_dtype = _TORCH_ACT[grad_dtype]
+    a.grad_norm_scale, a.grad_norm_offset = at["layerNormScale"], at["layerNormOffset"]
+    a.grad_w1, a.grad_b1 = at["firstWeight"], at.get("firstBias")
+    a.grad_w2, a.grad_b2 = at["secondWeight"], at.get("secondBias")
+    check(ctx.lib.lf_transition_backward(ctx.handle, C.byref(a)))
+    return out, grads

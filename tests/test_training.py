@@ -1,0 +1,715 @@
+"""Training operators: LayerNorm and its gradient, activations kept in 8 bits, 8-bit products, weight
+gradients and the transition's training step, against float64 restatements.
+
+Tolerances.  U = 2^-24 is half a step of float32; a sum whose terms pass through at most D additions is
+off by at most D * 2U times the sum of magnitudes (2U: an addition may cut instead of round).  A stored
+value adds half a step of its type, relative to it.  The 8-bit matrix instruction drops, of 8 products
+that it adds at a time, what lies 2^-13 below the largest: at most 8 * 2^-13 of the magnitudes' sum."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+U = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+TINY = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -133}
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+# ---- float64 restatements ------------------------------------------------------------------------
+
+def e4m3_values():
+    c = np.arange(256)
+    e, m = (c >> 3) & 15, c & 7
+    v = np.where(e == 0, m * 2.0 ** -9, (8 + m) * 2.0 ** (e - 10.0))
+    v[(c & 127) == 127] = np.nan
+    return np.where(c >= 128, -v, v)
+
+
+VALUES = e4m3_values()
+
+
+def round_e4m3(v):
+    a = np.abs(v)
+    e = np.maximum(np.floor(np.log2(np.where(a > 0, a, 1.0))), -6)
+    step = 2.0 ** (e - 3)
+    return np.round(v / step) * step      # half to even
+
+
+def scale_of(most):
+    """The smallest power of two, at least 2^-126, that puts `most` within 448."""
+    m, e = np.frexp(most)
+    return np.where(most > 0, 2.0 ** np.maximum(e - 9 + (m > 0.875), -126.0), 2.0 ** -126)
+
+
+def kept64(x):
+    """x after a round trip through 8 bits."""
+    out = np.array(x, np.float64)
+    for g in range(0, x.shape[1], 128):
+        p = out[:, g:g + 128]
+        f = scale_of(np.max(np.where(np.isfinite(p), np.abs(p), 0.0), axis=1, keepdims=True))
+        with np.errstate(invalid="ignore"):
+            out[:, g:g + 128] = np.where(np.isfinite(p), round_e4m3(np.where(np.isfinite(p), p, 0) / f) * f, np.nan)
+    return out
+
+
+def kept_weight64(w):
+    out = np.array(w, np.float64)
+    for i in range(0, w.shape[0], 128):
+        for j in range(0, w.shape[1], 128):
+            p = out[i:i + 128, j:j + 128]
+            f = scale_of(np.max(np.abs(p)))
+            out[i:i + 128, j:j + 128] = round_e4m3(p / f) * f
+    return out
+
+
+def values_of(kept):
+    """What a Checkpoint's codes stand for, read here from its documented layout."""
+    codes, scales = kept.codes.cpu().numpy(), kept.scales.cpu().numpy()
+    f = 2.0 ** (scales[:, :kept.rows].T.astype(np.float64) - 127)
+    return VALUES[codes[:, :kept.cols]] * np.repeat(f, 128, axis=1)[:, :kept.cols]
+
+
+def weight_values(w):
+    codes, scales = w.codes.cpu().numpy(), w.scales.cpu().numpy()
+    f = np.repeat(np.repeat(2.0 ** (scales.astype(np.float64) - 127), 128, 0), 128, 1)
+    return VALUES[codes[:, :w.inputs]] * f[:w.outputs, :w.inputs]
+
+
+def norm64(x, s, o, eps, fast=False):
+    m = x.mean(1, keepdims=True)
+    v = (x * x).mean(1, keepdims=True) - m * m if fast else ((x - m) ** 2).mean(1, keepdims=True)
+    r = 1 / np.sqrt(v + eps)
+    return (x - m) * r * s + o, m, r
+
+
+def norm_backward64(dy, x, s, m, r):
+    h, g = (x - m) * r, dy * s
+    dx = r * (g - g.mean(1, keepdims=True) - h * (g * h).mean(1, keepdims=True))
+    return dx, (dy * h).sum(0), dy.sum(0)
+
+
+def test_norm_backward_formula_by_differences():
+    rng = np.random.default_rng(0)
+    x, dy, s, o = rng.normal(size=(3, 7)), rng.normal(size=(3, 7)), rng.normal(size=7), rng.normal(size=7)
+    _, m, r = norm64(x, s, o, 1e-5)
+    dx, ds, do = norm_backward64(dy, x, s, m, r)
+
+    def loss(x, s, o):
+        return (norm64(x, s, o, 1e-5)[0] * dy).sum()
+
+    for a, d, f in ((x, dx, lambda t: loss(t, s, o)), (s, ds, lambda t: loss(x, t, o)), (o, do, lambda t: loss(x, s, t))):
+        for i in np.ndindex(a.shape):
+            e = np.zeros_like(a)
+            e[i] = 1e-6
+            assert abs((f(a + e) - f(a - e)) / 2e-6 - d[i]) < 1e-7
+
+
+def test_checkpoint_layout_is_checked():
+    from localfold_amd import device as D
+    c = D.checkpoint_empty(17, 130, "cpu")
+    assert c.codes.shape == (17, 192) and c.scales.shape == (2, 32)
+    with pytest.raises(ValueError):
+        D.Checkpoint(17, 130, c.codes[:, :130], c.scales)
+    with pytest.raises(ValueError):
+        D.Checkpoint(17, 130, c.codes, c.scales[:, :17].contiguous())
+    with pytest.raises(ValueError):
+        D.Fp8Weight(130, 70, torch.zeros(130, 128, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.uint8))
+
+
+def test_scratch_sizes_need_no_device():
+    from localfold_amd import capi
+    lib = capi.load()
+    assert lib.lf_layer_norm_backward_scratch(5, 128) >= 2 * 128 * 4
+    assert lib.lf_fp8_weight_grad_scratch(5, 30, 40) >= 30 * 40 * 4
+    assert lib.lf_transition_backward_scratch(5, 64, 256) > lib.lf_transition_train_scratch(5, 64, 256) > 0
+    assert lib.lf_fp8_weight_grad_scratch(0, 30, 40) == lib.lf_transition_train_scratch(5, -1, 4) == 0
+
+
+def test_entry_points_refuse_null():
+    import ctypes as C
+    from localfold_amd import capi
+    lib = capi.load()
+    for name in ("lf_checkpoint_pack", "lf_layer_norm", "lf_layer_norm_backward", "lf_fp8_linear", "lf_transition_train"):
+        fn = getattr(lib, name)
+        assert fn(None, None) == capi.LF_ERR_INVALID and name.encode() in lib.lf_last_error()
+
+
+# ---- on the GPU ----------------------------------------------------------------------------------
+
+def rows_of(rng, rows, c, dt, spread=1.0):
+    x = rng.normal(size=(rows, c)) * np.exp(spread * rng.normal(size=(rows, 1))) + 0.3 * rng.normal(size=c)
+    return torch.as_tensor(x).to(dt)
+
+
+def f64(t):
+    return t.detach().cpu().double().numpy()
+
+
+def vec(rng, ctx, n, spread, centre=0.0):
+    return torch.as_tensor(centre + spread * rng.uniform(-1, 1, n)).float().to(ctx.device)
+
+
+def close(got, want, slack, dt, label=""):
+    """|got - want| within `slack` (before the store) and the store's half step."""
+    got = f64(got) if isinstance(got, torch.Tensor) else got
+    bound = slack + HALF[dt] * (np.abs(want) + slack) + TINY[dt]
+    bad = ~(np.abs(got - want) <= bound)
+    assert not bad.any(), (label, int(bad.sum()), np.argwhere(bad)[:4].tolist(),
+                           float(np.nanmax(np.abs(got - want) / np.maximum(bound, 1e-300))))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rows,c", [(1, 1), (1, 128), (3, 22), (17, 64), (50, 65), (33, 127), (129, 128), (64, 129),
+                                    (7, 200), (20, 384), (5, 1000), (1000, 256), (2, 5000)])
+def test_checkpoint_round_trip(ctx, dt, rows, c):
+    from localfold_amd import device as D
+    rng = np.random.default_rng(rows * 7 + c)
+    x = rows_of(rng, rows, c, dt)
+    x[rows // 2] = 0
+    kept = D.checkpoint_pack(ctx, x.to(ctx.device))
+    back = D.checkpoint_unpack(ctx, kept)
+    torch.cuda.synchronize()
+    want = kept64(f64(x))
+    assert np.array_equal(values_of(kept), want)
+    assert np.array_equal(f64(back), want)
+    assert (kept.codes[:, c:] == 0).all()
+    b16 = f64(D.checkpoint_unpack(ctx, kept, torch.bfloat16))
+    assert np.array_equal(b16, want)
+
+
+@pytest.mark.gpu
+def test_checkpoint_special_values(ctx):
+    """Scales at their ends, groups whose largest value sits on 448 and just above, halves between
+    codes, infinities and NaN, float32 subnormals."""
+    from localfold_amd import device as D
+    x = np.zeros((13, 256), np.float32)
+    x[0, :3] = [448, -447, 1]
+    x[1, :3] = [np.nextafter(np.float32(448), np.float32(500)), 1, 2 ** -9]
+    x[2, 0], x[2, 1] = np.float32(3.4e38), 1
+    x[3, 0] = np.float32(1e-40)
+    x[4, :4] = [np.inf, 2.5, -np.inf, np.nan]
+    x[5, 200] = np.nan
+    grid = np.concatenate([VALUES[:127], (VALUES[:126] + VALUES[1:127]) / 2]).astype(np.float32)
+    x[6, :127], x[6, 127] = grid[:127], 448
+    x[7, :126], x[7, 127] = grid[127:], 448
+    x[8] = -x[6]
+    x[9] = -x[7]
+    x[10, 128:] = 2.0 ** -126
+    x[11, :] = np.finfo(np.float32).tiny * np.linspace(-3, 3, 256)
+    x[12] = np.inf
+    kept = D.checkpoint_pack(ctx, torch.as_tensor(x).to(ctx.device))
+    back = D.checkpoint_unpack(ctx, kept)
+    torch.cuda.synchronize()
+    want = kept64(x.astype(np.float64))
+    assert np.array_equal(values_of(kept), want, equal_nan=True)
+    # 3.4e38 lies above 15.5 / 16 of 2^128, so its code stands for 2^128, which float32 stores as infinity
+    assert want[2, 0] == 2.0 ** 128
+    with np.errstate(over="ignore"):
+        assert np.array_equal(back.cpu().numpy(), want.astype(np.float32), equal_nan=True)
+
+
+@pytest.mark.gpu
+def test_checkpoint_leaves_the_neighbours(ctx):
+    """Rows behind the last and codes behind the buffer stay as they were."""
+    from localfold_amd import device as D
+    big = torch.full((40, 192), 77, dtype=torch.uint8, device=ctx.device)
+    scales = torch.full((2, 32), 78, dtype=torch.uint8, device=ctx.device)
+    x = torch.randn(19, 130, device=ctx.device)
+    D.checkpoint_pack(ctx, x, out=D.Checkpoint(19, 130, big[:19], scales))
+    torch.cuda.synchronize()
+    assert (big[19:] == 77).all() and (scales[:, 19:] == 78).all() and (scales[:, :19] != 78).any()
+
+
+def norm_slack(x, s, o, m, r, c, kept=False):
+    # sums over c values pass through at most c / 8 + 16 additions whatever the team, never over 64
+    depth = min(c, 64) + 8
+    size = np.abs(x).mean(1, keepdims=True) + np.abs(x)
+    # the variance's relative error, halved by the root, times |h|; m's error times r; each product's rounding
+    rel = 2 * depth * U * (1 + r * r * (x * x).mean(1, keepdims=True))
+    return (np.abs((x - m) * r) * rel + depth * 2 * U * size * r) * np.abs(s) + 4 * U * (np.abs((x - m) * r * s) + np.abs(o))
+
+
+NORM_SHAPES = [(1, 1), (1, 128), (59, 384), (5, 22), (33, 49), (40, 64), (100, 65), (300, 128), (17, 129), (70, 256),
+               (9, 385), (6, 513), (11, 1024), (3, 1025), (5, 1536), (4, 2048), (2, 2049), (3, 4095), (2, 4096)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rows,c", NORM_SHAPES)
+def test_layer_norm(ctx, dt, rows, c):
+    from localfold_amd import device as D
+    rng = np.random.default_rng(rows + 31 * c)
+    for fast in (False, True):
+        x, s, o = rows_of(rng, rows, c, dt, 0.3), vec(rng, ctx, c, 0.3, 1.0), vec(rng, ctx, c, 0.2)
+        xd = x.to(ctx.device)
+        stats = torch.empty(2, rows, device=ctx.device)
+        xs, ys = D.checkpoint_empty(rows, c, ctx.device), D.checkpoint_empty(rows, c, ctx.device)
+        out = D.layer_norm(ctx, xd, s, o, fast_variance=fast, out=torch.empty_like(xd), stats=stats, x_saved=xs, y_saved=ys)
+        alone = D.layer_norm(ctx, xd, s, o, fast_variance=fast)
+        torch.cuda.synchronize()
+        x64, s64, o64 = f64(x), f64(s), f64(o)
+        y, m, r = norm64(x64, s64, o64, float(np.float32(1e-5)), fast)
+        slack = norm_slack(x64, s64, o64, m, r, c)
+        if c == 1 and fast:     # the variance's true value is zero: its rounding decides; y - o = 0 all the same
+            slack = slack + 1e-6
+        close(out, y, slack, dt, f"y {fast}")
+        assert torch.equal(out, alone)
+        assert np.array_equal(values_of(xs), kept64(x64))
+        # y kept: y's own slack, then half a step of the code (2^-4, or 2^-10 of the scale below 2^-6 of it)
+        f = np.repeat(scale_of(np.stack([np.abs(y[:, g:g + 128]).max(1) * (1 + 1e-5) for g in range(0, c, 128)], 1)), 128, 1)[:, :c]
+        assert (np.abs(values_of(ys) - y) <= slack + (np.abs(y) + slack) * 2.0 ** -4 + f * 2.0 ** -10).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rows,c", NORM_SHAPES + [(5000, 128), (2100, 384)])
+def test_layer_norm_backward(ctx, dt, rows, c):
+    from localfold_amd import device as D
+    rng = np.random.default_rng(rows + 17 * c)
+    x, dy, s = rows_of(rng, rows, c, dt, 0.3), rows_of(rng, rows, c, dt, 1.0), vec(rng, ctx, c, 0.3, 1.0)
+    if rows > 2:
+        dy[rows // 2] = 0      # a padded row
+    res = rows_of(rng, rows, c, dt)
+    kept = D.checkpoint_pack(ctx, x.to(ctx.device))
+    _, m, r = norm64(f64(x), 1.0, 0.0, 1e-5)
+    stats = torch.as_tensor(np.concatenate([m, r], 1).T.copy()).float().to(ctx.device)
+    m32, r32 = f64(stats)[0][:, None], f64(stats)[1][:, None]
+    for xin, x64, residual in ((x.to(ctx.device), f64(x), None), (kept, values_of(kept), res.to(ctx.device))):
+        out, gs, go = D.layer_norm_backward(ctx, dy.to(ctx.device), xin, s, stats, residual=residual)
+        torch.cuda.synchronize()
+        d64, s64 = f64(dy), f64(s)
+        dx, ds, do = norm_backward64(d64, x64, s64, m32, r32)
+        h, g = (x64 - m32) * r32, d64 * s64
+        dh = 2 * U * (np.abs(x64) + np.abs(m32)) * r32        # h's own error
+        depth = min(c, 64) + 8
+        b = np.abs(g * h).mean(1, keepdims=True)
+        slack = r32 * (4 * U * np.abs(g) + depth * 2 * U * np.abs(g).mean(1, keepdims=True)
+                       + np.abs(h) * (depth * 2 * U * b + (np.abs(g) * dh).mean(1, keepdims=True)) + dh * b)
+        slack = slack + 4 * U * np.abs(dx)
+        if residual is not None:
+            dx = dx + f64(res)
+            slack = slack + 2 * U * np.abs(dx)
+        close(out, dx, slack, dt, "dx")
+        # rows of one block, a block's teams, the blocks
+        depth = 32 + 16 + 80
+        close(gs, ds, depth * 2 * U * np.abs(d64 * h).sum(0) + (np.abs(d64) * dh).sum(0), torch.float32, "dscale")
+        close(go, do, depth * 2 * U * np.abs(d64).sum(0), torch.float32, "doffset")
+
+
+@pytest.mark.gpu
+def test_layer_norm_backward_in_place_types_and_repeats(ctx):
+    """The gradient written over grad and over the residual, 16-bit parameter gradients, the parts
+    alone, and the same bits from the same call."""
+    from localfold_amd import device as D
+    rng = np.random.default_rng(5)
+    rows, c = 777, 128
+    x, dy, s = (t.to(ctx.device) for t in (rows_of(rng, rows, c, torch.bfloat16), rows_of(rng, rows, c, torch.bfloat16),
+                                           vec(rng, ctx, c, 0.3, 1.0)))
+    stats = torch.empty(2, rows, device=ctx.device)
+    D.layer_norm(ctx, x, s, s, stats=stats)
+    want, gs, go = D.layer_norm_backward(ctx, dy, x, s, stats, residual=x)
+    g2 = dy.clone()
+    _, hs, ho = D.layer_norm_backward(ctx, g2, x, s, stats, residual=x, out=g2, grad_dtype=torch.bfloat16)
+    x2 = x.clone()
+    D.layer_norm_backward(ctx, dy, x, s, stats, residual=x2, out=x2)
+    for _ in range(3):
+        again = D.layer_norm_backward(ctx, dy, x, s, stats, residual=x)
+        assert all(torch.equal(p, q) for p, q in zip(again, (want, gs, go)))
+    torch.cuda.synchronize()
+    assert torch.equal(g2, want) and torch.equal(x2, want)
+    assert torch.equal(hs, gs.bfloat16()) and torch.equal(ho, go.bfloat16())
+    y = x.clone()
+    D.layer_norm(ctx, y, s, s, out=y)
+    assert torch.equal(y, D.layer_norm(ctx, x, s, s))
+
+
+@pytest.mark.gpu
+def test_layer_norm_extreme_rows(ctx):
+    """Constant rows, rows far from zero, rows with an infinity or a NaN beside ordinary ones."""
+    from localfold_amd import device as D
+    rng = np.random.default_rng(6)
+    x = rng.normal(size=(8, 128))
+    x[0], x[1] = 5.0, x[1] + 1000
+    x[2, 7], x[3, 9], x[4] = np.inf, np.nan, x[4] * 1e-20
+    xt = torch.as_tensor(x).float()
+    one, zero = torch.ones(128, device=ctx.device), torch.zeros(128, device=ctx.device)
+    ys = D.checkpoint_empty(8, 128, ctx.device)
+    out = D.layer_norm(ctx, xt.to(ctx.device), one, zero, out=torch.empty(8, 128, device=ctx.device), y_saved=ys)
+    torch.cuda.synchronize()
+    got, x64 = f64(out), f64(xt)
+    assert np.isnan(got[2]).all() and np.isnan(got[3]).all() and np.isnan(values_of(ys)[2:4]).all()
+    for i in (0, 1, 4, 5, 6, 7):
+        y, m, r = norm64(x64[i:i + 1], 1.0, 0.0, float(np.float32(1e-5)))
+        close(got[i:i + 1], y, norm_slack(x64[i:i + 1], np.ones(128), np.zeros(128), m, r, 128), torch.float32, str(i))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("a,b", [(1, 1), (64, 256), (128, 128), (130, 70), (300, 513), (384, 22)])
+def test_weight_pack(ctx, dt, a, b):
+    from localfold_amd import capi, device as D
+    rng = np.random.default_rng(a + b)
+    w = torch.as_tensor(rng.normal(size=(a, b)) * np.exp(rng.normal(size=(a, 1)))).to(dt)
+    wd = w.to(ctx.device)
+    plain, turned = kept_weight64(f64(w)), kept_weight64(f64(w)).T
+    for layout, backward, want in ((capi.LF_OUT_IN, False, plain), (capi.LF_IN_OUT, False, turned),
+                                   (capi.LF_OUT_IN, True, turned), (capi.LF_IN_OUT, True, plain)):
+        p = D.fp8_weight(ctx, wd, layout, backward)
+        torch.cuda.synchronize()
+        assert (p.outputs, p.inputs) == want.shape
+        assert np.array_equal(weight_values(p), want)
+        assert (p.codes[:, p.inputs:] == 0).all()
+
+
+LINEAR_SHAPES = [(1, 1, 1), (1, 128, 128), (3, 22, 49), (16, 64, 64), (59, 384, 1536), (77, 100, 130), (130, 129, 257),
+                 (257, 128, 512), (300, 192, 100), (65, 640, 64), (513, 256, 256), (260, 1000, 300), (40, 65, 384),
+                 (1030, 64, 128), (700, 512, 768)]
+
+
+def linear_slack(xv, wv, k, exact):
+    size = np.abs(xv) @ np.abs(wv).T
+    depth = 32 + k / 32 + 4
+    return size * (depth * 2 * U + (0 if exact else 2.0 ** -10))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rows,k,n", LINEAR_SHAPES)
+def test_linear(ctx, dt, rows, k, n):
+    from localfold_amd import capi, device as D
+    rng = np.random.default_rng(rows + k + n)
+    x8 = D.checkpoint_pack(ctx, rows_of(rng, rows, k, torch.float32, 2.0).to(ctx.device))
+    w8 = D.fp8_weight(ctx, torch.as_tensor(rng.normal(size=(n, k)) / math.sqrt(k)).float().to(ctx.device), capi.LF_OUT_IN)
+    bias, res = vec(rng, ctx, n, 1.0), rows_of(rng, rows, n, dt).to(ctx.device)
+    xv, wv = values_of(x8), weight_values(w8)
+    plain = xv @ wv.T
+    slack = linear_slack(xv, wv, k, dt == torch.float32)
+    close(D.fp8_linear(ctx, x8, w8, dtype=dt), plain, slack, dt, "plain")
+    with_bias = plain + f64(bias)
+    slack = slack + 2 * U * np.abs(with_bias)
+    close(D.fp8_linear(ctx, x8, w8, bias, relu=True, dtype=dt), np.maximum(with_bias, 0), slack, dt, "relu")
+    mask = D.checkpoint_pack(ctx, rows_of(rng, rows, n, torch.float32).to(ctx.device))
+    gated = np.where(values_of(mask) > 0, plain, 0)
+    close(D.fp8_linear(ctx, x8, w8, relu_of=mask, dtype=dt), gated, np.where(values_of(mask) > 0, slack, 0), dt, "gate")
+    total = with_bias + f64(res)
+    want_slack = slack + 2 * U * np.abs(total)
+    close(D.fp8_linear(ctx, x8, w8, bias, residual=res, out=torch.empty_like(res)), total, want_slack, dt, "residual")
+    close(D.fp8_linear(ctx, x8, w8, bias, residual=res, out=res), total, want_slack, dt, "in place")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,n", LINEAR_SHAPES)
+def test_linear_kept(ctx, rows, k, n):
+    """A product kept in 8 bits: within half a code of the float64 product, scales as documented, zero
+    codes in the padding and nothing behind the last row."""
+    from localfold_amd import capi, device as D
+    rng = np.random.default_rng(rows + 3 * k + n)
+    x8 = D.checkpoint_pack(ctx, rows_of(rng, rows, k, torch.float32).to(ctx.device))
+    w8 = D.fp8_weight(ctx, torch.as_tensor(rng.normal(size=(n, k)) / math.sqrt(k)).float().to(ctx.device), capi.LF_OUT_IN)
+    bias = vec(rng, ctx, n, 1.0)
+    codes = torch.full((rows + 3, -(-n // 64) * 64), 9, dtype=torch.uint8, device=ctx.device)
+    scales = torch.full((-(-n // 128), -(-rows // 16) * 16), 9, dtype=torch.uint8, device=ctx.device)
+    out = D.Checkpoint(rows, n, codes[:rows], scales)
+    D.fp8_linear(ctx, x8, w8, bias, relu=True, out=out)
+    torch.cuda.synchronize()
+    xv, wv = values_of(x8), weight_values(w8)
+    want = np.maximum(xv @ wv.T + f64(bias), 0)
+    slack = linear_slack(xv, wv, k, False) + 2 * U * np.abs(want)
+    got = values_of(out)
+    top = np.stack([(want + slack)[:, g:g + 128].max(1) for g in range(0, n, 128)], 1)
+    low = np.stack([np.maximum(want - slack, 0)[:, g:g + 128].max(1) for g in range(0, n, 128)], 1)
+    f = 2.0 ** (scales.cpu().numpy()[:, :rows].T.astype(np.float64) - 127)
+    assert (f <= scale_of(top)).all() and (f >= scale_of(low)).all()
+    wide = np.repeat(scale_of(top), 128, 1)[:, :n]
+    assert (np.abs(got - want) <= slack + (want + slack) * 2.0 ** -4 + wide * 2.0 ** -10).all()
+    assert (codes[:rows, n:] == 0).all() and (codes[rows:] == 9).all() and (scales[:, rows:] == 9).all()
+
+
+@pytest.mark.gpu
+def test_linear_specials(ctx):
+    """A NaN in a row stays in that row, in a weight's row in that column; ReLU keeps it; rows of very
+    different size do not disturb each other."""
+    from localfold_amd import capi, device as D
+    rng = np.random.default_rng(3)
+    x = rng.normal(size=(300, 256)) * 10.0 ** rng.integers(-12, 12, size=(300, 1))
+    x[5, 200] = np.nan
+    w = rng.normal(size=(200, 256)) / 16
+    w8 = D.fp8_weight(ctx, torch.as_tensor(w).float().to(ctx.device), capi.LF_OUT_IN)
+    x8 = D.checkpoint_pack(ctx, torch.as_tensor(x).float().to(ctx.device))
+    for dt in (torch.float32, torch.bfloat16):
+        out = f64(D.fp8_linear(ctx, x8, w8, relu=True, dtype=dt))
+        assert np.isnan(out[5]).all()
+        xv, wv = values_of(x8), weight_values(w8)
+        xv[5] = 0
+        out[5] = 0
+        close(out, np.maximum(xv @ wv.T, 0), linear_slack(xv, wv, 256, dt == torch.float32), dt)
+    kept = D.checkpoint_empty(300, 200, ctx.device)
+    D.fp8_linear(ctx, x8, w8, out=kept)
+    v = values_of(kept)
+    assert np.isnan(v[5]).all() and np.isfinite(v[:5]).all() and np.isfinite(v[6:]).all()
+
+
+GRAD_SHAPES = [(1, 1, 1), (1, 128, 128), (15, 22, 49), (64, 64, 64), (100, 130, 70), (333, 128, 512), (1000, 384, 129),
+               (257, 512, 256), (4100, 256, 64), (70000, 64, 128), (37, 1536, 384)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,k", GRAD_SHAPES)
+def test_weight_grad(ctx, rows, n, k):
+    from localfold_amd import capi, device as D
+    rng = np.random.default_rng(rows + n + k)
+    g8 = D.checkpoint_pack(ctx, rows_of(rng, rows, n, torch.float32).to(ctx.device))
+    x8 = D.checkpoint_pack(ctx, rows_of(rng, rows, k, torch.float32).to(ctx.device))
+    gv, xv = values_of(g8), values_of(x8)
+    want, size = gv.T @ xv, np.abs(gv).T @ np.abs(xv)
+    # 32 products an instruction, at most 1024 instructions a split, at most 1024 splits joined in runs
+    depth = 32 + min(rows / 32, 1024) + min(rows / 32, 80)
+    for layout, dt in ((capi.LF_OUT_IN, torch.float32), (capi.LF_IN_OUT, torch.float32), (capi.LF_IN_OUT, torch.bfloat16)):
+        bias = torch.empty(n, dtype=dt, device=ctx.device)
+        out = D.fp8_weight_grad(ctx, g8, x8, layout, bias_out=bias, grad_dtype=dt)
+        alone = D.fp8_weight_grad(ctx, g8, x8, layout, grad_dtype=dt)
+        torch.cuda.synchronize()
+        turn = (lambda t: t) if layout == capi.LF_OUT_IN else np.transpose
+        close(out, turn(want), depth * 2 * U * turn(size), dt, f"dw {layout} {dt}")
+        close(bias, gv.sum(0), depth * 2 * U * np.abs(gv).sum(0), dt, "db")
+        assert torch.equal(out, alone)
+
+
+def transition_case(ctx, rng, c, h, dt, bias=True):
+    w = {"layerNormScale": vec(rng, ctx, c, 0.2, 1.0), "layerNormOffset": vec(rng, ctx, c, 0.1),
+         "firstWeight": torch.as_tensor(rng.normal(size=(c, h)) / math.sqrt(c)).to(dt).to(ctx.device),
+         "secondWeight": torch.as_tensor(rng.normal(size=(h, c)) / math.sqrt(h)).to(dt).to(ctx.device)}
+    if bias:
+        w["firstBias"], w["secondBias"] = vec(rng, ctx, h, 0.1), vec(rng, ctx, c, 0.1)
+    return w
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,c,h,dt,wdt,residual,fast", [
+    (1, 128, 512, torch.float32, torch.float32, True, False), (37, 64, 256, torch.float16, torch.float32, True, True),
+    (300, 128, 512, torch.bfloat16, torch.bfloat16, True, False), (150, 256, 1024, torch.float32, torch.float16, False, False),
+    (90, 384, 100, torch.bfloat16, torch.float32, False, True), (45, 22, 70, torch.float32, torch.float32, True, False),
+    (600, 49, 130, torch.float16, torch.bfloat16, False, False)])
+def test_transition_step(ctx, rows, c, h, dt, wdt, residual, fast):
+    """The training step stage by stage: each stage's float64 form from what the stage before it kept,
+    so that a code that falls the other way is no difference."""
+    from localfold_amd import device as D
+    rng = np.random.default_rng(rows + c)
+    w = transition_case(ctx, rng, c, h, wdt, bias=rows != 45)
+    ws, saved = D.transition_train_weights(w), D.transition_saved(rows, c, h, ctx.device)
+    x, grad = rows_of(rng, rows, c, dt, 0.3).to(ctx.device), (rows_of(rng, rows, c, dt) * 0.01).to(dt).to(ctx.device)
+    out = D.transition_train(ctx, x, ws, saved, accumulate=residual, fast_variance=fast)
+    dx, grads = D.transition_backward(ctx, grad, ws, saved, accumulate=residual)
+    torch.cuda.synchronize()
+    x64, g64 = f64(x), f64(grad)
+    zero = {"firstBias": np.zeros(h), "secondBias": np.zeros(c)}
+    p = {k: f64(w[k]) if k in w else zero[k] for k in ("layerNormScale", "layerNormOffset", "firstWeight", "firstBias",
+                                                       "secondWeight", "secondBias")}
+    w1, w2 = kept_weight64(p["firstWeight"]), kept_weight64(p["secondWeight"])
+    y, m, r = norm64(x64, p["layerNormScale"], p["layerNormOffset"], float(np.float32(1e-5)), fast)
+    assert np.array_equal(values_of(saved.act), kept64(x64))
+    y8, h8 = values_of(saved.normed), values_of(saved.hidden)
+    code = 2.0 ** -4 + 2.0 ** -9      # half a code, and what moves a value to the next one
+    low = 2.0 ** -10 * 2.0 ** -7      # half the smallest code, relative to the group's largest value
+    top = np.abs(y).max(1, keepdims=True)
+    assert (np.abs(y8 - y) <= np.abs(y) * code + top * low).all()
+    pre = np.maximum(y8 @ w1 + p["firstBias"], 0)
+    top = np.maximum(pre.max(1, keepdims=True), 1e-30)
+    assert (np.abs(h8 - pre) <= pre * code + top * low + 2.0 ** -10 * (np.abs(y8) @ np.abs(w1))).all()
+    upd = h8 @ w2 + p["secondBias"]
+    total = upd + x64 if residual else upd
+    close(out, total, (np.abs(h8) @ np.abs(w2)) * (2.0 ** -10 + 2 * U * 80) + 4 * U * (np.abs(total) + np.abs(x64)), dt, "out")
+
+    d8 = kept64(g64)
+    size = np.abs(h8).T @ np.abs(d8)
+    close(grads["secondWeight"], h8.T @ d8, 200 * 2 * U * size, torch.float32, "dw2")
+    pre_e = np.where(h8 > 0, d8 @ w2.T, 0)
+    slack_e = np.where(h8 > 0, np.abs(pre_e) * code + np.abs(pre_e).max(1, keepdims=True) * low
+                       + 2.0 ** -10 * (np.abs(d8) @ np.abs(w2.T)), 0)
+    close(grads["firstWeight"], y8.T @ pre_e, np.abs(y8).T @ slack_e + 1e-6 * (np.abs(y8).T @ np.abs(pre_e)), torch.float32, "dw1")
+    if "firstBias" in w:
+        close(grads["firstBias"], pre_e.sum(0), slack_e.sum(0) + 1e-6 * np.abs(pre_e).sum(0), torch.float32, "db1")
+        close(grads["secondBias"], d8.sum(0), 200 * 2 * U * np.abs(d8).sum(0), torch.float32, "db2")
+    dy = pre_e @ w1.T
+    slack_y = slack_e @ np.abs(w1.T) + (np.abs(pre_e) @ np.abs(w1.T)) * 2.0 ** -9 + np.abs(dy) * HALF[dt] + TINY[dt]
+    st = f64(saved.stats)
+    x8, s = values_of(saved.act), p["layerNormScale"]
+    m32, r32 = st[0][:, None], st[1][:, None]
+    want, ds, do = norm_backward64(dy, x8, s, m32, r32)
+    hh, gs = (x8 - m32) * r32, slack_y * np.abs(s)
+    slack = r32 * (gs + gs.mean(1, keepdims=True) + np.abs(hh) * (gs * np.abs(hh)).mean(1, keepdims=True)) + 1e-5 * np.abs(want)
+    if residual:
+        want = want + g64
+    close(dx, want, slack + 1e-5 * np.abs(want), dt, "dx")
+    close(grads["layerNormScale"], ds, (slack_y * np.abs(hh)).sum(0) + 1e-5 * np.abs(dy * hh).sum(0), torch.float32, "ds")
+    close(grads["layerNormOffset"], do, slack_y.sum(0) + 1e-5 * np.abs(dy).sum(0), torch.float32, "do")
+
+
+@pytest.mark.gpu
+def test_transition_gradients_by_differences(ctx):
+    """The step's gradients against differences of its own float32 forward pass along random
+    directions.  The codes' roundings (2^-4 each, unbiased, over rows x hidden of them) leave a few
+    percent; a wrong factor, sign or missing term is far outside."""
+    from localfold_amd import device as D
+    rng = np.random.default_rng(11)
+    rows, c, h = 2048, 128, 512
+    w = transition_case(ctx, rng, c, h, torch.float32)
+    x, grad = (torch.as_tensor(rng.normal(size=(rows, c))).float().to(ctx.device) for _ in range(2))
+    saved = D.transition_saved(rows, c, h, ctx.device)
+    ws = D.transition_train_weights(w)
+    D.transition_train(ctx, x, ws, saved, accumulate=True)
+    dx, grads = D.transition_backward(ctx, grad, ws, saved, accumulate=True)
+    torch.cuda.synchronize()
+
+    def loss(x, w):
+        y, _, _ = norm64(f64(x), f64(w["layerNormScale"]), f64(w["layerNormOffset"]), 1e-5)
+        hid = np.maximum(y @ f64(w["firstWeight"]) + f64(w["firstBias"]), 0)
+        return ((f64(x) + hid @ f64(w["secondWeight"]) + f64(w["secondBias"])) * f64(grad)).sum()
+
+    # along the gradient itself: the difference is its squared length
+    for name, t, g in [("x", x, dx)] + [(k, w[k], grads[k]) for k in grads]:
+        d = g.double()
+        length = float((d * d).sum())
+        eps = 1e-3 * float(t.double().norm()) / max(float(d.norm()), 1e-30)
+        up, down = (t.double() + eps * d).to(t.dtype), (t.double() - eps * d).to(t.dtype)
+        if name == "x":
+            got = (loss(up, w) - loss(down, w)) / (2 * eps)
+        else:
+            got = (loss(x, {**w, name: up}) - loss(x, {**w, name: down})) / (2 * eps)
+        assert abs(got - length) < 0.1 * length, (name, got, length)
+
+
+@pytest.mark.gpu
+def test_training_step_in_place_and_other_stream(ctx):
+    """out written over the activations, dx over the gradient; the whole step on another stream."""
+    from localfold_amd import device as D
+    rng = np.random.default_rng(2)
+    rows, c, h = 500, 128, 512
+    w = transition_case(ctx, rng, c, h, torch.bfloat16)
+    ws, saved = D.transition_train_weights(w), D.transition_saved(rows, c, h, ctx.device)
+    x, grad = rows_of(rng, rows, c, torch.bfloat16).to(ctx.device), rows_of(rng, rows, c, torch.bfloat16).to(ctx.device)
+    want = D.transition_train(ctx, x, ws, saved, accumulate=True)
+    dx, grads = D.transition_backward(ctx, grad, ws, saved, accumulate=True)
+    x2, g2 = x.clone(), grad.clone()
+    D.transition_train(ctx, x2, ws, saved, out=x2, accumulate=True)
+    _, again = D.transition_backward(ctx, g2, ws, saved, out=g2, accumulate=True)
+    torch.cuda.synchronize()
+    assert torch.equal(x2, want) and torch.equal(g2, dx) and all(torch.equal(grads[k], again[k]) for k in grads)
+    s = torch.cuda.Stream()
+    try:
+        with torch.cuda.stream(s):
+            ctx.bind_stream()
+            x3, g3 = x.clone(), grad.clone()
+            D.transition_train(ctx, x3, ws, saved, out=x3, accumulate=True)
+            _, third = D.transition_backward(ctx, g3, ws, saved, out=g3, accumulate=True)
+        s.synchronize()
+    finally:
+        ctx.bind_stream()
+    assert torch.equal(x3, want) and torch.equal(g3, dx) and all(torch.equal(grads[k], third[k]) for k in grads)
+
+
+@pytest.mark.gpu
+def test_training_step_in_a_graph(ctx):
+    """Two captured steps with scratch of their own, replayed in turn with eager steps (which move the
+    context's workspace) between them, against the eager results; without scratch the capture is refused."""
+    from localfold_amd import capi, device as D
+    rng = np.random.default_rng(4)
+    rows, c, h = 700, 128, 256
+    cases = []
+    for k in range(2):
+        w = transition_case(ctx, rng, c, h, torch.float32)
+        ws, saved = D.transition_train_weights(w), D.transition_saved(rows, c, h, ctx.device)
+        x, grad = rows_of(rng, rows, c, torch.float32).to(ctx.device), rows_of(rng, rows, c, torch.float32).to(ctx.device)
+        out, dx = torch.empty_like(x), torch.empty_like(x)
+        grads = {n: torch.zeros_like(w[n]) for n in w}
+        need = max(ctx.lib.lf_transition_train_scratch(rows, c, h), ctx.lib.lf_transition_backward_scratch(rows, c, h))
+        scratch = torch.empty(need, dtype=torch.uint8, device=ctx.device)
+
+        def step(scratch, x=x, grad=grad, ws=ws, saved=saved, out=out, dx=dx, grads=grads):
+            D.transition_train(ctx, x, ws, saved, out=out, accumulate=True, scratch=scratch)
+            D.transition_backward(ctx, grad, ws, saved, out=dx, accumulate=True, grads=grads, scratch=scratch)
+
+        step(scratch)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        try:
+            with torch.cuda.graph(g):
+                ctx.bind_stream()
+                with pytest.raises(capi.LocalfoldError, match="scratch"):
+                    step(None)
+                step(scratch)
+        finally:
+            ctx.bind_stream()
+        cases.append((g, x, w, (out, dx, grads), step))
+    for turn in range(4):
+        for g, x, w, (out, dx, grads), step in cases:
+            x += 0.25
+            w["secondWeight"] *= 0.9
+            g.replay()
+            torch.cuda.synchronize()
+            got = [out.clone(), dx.clone()] + [grads[n].clone() for n in sorted(grads)]
+            big = torch.randn(4000 * (turn + 1), 128, device=ctx.device)      # moves the workspace
+            D.layer_norm_backward(ctx, big, big, w["layerNormScale"], torch.ones(2, big.shape[0], device=ctx.device))
+            step(None)
+            torch.cuda.synchronize()
+            want = [out, dx] + [grads[n] for n in sorted(grads)]
+            assert all(torch.equal(p, q) for p, q in zip(got, want)), turn
+
+
+@pytest.mark.gpu
+def test_refusals(ctx):
+    import ctypes as C
+    from localfold_amd import capi, device as D
+    dev = ctx.device
+    x = torch.randn(10, 128, device=dev)
+    s = torch.ones(128, device=dev)
+    k = D.checkpoint_pack(ctx, x)
+    w = D.fp8_weight(ctx, torch.randn(128, 64, device=dev))
+    stats = torch.ones(2, 10, device=dev)
+    with pytest.raises(ValueError):
+        D.checkpoint_pack(ctx, x[:, ::2])
+    with pytest.raises(TypeError):
+        D.checkpoint_pack(ctx, x.double())
+    with pytest.raises(ValueError):
+        D.layer_norm(ctx, x.cpu(), s, s)
+    with pytest.raises(TypeError):
+        D.layer_norm(ctx, x, s.half(), s)
+    with pytest.raises(ValueError):
+        D.layer_norm(ctx, x, s[:64].contiguous(), s)
+    with pytest.raises(capi.LocalfoldError, match="epsilon"):
+        D.layer_norm(ctx, x, s, s, epsilon=0.0)
+    with pytest.raises(capi.LocalfoldError, match="wide"):
+        D.layer_norm(ctx, torch.randn(2, 4097, device=dev), torch.ones(4097, device=dev), torch.ones(4097, device=dev))
+    with pytest.raises(capi.LocalfoldError, match="positive"):
+        D.layer_norm(ctx, torch.empty(0, 128, device=dev), s, s)
+    with pytest.raises(ValueError):
+        D.fp8_linear(ctx, D.checkpoint_pack(ctx, x[:, :100].contiguous()), w)
+    with pytest.raises(ValueError):
+        D.fp8_linear(ctx, k, w, residual=torch.zeros(10, 64, device=dev), out=D.checkpoint_empty(10, 64, dev))
+    with pytest.raises(ValueError):
+        D.fp8_weight_grad(ctx, k, D.checkpoint_empty(11, 128, dev))
+    with pytest.raises(capi.LocalfoldError, match="scratch has"):
+        D.fp8_weight_grad(ctx, k, k, scratch=torch.empty(16, dtype=torch.uint8, device=dev))
+    with pytest.raises(capi.LocalfoldError, match="aligned"):
+        D.layer_norm_backward(ctx, x, x, s, stats, scratch=torch.empty(1 << 20, dtype=torch.uint8, device=dev)[3:])
+    bad = D.Checkpoint(10, 128, torch.empty(10 * 128 + 8, dtype=torch.uint8, device=dev)[8:].view(10, 128), k.scales)
+    with pytest.raises(capi.LocalfoldError, match="aligned"):
+        D.checkpoint_pack(ctx, x, out=bad)
+    a = capi.lf_layer_norm_backward_args()
+    a.rows, a.channels, a.act_dtype, a.grad = 10, 128, capi.LF_F32, x.data_ptr()
+    assert ctx.lib.lf_layer_norm_backward(ctx.handle, C.byref(a)) == capi.LF_ERR_INVALID
+    assert b"either act or act_kept" in ctx.lib.lf_last_error()
+    weights = transition_case(ctx, np.random.default_rng(0), 128, 64, torch.float32)
+    ws = D.transition_train_weights(weights)
+    with pytest.raises(ValueError):
+        D.transition_train(ctx, x, ws, D.transition_saved(11, 128, 64, dev))
+    with pytest.raises(capi.LocalfoldError, match="hidden"):
+        D.transition_train(ctx, x, ws, D.transition_saved(10, 128, 65, dev))
+    ws.w1.dtype = capi.LF_INT8
+    with pytest.raises(capi.LocalfoldError, match="not trained"):
+        D.transition_train(ctx, x, ws, D.transition_saved(10, 128, 64, dev))
+    before = torch.cuda.current_device()
+    assert before == 0
