@@ -40,39 +40,55 @@ struct PackBatch {
   int count;
 };
 
-// One block packs one tile of 128 x 128 of the stored matrix: read once (coalesced along the stored
-// rows) into LDS, its largest magnitude, then the codes, written along the packed rows.
-__global__ __launch_bounds__(256) void pack_weight_kernel(PackBatch b) {
+// One block packs one tile of 128 x 128 of the stored matrix: read once into LDS, 8 consecutive values a
+// lane, its largest magnitude, then the codes, 8 consecutive of a packed row a lane.  A matrix has few
+// tiles, so a block is as large as it can be: latency is what a pack costs.
+template <int ACT>
+__device__ __forceinline__ float pack_weight_load(const PackWeight& w, int r0, int c0, float (*tile)[GROUP + 1]) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int e = i * 1024 + threadIdx.x, r = e >> 4, c = (e & 15) * 8;
+    float v[8] = {};
+    if (r0 + r < w.rows)
+      load8<ACT>(static_cast<const typename Act<ACT>::T*>(w.data) + (size_t)(r0 + r) * w.cols + c0 + c, w.cols - c0 - c, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) tile[r][c + k] = v[k];
+    top = fmaxf(top, amax8_finite(v));
+  }
+  return top;
+}
+
+__global__ __launch_bounds__(1024) void pack_weight_kernel(PackBatch b) {
   __shared__ float tile[GROUP][GROUP + 1];
-  __shared__ float sm[4];
+  __shared__ float sm[16];
   int m = 0;
   while (m + 1 < b.count && (int)blockIdx.x >= b.first[m + 1]) ++m;
   const PackWeight& w = b.w[m];
   const int tc = (w.cols + GROUP - 1) / GROUP;
-  const int t = blockIdx.x - b.first[m], tr = t / tc, r0 = tr * GROUP, c0 = (t % tc) * GROUP;
-  float top = 0.f;
-  for (int e = threadIdx.x; e < GROUP * GROUP; e += 256) {
-    const int r = e / GROUP, c = e % GROUP;
-    float v = 0.f;
-    if (r0 + r < w.rows && c0 + c < w.cols) v = load_act(w.data, w.dtype, (size_t)(r0 + r) * w.cols + c0 + c);
-    tile[r][c] = v;
-    top = fmaxf(top, fabsf(v) < __builtin_inff() ? fabsf(v) : 0.f);
-  }
+  const int t = blockIdx.x - b.first[m], r0 = t / tc * GROUP, c0 = t % tc * GROUP;
+  float top = w.dtype == DT_F32   ? pack_weight_load<DT_F32>(w, r0, c0, tile)
+              : w.dtype == DT_F16 ? pack_weight_load<DT_F16>(w, r0, c0, tile)
+                                  : pack_weight_load<DT_BF16>(w, r0, c0, tile);
   top = team_reduce<64, OpMax>(top);
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = top;
   __syncthreads();
-  const int byte = scale_byte(fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])));
-  const float inv = scale_inverse(byte);
+  top = team_reduce<16, OpMax>(sm[threadIdx.x & 15]);
+  const int byte = scale_byte(top);
+  const float f = scale_value(byte);
   const int rows = w.transpose ? w.cols : w.rows, cols = w.transpose ? w.rows : w.cols;   // of the packed matrix
   const int p0 = w.transpose ? c0 : r0, q0 = w.transpose ? r0 : c0;
   const int pitch = (int)LF_CHECKPOINT_PITCH(cols);
-  for (int e = threadIdx.x; e < GROUP * GROUP / 8; e += 256) {
-    const int r = e / (GROUP / 8), c = e % (GROUP / 8) * 8;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int e = i * 1024 + threadIdx.x;
+    // transposed, neighbouring lanes take neighbouring rows: LDS columns without bank conflicts
+    const int r = w.transpose ? e & 127 : e >> 4, c = w.transpose ? (e >> 7) * 8 : (e & 15) * 8;
     if (p0 + r >= rows || q0 + c >= pitch) continue;
     float v[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = w.transpose ? tile[c + k][r] : tile[r][c + k];
-    *reinterpret_cast<uint2*>(w.codes + (size_t)(p0 + r) * pitch + q0 + c) = encode8(v, inv);
+    *reinterpret_cast<uint2*>(w.codes + (size_t)(p0 + r) * pitch + q0 + c) = encode8(v, f);
   }
   if (threadIdx.x == 0) w.scales[(size_t)(p0 / GROUP) * ((cols + GROUP - 1) / GROUP) + q0 / GROUP] = (uint8_t)byte;
 }
@@ -121,7 +137,7 @@ int run_pack_weights(lf_context* ctx, const PackWeight* w, int count) {
     b.first[i + 1] = b.first[i] + (int)(LF_CHECKPOINT_GROUPS(w[i].rows) * LF_CHECKPOINT_GROUPS(w[i].cols));
   }
   LaunchScope ls(ctx, "fp8.pack_weight");
-  hipLaunchKernelGGL(pack_weight_kernel, dim3(b.first[count]), dim3(256), 0, ctx->stream, b);
+  hipLaunchKernelGGL(pack_weight_kernel, dim3(b.first[count]), dim3(1024), 0, ctx->stream, b);
   return check_hip(hipGetLastError(), "fp8 weight pack launch");
 }
 

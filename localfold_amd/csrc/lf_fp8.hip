@@ -181,7 +181,7 @@ __device__ __forceinline__ void finish(f4 (&acc)[8][4], const LinearParams& p, l
     for (int t = 0; t < 8; ++t) {
       if (p.relu) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[t][q][j] = acc[t][q][j] < 0.f ? 0.f : acc[t][q][j];    // keeps NaN
+        for (int j = 0; j < 4; ++j) acc[t][q][j] = __builtin_elementwise_maximum(acc[t][q][j], 0.f);   // keeps NaN
       }
     }
     if (p.relu_of) {
@@ -201,14 +201,18 @@ __device__ __forceinline__ void finish(f4 (&acc)[8][4], const LinearParams& p, l
       }
     }
     if constexpr (OUT == OUT_KEPT) {
+      if (nb * GROUP + GROUP > N) {    // codes behind the last output are zeros
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (nb * GROUP + n_of<OUT>(t, 4 * g) + j >= N) acc[t][q][j] = 0.f;
+      }
       float top = 0.f;
 #pragma unroll
       for (int t = 0; t < 8; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (nb * GROUP + GROUP > N && nb * GROUP + n_of<OUT>(t, 4 * g) + j >= N) acc[t][q][j] = 0.f;
-          top = fmaxf(top, fabsf(acc[t][q][j]));
-        }
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(acc[t][q][j]));
       top = lanes4_max(top);
       if (__builtin_expect(__any(top == __builtin_inff()), 0)) {
         float f = 0.f;
@@ -219,19 +223,18 @@ __device__ __forceinline__ void finish(f4 (&acc)[8][4], const LinearParams& p, l
         top = lanes4_max(f);
       }
       const int byte = scale_byte(top);
-      const float inv = scale_inverse(byte);
+      const float f = scale_value(byte);
       uint8_t* dst = p.q.codes + row * p.q.pitch + nb * GROUP;
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
-        int c[4];
+        u32x4 c;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          const f4 v = acc[a * 4 + b][q] * inv;
-          c[b] = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
-          c[b] = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], c[b], true);
+          const f4 v = acc[a * 4 + b][q];
+          c[b] = encode4(v[0], v[1], v[2], v[3], f);
         }
         const int nl = a * 64 + g * 16;
-        if (row_ok && nb * GROUP + nl < p.q.pitch) *reinterpret_cast<u32x4*>(dst + nl) = u32x4{(uint32_t)c[0], (uint32_t)c[1], (uint32_t)c[2], (uint32_t)c[3]};
+        if (row_ok && nb * GROUP + nl < p.q.pitch) *reinterpret_cast<u32x4*>(dst + nl) = c;
       }
       if (row_ok && g == 0) p.q.scales[(size_t)nb * p.q.sp + row] = (uint8_t)byte;
     } else {
@@ -309,30 +312,37 @@ __global__ __launch_bounds__(NT, 2) void fp8_linear_resident_kernel(LinearParams
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
 
+  // this block's units, of (rows / 64) x per, and the wave's first; a unit is (row tile, output group)
   const long long units = ((long long)p.rows + MROWS - 1) / MROWS * per;
-  const long long u0 = units * blk / q.blocks, u1 = units * (blk + 1) / q.blocks;
+  const int u0 = (int)(units * blk / q.blocks), u1 = (int)(units * (blk + 1) / q.blocks);
   const int i16 = n_of<OUT>(0, r);
   const uint8_t* wl = fp8_smem + i16 * GROUP + ((g ^ key_of<OUT>(i16)) << 4);
   const uint8_t* wlx = fp8_smem + i16 * GROUP + ((g ^ key_of<OUT>(i16) ^ 4) << 4);
   f4 acc[8][4];
   XFrag x, xn;
-  long long u = u0 + wave;
-  int kb = 0;
+  int u = u0 + wave, kb = 0, mt = u / per, nb = u % per;
+  const int mstep = WAVES / per, nstep = WAVES % per;
   if (u >= u1) return;
-  x_load(x, p, u / per * MROWS, 0, r, g);
+  x_load(x, p, (long long)mt * MROWS, 0, r, g);
   for (;;) {
-    const long long u_now = u;
-    const int kb_now = kb, nb = (int)(u_now % per);
+    const int kb_now = kb, mt_now = mt, nb_now = nb;
     if (++kb == kbs) {
       kb = 0;
       u += WAVES;
+      if (u < u1) {      // past the last step the same rows again, which nothing uses
+        mt += mstep;
+        nb += nstep;
+        if (nb >= per) {
+          nb -= per;
+          ++mt;
+        }
+      }
     }
-    const long long ul = min(u, u1 - 1);     // past the last step: rows that nothing uses
-    if (kb_now == 0) start<OUT>(acc, bias + nb * GROUP, g);
-    const int at = (nb * kbs + kb_now) * WTILE;
-    mma<OUT>(acc, wl + at, wlx + at, x, p.ws[(size_t)(nb0 + nb) * kbs + kb_now],
-             [&]() __attribute__((always_inline)) { x_load(xn, p, ul / per * MROWS, kb, r, g); });
-    if (kb_now == kbs - 1) finish<OUT>(acc, p, u_now / per * MROWS, nb0 + nb, r, g);
+    if (kb_now == 0) start<OUT>(acc, bias + nb_now * GROUP, g);
+    const int at = (nb_now * kbs + kb_now) * WTILE;
+    mma<OUT>(acc, wl + at, wlx + at, x, p.ws[(nb0 + nb_now) * kbs + kb_now],
+             [&]() __attribute__((always_inline)) { x_load(xn, p, (long long)mt * MROWS, kb, r, g); });
+    if (kb_now == kbs - 1) finish<OUT>(acc, p, (long long)mt_now * MROWS, nb0 + nb_now, r, g);
     if (u >= u1) break;
     x = xn;
   }
@@ -340,7 +350,8 @@ __global__ __launch_bounds__(NT, 2) void fp8_linear_resident_kernel(LinearParams
 
 // Long reductions: a block of 512 rows and one output group walks the columns, its weight tiles in two LDS
 // buffers in turn.  One barrier a step; the next step's tile and rows are under way during this one's
-// products.
+// products.  Blocks begin at different columns: with rows a power of two apart, one column of all rows
+// lies on one memory channel.
 template <int OUT>
 __global__ __launch_bounds__(NT, 2) void fp8_linear_stream_kernel(LinearParams p, LinearGrid q) {
   __shared__ __attribute__((aligned(16))) uint8_t W[2][WTILE];
@@ -361,17 +372,19 @@ __global__ __launch_bounds__(NT, 2) void fp8_linear_stream_kernel(LinearParams p
   const int wl = i16 * GROUP + ((g ^ key_of<OUT>(i16)) << 4), wlx = wl ^ 64;
   f4 acc[8][4];
   XFrag x, xn;
-  stage(W[0], 0);
-  x_load(x, p, mx, 0, r, g);
-  for (int kb = 0; kb < kbs; ++kb) {
+  int kb = slot % kbs;
+  stage(W[0], kb);
+  x_load(x, p, mx, kb, r, g);
+  for (int s = 0; s < kbs; ++s) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();     // tile kb in LDS for every wave; every wave done with the other buffer
-    if (kb == 0) start<OUT>(acc, bias, g);
-    const int kn = min(kb + 1, kbs - 1);
-    stage(W[(kb + 1) & 1], kn);
-    mma<OUT>(acc, W[kb & 1] + wl, W[kb & 1] + wlx, x, p.ws[(size_t)nb * kbs + kb],
+    __syncthreads();     // step s in LDS for every wave; every wave done with the other buffer
+    if (s == 0) start<OUT>(acc, bias, g);
+    const int kn = kb + 1 < kbs ? kb + 1 : 0;
+    stage(W[(s + 1) & 1], kn);
+    mma<OUT>(acc, W[s & 1] + wl, W[s & 1] + wlx, x, p.ws[(size_t)nb * kbs + kb],
              [&]() __attribute__((always_inline)) { x_load(xn, p, mx, kn, r, g); });
     x = xn;
+    kb = kn;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last copy, which nothing reads
   if (live) finish<OUT>(acc, p, m0, nb, r, g);

@@ -210,23 +210,44 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(NormGradParams p) {
   }
 }
 
-// Columns of [blocks][cols] partial sums added in order of the blocks, 16 runs of them at a time.
+// Columns of [blocks][2 C] partial sums added in order of the blocks: 64 columns a block, four a lane, in
+// 64 runs of the blocks, then 8 of 8 runs, then those.
 template <int OUT>
 __global__ __launch_bounds__(1024) void norm_join_kernel(const float* partial, int blocks, int C, void* ds, void* dof) {
-  __shared__ float sm[16][64];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
-  const int per = (blocks + 15) / 16, b0 = part * per, b1 = min(blocks, b0 + per);
-  float t = 0.f;
-  if (c < 2 * C)
-    for (int b = b0; b < b1; ++b) t += partial[(size_t)b * 2 * C + c];
-  sm[part][threadIdx.x & 63] = t;
+  __shared__ f4 sm[64][16];
+  const int lane = threadIdx.x & 15, run = threadIdx.x >> 4, c = blockIdx.x * 64 + lane * 4;
+  const int per = (blocks + 63) / 64, b0 = run * per, b1 = min(blocks, b0 + per);
+  f4 t = {0.f, 0.f, 0.f, 0.f};
+  if (c + 4 <= 2 * C) {
+#pragma unroll 8
+    for (int b = b0; b < b1; ++b) {
+      f4 v;
+      __builtin_memcpy(&v, partial + (size_t)b * 2 * C + c, 16);   // rows may be unaligned
+      t += v;
+    }
+  } else {
+    for (int b = b0; b < b1; ++b)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (c + k < 2 * C) t[k] += partial[(size_t)b * 2 * C + c + k];
+  }
+  sm[run][lane] = t;
   __syncthreads();
-  if (part == 0 && c < 2 * C) {
-    t = 0.f;
-    for (int i = 0; i < 16; ++i) t += sm[i][threadIdx.x];
-    typedef typename Act<OUT>::T T;
-    if (c < C) Act<OUT>::st(static_cast<T*>(ds) + c, t);
-    else Act<OUT>::st(static_cast<T*>(dof) + c - C, t);
+  if (run < 8) {
+    t = sm[run * 8][lane];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) t += sm[run * 8 + i][lane];
+    sm[run * 8][lane] = t;
+  }
+  __syncthreads();
+  if (run != 0) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) t += sm[i * 8][lane];
+  typedef typename Act<OUT>::T T;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (c + k < C) Act<OUT>::st(static_cast<T*>(ds) + c + k, t[k]);
+    else if (c + k < 2 * C) Act<OUT>::st(static_cast<T*>(dof) + c + k - C, t[k]);
   }
 }
 

@@ -131,24 +131,26 @@ __device__ __forceinline__ float amax8_finite(const float (&v)[8]) {
 }
 
 // The stored byte of the smallest power of two that puts m within 448 = 1.75 * 2^8: m = f * 2^p with
-// f in [1, 2) needs 2^(p - 8), or 2^(p - 7) when f > 1.75.  At least 1, so that the power and its
-// inverse are normal numbers.
+// f in [1, 2) needs 2^(p - 8), or 2^(p - 7) when f > 1.75.  At least 1, so that the power is a normal
+// number.
 __device__ __forceinline__ int scale_byte(float m) {
   const uint32_t u = __float_as_uint(m);
   const int b = (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
   return b < 1 ? 1 : b;
 }
 __device__ __forceinline__ float scale_value(int b) { return __uint_as_float((uint32_t)b << 23); }
-__device__ __forceinline__ float scale_inverse(int b) { return __uint_as_float((uint32_t)(254 - b) << 23); }
 
-// Codes of eight values over the scale whose inverse is given.  Within 448 by the choice of the scale;
-// v_cvt_pk_fp8_f32 rounds to nearest even and makes infinities and NaN the NaN code.
-__device__ __forceinline__ uint2 encode8(const float (&v)[8], float inv) {
-  int a = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
-  a = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, a, true);
-  int b = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * inv, v[5] * inv, 0, false);
-  b = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * inv, v[7] * inv, b, true);
-  return make_uint2((uint32_t)a, (uint32_t)b);
+// Four values over a power of two as codes.  Within 448 by the choice of the scale; the instruction divides
+// exactly, rounds to nearest even and makes infinities and NaN the NaN code.
+__device__ __forceinline__ uint32_t encode4(float v0, float v1, float v2, float v3, float scale) {
+  typedef short s2v __attribute__((ext_vector_type(2)));
+  s2v c = {0, 0};
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, v0, v1, scale, false);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, v2, v3, scale, true);
+  return __builtin_bit_cast(uint32_t, c);
+}
+__device__ __forceinline__ uint2 encode8(const float (&v)[8], float scale) {
+  return make_uint2(encode4(v[0], v[1], v[2], v[3], scale), encode4(v[4], v[5], v[6], v[7], scale));
 }
 
 __device__ __forceinline__ void decode4(uint32_t w, float s, float* v) {
@@ -169,7 +171,7 @@ __device__ __forceinline__ void keep8(const Kept& k, size_t row, int c0, const f
     m = m < 0.f ? f : m;
   }
   const int b = scale_byte(m);
-  const uint2 q = encode8(v, scale_inverse(b));
+  const uint2 q = encode8(v, scale_value(b));
   if (write && c0 < k.pitch) {
     *reinterpret_cast<uint2*>(k.codes + row * (size_t)k.pitch + c0) = q;
     if ((c0 & (GROUP - 1)) == 0) k.scales[(size_t)(c0 / GROUP) * k.sp + row] = (uint8_t)b;
