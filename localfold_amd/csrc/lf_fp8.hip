@@ -288,8 +288,9 @@ __device__ __forceinline__ void finish(f4 (&acc)[8][4], const LinearParams& p, l
 }
 
 struct LinearGrid {
-  int per;                      // output groups of a subset (resident) or 1
-  int subsets, blocks;          // blocks of a subset
+  int per;                      // resident: output groups of a subset
+  int subsets;                  // subsets; stream: pairs of output groups
+  int blocks;                   // blocks of a subset; stream: row tiles of 256
 };
 
 // Weights resident: a block copies its subset of output groups, all their columns, to LDS once; its waves
@@ -348,46 +349,79 @@ __global__ __launch_bounds__(NT, 2) void fp8_linear_resident_kernel(LinearParams
   }
 }
 
-// Long reductions: a block of 512 rows and one output group walks the columns, its weight tiles in two LDS
-// buffers in turn.  One barrier a step; the next step's tile and rows are under way during this one's
-// products.  Blocks begin at different columns: with rows a power of two apart, one column of all rows
-// lies on one memory channel.
+// Rows m0 .. m0 + 63 of column group kb as x_load's fragments, from an LDS tile of 64 x 128 codes whose
+// chunk c of row m lies at c ^ ((m >> 2) & 7), and their scale bytes from memory.
+__device__ __forceinline__ void x_stage(uint8_t* dst, const LinearParams& p, long long m0, int kb, int part, int lane) {
+  const int row = part * 8 + (lane >> 3), c = (lane & 7) ^ (row >> 2 & 7);
+  const long long m = min(m0 + row, (long long)p.rows - 1);
+  const uint8_t* src = p.x.codes + (size_t)m * p.x.pitch + kb * GROUP + c * 16;
+  if (kb * GROUP + c * 16 >= p.x.pitch) src = reinterpret_cast<const uint8_t*>(&fp8_zero16);
+#if __HIP_DEVICE_COMPILE__
+  __builtin_amdgcn_global_load_lds(src, dst + part * 1024, 16, 0, 0);
+#else
+  (void)src;
+#endif
+}
+
+// Long reductions: a block of 256 rows and two output groups walks the columns 128 at a time, tiles of both
+// operands in two LDS buffers in turn.  One barrier a step; the next step's tiles are under way during this
+// one's products.  Blocks on one XCD run through 4 row tiles and then the outputs, so its L2 serves both.
 template <int OUT>
 __global__ __launch_bounds__(NT, 2) void fp8_linear_stream_kernel(LinearParams p, LinearGrid q) {
-  __shared__ __attribute__((aligned(16))) uint8_t W[2][WTILE];
-  __shared__ __attribute__((aligned(16))) float bias[GROUP];
+  extern __shared__ __attribute__((aligned(16))) uint8_t fp8_smem[];   // [2][2 weight tiles, 4 x tiles of 64 rows]
+  __shared__ __attribute__((aligned(16))) float bias[2 * GROUP];
+  constexpr int STAGE = 2 * WTILE + 4 * MROWS * GROUP;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int kbs = (p.inputs + GROUP - 1) / GROUP;
-  const int slot = blockIdx.x >> 3, nb = slot % q.subsets, blk = slot / q.subsets * 8 + (blockIdx.x & 7);
-  if (blk >= q.blocks) return;
-  const long long m0 = ((long long)blk * WAVES + wave) * MROWS;
-  const bool live = m0 < p.rows;     // uniform in a wave; idle waves still copy their part of the tiles
-  const long long mx = live ? m0 : 0;
-  for (int i = threadIdx.x; i < GROUP; i += NT) bias[i] = p.bias && nb * GROUP + i < p.outputs ? p.bias[nb * GROUP + i] : 0.f;
-  auto stage = [&](uint8_t* W, int kb) __attribute__((always_inline)) {
-    w_stage<OUT>(W, p, nb, kb, wave * 2, lane);
-    w_stage<OUT>(W, p, nb, kb, wave * 2 + 1, lane);
+  const int kbs = (p.inputs + GROUP - 1) / GROUP, nbs = (p.outputs + GROUP - 1) / GROUP;
+  const int slot = blockIdx.x >> 3, nt = q.subsets, turn = slot / (4 * nt), in = slot % (4 * nt);
+  const int mblk = (turn * 4 + in % 4) * 8 + (blockIdx.x & 7), nblk = in / 4;
+  if (mblk >= q.blocks) return;
+  const int wn = wave & 1, wm = wave >> 1, nb = nblk * 2 + wn;
+  const long long m0 = (long long)mblk * 4 * MROWS + wm * MROWS;
+  const int nbl = min(nb, nbs - 1);
+  for (int i = threadIdx.x; i < 2 * GROUP; i += NT) {
+    const int n = nblk * 2 * GROUP + i;
+    bias[i] = p.bias && n < p.outputs ? p.bias[n] : 0.f;
+  }
+  auto stage = [&](uint8_t* dst, int kb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int part = wave * 4 + i;
+      w_stage<OUT>(dst + (part >> 4) * WTILE, p, min(nblk * 2 + (part >> 4), nbs - 1), kb, part & 15, lane);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int part = wave * 4 + i;
+      x_stage(dst + 2 * WTILE + (part >> 3) * MROWS * GROUP, p, (long long)(mblk * 4 + (part >> 3)) * MROWS, kb, part & 7, lane);
+    }
   };
   const int i16 = n_of<OUT>(0, r);
-  const int wl = i16 * GROUP + ((g ^ key_of<OUT>(i16)) << 4), wlx = wl ^ 64;
+  const int wl = wn * WTILE + i16 * GROUP + ((g ^ key_of<OUT>(i16)) << 4), wlx = wl ^ 64;
+  // rows 4 r + t: chunk g ^ (r & 7)
+  const int xl = 2 * WTILE + wm * MROWS * GROUP + r * 4 * GROUP + ((g ^ (r & 7)) << 4), xlx = xl ^ 64;
+  const long long srow = min(m0 + 4 * r, (long long)p.x.sp - 4);
   f4 acc[8][4];
-  XFrag x, xn;
-  int kb = slot % kbs;
-  stage(W[0], kb);
-  x_load(x, p, mx, kb, r, g);
-  for (int s = 0; s < kbs; ++s) {
+  stage(fp8_smem, 0);
+  uint32_t scale = *reinterpret_cast<const uint32_t*>(p.x.scales + srow);
+  for (int kb = 0; kb < kbs; ++kb) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();     // step s in LDS for every wave; every wave done with the other buffer
-    if (s == 0) start<OUT>(acc, bias, g);
-    const int kn = kb + 1 < kbs ? kb + 1 : 0;
-    stage(W[(s + 1) & 1], kn);
-    mma<OUT>(acc, W[s & 1] + wl, W[s & 1] + wlx, x, p.ws[(size_t)nb * kbs + kb],
-             [&]() __attribute__((always_inline)) { x_load(xn, p, mx, kn, r, g); });
-    x = xn;
-    kb = kn;
+    __syncthreads();     // step kb in LDS for every wave; every wave done with the other buffer
+    if (kb == 0) start<OUT>(acc, bias + wn * GROUP, g);
+    const int kn = min(kb + 1, kbs - 1);
+    const uint8_t* buf = fp8_smem + (kb & 1) * STAGE;
+    XFrag x;
+    x.scale = scale;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      x.v[t][0] = *reinterpret_cast<const u32x4*>(buf + xl + t * GROUP);
+      x.v[t][1] = *reinterpret_cast<const u32x4*>(buf + xlx + t * GROUP);
+    }
+    stage(fp8_smem + ((kb + 1) & 1) * STAGE, kn);
+    scale = *reinterpret_cast<const uint32_t*>(p.x.scales + (size_t)kn * p.x.sp + srow);
+    mma<OUT>(acc, buf + wl, buf + wlx, x, p.ws[(size_t)nbl * kbs + kb], []() {});
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last copy, which nothing reads
-  if (live) finish<OUT>(acc, p, m0, nb, r, g);
+  if (m0 < p.rows && nb < nbs) finish<OUT>(acc, p, m0, nb, r, g);
 }
 
 namespace {
@@ -405,22 +439,22 @@ int go(lf_context* ctx, const LinearParams& p) {
     q.per = (int)std::min<long long>(std::min(fit, nbs), busy);
     q.subsets = (nbs + q.per - 1) / q.per;
     q.blocks = (int)std::min<long long>((mt * q.per + WAVES - 1) / WAVES, std::max(1, cus / q.subsets));
-    static const bool lds = [] {
-      return hipFuncSetAttribute(reinterpret_cast<const void*>(&fp8_linear_resident_kernel<OUT>),
-                                 hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) == hipSuccess;
-    }();
+    static const bool lds = hipFuncSetAttribute(reinterpret_cast<const void*>(&fp8_linear_resident_kernel<OUT>),
+                                                hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) == hipSuccess;
+    if (!lds) return set_error(LF_ERR_DEVICE, "fp8 linear: the device refuses the LDS it needs");
     const size_t smem = (size_t)q.per * (kbs * WTILE + GROUP * 4);
-    if (lds || smem <= 64 * 1024) {
-      const unsigned grid = (unsigned)((q.blocks + 7) / 8 * q.subsets * 8);
-      hipLaunchKernelGGL((fp8_linear_resident_kernel<OUT>), dim3(grid), dim3(NT), smem, ctx->stream, p, q);
-      return check_hip(hipGetLastError(), "fp8 linear launch");
-    }
+    const unsigned grid = (unsigned)((q.blocks + 7) / 8 * q.subsets * 8);
+    hipLaunchKernelGGL((fp8_linear_resident_kernel<OUT>), dim3(grid), dim3(NT), smem, ctx->stream, p, q);
+    return check_hip(hipGetLastError(), "fp8 linear launch");
   }
-  q.per = 1;
-  q.subsets = nbs;
-  q.blocks = (int)((mt + WAVES - 1) / WAVES);
-  const unsigned grid = (unsigned)(((long long)q.blocks + 7) / 8 * nbs * 8);
-  hipLaunchKernelGGL((fp8_linear_stream_kernel<OUT>), dim3(grid), dim3(NT), 0, ctx->stream, p, q);
+  constexpr int smem = 2 * (2 * WTILE + 4 * MROWS * GROUP);
+  static const bool lds = hipFuncSetAttribute(reinterpret_cast<const void*>(&fp8_linear_stream_kernel<OUT>),
+                                              hipFuncAttributeMaxDynamicSharedMemorySize, smem) == hipSuccess;
+  if (!lds) return set_error(LF_ERR_DEVICE, "fp8 linear: the device refuses the LDS it needs");
+  q.subsets = (nbs + 1) / 2;
+  q.blocks = (int)((mt + 3) / 4);
+  const unsigned grid = (unsigned)(((long long)q.blocks + 31) / 32 * 32 * q.subsets);
+  hipLaunchKernelGGL((fp8_linear_stream_kernel<OUT>), dim3(grid), dim3(NT), smem, ctx->stream, p, q);
   return check_hip(hipGetLastError(), "fp8 linear launch");
 }
 
