@@ -4,7 +4,7 @@
 // The reduction runs over the rows, along which each value has a scale of its own, so the codes are turned
 // into bf16 (exactly) as they are staged into LDS, and the fragments, whose lanes need 8 rows of a column,
 // are read from there by transposing reads.  A block of two teams of four waves computes a tile of
-// 32 FI x 128 outputs over its share of the rows, the teams on alternate steps of 32 rows, joined in LDS;
+// 128 x 128 outputs over its share of the rows, the teams on alternate steps of 32 rows, joined in LDS;
 // the blocks' partial sums are added in order by a second kernel.  Column sums are a product with ones.
 #include <algorithm>
 
@@ -16,8 +16,9 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 typedef short s4v __attribute__((ext_vector_type(4)));
 
-constexpr int GN = 128;                   // outputs of a block along j
+constexpr int GN = GROUP;                 // outputs of a block, either way: one group of both operands
 constexpr int GSTEP = 32;                 // rows of a step
+constexpr int RING = 4;                   // steps between a load and its use
 
 struct GradParams {
   Kept a, b;
@@ -25,19 +26,15 @@ struct GradParams {
   float* colsum;                          // [splits][cols of the summed one], or null
   int sum_of;                             // 0: no column sums, 1: of a, 2: of b
   int splits, tiles, tiles_j;
-  long long rows_per;                     // rows of a split, a multiple of 2 GSTEP
+  long long rows_per;                     // rows of a split, a multiple of 2 RING GSTEP
   void *out, *bias;
   int dt, swapped;                        // out is [b.cols][a.cols]
 };
 
-template <int FI>
-struct GradShape {
-  static constexpr int TI = 32 * FI;                       // outputs along i
-  static constexpr int PA = TI * 2 + 32, PB = GN * 2 + 32; // LDS row pitches: 4 rows apart by 32 bytes mod 128
-  static constexpr int BUF = GSTEP * (PA + PB);            // one team's buffer
-  static constexpr int ITEMS = GSTEP * (TI + GN) / 16 / 256;   // 16-code pieces a lane stages
-  static constexpr size_t SMEM = (size_t)(4 * BUF > TI * GN * 4 ? 4 * BUF : TI * GN * 4);
-};
+constexpr int PITCH = GN * 2 + 32;        // LDS bytes of a row of bf16: 4 rows apart by 32 bytes mod 128
+constexpr int BUF = 2 * GSTEP * PITCH;    // one team's buffer: rows of a, then of b
+constexpr size_t GRAD_SMEM = 4 * BUF;     // two teams, two buffers; the joining teams use 64 KB of it
+static_assert(GRAD_SMEM >= (size_t)GN * GN * 4, "the teams' join");
 
 // The transposing read: of each 16 lanes, lanes 4k .. 4k+3 address row k's 16 columns, 4 each; lane i
 // receives column i of the 4 rows.
@@ -52,12 +49,12 @@ __device__ __forceinline__ void tr_read(uint32_t (&o)[2], const uint8_t* p) {
 #endif
 }
 // 16 columns of 32 rows as a bf16 fragment: lane group g has rows 4g .. and 16 + 4g ..
-__device__ __forceinline__ b8 tr_frag(const uint8_t* p, int pitch) {
+__device__ __forceinline__ b8 tr_frag(const uint8_t* p) {
   uint32_t w[4], h[2];
   tr_read(h, p);
   w[0] = h[0];
   w[1] = h[1];
-  tr_read(h, p + 16 * pitch);
+  tr_read(h, p + 16 * PITCH);
   w[2] = h[0];
   w[3] = h[1];
   b8 o;
@@ -65,168 +62,181 @@ __device__ __forceinline__ b8 tr_frag(const uint8_t* p, int pitch) {
   return o;
 }
 
-template <int FI>
+// SUM: 0 no column sums, 1 of a, 2 of b.
+template <int SUM>
 __global__ __launch_bounds__(512, 2) void weight_grad_kernel(GradParams p) {
-  using S = GradShape<FI>;
   extern __shared__ __attribute__((aligned(16))) uint8_t grad_smem[];
   const int slot = blockIdx.x >> 3, tile = slot % p.tiles, split = slot / p.tiles * 8 + (blockIdx.x & 7);
   if (split >= p.splits) return;
-  const int i0 = tile / p.tiles_j * S::TI, j0 = tile % p.tiles_j * GN;
+  const int i0 = tile / p.tiles_j * GN, j0 = tile % p.tiles_j * GN;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int team = wave >> 2, wi = (wave >> 1) & 1, wj = wave & 1, tid = threadIdx.x & 255;
-  const long long m0 = split * p.rows_per, m1 = min((long long)p.a.rows, m0 + p.rows_per);
-  const int steps = (int)((m1 - m0 + 2 * GSTEP - 1) / (2 * GSTEP));
-  uint8_t* mine = grad_smem + team * 2 * S::BUF;
+  const long long m0 = split * p.rows_per;
+  const int n = (int)min(p.a.rows - m0, p.rows_per);            // rows of the split
+  const int steps = (n + 2 * GSTEP - 1) / (2 * GSTEP);
+  uint8_t* mine = grad_smem + team * 2 * BUF;
 
-  u32x4 raw[S::ITEMS];
-  int sc[S::ITEMS];
-  auto load = [&](int s) __attribute__((always_inline)) {
-    const long long base = m0 + (long long)(2 * s + team) * GSTEP;
-#pragma unroll
-    for (int k = 0; k < S::ITEMS; ++k) {
-      const int item = k * 256 + tid;
-      const bool of_a = item < GSTEP * S::TI / 16;       // whole waves: the boundary is a multiple of 256
-      const int e = of_a ? item : item - GSTEP * S::TI / 16, per = of_a ? S::TI / 16 : GN / 16;
-      const int r = e / per, col = (of_a ? i0 : j0) + e % per * 16;
-      const Kept& q = of_a ? p.a : p.b;
-      raw[k] = u32x4{0, 0, 0, 0};
-      sc[k] = 127;
-      if (base + r < m1 && col < q.pitch) {
-        raw[k] = *reinterpret_cast<const u32x4*>(q.codes + (size_t)(base + r) * q.pitch + col);
-        sc[k] = q.scales[(size_t)(col / GROUP) * q.sp + base + r];
-      }
-    }
+  // A step is 32 rows, 16 codes a lane of a and of b, at a uniform base that moves with the step and a 32-bit
+  // lane offset.  The loads have no condition, or the compiler could not count those in flight: rows past
+  // the end read the last one, and are made zeros when they are stored; columns past the pitch read the
+  // last ones, for outputs that do not exist.
+  const int row = tid >> 3, pc = tid & 7;
+  const uint8_t* code[2] = {p.a.codes + (size_t)m0 * p.a.pitch, p.b.codes + (size_t)m0 * p.b.pitch};
+  const uint8_t* scale[2] = {p.a.scales + (size_t)(i0 / GROUP) * p.a.sp + m0, p.b.scales + (size_t)(j0 / GROUP) * p.b.sp + m0};
+  const int pitch[2] = {p.a.pitch, p.b.pitch};
+  const int col[2] = {min(i0 + pc * 16, pitch[0] - 16), min(j0 + pc * 16, pitch[1] - 16)};
+  u32x4 raw[RING][2];
+  int sc[RING][2];
+  // 24-bit products: the 64-bit multiply-add that the compiler would take reads a register pair whose other
+  // half may be a load in flight, and waits for it
+  auto load = [&](int s, int slot4, int k) __attribute__((always_inline)) {
+    const int m = min((2 * s + team) * GSTEP, n - 1), r = min(row, n - 1 - m);
+    raw[slot4][k] = *reinterpret_cast<const u32x4*>(code[k] + (size_t)m * pitch[k] + (__umul24(r, pitch[k]) + col[k]));
+    sc[slot4][k] = (scale[k] + m)[(uint32_t)r];
   };
-  auto store = [&](int s) __attribute__((always_inline)) {
-    uint8_t* buf = mine + (s & 1) * S::BUF;
+  uint8_t* const dst = mine + row * PITCH + pc * 32;
+  auto store = [&](int s, int slot4, int k) __attribute__((always_inline)) {
+    const bool ok = row < n - (2 * s + team) * GSTEP;
+    const float f = scale_value(sc[slot4][k]);
+    uint32_t w[8];
 #pragma unroll
-    for (int k = 0; k < S::ITEMS; ++k) {
-      const int item = k * 256 + tid;
-      const bool of_a = item < GSTEP * S::TI / 16;
-      const int e = of_a ? item : item - GSTEP * S::TI / 16, per = of_a ? S::TI / 16 : GN / 16;
-      uint8_t* dst = buf + (of_a ? 0 : GSTEP * S::PA) + e / per * (of_a ? S::PA : S::PB) + e % per * 32;
-      const float f = scale_value(sc[k]);
-      uint32_t w[8];
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        w[2 * d] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)raw[k][d], f, false));
-        w[2 * d + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)raw[k][d], f, true));
-      }
-      *reinterpret_cast<u32x4*>(dst) = u32x4{w[0], w[1], w[2], w[3]};
-      *reinterpret_cast<u32x4*>(dst + 16) = u32x4{w[4], w[5], w[6], w[7]};
+    for (int d = 0; d < 4; ++d) {
+      const int c = ok ? (int)raw[slot4][k][d] : 0;
+      w[2 * d] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, f, false));
+      w[2 * d + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, f, true));
     }
+    uint8_t* to = dst + (s & 1) * BUF + k * GSTEP * PITCH;
+    *reinterpret_cast<u32x4*>(to) = u32x4{w[0], w[1], w[2], w[3]};
+    *reinterpret_cast<u32x4*>(to + 16) = u32x4{w[4], w[5], w[6], w[7]};
   };
 
-  f4 acc[FI][4], sums[FI / 2];
+  // A wave has a 64 x 64 part of the tile.  Its fragments are numbered so that fragments 0 and 2 of the two
+  // waves that share them are different ones: each sums those.
+  f4 acc[4][4], sums[2];
 #pragma unroll
-  for (int i = 0; i < FI; ++i)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < FI / 2; ++i) sums[i] = f4{0.f, 0.f, 0.f, 0.f};
-  // column sums: blocks at the other operand's first tile, each fragment by one of the two waves that read it
-  const bool sum_a = p.sum_of == 1 && j0 == 0, sum_b = p.sum_of == 2 && i0 == 0;
+  sums[0] = sums[1] = f4{0.f, 0.f, 0.f, 0.f};
+  const bool sum = SUM == 1 ? j0 == 0 : SUM == 2 ? i0 == 0 : false;   // blocks at the other operand's first tile
   b8 ones;
 #pragma unroll
   for (int k = 0; k < 8; ++k) ones[k] = (__bf16)1.0f;
+  const int xi = SUM == 1 ? wj : 0, xj = SUM == 2 ? wi : 0;
   const int g = lane >> 4, l16 = lane & 15;
-  const int row = 4 * g + (l16 >> 2), cb = (l16 & 3) * 8;
-  const int ao = row * S::PA + wi * FI * 32 + cb, bo = GSTEP * S::PA + row * S::PB + wj * 128 + cb;
+  const uint8_t* const from = mine + (4 * g + (l16 >> 2)) * PITCH + (l16 & 3) * 8;
+  const uint8_t* const from_a = from + wi * 128 + xi * 32;
+  const uint8_t* const from_b = from + GSTEP * PITCH + wj * 128 + xj * 32;
+  auto read_a = [&](int s, int i) __attribute__((always_inline)) {     // fragment i ^ xi
+    return tr_frag((i & 1) ? from_a + (s & 1) * BUF + (i - 1) * 32 + (1 - 2 * xi) * 32 : from_a + (s & 1) * BUF + i * 32);
+  };
+  auto read_b = [&](int s, int j) __attribute__((always_inline)) {
+    return tr_frag((j & 1) ? from_b + (s & 1) * BUF + (j - 1) * 32 + (1 - 2 * xj) * 32 : from_b + (s & 1) * BUF + j * 32);
+  };
 
-  load(0);
-  store(0);
-  load(1);
-  for (int s = 0; s < steps; ++s) {
-    __syncthreads();     // step s in LDS; every wave done with the other buffer
-    const uint8_t* buf = mine + (s & 1) * S::BUF;
-    b8 fb[4];
+  // Step s multiplies fragments that step s - 1 read, reads step s + 1's, and turns step s + 2's codes,
+  // loaded RING steps ago, into the buffer that step s - 1 read from.
 #pragma unroll
-    for (int j = 0; j < 4; ++j) fb[j] = tr_frag(buf + bo + j * 32, S::PB);
-    b8 fa[2];
-    fa[0] = tr_frag(buf + ao, S::PA);
-    if (s + 1 < steps) store(s + 1);
-    load(s + 2);         // past the end: nothing is read
+  for (int q = 0; q < RING; ++q) {
+    load(q, q, 0);
+    load(q, q, 1);
+  }
 #pragma unroll
-    for (int i = 0; i < FI; ++i) {
-      if (i + 1 < FI) fa[(i + 1) & 1] = tr_frag(buf + ao + (i + 1) * 32, S::PA);
+  for (int q = 0; q < 2; ++q)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i & 1], fb[j], acc[i][j], 0, 0, 0);
-      if (sum_a && (i & 1) == wj) sums[i >> 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i & 1], ones, sums[i >> 1], 0, 0, 0);
-      __builtin_amdgcn_sched_barrier(0);
+    for (int k = 0; k < 2; ++k) {
+      store(q, q, k);
+      load(q + RING, q, k);
     }
-    if (sum_b) {
+  __syncthreads();
+  b8 fa[4], fb[2][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if ((j & 1) == wi) sums[j >> 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fb[j], sums[j >> 1], 0, 0, 0);
+  for (int j = 0; j < 4; ++j) fb[0][j] = read_b(0, j);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) fa[i] = read_a(0, i);
+  for (int s0 = 0; s0 < steps; s0 += RING) {     // past the last step: zeros
+#pragma unroll
+    for (int u = 0; u < RING; ++u) {
+      const int s = s0 + u, slot4 = (u + 2) % RING;
+      __syncthreads();     // step s + 1 in LDS; every wave has read step s
+      if (sum) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          sums[h] = SUM == 1 ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[2 * h], ones, sums[h], 0, 0, 0)
+                             : __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fb[u & 1][2 * h], sums[h], 0, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) fb[(u + 1) & 1][j] = read_b(u + 1, j);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[u & 1][j], acc[i][j], 0, 0, 0);
+        fa[i] = read_a(u + 1, i);
+        if (i & 1) {
+          store(s + 2, slot4, i >> 1);
+          load(s + 2 + RING, slot4, i >> 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
 
   // the second team's sums are added to the first's
-  const int wt = wi * 2 + wj;
-  f4* half = reinterpret_cast<f4*>(grad_smem) + wt * 64 + lane;      // [FI * 4][4 waves][64]
+  f4* half = reinterpret_cast<f4*>(grad_smem) + (wi * 2 + wj) * 64 + lane;      // [16][4 waves][64]
   __syncthreads();
   if (team == 1) {
 #pragma unroll
-    for (int i = 0; i < FI; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) half[(i * 4 + j) * 256] = acc[i][j];
   }
   __syncthreads();
   if (team == 0) {
 #pragma unroll
-    for (int i = 0; i < FI; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] += half[(i * 4 + j) * 256];
   }
-  if (sum_a || sum_b) {     // uniform in the block
+  if (sum) {     // uniform in the block
     __syncthreads();
-    if (team == 1)
-#pragma unroll
-      for (int i = 0; i < FI / 2; ++i) half[i * 256] = sums[i];
+    if (team == 1) {
+      half[0] = sums[0];
+      half[256] = sums[1];
+    }
     __syncthreads();
-    if (team == 0)
-#pragma unroll
-      for (int i = 0; i < FI / 2; ++i) sums[i] += half[i * 256];
+    if (team == 0) {
+      sums[0] += half[0];
+      sums[1] += half[256];
+    }
   }
   if (team == 1) return;
-  const int ca = p.a.cols, cb2 = p.b.cols;
-  float* dst = p.partial ? p.partial + (size_t)split * ca * cb2 : nullptr;
+  const int ca = p.a.cols, cb = p.b.cols;
+  float* part = p.partial ? p.partial + (size_t)split * ca * cb : nullptr;
 #pragma unroll
-  for (int i = 0; i < FI; ++i)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int ci = i0 + (wi * FI + i) * 16 + 4 * g, cj = j0 + wj * 64 + j * 16 + l16;
+      const int ci = i0 + wi * 64 + (i ^ xi) * 16 + 4 * g, cj = j0 + wj * 64 + (j ^ xj) * 16 + l16;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (ci + k < ca && cj < cb2) {
-          if (dst) dst[(size_t)(ci + k) * cb2 + cj] = acc[i][j][k];
-          else store_act(p.out, p.dt, p.swapped ? (size_t)cj * ca + ci + k : (size_t)(ci + k) * cb2 + cj, acc[i][j][k]);
+        if (ci + k < ca && cj < cb) {
+          if (part) part[(size_t)(ci + k) * cb + cj] = acc[i][j][k];
+          else store_act(p.out, p.dt, p.swapped ? (size_t)cj * ca + ci + k : (size_t)(ci + k) * cb + cj, acc[i][j][k]);
         }
     }
-  if (sum_a) {
+  if (!sum) return;
+  // of a: lane group g has columns 4g .. 4g + 3 of a fragment, in every lane; of b: lane l16 column l16
+  const int cn = SUM == 1 ? ca : cb;
 #pragma unroll
-    for (int i = 0; i < FI; ++i)
-      if ((i & 1) == wj && l16 == 0)
+  for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int c = i0 + (wi * FI + i) * 16 + 4 * g + k;
-          if (c < ca) {
-            if (dst) p.colsum[(size_t)split * ca + c] = sums[i >> 1][k];
-            else store_act(p.bias, p.dt, c, sums[i >> 1][k]);
-          }
-        }
-  }
-  if (sum_b) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if ((j & 1) == wi && g == 0) {
-        const int c = j0 + wj * 64 + j * 16 + l16;
-        if (c < cb2) {
-          if (dst) p.colsum[(size_t)split * cb2 + c] = sums[j >> 1][0];
-          else store_act(p.bias, p.dt, c, sums[j >> 1][0]);
-        }
+    for (int k = 0; k < (SUM == 1 ? 4 : 1); ++k) {
+      const int c = SUM == 1 ? i0 + wi * 64 + (2 * h + xi) * 16 + 4 * g + k : j0 + wj * 64 + (2 * h + xj) * 16 + l16;
+      if ((SUM == 1 ? l16 : g) == 0 && c < cn) {
+        if (part) p.colsum[(size_t)split * cn + c] = sums[h][k];
+        else store_act(p.bias, p.dt, c, sums[h][k]);
       }
-  }
+    }
 }
 
 // Partial sums added in order: 64 outputs a block, 16 runs of the splits at a time.
@@ -264,30 +274,27 @@ __global__ __launch_bounds__(256) void weight_grad_join_kernel(GradParams p, lon
 namespace {
 
 struct GradPlan {
-  int fi, tiles, tiles_j, splits;
+  int tiles, tiles_j, splits;
   long long rows_per;
 };
-// i is the wider matrix (ci >= cj).
 GradPlan grad_plan(long long rows, int ci, int cj) {
   GradPlan q{};
-  q.fi = ci > 128 ? 8 : 4;
   q.tiles_j = (cj + GN - 1) / GN;
-  q.tiles = (ci + 32 * q.fi - 1) / (32 * q.fi) * q.tiles_j;
+  q.tiles = (ci + GN - 1) / GN * q.tiles_j;
   const long long want = std::max<long long>(1, 256 / q.tiles);      // a block a CU
-  const long long steps = (rows + 2 * GSTEP - 1) / (2 * GSTEP);
-  q.rows_per = (steps + want - 1) / want * (2 * GSTEP);
+  const long long turns = (rows + 2 * RING * GSTEP - 1) / (2 * RING * GSTEP);
+  q.rows_per = (turns + want - 1) / want * (2 * RING * GSTEP);
   q.splits = (int)((rows + q.rows_per - 1) / q.rows_per);
   return q;
 }
 
-template <int FI>
+template <int SUM>
 int go(lf_context* ctx, const GradParams& p) {
-  static const bool lds = hipFuncSetAttribute(reinterpret_cast<const void*>(&weight_grad_kernel<FI>),
-                                              hipFuncAttributeMaxDynamicSharedMemorySize,
-                                              (int)GradShape<FI>::SMEM) == hipSuccess;
+  static const bool lds = hipFuncSetAttribute(reinterpret_cast<const void*>(&weight_grad_kernel<SUM>),
+                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)GRAD_SMEM) == hipSuccess;
   if (!lds) return set_error(LF_ERR_DEVICE, "weight gradient: the device refuses the LDS it needs");
   const unsigned grid = (unsigned)((p.splits + 7) / 8 * p.tiles * 8);
-  hipLaunchKernelGGL((weight_grad_kernel<FI>), dim3(grid), dim3(512), GradShape<FI>::SMEM, ctx->stream, p);
+  hipLaunchKernelGGL((weight_grad_kernel<SUM>), dim3(grid), dim3(512), GRAD_SMEM, ctx->stream, p);
   return check_hip(hipGetLastError(), "weight gradient launch");
 }
 
@@ -322,7 +329,7 @@ int run_weight_grad(lf_context* ctx, const Kept& a, const Kept& b, void* out, vo
   }
   {
     LaunchScope ls(ctx, label);
-    LF_TRY(q.fi == 8 ? go<8>(ctx, p) : go<4>(ctx, p));
+    LF_TRY(p.sum_of == 0 ? go<0>(ctx, p) : p.sum_of == 1 ? go<1>(ctx, p) : go<2>(ctx, p));
   }
   if (q.splits == 1) return LF_OK;
   const int cn = p.sum_of == 0 ? 0 : p.sum_of == 1 ? p.a.cols : p.b.cols;
