@@ -352,11 +352,15 @@ int run_layer_norm_backward(lf_context* ctx, const lf_layer_norm_backward_args& 
   }
   LF_TRY(check_hip(hipGetLastError(), "layer_norm backward launch"));
   if (!a.grad_scale) return LF_OK;
+  return run_norm_join(ctx, p.partial, blocks, a.channels, a.grad_scale, a.grad_offset, a.grad_dtype);
+}
+
+int run_norm_join(lf_context* ctx, const float* partial, int blocks, int channels, void* grad_scale, void* grad_offset,
+                  int dt) {
   LaunchScope ls(ctx, "layer_norm.join");
-  const dim3 grid((2 * a.channels + 63) / 64);
-  auto k = a.grad_dtype == LF_F32 ? norm_join_kernel<DT_F32> : a.grad_dtype == LF_F16 ? norm_join_kernel<DT_F16>
-                                                                                      : norm_join_kernel<DT_BF16>;
-  hipLaunchKernelGGL(k, grid, dim3(1024), 0, ctx->stream, p.partial, blocks, a.channels, a.grad_scale, a.grad_offset);
+  const dim3 grid((2 * channels + 63) / 64);
+  auto k = dt == LF_F32 ? norm_join_kernel<DT_F32> : dt == LF_F16 ? norm_join_kernel<DT_F16> : norm_join_kernel<DT_BF16>;
+  hipLaunchKernelGGL(k, grid, dim3(1024), 0, ctx->stream, partial, blocks, channels, grad_scale, grad_offset);
   return check_hip(hipGetLastError(), "layer_norm join launch");
 }
 

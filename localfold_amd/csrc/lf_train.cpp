@@ -246,7 +246,7 @@ struct Carve {
 size_t train_bytes(int, int c, int h) { return packed_bytes(h, c) + packed_bytes(c, h); }
 size_t backward_bytes(int rows, int c, int h) {
   const size_t partials = std::max(std::max(weight_grad_partials(rows, c, h), weight_grad_partials(rows, h, c)),
-                                   layer_norm_partials(rows, c));
+                                   std::max(layer_norm_partials(rows, c), train_partials(c)));
   return packed_bytes(h, c) + packed_bytes(c, h) + kept_bytes(rows, c) + kept_bytes(rows, h) +
          up((size_t)rows * c * 4) + up(partials);
 }
@@ -290,6 +290,7 @@ int transition_train(lf_context* ctx, const lf_transition_train_args& a) {
   StageScope stage(ctx, "transition.train");
   const PackWeight packs[2] = {pack_of(w.w1, false, w1.codes, w1.scales), pack_of(w.w2, false, w2.codes, w2.scales)};
   LF_TRY(run_pack_weights(ctx, packs, 2));
+  if (train_fused(c, h, a.act, a.out)) return run_train_forward(ctx, a, w1, w2);
 
   lf_layer_norm_args n{};
   n.rows = a.rows;
@@ -347,9 +348,15 @@ int transition_backward(lf_context* ctx, const lf_transition_backward_args& a) {
   StageScope stage(ctx, "transition.backward");
   const PackWeight packs[2] = {pack_of(w.w2, true, w2.codes, w2.scales), pack_of(w.w1, true, w1.codes, w1.scales)};
   LF_TRY(run_pack_weights(ctx, packs, 2));
-  LF_TRY(run_checkpoint_pack(ctx, a.grad, a.act_dtype, kept_view(d)));
-
   const bool t2 = w.w2.layout == LF_IN_OUT, t1 = w.w1.layout == LF_IN_OUT;
+  if (train_fused(c, h, a.grad, a.out)) {
+    LF_TRY(run_train_backward(ctx, a, w2, w1, kept_view(d), kept_view(e), static_cast<float*>(partials)));
+    LF_TRY(run_weight_grad(ctx, kept_view(t2 ? s.hidden : d), kept_view(t2 ? d : s.hidden), a.grad_w2, a.grad_b2, t2,
+                           a.grad_dtype, partials, "fp8.weight_grad2"));
+    return run_weight_grad(ctx, kept_view(t1 ? s.normed : e), kept_view(t1 ? e : s.normed), a.grad_w1, a.grad_b1, t1,
+                           a.grad_dtype, partials, "fp8.weight_grad1");
+  }
+  LF_TRY(run_checkpoint_pack(ctx, a.grad, a.act_dtype, kept_view(d)));
   LF_TRY(run_weight_grad(ctx, kept_view(t2 ? s.hidden : d), kept_view(t2 ? d : s.hidden), a.grad_w2, a.grad_b2, t2,
                          a.grad_dtype, partials, "fp8.weight_grad2"));
   lf_fp8_linear_args l{};

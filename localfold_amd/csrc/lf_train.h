@@ -50,6 +50,17 @@ size_t weight_grad_partials(int rows, int outputs, int inputs);
 int run_weight_grad(lf_context* ctx, const Kept& a, const Kept& b, void* out, void* bias, bool bias_of_b, int dt,
                     void* scratch, const char* label);
 
+// Adds [blocks][2 channels] partial sums of scale and offset gradients.
+int run_norm_join(lf_context* ctx, const float* partial, int blocks, int channels, void* grad_scale, void* grad_offset,
+                  int dt);
+// The transition's training step in one kernel each way, where train_fused says that there is one: packed
+// weights of the forward pass w1, w2, of the backward w2, w1; d, e: the kept gradients of out and hidden.
+bool train_fused(int channels, int hidden, const void* in, const void* out);
+int run_train_forward(lf_context* ctx, const lf_transition_train_args& a, const lf_fp8_weight& w1, const lf_fp8_weight& w2);
+size_t train_partials(int channels);
+int run_train_backward(lf_context* ctx, const lf_transition_backward_args& a, const lf_fp8_weight& w2,
+                       const lf_fp8_weight& w1, const Kept& d, const Kept& e, float* partial);
+
 // ---- device helpers ---------------------------------------------------------------------------
 
 template <int CTRL>
