@@ -4,7 +4,7 @@
 // The reduction runs over the rows, along which each value has a scale of its own, so the codes are turned
 // into bf16 (exactly) as they are staged into LDS, and the fragments, whose lanes need 8 rows of a column,
 // are read from there by transposing reads.  A block of two teams of four waves computes a tile of
-// 128 x 128 outputs over its share of the rows, the teams on alternate steps of 32 rows, joined in LDS;
+// 128 x 128 outputs over its share of the rows, the teams on alternate steps of 64 rows, joined in LDS;
 // the blocks' partial sums are added in order by a second kernel.  Column sums are a product with ones.
 #include <algorithm>
 
@@ -17,8 +17,8 @@ typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 typedef short s4v __attribute__((ext_vector_type(4)));
 
 constexpr int GN = GROUP;                 // outputs of a block, either way: one group of both operands
-constexpr int GSTEP = 32;                 // rows of a step
-constexpr int RING = 4;                   // steps between a load and its use
+constexpr int GSTEP = 64;                 // rows of a step, multiplied in two halves
+constexpr int RING = 2;                   // steps between a load and its use
 
 struct GradParams {
   Kept a, b;
@@ -76,38 +76,41 @@ __global__ __launch_bounds__(512, 2) void weight_grad_kernel(GradParams p) {
   const int steps = (n + 2 * GSTEP - 1) / (2 * GSTEP);
   uint8_t* mine = grad_smem + team * 2 * BUF;
 
-  // A step is 32 rows, 16 codes a lane of a and of b, at a uniform base that moves with the step and a 32-bit
-  // lane offset.  The loads have no condition, or the compiler could not count those in flight: rows past
-  // the end read the last one, and are made zeros when they are stored; columns past the pitch read the
-  // last ones, for outputs that do not exist.
+  // Half a step is 32 rows, 16 codes a lane of a and of b, at a uniform base that moves with the step and a
+  // 32-bit lane offset.  The loads have no condition, or the compiler could not count those in flight:
+  // rows past the end read the last one, and are made zeros when they are stored; columns past the pitch
+  // read the last ones, for outputs that do not exist.
   const int row = tid >> 3, pc = tid & 7;
   const uint8_t* code[2] = {p.a.codes + (size_t)m0 * p.a.pitch, p.b.codes + (size_t)m0 * p.b.pitch};
   const uint8_t* scale[2] = {p.a.scales + (size_t)(i0 / GROUP) * p.a.sp + m0, p.b.scales + (size_t)(j0 / GROUP) * p.b.sp + m0};
   const int pitch[2] = {p.a.pitch, p.b.pitch};
   const int col[2] = {min(i0 + pc * 16, pitch[0] - 16), min(j0 + pc * 16, pitch[1] - 16)};
-  u32x4 raw[RING][2];
-  int sc[RING][2];
+  u32x4 raw[RING][2][2];        // [step][half][a or b]
+  int sc[RING][2][2];
   // 24-bit products: the 64-bit multiply-add that the compiler would take reads a register pair whose other
   // half may be a load in flight, and waits for it
-  auto load = [&](int s, int slot4, int k) __attribute__((always_inline)) {
-    const int m = min((2 * s + team) * GSTEP, n - 1), r = min(row, n - 1 - m);
-    raw[slot4][k] = *reinterpret_cast<const u32x4*>(code[k] + (size_t)m * pitch[k] + (__umul24(r, pitch[k]) + col[k]));
-    sc[slot4][k] = (scale[k] + m)[(uint32_t)r];
+  auto load = [&](int s, int ring, int h, int k) __attribute__((always_inline)) {
+    const int m = min((2 * s + team) * GSTEP + h * 32, n - 1), r = min(row, n - 1 - m);
+    raw[ring][h][k] = *reinterpret_cast<const u32x4*>(code[k] + (size_t)m * pitch[k] + (__umul24(r, pitch[k]) + col[k]));
+    sc[ring][h][k] = (scale[k] + m)[(uint32_t)r];
   };
-  uint8_t* const dst = mine + row * PITCH + pc * 32;
-  auto store = [&](int s, int slot4, int k) __attribute__((always_inline)) {
-    const bool ok = row < n - (2 * s + team) * GSTEP;
-    const float f = scale_value(sc[slot4][k]);
+  // A lane's 16 values are two 16-byte pieces; in the upper half of a row they lie the other way round, so
+  // that the 8 lanes of a row store to all banks at once.
+  uint8_t* const dst = mine + row * PITCH + pc * 32 + (pc & 4 ? 16 : 0);
+  uint8_t* const dst1 = mine + row * PITCH + pc * 32 + (pc & 4 ? 0 : 16);
+  auto store = [&](int s, int ring, int h, int k) __attribute__((always_inline)) {
+    const bool ok = row < n - (2 * s + team) * GSTEP - h * 32;
+    const float f = scale_value(sc[ring][h][k]);
     uint32_t w[8];
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
-      const int c = ok ? (int)raw[slot4][k][d] : 0;
+      const int c = ok ? (int)raw[ring][h][k][d] : 0;
       w[2 * d] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, f, false));
       w[2 * d + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, f, true));
     }
-    uint8_t* to = dst + (s & 1) * BUF + k * GSTEP * PITCH;
-    *reinterpret_cast<u32x4*>(to) = u32x4{w[0], w[1], w[2], w[3]};
-    *reinterpret_cast<u32x4*>(to + 16) = u32x4{w[4], w[5], w[6], w[7]};
+    const int to = (s & 1) * BUF + (k * GSTEP + h * 32) * PITCH;
+    *reinterpret_cast<u32x4*>(dst + to) = u32x4{w[0], w[1], w[2], w[3]};
+    *reinterpret_cast<u32x4*>(dst1 + to) = u32x4{w[4], w[5], w[6], w[7]};
   };
 
   // A wave has a 64 x 64 part of the tile.  Its fragments are numbered so that fragments 0 and 2 of the two
@@ -124,59 +127,66 @@ __global__ __launch_bounds__(512, 2) void weight_grad_kernel(GradParams p) {
   for (int k = 0; k < 8; ++k) ones[k] = (__bf16)1.0f;
   const int xi = SUM == 1 ? wj : 0, xj = SUM == 2 ? wi : 0;
   const int g = lane >> 4, l16 = lane & 15;
-  const uint8_t* const from = mine + (4 * g + (l16 >> 2)) * PITCH + (l16 & 3) * 8;
-  const uint8_t* const from_a = from + wi * 128 + xi * 32;
-  const uint8_t* const from_b = from + GSTEP * PITCH + wj * 128 + xj * 32;
-  auto read_a = [&](int s, int i) __attribute__((always_inline)) {     // fragment i ^ xi
-    return tr_frag((i & 1) ? from_a + (s & 1) * BUF + (i - 1) * 32 + (1 - 2 * xi) * 32 : from_a + (s & 1) * BUF + i * 32);
+  const uint8_t* const from = mine + (4 * g + (l16 >> 2)) * PITCH;
+  const uint8_t* const from_a = from + wi * 128 + ((l16 & 3) * 8 ^ wi * 16) + xi * 32;
+  const uint8_t* const from_b = from + GSTEP * PITCH + wj * 128 + ((l16 & 3) * 8 ^ wj * 16) + xj * 32;
+  auto read_a = [&](int s, int h, int i) __attribute__((always_inline)) {     // fragment i ^ xi
+    const int at = (s & 1) * BUF + h * 32 * PITCH;
+    return tr_frag(from_a + (i & 1 ? at + (i - 1) * 32 + (1 - 2 * xi) * 32 : at + i * 32));
   };
-  auto read_b = [&](int s, int j) __attribute__((always_inline)) {
-    return tr_frag((j & 1) ? from_b + (s & 1) * BUF + (j - 1) * 32 + (1 - 2 * xj) * 32 : from_b + (s & 1) * BUF + j * 32);
+  auto read_b = [&](int s, int h, int j) __attribute__((always_inline)) {
+    const int at = (s & 1) * BUF + h * 32 * PITCH;
+    return tr_frag(from_b + (j & 1 ? at + (j - 1) * 32 + (1 - 2 * xj) * 32 : at + j * 32));
   };
 
-  // Step s multiplies fragments that step s - 1 read, reads step s + 1's, and turns step s + 2's codes,
-  // loaded RING steps ago, into the buffer that step s - 1 read from.
+  // Half (s, h) multiplies fragments that the half before it read, and reads the next one's.  Step s stores
+  // (s + 2, 0) where (s, 0) was, read in step s - 1, and (s + 1, 1) where (s - 1, 1) was, read in that step
+  // too: one barrier a step.
 #pragma unroll
-  for (int q = 0; q < RING; ++q) {
-    load(q, q, 0);
-    load(q, q, 1);
+  for (int q = 0; q < RING; ++q)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) load(q, q, k >> 1, k & 1);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    store(0, 0, 0, k);
+    load(2, 0, 0, k);
+    store(0, 0, 1, k);
+    load(2, 0, 1, k);
+    store(1, 1, 0, k);
+    load(3, 1, 0, k);
   }
-#pragma unroll
-  for (int q = 0; q < 2; ++q)
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      store(q, q, k);
-      load(q + RING, q, k);
-    }
   __syncthreads();
   b8 fa[4], fb[2][4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) fb[0][j] = read_b(0, j);
+  for (int j = 0; j < 4; ++j) fb[0][j] = read_b(0, 0, j);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) fa[i] = read_a(0, i);
+  for (int i = 0; i < 4; ++i) fa[i] = read_a(0, 0, i);
   for (int s0 = 0; s0 < steps; s0 += RING) {     // past the last step: zeros
 #pragma unroll
     for (int u = 0; u < RING; ++u) {
-      const int s = s0 + u, slot4 = (u + 2) % RING;
-      __syncthreads();     // step s + 1 in LDS; every wave has read step s
-      if (sum) {
+      __syncthreads();
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          sums[h] = SUM == 1 ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[2 * h], ones, sums[h], 0, 0, 0)
-                             : __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fb[u & 1][2 * h], sums[h], 0, 0, 0);
-      }
+      for (int h = 0; h < 2; ++h) {
+        const int s = s0 + u, sn = u + h, st = h ? s + 1 : s + 2, ring = (u + h) & 1;
+        if (sum) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) fb[(u + 1) & 1][j] = read_b(u + 1, j);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[u & 1][j], acc[i][j], 0, 0, 0);
-        fa[i] = read_a(u + 1, i);
-        if (i & 1) {
-          store(s + 2, slot4, i >> 1);
-          load(s + 2 + RING, slot4, i >> 1);
+          for (int f = 0; f < 2; ++f)
+            sums[f] = SUM == 1 ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[2 * f], ones, sums[f], 0, 0, 0)
+                               : __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fb[h][2 * f], sums[f], 0, 0, 0);
         }
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) fb[1 - h][j] = read_b(sn, 1 - h, j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[h][j], acc[i][j], 0, 0, 0);
+          fa[i] = read_a(sn, 1 - h, i);
+          if (i & 1) {
+            store(st, ring, h, i >> 1);
+            load(st + RING, ring, h, i >> 1);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
   }
