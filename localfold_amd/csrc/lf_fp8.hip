@@ -152,29 +152,17 @@ __global__ __launch_bounds__(RW * 64) void fp8_linear_resident_kernel(LinearPara
 
 constexpr int SW = 8, SM = 4, MROWS = 16 * SM;   // the streaming kernel's waves, tiles and rows of a wave
 
-// Copies rows m0 .. m0 + 63 of column group kb to an LDS tile whose chunk c of row m lies at
-// c ^ ((m >> 2) & 7); instruction `part` of 8 fills 8 rows.
-__device__ __forceinline__ void x_stage(uint8_t* dst, const LinearParams& p, long long m0, int kb, int part, int lane) {
-  const int row = part * 8 + (lane >> 3), c = (lane & 7) ^ (row >> 2 & 7);
-  const long long m = min(m0 + row, (long long)p.rows - 1);
-  const uint8_t* src = p.x.codes + (size_t)m * p.x.pitch + kb * GROUP + c * 16;
-  if (kb * GROUP + c * 16 >= p.x.pitch) src = reinterpret_cast<const uint8_t*>(&fp8_zero16);
-#if __HIP_DEVICE_COMPILE__
-  __builtin_amdgcn_global_load_lds(src, dst + part * 1024, 16, 0, 0);
-#else
-  (void)src;
-#endif
-}
-
 // Long reductions: a block of 256 rows and two output groups walks the columns 128 at a time, tiles of both
 // operands in two LDS buffers in turn.  One barrier a step; the next step's tiles are under way during this
 // one's products.  Blocks on one XCD run through 4 row tiles and then the outputs, so its L2 serves both.
 template <int OUT>
 __global__ __launch_bounds__(SW * 64, 2) void fp8_linear_stream_kernel(LinearParams p, LinearGrid q) {
   constexpr bool FAST = OUT == DT_F16 || OUT == DT_BF16;
-  extern __shared__ __attribute__((aligned(16))) uint8_t fp8_smem[];   // [2][2 weight tiles, 4 x tiles of 64 rows]
-  __shared__ __attribute__((aligned(16))) float bias[2 * GROUP];
+  // Two weight tiles and 4 tiles of 64 rows each.  Separate objects: reads of one are then known not to wait
+  // for copies into the other.
   constexpr int STAGE = 2 * WTILE + 4 * MROWS * GROUP;
+  __shared__ __attribute__((aligned(16))) uint8_t S0[STAGE], S1[STAGE];
+  __shared__ __attribute__((aligned(16))) float bias[2 * GROUP];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int kbs = (p.inputs + GROUP - 1) / GROUP, nbs = (p.outputs + GROUP - 1) / GROUP;
   const int slot = blockIdx.x >> 3, nt = q.subsets, turn = slot / (4 * nt), in = slot % (4 * nt);
@@ -187,37 +175,57 @@ __global__ __launch_bounds__(SW * 64, 2) void fp8_linear_stream_kernel(LinearPar
     const int n = nblk * 2 * GROUP + i;
     bias[i] = p.bias && n < p.outputs ? p.bias[n] : 0.f;
   }
+  // A step's copies: 8 rows of 128 bytes an instruction, four of weights and four of x a wave, at uniform bases
+  // that move with the step and 32-bit lane offsets.  Rows past the end repeat the last one; the missing
+  // half of a half group repeats its first, which x's zeros (below) take out of the sums.  Chunk c of x's
+  // row m lies at c ^ (m >> 2 & 7).
+  const uint8_t* const wbase = p.w + (size_t)nblk * 2 * GROUP * p.x.pitch;
+  const uint8_t* const xbase = p.x.codes + (size_t)mblk * 4 * MROWS * p.x.pitch;
+  uint32_t woff[4], xoff[4];    // bit 0: in the upper half of the group
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = (wave * 4 + i) * 8 + (lane >> 3);
+    const int cw = (lane & 7) ^ key_of<OUT>(row & (GROUP - 1)), cx = (lane & 7) ^ (row >> 2 & 7);
+    woff[i] = __umul24(min(row, p.outputs - 1 - nblk * 2 * GROUP), p.x.pitch) + (cw & 3) * 16 + (cw >> 2);
+    xoff[i] = __umul24((int)min((long long)row, p.rows - 1 - (long long)mblk * 4 * MROWS), p.x.pitch) + (cx & 3) * 16 + (cx >> 2);
+  }
+  // Buffer instructions: after a global load into LDS every wait for LDS becomes a wait for that load too.
   auto stage = [&](uint8_t* dst, int kb) __attribute__((always_inline)) {
+#if __HIP_DEVICE_COMPILE__
+    const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc((void*)wbase, 0, 0xffffffffu, 0x27000);
+    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc((void*)xbase, 0, 0xffffffffu, 0x27000);
+    const uint32_t up = kb * GROUP + 64 < p.x.pitch ? 63 : -1;     // uniform
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int part = wave * 4 + i;
-      w_stage<OUT>(dst + (part >> 4) * WTILE, p.w, p.x.pitch, p.outputs, min(nblk * 2 + (part >> 4), nbs - 1), kb,
-                   part & 15, lane);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, dst + (wave * 4 + i) * 1024, 16, woff[i] + (woff[i] & 1) * up, kb * GROUP, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, dst + 2 * WTILE + (wave * 4 + i) * 1024, 16,
+                                               xoff[i] + (xoff[i] & 1) * up, kb * GROUP, 0, 0);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int part = wave * 4 + i;
-      x_stage(dst + 2 * WTILE + (part >> 3) * MROWS * GROUP, p, (long long)(mblk * 4 + (part >> 3)) * MROWS, kb, part & 7, lane);
-    }
+#else
+    (void)dst;
+    (void)kb;
+#endif
   };
   const int i16 = n_of<OUT>(0, r);
   const int wl = wn * WTILE + i16 * GROUP + ((g ^ key_of<OUT>(i16)) << 4), wlx = wl ^ 64;
   // rows 4 r + t: chunk g ^ (r & 7)
   const int xl = 2 * WTILE + wm * MROWS * GROUP + r * 4 * GROUP + ((g ^ (r & 7)) << 4), xlx = xl ^ 64;
   const long long srow = min(m0 + 4 * r, (long long)p.x.sp - 4);
-  stage(fp8_smem, 0);
+  stage(S0, 0);
   __syncthreads();     // the biases
   f4 acc[8][SM];
 #pragma unroll
   for (int t = 0; t < 8; ++t)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) acc[t][q] = *reinterpret_cast<const f4*>(bias + wn * GROUP + n_of<OUT>(t, 4 * g));
+    for (int q = 0; q < SM; ++q) acc[t][q] = *reinterpret_cast<const f4*>(bias + wn * GROUP + n_of<OUT>(t, 4 * g));
+  // the step's scales are loaded a step ahead too, before its copies: a wait for them is no wait for those
   uint32_t scale = *reinterpret_cast<const uint32_t*>(p.x.scales + srow);
-  for (int kb = 0; kb < kbs; ++kb) {
+  const uint8_t* const ws = p.ws + (size_t)nbl * kbs;
+  int wscale = ws[0];
+  auto step = [&](int kb, const uint8_t* buf, uint8_t* other) __attribute__((always_inline)) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();     // step kb in LDS for every wave; every wave done with the other buffer
     const int kn = min(kb + 1, kbs - 1);
-    const uint8_t* buf = fp8_smem + (kb & 1) * STAGE;
     XFrag<SM> x;
     x.scale = scale;
 #pragma unroll
@@ -225,10 +233,26 @@ __global__ __launch_bounds__(SW * 64, 2) void fp8_linear_stream_kernel(LinearPar
       x.v[t][0] = *reinterpret_cast<const u32x4*>(buf + xl + t * GROUP);
       x.v[t][1] = *reinterpret_cast<const u32x4*>(buf + xlx + t * GROUP);
     }
-    stage(fp8_smem + ((kb + 1) & 1) * STAGE, kn);
+    x_zero(x, p, kb);
+    const int wnow = wscale;
     scale = *reinterpret_cast<const uint32_t*>(p.x.scales + (size_t)kn * p.x.sp + srow);
-    mma<OUT, FAST, false, false>(acc, buf + wl, buf + wlx, x, p.ws[(size_t)nbl * kbs + kb], bias, g, []() {});
+    wscale = ws[kn];
+    __builtin_amdgcn_sched_barrier(0);
+    stage(other, kn);
+    __builtin_amdgcn_sched_barrier(0);     // the copies are under way first, the fragments come one by one
+    mma<OUT, FAST, false, false>(acc, buf + wl, buf + wlx, x, wnow, bias, g, []() {});
+    // products touch no memory: without this they would be moved past the next step's barrier
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int q = 0; q < SM; ++q) asm volatile("" : "+v"(acc[t][q]));
+  };
+  int kb = 0;
+  for (; kb + 1 < kbs; kb += 2) {
+    step(kb, S0, S1);
+    step(kb + 1, S1, S0);
   }
+  if (kb < kbs) step(kb, S0, S1);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last copy, which nothing reads
   if (m0 >= p.rows || nb >= nbs) return;
   if constexpr (OUT == OUT_KEPT) finish_kept(acc, p, m0, nb, r, g);
@@ -259,14 +283,10 @@ int go(lf_context* ctx, const LinearParams& p) {
     return check_hip(hipGetLastError(), "fp8 linear launch");
   }
   const long long mt = ((long long)p.rows + MROWS - 1) / MROWS;
-  constexpr int smem = 2 * (2 * WTILE + 4 * MROWS * GROUP);
-  static const bool lds = hipFuncSetAttribute(reinterpret_cast<const void*>(&fp8_linear_stream_kernel<OUT>),
-                                              hipFuncAttributeMaxDynamicSharedMemorySize, smem) == hipSuccess;
-  if (!lds) return set_error(LF_ERR_DEVICE, "fp8 linear: the device refuses the LDS it needs");
   q.subsets = (nbs + 1) / 2;
   q.blocks = (int)((mt + 3) / 4);
   const unsigned grid = (unsigned)(((long long)q.blocks + 31) / 32 * 32 * q.subsets);
-  hipLaunchKernelGGL((fp8_linear_stream_kernel<OUT>), dim3(grid), dim3(SW * 64), smem, ctx->stream, p, q);
+  hipLaunchKernelGGL((fp8_linear_stream_kernel<OUT>), dim3(grid), dim3(SW * 64), 0, ctx->stream, p, q);
   return check_hip(hipGetLastError(), "fp8 linear launch");
 }
 

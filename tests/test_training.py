@@ -452,6 +452,44 @@ def test_linear_specials(ctx):
     assert np.isnan(v[5]).all() and np.isfinite(v[:5]).all() and np.isfinite(v[6:]).all()
 
 
+# Reductions too long for resident weights: steps of whole groups, half a group at the end, tails of rows
+# and outputs on both sides of a 256 x 256 tile.
+LONG_SHAPES = [(1, 1153, 1), (3, 1216, 130), (257, 1280, 257), (300, 2112, 384), (59, 4096, 64), (1025, 1408, 500),
+               (2100, 1500, 129)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rows,k,n", LONG_SHAPES)
+def test_linear_long(ctx, dt, rows, k, n):
+    test_linear(ctx, dt, rows, k, n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,n", LONG_SHAPES)
+def test_linear_long_kept(ctx, rows, k, n):
+    test_linear_kept(ctx, rows, k, n)
+
+
+@pytest.mark.gpu
+def test_linear_long_specials(ctx):
+    """NaN stays in its row and its column, and garbage scales behind the last row change nothing."""
+    from localfold_amd import capi, device as D
+    rng = np.random.default_rng(4)
+    x = rng.normal(size=(270, 1344)) * 10.0 ** rng.integers(-12, 12, size=(270, 1))
+    x[5, 1340] = np.nan
+    w8 = D.fp8_weight(ctx, torch.as_tensor(rng.normal(size=(200, 1344)) / 36).float().to(ctx.device), capi.LF_OUT_IN)
+    x8 = D.checkpoint_pack(ctx, torch.as_tensor(x).float().to(ctx.device))
+    x8.scales[:, 270:] = 255
+    for dt in (torch.float32, torch.bfloat16):
+        out = f64(D.fp8_linear(ctx, x8, w8, relu=True, dtype=dt))
+        assert np.isnan(out[5]).all()
+        xv, wv = values_of(x8), weight_values(w8)
+        xv[5] = 0
+        out[5] = 0
+        close(out, np.maximum(xv @ wv.T, 0), linear_slack(xv, wv, 1344, dt == torch.float32), dt)
+
+
 GRAD_SHAPES = [(1, 1, 1), (1, 128, 128), (15, 22, 49), (64, 64, 64), (100, 130, 70), (333, 128, 512), (1000, 384, 129),
                (257, 512, 256), (4100, 256, 64), (70000, 64, 128), (37, 1536, 384)]
 
