@@ -17,8 +17,9 @@ typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 typedef short s4v __attribute__((ext_vector_type(4)));
 
 constexpr int GN = GROUP;                 // outputs of a block, either way: one group of both operands
-constexpr int GSTEP = 64;                 // rows of a step, multiplied in two halves
-constexpr int RING = 2;                   // steps between a load and its use
+constexpr int GSTEP = 32;                 // rows of a step: one matrix instruction's
+constexpr int TEAMS = 4;                  // of four waves, on steps in turn
+constexpr int GWAVES = 4 * TEAMS;
 
 struct GradParams {
   Kept a, b;
@@ -26,15 +27,15 @@ struct GradParams {
   float* colsum;                          // [splits][cols of the summed one], or null
   int sum_of;                             // 0: no column sums, 1: of a, 2: of b
   int splits, tiles, tiles_j;
-  long long rows_per;                     // rows of a split, a multiple of 2 RING GSTEP
+  long long rows_per;                     // rows of a split, a multiple of TEAMS GSTEP
   void *out, *bias;
   int dt, swapped;                        // out is [b.cols][a.cols]
 };
 
 constexpr int PITCH = GN * 2 + 32;        // LDS bytes of a row of bf16: 4 rows apart by 32 bytes mod 128
 constexpr int BUF = 2 * GSTEP * PITCH;    // one team's buffer: rows of a, then of b
-constexpr size_t GRAD_SMEM = 4 * BUF;     // two teams, two buffers; the joining teams use 64 KB of it
-static_assert(GRAD_SMEM >= (size_t)GN * GN * 4, "the teams' join");
+constexpr size_t GRAD_SMEM = TEAMS * 2 * BUF;
+static_assert(GRAD_SMEM >= (size_t)2 * GN * GN * 4 && GRAD_SMEM <= 160 * 1024, "the join of two teams at a time; LDS");
 
 // The transposing read: of each 16 lanes, lanes 4k .. 4k+3 address row k's 16 columns, 4 each; lane i
 // receives column i of the 4 rows.
@@ -64,7 +65,7 @@ __device__ __forceinline__ b8 tr_frag(const uint8_t* p) {
 
 // SUM: 0 no column sums, 1 of a, 2 of b.
 template <int SUM>
-__global__ __launch_bounds__(512, 2) void weight_grad_kernel(GradParams p) {
+__global__ __launch_bounds__(GWAVES * 64) void weight_grad_kernel(GradParams p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t grad_smem[];
   const int slot = blockIdx.x >> 3, tile = slot % p.tiles, split = slot / p.tiles * 8 + (blockIdx.x & 7);
   if (split >= p.splits) return;
@@ -73,44 +74,43 @@ __global__ __launch_bounds__(512, 2) void weight_grad_kernel(GradParams p) {
   const int team = wave >> 2, wi = (wave >> 1) & 1, wj = wave & 1, tid = threadIdx.x & 255;
   const long long m0 = split * p.rows_per;
   const int n = (int)min(p.a.rows - m0, p.rows_per);            // rows of the split
-  const int steps = (n + 2 * GSTEP - 1) / (2 * GSTEP);
-  uint8_t* mine = grad_smem + team * 2 * BUF;
+  const int steps = (n + TEAMS * GSTEP - 1) / (TEAMS * GSTEP);
+  uint8_t* const mine = grad_smem + team * 2 * BUF;
 
-  // Half a step is 32 rows, 16 codes a lane of a and of b, at a uniform base that moves with the step and a
-  // 32-bit lane offset.  The loads have no condition, or the compiler could not count those in flight:
-  // rows past the end read the last one, and are made zeros when they are stored; columns past the pitch
-  // read the last ones, for outputs that do not exist.
+  // A step is 16 codes a lane of a and of b, at a uniform base that moves with the step and a 32-bit lane
+  // offset.  The loads have no condition, or the compiler could not count those in flight: rows past the
+  // end read the last one, and are made zeros when they are stored; columns past the pitch read the last
+  // ones, for outputs that do not exist.
   const int row = tid >> 3, pc = tid & 7;
-  const uint8_t* code[2] = {p.a.codes + (size_t)m0 * p.a.pitch, p.b.codes + (size_t)m0 * p.b.pitch};
-  const uint8_t* scale[2] = {p.a.scales + (size_t)(i0 / GROUP) * p.a.sp + m0, p.b.scales + (size_t)(j0 / GROUP) * p.b.sp + m0};
+  const uint8_t* const code[2] = {p.a.codes + (size_t)m0 * p.a.pitch, p.b.codes + (size_t)m0 * p.b.pitch};
+  const uint8_t* const scale[2] = {p.a.scales + (size_t)(i0 / GROUP) * p.a.sp + m0, p.b.scales + (size_t)(j0 / GROUP) * p.b.sp + m0};
   const int pitch[2] = {p.a.pitch, p.b.pitch};
   const int col[2] = {min(i0 + pc * 16, pitch[0] - 16), min(j0 + pc * 16, pitch[1] - 16)};
-  u32x4 raw[RING][2][2];        // [step][half][a or b]
-  int sc[RING][2][2];
+  u32x4 raw[2];        // a, b
+  int sc[2];
   // 24-bit products: the 64-bit multiply-add that the compiler would take reads a register pair whose other
   // half may be a load in flight, and waits for it
-  auto load = [&](int s, int ring, int h, int k) __attribute__((always_inline)) {
-    const int m = min((2 * s + team) * GSTEP + h * 32, n - 1), r = min(row, n - 1 - m);
-    raw[ring][h][k] = *reinterpret_cast<const u32x4*>(code[k] + (size_t)m * pitch[k] + (__umul24(r, pitch[k]) + col[k]));
-    sc[ring][h][k] = (scale[k] + m)[(uint32_t)r];
+  auto load = [&](int s, int k) __attribute__((always_inline)) {
+    const int m = (int)min(((uint32_t)s * TEAMS + team) * GSTEP, (uint32_t)n - 1), r = min(row, n - 1 - m);
+    raw[k] = *reinterpret_cast<const u32x4*>(code[k] + (size_t)m * pitch[k] + (__umul24(r, pitch[k]) + col[k]));
+    sc[k] = (scale[k] + m)[(uint32_t)r];
   };
   // A lane's 16 values are two 16-byte pieces; in the upper half of a row they lie the other way round, so
   // that the 8 lanes of a row store to all banks at once.
-  uint8_t* const dst = mine + row * PITCH + pc * 32 + (pc & 4 ? 16 : 0);
-  uint8_t* const dst1 = mine + row * PITCH + pc * 32 + (pc & 4 ? 0 : 16);
-  auto store = [&](int s, int ring, int h, int k) __attribute__((always_inline)) {
-    const bool ok = row < n - (2 * s + team) * GSTEP - h * 32;
-    const float f = scale_value(sc[ring][h][k]);
+  const int dst = row * PITCH + pc * 32 + (pc & 4 ? 16 : 0);
+  auto store = [&](int s, int k) __attribute__((always_inline)) {
+    const bool ok = row < (int)(n - ((uint32_t)s * TEAMS + team) * GSTEP);
+    const float f = scale_value(sc[k]);
     uint32_t w[8];
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
-      const int c = ok ? (int)raw[ring][h][k][d] : 0;
+      const int c = ok ? (int)raw[k][d] : 0;
       w[2 * d] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, f, false));
       w[2 * d + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, f, true));
     }
-    const int to = (s & 1) * BUF + (k * GSTEP + h * 32) * PITCH;
-    *reinterpret_cast<u32x4*>(dst + to) = u32x4{w[0], w[1], w[2], w[3]};
-    *reinterpret_cast<u32x4*>(dst1 + to) = u32x4{w[4], w[5], w[6], w[7]};
+    uint8_t* const to = mine + (s & 1) * BUF + k * GSTEP * PITCH;
+    *reinterpret_cast<u32x4*>(to + dst) = u32x4{w[0], w[1], w[2], w[3]};
+    *reinterpret_cast<u32x4*>(to + (dst ^ 16)) = u32x4{w[4], w[5], w[6], w[7]};
   };
 
   // A wave has a 64 x 64 part of the tile.  Its fragments are numbered so that fragments 0 and 2 of the two
@@ -130,96 +130,73 @@ __global__ __launch_bounds__(512, 2) void weight_grad_kernel(GradParams p) {
   const uint8_t* const from = mine + (4 * g + (l16 >> 2)) * PITCH;
   const uint8_t* const from_a = from + wi * 128 + ((l16 & 3) * 8 ^ wi * 16) + xi * 32;
   const uint8_t* const from_b = from + GSTEP * PITCH + wj * 128 + ((l16 & 3) * 8 ^ wj * 16) + xj * 32;
-  auto read_a = [&](int s, int h, int i) __attribute__((always_inline)) {     // fragment i ^ xi
-    const int at = (s & 1) * BUF + h * 32 * PITCH;
-    return tr_frag(from_a + (i & 1 ? at + (i - 1) * 32 + (1 - 2 * xi) * 32 : at + i * 32));
-  };
-  auto read_b = [&](int s, int h, int j) __attribute__((always_inline)) {
-    const int at = (s & 1) * BUF + h * 32 * PITCH;
-    return tr_frag(from_b + (j & 1 ? at + (j - 1) * 32 + (1 - 2 * xj) * 32 : at + j * 32));
-  };
+  const int odd_a = (1 - 2 * xi) * 32, odd_b = (1 - 2 * xj) * 32;
 
-  // Half (s, h) multiplies fragments that the half before it read, and reads the next one's.  Step s stores
-  // (s + 2, 0) where (s, 0) was, read in step s - 1, and (s + 1, 1) where (s - 1, 1) was, read in that step
-  // too: one barrier a step.
-#pragma unroll
-  for (int q = 0; q < RING; ++q)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) load(q, q, k >> 1, k & 1);
+  // Step s is multiplied while step s + 1 is converted and stored and step s + 2 is loaded.
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    store(0, 0, 0, k);
-    load(2, 0, 0, k);
-    store(0, 0, 1, k);
-    load(2, 0, 1, k);
-    store(1, 1, 0, k);
-    load(3, 1, 0, k);
+    load(0, k);
+    store(0, k);
+    load(1, k);
   }
-  __syncthreads();
-  b8 fa[4], fb[2][4];
+  for (int s = 0; s < steps; ++s) {
+    __syncthreads();
+    const int at = (s & 1) * BUF;
+    b8 fa[4], fb[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) fb[0][j] = read_b(0, 0, j);
+    for (int j = 0; j < 4; ++j) fb[j] = tr_frag(from_b + (j & 1 ? at + (j - 1) * 32 + odd_b : at + j * 32));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) fa[i] = read_a(0, 0, i);
-  for (int s0 = 0; s0 < steps; s0 += RING) {     // past the last step: zeros
+    for (int i = 0; i < 4; ++i) fa[i] = tr_frag(from_a + (i & 1 ? at + (i - 1) * 32 + odd_a : at + i * 32));
 #pragma unroll
-    for (int u = 0; u < RING; ++u) {
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+      if (i & 1) {
+        store(s + 1, i >> 1);
+        load(s + 2, i >> 1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (sum) {
+#pragma unroll
+      for (int f = 0; f < 2; ++f)
+        sums[f] = SUM == 1 ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[2 * f], ones, sums[f], 0, 0, 0)
+                           : __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fb[2 * f], sums[f], 0, 0, 0);
+    }
+  }
+
+  // the teams' sums, joined in halves: 2 and 3 to 0 and 1, then 1 to 0
+#pragma unroll
+  for (int to = TEAMS / 2; to > 0; to >>= 1) {
+    f4* const at = reinterpret_cast<f4*>(grad_smem) + ((team & (to - 1)) * 16 * 4 + (wi * 2 + wj)) * 64 + lane;   // [to][16][4 waves][64]
+    __syncthreads();
+    if (team >= to && team < 2 * to) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) at[(i * 4 + j) * 256] = acc[i][j];
+    }
+    __syncthreads();
+    if (team < to) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] += at[(i * 4 + j) * 256];
+    }
+    if (sum) {     // uniform in the block
       __syncthreads();
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int s = s0 + u, sn = u + h, st = h ? s + 1 : s + 2, ring = (u + h) & 1;
-        if (sum) {
-#pragma unroll
-          for (int f = 0; f < 2; ++f)
-            sums[f] = SUM == 1 ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[2 * f], ones, sums[f], 0, 0, 0)
-                               : __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fb[h][2 * f], sums[f], 0, 0, 0);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) fb[1 - h][j] = read_b(sn, 1 - h, j);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[h][j], acc[i][j], 0, 0, 0);
-          fa[i] = read_a(sn, 1 - h, i);
-          if (i & 1) {
-            store(st, ring, h, i >> 1);
-            load(st + RING, ring, h, i >> 1);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
+      if (team >= to && team < 2 * to) {
+        at[0] = sums[0];
+        at[256] = sums[1];
+      }
+      __syncthreads();
+      if (team < to) {
+        sums[0] += at[0];
+        sums[1] += at[256];
       }
     }
   }
-
-  // the second team's sums are added to the first's
-  f4* half = reinterpret_cast<f4*>(grad_smem) + (wi * 2 + wj) * 64 + lane;      // [16][4 waves][64]
-  __syncthreads();
-  if (team == 1) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) half[(i * 4 + j) * 256] = acc[i][j];
-  }
-  __syncthreads();
-  if (team == 0) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] += half[(i * 4 + j) * 256];
-  }
-  if (sum) {     // uniform in the block
-    __syncthreads();
-    if (team == 1) {
-      half[0] = sums[0];
-      half[256] = sums[1];
-    }
-    __syncthreads();
-    if (team == 0) {
-      sums[0] += half[0];
-      sums[1] += half[256];
-    }
-  }
-  if (team == 1) return;
+  if (team != 0) return;
   const int ca = p.a.cols, cb = p.b.cols;
   float* part = p.partial ? p.partial + (size_t)split * ca * cb : nullptr;
 #pragma unroll
@@ -292,8 +269,8 @@ GradPlan grad_plan(long long rows, int ci, int cj) {
   q.tiles_j = (cj + GN - 1) / GN;
   q.tiles = (ci + GN - 1) / GN * q.tiles_j;
   const long long want = std::max<long long>(1, 256 / q.tiles);      // a block a CU
-  const long long turns = (rows + 2 * RING * GSTEP - 1) / (2 * RING * GSTEP);
-  q.rows_per = (turns + want - 1) / want * (2 * RING * GSTEP);
+  const long long turns = (rows + TEAMS * GSTEP - 1) / (TEAMS * GSTEP);
+  q.rows_per = (turns + want - 1) / want * (TEAMS * GSTEP);
   q.splits = (int)((rows + q.rows_per - 1) / q.rows_per);
   return q;
 }
@@ -304,7 +281,7 @@ int go(lf_context* ctx, const GradParams& p) {
                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)GRAD_SMEM) == hipSuccess;
   if (!lds) return set_error(LF_ERR_DEVICE, "weight gradient: the device refuses the LDS it needs");
   const unsigned grid = (unsigned)((p.splits + 7) / 8 * p.tiles * 8);
-  hipLaunchKernelGGL((weight_grad_kernel<SUM>), dim3(grid), dim3(512), GRAD_SMEM, ctx->stream, p);
+  hipLaunchKernelGGL((weight_grad_kernel<SUM>), dim3(grid), dim3(GWAVES * 64), GRAD_SMEM, ctx->stream, p);
   return check_hip(hipGetLastError(), "weight gradient launch");
 }
 
