@@ -103,6 +103,9 @@ __global__ __launch_bounds__(RW * 64) void fp8_linear_resident_kernel(LinearPara
     w_stage<OUT>(fp8_smem + (i >> 4) * WTILE, p.w, p.x.pitch, p.outputs, nb0 + (i >> 4) / kbs, (i >> 4) % kbs, i & 15, lane);
   for (int i = threadIdx.x; i < per * GROUP; i += RW * 64)
     bias[i] = p.bias && nb0 * GROUP + i < p.outputs ? p.bias[nb0 * GROUP + i] : 0.f;
+  // The scales too: a load from memory between the products would have to wait for the stores before it.
+  uint8_t* wscales = reinterpret_cast<uint8_t*>(bias + q.per * GROUP);
+  for (int i = threadIdx.x; i < per * kbs; i += RW * 64) wscales[i] = p.ws[nb0 * kbs + i];
   // this block's units, of (rows / 32) x per, and the wave's first; a unit is (row tile, output group)
   const long long units = ((long long)p.rows + 16 * RM - 1) / (16 * RM) * per;
   const int u0 = (int)(units * blk / q.blocks), u1 = (int)(units * (blk + 1) / q.blocks);
@@ -129,7 +132,7 @@ __global__ __launch_bounds__(RW * 64) void fp8_linear_resident_kernel(LinearPara
         ++mt;
       }
     }
-    const uint8_t* const ws = p.ws + (nb0 + nb_now) * kbs;
+    const uint8_t* const ws = wscales + nb_now * kbs;
     const float* const bn = bias + nb_now * GROUP;
     int at = nb_now * kbs * WTILE;
     x_zero(x, p, 0);
@@ -277,7 +280,7 @@ int go(lf_context* ctx, const LinearParams& p) {
     static const bool lds = hipFuncSetAttribute(reinterpret_cast<const void*>(&fp8_linear_resident_kernel<OUT>),
                                                 hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) == hipSuccess;
     if (!lds) return set_error(LF_ERR_DEVICE, "fp8 linear: the device refuses the LDS it needs");
-    const size_t smem = (size_t)q.per * (kbs * WTILE + GROUP * 4);
+    const size_t smem = (size_t)q.per * (kbs * WTILE + GROUP * 4 + kbs);
     const unsigned grid = (unsigned)((q.blocks + 7) / 8 * q.subsets * 8);
     hipLaunchKernelGGL((fp8_linear_resident_kernel<OUT>), dim3(grid), dim3(RW * 64), smem, ctx->stream, p, q);
     return check_hip(hipGetLastError(), "fp8 linear launch");

@@ -98,6 +98,14 @@ __device__ __forceinline__ void stage_all(uint8_t* smem, const TrainParams& p, i
   }
 }
 
+// The weights' scale bytes of up to 4 groups, one byte each.  Loaded once: a load in the loop would have to
+// wait for the stores before it.
+__device__ __forceinline__ uint32_t scale_word(const uint8_t* s, int groups) {
+  uint32_t w = 0;
+  for (int i = 0; i < groups; ++i) w |= (uint32_t)s[i] << (8 * i);
+  return __builtin_amdgcn_readfirstlane(w);
+}
+
 // Tiles of 32 rows of this block, dealt out to its waves in turn.
 struct Tiles {
   int first, end;
@@ -122,6 +130,7 @@ __global__ __launch_bounds__(TW * 64, 2) void train_forward_kernel(TrainParams p
     vec[2 * C + i] = p.b2 ? p.b2[i] : 0.f;
   }
   for (int i = threadIdx.x; i < p.hidden; i += TW * 64) vec[3 * C + i] = p.b1 ? p.b1[i] : 0.f;
+  const uint32_t s1 = scale_word(p.s1, groups), s2 = scale_word(p.s2, groups);
   const Tiles tiles = block_tiles(p.rows, wave);
   RowWords<ACT, C> x;
   auto load = [&](int tile) __attribute__((always_inline)) {
@@ -208,7 +217,7 @@ __global__ __launch_bounds__(TW * 64, 2) void train_forward_kernel(TrainParams p
       for (int q = 0; q < TM; ++q) acc[t][q] = *reinterpret_cast<const f4*>(vec + 2 * C + n_of<ACT>(t, 4 * g));
     for (int hb = 0; hb < groups; ++hb) {
       f4 hid[8][TM];
-      mma<OUT_KEPT, false, true, C == 64>(hid, wa + hb * WTILE, wax + hb * WTILE, y8, p.s1[hb], vec + 3 * C + hb * GROUP, g,
+      mma<OUT_KEPT, false, true, C == 64>(hid, wa + hb * WTILE, wax + hb * WTILE, y8, s1 >> (8 * hb) & 255, vec + 3 * C + hb * GROUP, g,
                                           [] {});
 #pragma unroll
       for (int t = 0; t < 8; ++t)
@@ -220,7 +229,7 @@ __global__ __launch_bounds__(TW * 64, 2) void train_forward_kernel(TrainParams p
       keep_tile(hid, h8);
       store_kept(h8, p.kh.codes + (size_t)m0 * p.hidden + hb * GROUP, p.kh.scales + (size_t)hb * p.kh.sp + m0, p.hidden,
                  left, GROUP, r, g);
-      mma<ACT, FAST, false, false>(acc, wb + hb * WTILE, wbx + hb * WTILE, h8, p.s2[hb], vec, g, [] {});
+      mma<ACT, FAST, false, false>(acc, wb + hb * WTILE, wbx + hb * WTILE, h8, s2 >> (8 * hb) & 255, vec, g, [] {});
     }
     finish<ACT>(acc, fin, m0, 0, r, g);
     if constexpr (ACT == DT_F32) load(min(tile + TW, tiles.end - 1));
@@ -250,6 +259,7 @@ __global__ __launch_bounds__(TW * 64, 2) void train_backward_kernel(TrainParams 
   for (int i = threadIdx.x; i < C; i += TW * 64) vec[i] = p.scale[i];
   for (int i = threadIdx.x; i < GROUP; i += TW * 64) vec[C + i] = 0.f;
   float* const sums = vec + C + GROUP;
+  const uint32_t s1 = scale_word(p.s1, groups), s2 = scale_word(p.s2, groups);
   const Tiles tiles = block_tiles(p.rows, wave);
   RowWords<ACT, C> x;
   auto load = [&](int tile) __attribute__((always_inline)) {
@@ -287,8 +297,8 @@ __global__ __launch_bounds__(TW * 64, 2) void train_backward_kernel(TrainParams 
     for (int t = 0; t < NT2; ++t)
 #pragma unroll
       for (int q = 0; q < TM; ++q) dy[t][q] = f4{0.f, 0.f, 0.f, 0.f};
-    for (int hb = 0; hb < groups; ++hb) {
-      u32x4 gate[TM][2];
+    u32x4 gate[TM][2];
+    auto load_gate = [&](int hb) __attribute__((always_inline)) {
 #pragma unroll
       for (int q = 0; q < TM; ++q)
 #pragma unroll
@@ -296,18 +306,22 @@ __global__ __launch_bounds__(TW * 64, 2) void train_backward_kernel(TrainParams 
           gate[q][a] = *reinterpret_cast<const u32x4*>(
               p.kh.codes + (size_t)m0 * p.hidden + hb * GROUP +
               (uint32_t)(__umul24(min(TM * r + q, left - 1), p.hidden) + 64 * a + 16 * g));
+    };
+    load_gate(0);
+    for (int hb = 0; hb < groups; ++hb) {
       f4 e[8][TM];
-      mma<OUT_KEPT, false, true, C == 64>(e, wa + hb * WTILE, wax + hb * WTILE, d8, p.s1[hb], vec + C, g, [] {});
+      mma<OUT_KEPT, false, true, C == 64>(e, wa + hb * WTILE, wax + hb * WTILE, d8, s1 >> (8 * hb) & 255, vec + C, g, [] {});
 #pragma unroll
       for (int t = 0; t < 8; ++t)
 #pragma unroll
         for (int q = 0; q < TM; ++q) gate4(e[t][q], gate[q][t >> 2][t & 3]);
+      load_gate(min(hb + 1, groups - 1));     // before the stores, which its wait would be for too
       XFrag<TM> e8;
       keep_tile(e, e8);
       store_kept(e8, p.k2.codes + (size_t)m0 * p.hidden + hb * GROUP, p.k2.scales + (size_t)hb * p.k2.sp + m0, p.hidden,
                  left, GROUP, r, g);
       const int at = (groups + hb) * WTILE;
-      mma<OUT_KEPT, FAST, false, false>(dy, wa + at, wax + at, e8, p.s2[hb], vec, g, [] {});
+      mma<OUT_KEPT, FAST, false, false>(dy, wa + at, wax + at, e8, s2 >> (8 * hb) & 255, vec, g, [] {});
     }
 
     // LayerNorm's gradient: a lane has columns 64 a + 16 g + 4 b + j of its rows in dy[4 a + b][q][j]
