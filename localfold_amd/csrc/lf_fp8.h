@@ -72,6 +72,43 @@ __device__ __forceinline__ void w_stage(uint8_t* dst, const uint8_t* w, int pitc
 #endif
 }
 
+// acc[q] += 16 outputs x 16 MT rows x 128 columns, w a lane's two pieces of its output's codes.
+template <bool FAST, int MT>
+__device__ __forceinline__ void mma_frag(f4 (&acc)[MT], const u32x4 (&w)[2], const XFrag<MT>& x, int wscale) {
+#if __HIP_DEVICE_COMPILE__
+  if constexpr (FAST) {
+    const i8v a = {(int)w[0].x, (int)w[0].y, (int)w[0].z, (int)w[0].w, (int)w[1].x, (int)w[1].y, (int)w[1].z, (int)w[1].w};
+#define LF_MM(q)                                                                                                           \
+  {                                                                                                                        \
+    const i8v b = {(int)x.v[q][0].x, (int)x.v[q][0].y, (int)x.v[q][0].z, (int)x.v[q][0].w,                                 \
+                   (int)x.v[q][1].x, (int)x.v[q][1].y, (int)x.v[q][1].z, (int)x.v[q][1].w};                                \
+    acc[q] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[q], 0, 0, 0, wscale, q, (int)x.scale);             \
+  }
+    static_assert(MT == 2, "");
+    LF_MM(0) LF_MM(1)
+#undef LF_MM
+  } else {
+    const float sw = scale_value(wscale);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const b8 a0 = codes_bf16(w[half].x, w[half].y, sw), a1 = codes_bf16(w[half].z, w[half].w, sw);
+#pragma unroll
+      for (int q = 0; q < MT; ++q) {
+        const float sx = scale_value((x.scale >> (8 * q)) & 255);
+        const u32x4 v = x.v[q][half];
+        acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, codes_bf16(v.x, v.y, sx), acc[q], 0, 0, 0);
+        acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, codes_bf16(v.z, v.w, sx), acc[q], 0, 0, 0);
+      }
+    }
+  }
+#else
+  (void)acc;
+  (void)w;
+  (void)x;
+  (void)wscale;
+#endif
+}
+
 // acc += one step: 16 NT outputs x 16 MT rows x 128 columns (HALF: 64, the others are zeros); FIRST: acc =
 // bias + the step, bias 16 NT floats in LDS.  FAST: the scaled 8-bit instruction, else bf16.  w: the
 // lane's place in an LDS tile, wx the same with the other half of the columns.  A tile's fragment is read
@@ -235,11 +272,11 @@ __device__ __forceinline__ uint32_t run_word(float v0, float v1) {
 
 // A wave's tile stored: ReLU or its gradient, then the residual.
 template <int OUT, int NT, int MT>
-__device__ __forceinline__ void finish(f4 (&acc)[NT][MT], const LinearParams& p, long long m0, int nb, int r, int g) {
+__device__ __forceinline__ void finish(f4 (&acc)[NT][MT], const LinearParams& p, long long m0, int n0, int r, int g) {
   typedef typename Act<OUT>::T T;
   constexpr int P = Run<OUT>::PER, L = 4 * P, RUNS = NT / P;    // a lane: RUNS runs of L outputs for each of MT rows
   constexpr int E = 4 / (int)sizeof(T);                        // outputs of a word
-  const int left = (int)min((long long)16 * MT, p.rows - m0), N = p.outputs - nb * GROUP;
+  const int left = (int)min((long long)16 * MT, p.rows - m0), N = p.outputs - n0;
 #pragma unroll
   for (int q = 0; q < MT; ++q) {
     __builtin_amdgcn_sched_barrier(0);   // one row of a lane at a time
@@ -250,17 +287,17 @@ __device__ __forceinline__ void finish(f4 (&acc)[NT][MT], const LinearParams& p,
         for (int j = 0; j < 4; ++j) acc[t][q][j] = __builtin_elementwise_maximum(acc[t][q][j], 0.f);   // keeps NaN
     }
     if (p.relu_of) {
-      const uint8_t* gate = p.relu_of + (size_t)(m0 + min(MT * r + q, left - 1)) * p.q.pitch + nb * GROUP;
+      const uint8_t* gate = p.relu_of + (size_t)(m0 + min(MT * r + q, left - 1)) * p.q.pitch + n0;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const int n = n_of<OUT>(t, 4 * g);
-        gate4(acc[t][q], *reinterpret_cast<const uint32_t*>(gate + min(n, p.q.pitch - nb * GROUP - 4)));
+        gate4(acc[t][q], *reinterpret_cast<const uint32_t*>(gate + min(n, p.q.pitch - n0 - 4)));
       }
     }
   }
-  T* const out = static_cast<T*>(p.out) + (size_t)m0 * p.outputs + nb * GROUP;
-  const T* const res = static_cast<const T*>(p.residual) + (size_t)m0 * p.outputs + nb * GROUP;
-  if (left == 16 * MT && (N >= GROUP || N % (16 * P) == 0)) {     // uniform: rows and runs exist as a whole
+  T* const out = static_cast<T*>(p.out) + (size_t)m0 * p.outputs + n0;
+  const T* const res = static_cast<const T*>(p.residual) + (size_t)m0 * p.outputs + n0;
+  if (left == 16 * MT && (N >= 16 * NT || N % (16 * P) == 0)) {     // uniform: rows and runs exist as a whole
     const char* const rb = reinterpret_cast<const char*>(res);
     char* const ob = reinterpret_cast<char*>(out);
 #pragma unroll

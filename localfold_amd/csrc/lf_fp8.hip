@@ -95,7 +95,7 @@ __global__ __launch_bounds__(RW * 64) void fp8_linear_resident_kernel(LinearPara
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int nbs = (p.outputs + GROUP - 1) / GROUP, kbs = (p.inputs + GROUP - 1) / GROUP;
   // blocks of the same rows and other subsets share an XCD (blocks are dealt out to 8 in turn)
-  const int slot = blockIdx.x >> 3, subset = slot % q.subsets, blk = slot / q.subsets * 8 + (blockIdx.x & 7);
+  const int index = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3), subset = index % q.subsets, blk = index / q.subsets;
   if (blk >= q.blocks) return;
   const int nb0 = subset * q.per, per = min(q.per, nbs - nb0);
   float* bias = reinterpret_cast<float*>(fp8_smem + (size_t)q.per * kbs * WTILE);
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(RW * 64) void fp8_linear_resident_kernel(LinearPara
       });
     }
     if constexpr (OUT == OUT_KEPT) finish_kept(acc, p, (long long)mt_now * 16 * RM, nb0 + nb_now, r, g);
-    else finish<OUT>(acc, p, (long long)mt_now * 16 * RM, nb0 + nb_now, r, g);
+    else finish<OUT>(acc, p, (long long)mt_now * 16 * RM, (nb0 + nb_now) * GROUP, r, g);
     if (u >= u1) break;
   }
 }
@@ -259,7 +259,87 @@ __global__ __launch_bounds__(SW * 64, 2) void fp8_linear_stream_kernel(LinearPar
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last copy, which nothing reads
   if (m0 >= p.rows || nb >= nbs) return;
   if constexpr (OUT == OUT_KEPT) finish_kept(acc, p, m0, nb, r, g);
-  else finish<OUT>(acc, p, m0, nb, r, g);
+  else finish<OUT>(acc, p, m0, nb * GROUP, r, g);
+}
+
+// Small products: what counts is the time to the last byte.  A block computes 32 rows by one run of outputs,
+// its waves a group of columns each, in turn, fragments straight from memory, sums joined in LDS.  59 rows of
+// 384 x 1536 in bf16: 3.5 us, where a block that stages its weights first takes 8.
+//
+// Every block reads its weights and its rows from L2 again, so larger products take the other kernels.  In
+// tiles of 32 x 32 outputs the times cross between 1000 (1024 x 256) and 2600 (64 x 256) for resident
+// weights (f32: 1350 and 3500), and at 3000 for streamed ones (f32: 4200).  bf16, us, small and other:
+// 384 x 1536: 1024 rows 8.2 and 8.1, 4096 rows 22 and 11; 128 x 512: 2048 rows 3.8 and 6.3, 16384 rows 17 and
+// 9.8; 4096 x 4096: 512 rows 60 and 89, 1024 rows 117 and 89.
+constexpr int FW = 8, FM = 2;             // most waves of a block, tiles of 16 rows
+constexpr int FEW_TILES = 1500, FEW_TILES_LONG = 3000;
+
+template <int OUT>
+__global__ __launch_bounds__(FW * 64) void fp8_linear_few_kernel(LinearParams p) {
+  constexpr bool FAST = OUT != DT_F32;
+  constexpr int NT = Run<OUT>::PER;
+  __shared__ f4 part[FW - 1][NT][FM][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int waves = blockDim.x >> 6, kbs = (p.inputs + GROUP - 1) / GROUP;
+  const int n0 = blockIdx.x * 16 * NT;
+  const long long m0 = (long long)blockIdx.y * 16 * FM;
+  const uint8_t* const wbase = p.w + (size_t)n0 * p.x.pitch;
+  const uint8_t* const ws = p.ws + (size_t)(n0 / GROUP) * kbs;
+  uint32_t woff[NT];
+  f4 acc[NT][FM], bias[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    woff[t] = __umul24(min(n_of<OUT>(t, r), p.outputs - 1 - n0), p.x.pitch) + 16 * g;
+#pragma unroll
+    for (int q = 0; q < FM; ++q) acc[t][q] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bias[t][j] = p.bias ? p.bias[min(n0 + n_of<OUT>(t, 4 * g) + j, p.outputs - 1)] : 0.f;
+  }
+  struct Step {
+    XFrag<FM> x;
+    u32x4 w[NT][2];
+    int ws;
+  };
+  auto load = [&](Step& s, int kb) __attribute__((always_inline)) {
+    const int second = kb * GROUP + 64 < p.x.pitch ? 64 : 0;    // uniform
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      s.w[t][0] = *reinterpret_cast<const u32x4*>(wbase + kb * GROUP + woff[t]);
+      s.w[t][1] = *reinterpret_cast<const u32x4*>(wbase + kb * GROUP + second + woff[t]);
+    }
+    x_load(s.x, p, m0, kb, r, g);
+    s.ws = ws[kb];
+  };
+  auto multiply = [&](Step& s, int kb) __attribute__((always_inline)) {
+    x_zero(s.x, p, kb);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) mma_frag<FAST>(acc[t], s.w[t], s.x, s.ws);
+  };
+  for (int kb = wave; kb < kbs; kb += 2 * waves) {
+    Step a, b;
+    load(a, kb);
+    load(b, min(kb + waves, kbs - 1));
+    multiply(a, kb);
+    if (kb + waves < kbs) multiply(b, kb + waves);
+  }
+  if (wave > 0) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int q = 0; q < FM; ++q) part[wave - 1][t][q][lane] = acc[t][q];
+  }
+  __syncthreads();
+  if (wave > 0) return;
+  for (int k = 1; k < waves; ++k)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int q = 0; q < FM; ++q) acc[t][q] += part[k - 1][t][q][lane];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int q = 0; q < FM; ++q) acc[t][q] += bias[t];
+  finish<OUT>(acc, p, m0, n0, r, g);
 }
 
 namespace {
@@ -269,6 +349,14 @@ int go(lf_context* ctx, const LinearParams& p) {
   const int nbs = (p.outputs + GROUP - 1) / GROUP, kbs = (p.inputs + GROUP - 1) / GROUP;
   const int cus = ctx->num_cus;
   LinearGrid q{};
+  if constexpr (OUT != OUT_KEPT) {
+    const long long mt = ((long long)p.rows + 16 * FM - 1) / (16 * FM), tiles = mt * ((p.outputs + 31) / 32);
+    if (tiles <= (kbs <= RESIDENT_TILES ? FEW_TILES : FEW_TILES_LONG)) {
+      const dim3 grid((p.outputs + 16 * Run<OUT>::PER - 1) / (16 * Run<OUT>::PER), (unsigned)mt);
+      hipLaunchKernelGGL((fp8_linear_few_kernel<OUT>), grid, dim3(std::min(kbs, FW) * 64), 0, ctx->stream, p);
+      return check_hip(hipGetLastError(), "fp8 linear launch");
+    }
+  }
   if (kbs <= RESIDENT_TILES) {
     const long long mt = ((long long)p.rows + 16 * RM - 1) / (16 * RM);
     // as many output groups a block as fit, but no more than keep every wave of the chip in units
@@ -276,12 +364,13 @@ int go(lf_context* ctx, const LinearParams& p) {
     const long long busy = std::max<long long>(1, mt * nbs / ((long long)cus * RW));
     q.per = (int)std::min<long long>(std::min(fit, nbs), busy);
     q.subsets = (nbs + q.per - 1) / q.per;
-    q.blocks = (int)std::min<long long>((mt * q.per + RW - 1) / RW, std::max(1, cus / q.subsets));
+    // a unit for every SIMD before a second one: 2048 rows of 128 x 512 in 6.3 us, in blocks of 16 units 10
+    q.blocks = (int)std::min<long long>((mt * q.per + 3) / 4, std::max(1, cus / q.subsets));
     static const bool lds = hipFuncSetAttribute(reinterpret_cast<const void*>(&fp8_linear_resident_kernel<OUT>),
                                                 hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) == hipSuccess;
     if (!lds) return set_error(LF_ERR_DEVICE, "fp8 linear: the device refuses the LDS it needs");
     const size_t smem = (size_t)q.per * (kbs * WTILE + GROUP * 4 + kbs);
-    const unsigned grid = (unsigned)((q.blocks + 7) / 8 * q.subsets * 8);
+    const unsigned grid = (unsigned)((q.blocks * q.subsets + 7) / 8 * 8);
     hipLaunchKernelGGL((fp8_linear_resident_kernel<OUT>), dim3(grid), dim3(RW * 64), smem, ctx->stream, p, q);
     return check_hip(hipGetLastError(), "fp8 linear launch");
   }

@@ -490,6 +490,18 @@ def test_linear_long_specials(ctx):
         close(out, np.maximum(xv @ wv.T, 0), linear_slack(xv, wv, 1344, dt == torch.float32), dt)
 
 
+# Products large enough for the kernels that stage weights, resident and streamed.
+MANY_SHAPES = [(20000, 64, 100), (9000, 128, 257), (6001, 192, 300), (3100, 1000, 512), (49001, 22, 17), (4000, 384, 513),
+               (12300, 128, 128), (25000, 1153, 130), (8200, 1216, 400), (5000, 2112, 650)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rows,k,n", MANY_SHAPES)
+def test_linear_many(ctx, dt, rows, k, n):
+    test_linear(ctx, dt, rows, k, n)
+
+
 GRAD_SHAPES = [(1, 1, 1), (1, 128, 128), (15, 22, 49), (64, 64, 64), (100, 130, 70), (333, 128, 512), (1000, 384, 129),
                (257, 512, 256), (4100, 256, 64), (70000, 64, 128), (37, 1536, 384)]
 
