@@ -9,7 +9,7 @@
 // 16-bit outputs take the scaled 8-bit instruction (16x16x128), which multiplies the powers of two itself
 // and has twice bfloat16's rate.  Of 8 products that it adds at a time it drops what lies 2^-13 below the
 // largest (measured: 1.6e-5 of the result for normal inputs, where bfloat16 and half round by 2e-3 and
-// 2e-4).  f32 outputs, and kept ones, whose codes would fall the other way near a border, take the bf16
+// 2e-4).  f32 outputs that a caller sees, and kept ones, whose codes would fall the other way near a border, take the bf16
 // instruction on operands converted in registers, exactly: codes times a power of two fit bfloat16.
 #pragma once
 #include "lf_train.h"
@@ -117,8 +117,8 @@ __device__ __forceinline__ void mma_frag(f4 (&acc)[MT], const u32x4 (&w)[2], con
 template <int OUT, bool FAST, bool FIRST, bool HALF, int NT, int MT, class NEXT>
 __device__ __forceinline__ void mma(f4 (&acc)[NT][MT], const uint8_t* w, const uint8_t* wx, const XFrag<MT>& x, int wscale,
                                     const float* bias, int g, NEXT next) {
-  f4 c;
 #if __HIP_DEVICE_COMPILE__
+  f4 c;
   if constexpr (FAST) {
     u32x4 a0[2], a1[2];
     a1[0] = a1[1] = u32x4{0, 0, 0, 0};

@@ -88,9 +88,8 @@ struct LinearGrid {
 // neighbouring waves.
 constexpr int RW = 16, RM = 2;            // waves of a block, tiles of 16 rows of a wave
 
-template <int OUT>
+template <int OUT, bool FAST>
 __global__ __launch_bounds__(RW * 64) void fp8_linear_resident_kernel(LinearParams p, LinearGrid q) {
-  constexpr bool FAST = OUT == DT_F16 || OUT == DT_BF16;
   extern __shared__ __attribute__((aligned(16))) uint8_t fp8_smem[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int nbs = (p.outputs + GROUP - 1) / GROUP, kbs = (p.inputs + GROUP - 1) / GROUP;
@@ -158,9 +157,8 @@ constexpr int SW = 8, SM = 4, MROWS = 16 * SM;   // the streaming kernel's waves
 // Long reductions: a block of 256 rows and two output groups walks the columns 128 at a time, tiles of both
 // operands in two LDS buffers in turn.  One barrier a step; the next step's tiles are under way during this
 // one's products.  Blocks on one XCD run through 4 row tiles and then the outputs, so its L2 serves both.
-template <int OUT>
+template <int OUT, bool FAST>
 __global__ __launch_bounds__(SW * 64, 2) void fp8_linear_stream_kernel(LinearParams p, LinearGrid q) {
-  constexpr bool FAST = OUT == DT_F16 || OUT == DT_BF16;
   // Two weight tiles and 4 tiles of 64 rows each.  Separate objects: reads of one are then known not to wait
   // for copies into the other.
   constexpr int STAGE = 2 * WTILE + 4 * MROWS * GROUP;
@@ -205,6 +203,8 @@ __global__ __launch_bounds__(SW * 64, 2) void fp8_linear_stream_kernel(LinearPar
                                                xoff[i] + (xoff[i] & 1) * up, kb * GROUP, 0, 0);
     }
 #else
+    (void)wbase;
+    (void)xbase;
     (void)dst;
     (void)kb;
 #endif
@@ -274,9 +274,8 @@ __global__ __launch_bounds__(SW * 64, 2) void fp8_linear_stream_kernel(LinearPar
 constexpr int FW = 8, FM = 2;             // most waves of a block, tiles of 16 rows
 constexpr int FEW_TILES = 1500, FEW_TILES_LONG = 3000;
 
-template <int OUT>
+template <int OUT, bool FAST>
 __global__ __launch_bounds__(FW * 64) void fp8_linear_few_kernel(LinearParams p) {
-  constexpr bool FAST = OUT != DT_F32;
   constexpr int NT = Run<OUT>::PER;
   __shared__ f4 part[FW - 1][NT][FM][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
@@ -344,7 +343,7 @@ __global__ __launch_bounds__(FW * 64) void fp8_linear_few_kernel(LinearParams p)
 
 namespace {
 
-template <int OUT>
+template <int OUT, bool FAST = OUT == DT_F16 || OUT == DT_BF16>
 int go(lf_context* ctx, const LinearParams& p) {
   const int nbs = (p.outputs + GROUP - 1) / GROUP, kbs = (p.inputs + GROUP - 1) / GROUP;
   const int cus = ctx->num_cus;
@@ -353,7 +352,7 @@ int go(lf_context* ctx, const LinearParams& p) {
     const long long mt = ((long long)p.rows + 16 * FM - 1) / (16 * FM), tiles = mt * ((p.outputs + 31) / 32);
     if (tiles <= (kbs <= RESIDENT_TILES ? FEW_TILES : FEW_TILES_LONG)) {
       const dim3 grid((p.outputs + 16 * Run<OUT>::PER - 1) / (16 * Run<OUT>::PER), (unsigned)mt);
-      hipLaunchKernelGGL((fp8_linear_few_kernel<OUT>), grid, dim3(std::min(kbs, FW) * 64), 0, ctx->stream, p);
+      hipLaunchKernelGGL((fp8_linear_few_kernel<OUT, FAST>), grid, dim3(std::min(kbs, FW) * 64), 0, ctx->stream, p);
       return check_hip(hipGetLastError(), "fp8 linear launch");
     }
   }
@@ -366,28 +365,28 @@ int go(lf_context* ctx, const LinearParams& p) {
     q.subsets = (nbs + q.per - 1) / q.per;
     // a unit for every SIMD before a second one: 2048 rows of 128 x 512 in 6.3 us, in blocks of 16 units 10
     q.blocks = (int)std::min<long long>((mt * q.per + 3) / 4, std::max(1, cus / q.subsets));
-    static const bool lds = hipFuncSetAttribute(reinterpret_cast<const void*>(&fp8_linear_resident_kernel<OUT>),
+    static const bool lds = hipFuncSetAttribute(reinterpret_cast<const void*>(&fp8_linear_resident_kernel<OUT, FAST>),
                                                 hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) == hipSuccess;
     if (!lds) return set_error(LF_ERR_DEVICE, "fp8 linear: the device refuses the LDS it needs");
     const size_t smem = (size_t)q.per * (kbs * WTILE + GROUP * 4 + kbs);
     const unsigned grid = (unsigned)((q.blocks * q.subsets + 7) / 8 * 8);
-    hipLaunchKernelGGL((fp8_linear_resident_kernel<OUT>), dim3(grid), dim3(RW * 64), smem, ctx->stream, p, q);
+    hipLaunchKernelGGL((fp8_linear_resident_kernel<OUT, FAST>), dim3(grid), dim3(RW * 64), smem, ctx->stream, p, q);
     return check_hip(hipGetLastError(), "fp8 linear launch");
   }
   const long long mt = ((long long)p.rows + MROWS - 1) / MROWS;
   q.subsets = (nbs + 1) / 2;
   q.blocks = (int)((mt + 3) / 4);
   const unsigned grid = (unsigned)(((long long)q.blocks + 31) / 32 * 32 * q.subsets);
-  hipLaunchKernelGGL((fp8_linear_stream_kernel<OUT>), dim3(grid), dim3(SW * 64), 0, ctx->stream, p, q);
+  hipLaunchKernelGGL((fp8_linear_stream_kernel<OUT, FAST>), dim3(grid), dim3(SW * 64), 0, ctx->stream, p, q);
   return check_hip(hipGetLastError(), "fp8 linear launch");
 }
 
 }  // namespace
 
-int run_fp8_linear(lf_context* ctx, const LinearParams& p, int out_dtype, const char* label) {
+int run_fp8_linear(lf_context* ctx, const LinearParams& p, int out_dtype, const char* label, bool fast) {
   LaunchScope ls(ctx, label);
   if (!p.out) return go<OUT_KEPT>(ctx, p);
-  if (out_dtype == LF_F32) return go<DT_F32>(ctx, p);
+  if (out_dtype == LF_F32) return fast ? go<DT_F32, true>(ctx, p) : go<DT_F32>(ctx, p);
   if (out_dtype == LF_F16) return go<DT_F16>(ctx, p);
   return go<DT_BF16>(ctx, p);
 }

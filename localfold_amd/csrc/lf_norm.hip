@@ -114,7 +114,7 @@ __global__ __launch_bounds__(256) void norm_kernel(NormParams p) {
 
 // Rows are dealt out to a fixed number of blocks, whose lanes add up their columns' ds and do in
 // registers; a block joins its teams in LDS and writes one row of partial sums.
-template <int ACT, int L, int NV>
+template <int ACT, int L, int NV, int DY>
 __global__ __launch_bounds__(256) void norm_grad_kernel(NormGradParams p) {
   typedef typename Act<ACT>::T T;
   constexpr int SLOTS = 256 / L;
@@ -133,7 +133,7 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(NormGradParams p) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c0 = (v * L + lr) * 8;
-      load8<ACT>(static_cast<const T*>(p.dy) + row * (size_t)C + c0, C - c0, dy[v]);
+      load8<DY>(static_cast<const typename Act<DY>::T*>(p.dy) + row * (size_t)C + c0, C - c0, dy[v]);
       if (p.x) {
         load8<ACT>(static_cast<const T*>(p.x) + row * (size_t)C + c0, C - c0, h[v]);
       } else {
@@ -301,7 +301,13 @@ struct GoNorm {
 template <int ACT, int L, int NV>
 struct GoNormGrad {
   static void go(const NormGradParams& p, dim3 grid, hipStream_t s) {
-    hipLaunchKernelGGL((norm_grad_kernel<ACT, L, NV>), grid, dim3(256), 0, s, p);
+    hipLaunchKernelGGL((norm_grad_kernel<ACT, L, NV, ACT>), grid, dim3(256), 0, s, p);
+  }
+};
+template <int ACT, int L, int NV>
+struct GoNormGradWide {     // from a gradient in f32
+  static void go(const NormGradParams& p, dim3 grid, hipStream_t s) {
+    hipLaunchKernelGGL((norm_grad_kernel<ACT, L, NV, DT_F32>), grid, dim3(256), 0, s, p);
   }
 };
 
@@ -332,7 +338,7 @@ size_t layer_norm_partials(int rows, int channels) {
   return (size_t)grad_blocks(rows, channels) * 2 * channels * sizeof(float);
 }
 
-int run_layer_norm_backward(lf_context* ctx, const lf_layer_norm_backward_args& a, void* scratch) {
+int run_layer_norm_backward(lf_context* ctx, const lf_layer_norm_backward_args& a, void* scratch, bool wide) {
   NormGradParams p{};
   p.dy = a.grad;
   p.x = a.act;
@@ -348,7 +354,9 @@ int run_layer_norm_backward(lf_context* ctx, const lf_layer_norm_backward_args& 
   const int blocks = grad_blocks(a.rows, a.channels);
   {
     LaunchScope ls(ctx, "layer_norm.backward");
-    by_type<GoNormGrad>(a.act_dtype, team_of(a.channels), p, dim3(blocks), ctx->stream);
+    const Team t = team_of(a.channels);
+    if (wide) by_type<GoNormGradWide>(a.act_dtype, t, p, dim3(blocks), ctx->stream);
+    else by_type<GoNormGrad>(a.act_dtype, t, p, dim3(blocks), ctx->stream);
   }
   LF_TRY(check_hip(hipGetLastError(), "layer_norm backward launch"));
   if (!a.grad_scale) return LF_OK;

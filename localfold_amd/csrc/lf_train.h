@@ -43,8 +43,10 @@ struct PackWeight {
 int run_pack_weights(lf_context* ctx, const PackWeight* w, int count);
 int run_layer_norm(lf_context* ctx, const lf_layer_norm_args& a);
 size_t layer_norm_partials(int rows, int channels);
-int run_layer_norm_backward(lf_context* ctx, const lf_layer_norm_backward_args& a, void* scratch);
-int run_fp8_linear(lf_context* ctx, const LinearParams& p, int out_dtype, const char* label);
+// wide: a.grad is f32, whatever act_dtype is.
+int run_layer_norm_backward(lf_context* ctx, const lf_layer_norm_backward_args& a, void* scratch, bool wide = false);
+// fast: f32 outputs by the 8-bit instruction too, for a caller whose results are of 16 bits.
+int run_fp8_linear(lf_context* ctx, const LinearParams& p, int out_dtype, const char* label, bool fast = false);
 size_t weight_grad_partials(int rows, int outputs, int inputs);
 // out = [a.cols, b.cols] = sum over rows of a^T b; bias = sum of a's rows, or of b's when bias_of_b
 int run_weight_grad(lf_context* ctx, const Kept& a, const Kept& b, void* out, void* bias, bool bias_of_b, int dt,
