@@ -109,8 +109,7 @@ __global__ __launch_bounds__(RW * 64) void fp8_linear_resident_kernel(LinearPara
   const long long units = ((long long)p.rows + 16 * RM - 1) / (16 * RM) * per;
   const int u0 = (int)(units * blk / q.blocks), u1 = (int)(units * (blk + 1) / q.blocks);
   const int i16 = n_of<OUT>(0, r);
-  const uint8_t* wl = fp8_smem + i16 * GROUP + ((g ^ key_of<OUT>(i16)) << 4);
-  const uint8_t* wlx = fp8_smem + i16 * GROUP + ((g ^ key_of<OUT>(i16) ^ 4) << 4);
+  const int wl = i16 * GROUP + ((g ^ key_of<OUT>(i16)) << 4);     // the other half of the columns: ^ 64
   f4 acc[8][RM];
   XFrag<RM> x;
   int u = u0 + wave, mt = u / per, nb = u % per;
@@ -133,16 +132,16 @@ __global__ __launch_bounds__(RW * 64) void fp8_linear_resident_kernel(LinearPara
     }
     const uint8_t* const ws = wscales + nb_now * kbs;
     const float* const bn = bias + nb_now * GROUP;
-    int at = nb_now * kbs * WTILE;
+    int at = nb_now * kbs * WTILE + wl;
     x_zero(x, p, 0);
-    mma<OUT, FAST, true, false>(acc, wl + at, wlx + at, x, ws[0], bn, g, [&]() __attribute__((always_inline)) {
+    mma<OUT, FAST, true, false>(acc, fp8_smem + at, fp8_smem + (at ^ 64), x, ws[0], bn, g, [&]() __attribute__((always_inline)) {
       x_load(x, p, (long long)(kbs == 1 ? mt : mt_now) * 16 * RM, kbs == 1 ? 0 : 1, r, g);
     });
     for (int kb = 1; kb < kbs; ++kb) {
       at += WTILE;
       const bool last = kb + 1 == kbs;
       x_zero(x, p, kb);
-      mma<OUT, FAST, false, false>(acc, wl + at, wlx + at, x, ws[kb], bn, g, [&]() __attribute__((always_inline)) {
+      mma<OUT, FAST, false, false>(acc, fp8_smem + at, fp8_smem + (at ^ 64), x, ws[kb], bn, g, [&]() __attribute__((always_inline)) {
         x_load(x, p, (long long)(last ? mt : mt_now) * 16 * RM, last ? 0 : kb + 1, r, g);
       });
     }

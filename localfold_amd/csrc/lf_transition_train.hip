@@ -421,7 +421,8 @@ __global__ __launch_bounds__(TW * 64, 2) void train_backward_kernel(TrainParams 
 namespace {
 
 int train_blocks(const lf_context* ctx, int rows) {
-  return (int)std::min<long long>(((long long)rows + TROWS * TW - 1) / (TROWS * TW), ctx->num_cus);
+  // a tile for every SIMD before a second one
+  return (int)std::min<long long>(((long long)rows + TROWS * 4 - 1) / (TROWS * 4), ctx->num_cus);
 }
 
 template <int ACT, int C>

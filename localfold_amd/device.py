@@ -1007,6 +1007,9 @@ def _transition_args(ctx: Context, a, x: torch.Tensor, out: torch.Tensor, wstruc
     a.rows, a.channels, a.hidden, a.act_dtype = rows, c, saved.hidden_size, act_code(x)
     a.out = _tensor(ctx, "out", out, x.shape, x.dtype)
     a.accumulate = int(accumulate)
+    for name, t in wstruct._owner.items():
+        if t is not None and t.device != ctx.device:
+            raise ValueError(f"{name} is on {t.device}; the context is on {ctx.device}")
     a.w, a.saved = C.pointer(wstruct), C.pointer(saved.struct)
     _scratch(ctx, a, scratch)
 

@@ -118,6 +118,26 @@ def test_checkpoint_layout_is_checked():
         D.Fp8Weight(130, 70, torch.zeros(130, 128, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.uint8))
 
 
+def test_struct_layouts(tmp_path):
+    """sizeof of the training structs in C and in Python."""
+    import ctypes as C
+    import os
+    import subprocess
+    from localfold_amd import capi
+    names = [n for n in dir(capi) if n.startswith(("lf_checkpoint", "lf_layer_norm", "lf_fp8", "lf_transition_saved",
+                                                   "lf_transition_train", "lf_transition_backward"))
+             and isinstance(getattr(capi, n), type) and issubclass(getattr(capi, n), C.Structure)]
+    assert len(names) >= 10
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include "localfold.h"\nint main(void) {\n' + "".join(
+        f'printf("{n} %zu\\n", sizeof({n}));\n' for n in names) + "return 0;}\n")
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["gcc", "-I", include, str(src), "-o", str(tmp_path / "sizes")], check=True)
+    for line in subprocess.run([str(tmp_path / "sizes")], check=True, capture_output=True, text=True).stdout.splitlines():
+        n, size = line.split()
+        assert C.sizeof(getattr(capi, n)) == int(size), n
+
+
 def test_scratch_sizes_need_no_device():
     from localfold_amd import capi
     lib = capi.load()
@@ -528,6 +548,27 @@ def test_weight_grad(ctx, rows, n, k):
         assert torch.equal(out, alone)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,k", [(5, 130, 70), (97, 64, 128), (1001, 200, 40), (16500, 128, 256)])
+def test_weight_grad_garbage_behind_the_rows(ctx, rows, n, k):
+    """Scales behind the last row may hold anything, and a NaN stays in its own output."""
+    from localfold_amd import device as D
+    rng = np.random.default_rng(rows)
+    g, x = rng.normal(size=(rows, n)), rng.normal(size=(rows, k)) * 10.0 ** rng.integers(-6, 6, size=(rows, 1))
+    g[rows - 1, n - 1] = np.nan
+    g8, x8 = (D.checkpoint_pack(ctx, torch.as_tensor(t).float().to(ctx.device)) for t in (g, x))
+    for t in (g8, x8):
+        t.scales[:, rows:] = 255
+    bias = torch.empty(n, device=ctx.device)
+    out = f64(D.fp8_weight_grad(ctx, g8, x8, bias_out=bias))
+    db = f64(bias)
+    gv, xv = values_of(g8), values_of(x8)
+    assert np.isnan(out[n - 1]).all() and np.isnan(db[n - 1])
+    depth = 32 + min(rows / 32, 1024) + min(rows / 32, 80)
+    close(out[:n - 1], (gv.T @ xv)[:n - 1], depth * 2 * U * (np.abs(gv).T @ np.abs(xv))[:n - 1], torch.float32, "dw")
+    close(db[:n - 1], gv.sum(0)[:n - 1], depth * 2 * U * np.abs(gv).sum(0)[:n - 1], torch.float32, "db")
+
+
 def transition_case(ctx, rng, c, h, dt, bias=True):
     w = {"layerNormScale": vec(rng, ctx, c, 0.2, 1.0), "layerNormOffset": vec(rng, ctx, c, 0.1),
          "firstWeight": torch.as_tensor(rng.normal(size=(c, h)) / math.sqrt(c)).to(dt).to(ctx.device),
@@ -537,13 +578,7 @@ def transition_case(ctx, rng, c, h, dt, bias=True):
     return w
 
 
-@pytest.mark.gpu
-@pytest.mark.parametrize("rows,c,h,dt,wdt,residual,fast", [
-    (1, 128, 512, torch.float32, torch.float32, True, False), (37, 64, 256, torch.float16, torch.float32, True, True),
-    (300, 128, 512, torch.bfloat16, torch.bfloat16, True, False), (150, 256, 1024, torch.float32, torch.float16, False, False),
-    (90, 384, 100, torch.bfloat16, torch.float32, False, True), (45, 22, 70, torch.float32, torch.float32, True, False),
-    (600, 49, 130, torch.float16, torch.bfloat16, False, False)])
-def test_transition_step(ctx, rows, c, h, dt, wdt, residual, fast):
+def transition_step(ctx, rows, c, h, dt, wdt, residual, fast, shift=0):
     """The training step stage by stage: each stage's float64 form from what the stage before it kept,
     so that a code that falls the other way is no difference."""
     from localfold_amd import device as D
@@ -551,8 +586,11 @@ def test_transition_step(ctx, rows, c, h, dt, wdt, residual, fast):
     w = transition_case(ctx, rng, c, h, wdt, bias=rows != 45)
     ws, saved = D.transition_train_weights(w), D.transition_saved(rows, c, h, ctx.device)
     x, grad = rows_of(rng, rows, c, dt, 0.3).to(ctx.device), (rows_of(rng, rows, c, dt) * 0.01).to(dt).to(ctx.device)
-    out = D.transition_train(ctx, x, ws, saved, accumulate=residual, fast_variance=fast)
-    dx, grads = D.transition_backward(ctx, grad, ws, saved, accumulate=residual)
+    out, dx = torch.empty_like(x), torch.empty_like(grad)
+    if shift:       # everything that many elements behind an aligned address
+        x, grad, out, dx = (torch.cat([t.new_zeros(shift), t.flatten()])[shift:].view(rows, c) for t in (x, grad, out, dx))
+    D.transition_train(ctx, x, ws, saved, out=out, accumulate=residual, fast_variance=fast)
+    _, grads = D.transition_backward(ctx, grad, ws, saved, out=dx, accumulate=residual)
     torch.cuda.synchronize()
     x64, g64 = f64(x), f64(grad)
     zero = {"firstBias": np.zeros(h), "secondBias": np.zeros(c)}
@@ -596,6 +634,34 @@ def test_transition_step(ctx, rows, c, h, dt, wdt, residual, fast):
     close(dx, want, slack + 1e-5 * np.abs(want), dt, "dx")
     close(grads["layerNormScale"], ds, (slack_y * np.abs(hh)).sum(0) + 1e-5 * np.abs(dy * hh).sum(0), torch.float32, "ds")
     close(grads["layerNormOffset"], do, slack_y.sum(0) + 1e-5 * np.abs(dy).sum(0), torch.float32, "do")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,c,h,dt,wdt,residual,fast", [
+    (1, 128, 512, torch.float32, torch.float32, True, False), (37, 64, 256, torch.float16, torch.float32, True, True),
+    (300, 128, 512, torch.bfloat16, torch.bfloat16, True, False), (150, 256, 1024, torch.float32, torch.float16, False, False),
+    (90, 384, 100, torch.bfloat16, torch.float32, False, True), (45, 22, 70, torch.float32, torch.float32, True, False),
+    (600, 49, 130, torch.float16, torch.bfloat16, False, False)])
+def test_transition_step(ctx, rows, c, h, dt, wdt, residual, fast):
+    transition_step(ctx, rows, c, h, dt, wdt, residual, fast)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,c,h,dt,wdt,residual,fast", [
+    (33, 64, 128, torch.bfloat16, torch.float32, True, False), (31, 128, 128, torch.float16, torch.float16, False, True),
+    (257, 64, 512, torch.float32, torch.float32, False, False), (1000, 128, 384, torch.float32, torch.bfloat16, True, True),
+    (66001, 64, 128, torch.bfloat16, torch.float32, True, False)])
+def test_transition_step_fused(ctx, rows, c, h, dt, wdt, residual, fast):
+    """Widths that run as one kernel a direction: tails, more tiles of rows than waves."""
+    transition_step(ctx, rows, c, h, dt, wdt, residual, fast)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,c,h,dt,shift", [(70, 128, 256, torch.bfloat16, 1), (70, 64, 128, torch.float16, 4),
+                                               (70, 128, 128, torch.float32, 1), (131, 64, 640, torch.bfloat16, 0)])
+def test_transition_step_composed(ctx, rows, c, h, dt, shift):
+    """The same widths where the fused kernels do not apply: activations off a 16-byte address, wide hidden layers."""
+    transition_step(ctx, rows, c, h, dt, torch.float32, True, False, shift)
 
 
 @pytest.mark.gpu
