@@ -16,8 +16,16 @@ constexpr long long MOST_ELEMENTS = 1LL << 34;   // of one matrix: launches coun
 
 bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+// What an error names, put together only where there is one.
+struct Name {
+  const char *fn, *argument;
+  std::string operator+(const std::string& rest) const {
+    return argument ? std::string(fn) + ": " + argument + rest : fn + rest;
+  }
+};
+
 int check_shape(const char* fn, long long rows, long long cols, long long most_cols) {
-  const std::string f(fn);
+  const Name f{fn, nullptr};
   LF_REQUIRE(rows > 0 && cols > 0, f + ": dimensions must be positive");
   LF_REQUIRE(cols <= most_cols, f + ": rows are at most " + std::to_string(most_cols) + " wide");
   LF_REQUIRE(rows * (long long)LF_CHECKPOINT_PITCH(cols) <= MOST_ELEMENTS, f + ": more than 2^34 elements");
@@ -25,14 +33,14 @@ int check_shape(const char* fn, long long rows, long long cols, long long most_c
 }
 
 int check_act(const char* fn, const char* name, const void* p, int dt) {
-  const std::string f(fn);
+  const Name f{fn, nullptr};
   LF_REQUIRE(act_dtype_ok(dt), f + ": dtypes are f32, f16 or bf16");
   LF_REQUIRE(aligned(p, act_bytes(dt)), f + ": " + name + " is not aligned to its type");
   return LF_OK;
 }
 
 int check_kept(const char* fn, const char* name, const lf_checkpoint& c, long long rows, long long cols) {
-  const std::string f = std::string(fn) + ": " + name;
+  const Name f{fn, name};
   LF_REQUIRE(c.codes && c.scales, f + " has NULL codes or scales");
   LF_REQUIRE(aligned(c.codes, 16) && aligned(c.scales, 16), f + " is not 16-byte aligned");
   LF_REQUIRE(c.rows == rows && c.cols == cols, f + " is " + std::to_string(c.rows) + " x " + std::to_string(c.cols) +
@@ -41,14 +49,14 @@ int check_kept(const char* fn, const char* name, const lf_checkpoint& c, long lo
 }
 
 int check_vec(const char* fn, const char* name, const void* p, bool optional = false) {
-  const std::string f(fn);
+  const Name f{fn, nullptr};
   LF_REQUIRE(p || optional, f + ": " + name + " is NULL");
   LF_REQUIRE(aligned(p, 4), f + ": " + name + " is not aligned to its type");
   return LF_OK;
 }
 
 int check_weight(const char* fn, const char* name, const lf_weight& w) {
-  const std::string f = std::string(fn) + ": " + name;
+  const Name f{fn, name};
   LF_REQUIRE(w.data, f + " is NULL");
   LF_REQUIRE(w.layout == LF_IN_OUT || w.layout == LF_OUT_IN, f + ": bad layout");
   if (w.dtype == LF_INT8 || w.dtype == LF_INT5)
@@ -62,7 +70,7 @@ int check_weight(const char* fn, const char* name, const lf_weight& w) {
 // Scratch of a call: the caller's, or the context's workspace.  The workspace moves when a later call
 // grows it, which a captured graph would not see.
 int take_scratch(lf_context* ctx, const char* fn, void* given, size_t given_bytes, size_t need, void** out) {
-  const std::string f(fn);
+  const Name f{fn, nullptr};
   if (given) {
     LF_REQUIRE(given_bytes >= need, f + ": scratch has " + std::to_string(given_bytes) + " bytes; needs " + std::to_string(need));
     LF_REQUIRE(aligned(given, 16), f + ": scratch is not 16-byte aligned");
@@ -78,7 +86,7 @@ int take_scratch(lf_context* ctx, const char* fn, void* given, size_t given_byte
 // ---- single operators ------------------------------------------------------------------------
 
 int checkpoint_args(const char* fn, const lf_checkpoint_args& a) {
-  const std::string f(fn);
+  const Name f{fn, nullptr};
   LF_REQUIRE(a.kept && a.act, f + ": NULL activations or checkpoint");
   LF_TRY(check_shape(fn, a.kept->rows, a.kept->cols, MOST_COLS));
   LF_TRY(check_kept(fn, "kept", *a.kept, a.kept->rows, a.kept->cols));
@@ -252,7 +260,7 @@ size_t backward_bytes(int rows, int c, int h) {
 }
 
 int check_transition(const char* fn, int rows, int c, int h, const lf_transition_weights* w, const lf_transition_saved* s) {
-  const std::string f(fn);
+  const Name f{fn, nullptr};
   LF_TRY(check_shape(fn, rows, c, MOST_CHANNELS));
   LF_TRY(check_shape(fn, rows, h, MOST_COLS));
   LF_REQUIRE(w, f + ": weights are NULL");

@@ -748,9 +748,9 @@ def _tensor(ctx: Context, name: str, t: torch.Tensor, shape=None, dtype=None) ->
         raise ValueError(f"{name} is on {t.device}; the context is on {ctx.device}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous, got strides {t.stride()}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}; expected {tuple(shape)}")
-    if dtype is not None and t.dtype != dtype:
+    if dtype is not None and t.dtype is not dtype:
         raise TypeError(f"{name} is {t.dtype}; expected {dtype}")
     return t.data_ptr()
 
@@ -762,9 +762,10 @@ def _scratch(ctx: Context, a, scratch: torch.Tensor):
 
 
 def _rows(t: torch.Tensor):
-    if t.dim() < 1 or t.shape[-1] == 0:
-        raise ValueError(f"activations need a last dimension, got shape {tuple(t.shape)}")
-    return t.numel() // t.shape[-1], t.shape[-1]
+    shape = t.shape
+    if len(shape) < 1 or shape[-1] == 0:
+        raise ValueError(f"activations need a last dimension, got shape {tuple(shape)}")
+    return t.numel() // shape[-1], shape[-1]
 
 
 class Checkpoint:
@@ -776,15 +777,18 @@ class Checkpoint:
         for name, t, shape in (("codes", codes, want[0]), ("scales", scales, want[1])):
             if tuple(t.shape) != shape or t.dtype != torch.uint8 or not t.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous uint8 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
-        self.rows, self.cols, self.codes, self.scales = rows, cols, codes, scales
+        if codes.device != scales.device:
+            raise ValueError(f"codes are on {codes.device}, scales on {scales.device}")
+        self.rows, self.cols, self.codes, self.scales, self.device = rows, cols, codes, scales, codes.device
         self.struct = capi.lf_checkpoint(rows, cols, codes.data_ptr(), scales.data_ptr())
+        self._pointer = C.pointer(self.struct)
 
     def _ref(self, ctx: Context, name: str, shape=None):
-        if self.codes.device != ctx.device or self.scales.device != ctx.device:
-            raise ValueError(f"{name} is on {self.codes.device}; the context is on {ctx.device}")
-        if shape is not None and (self.rows, self.cols) != tuple(shape):
+        if self.device != ctx.device:
+            raise ValueError(f"{name} is on {self.device}; the context is on {ctx.device}")
+        if shape is not None and (self.rows, self.cols) != shape:
             raise ValueError(f"{name} is {self.rows} x {self.cols}; expected {shape[0]} x {shape[1]}")
-        return C.pointer(self.struct)
+        return self._pointer
 
 
 def checkpoint_empty(rows: int, cols: int, device) -> Checkpoint:
@@ -823,12 +827,9 @@ def layer_norm(ctx: Context, x: torch.Tensor, scale: torch.Tensor, offset: torch
     rows, c = _rows(x)
     if out is None and x_saved is None and y_saved is None:
         out = torch.empty_like(x)
-    a = capi.lf_layer_norm_args()
-    a.rows, a.channels, a.act_dtype, a.act = rows, c, act_code(x), _tensor(ctx, "x", x)
-    a.scale = _tensor(ctx, "scale", scale, (c,), torch.float32)
-    a.offset = _tensor(ctx, "offset", offset, (c,), torch.float32)
-    a.epsilon, a.fast_variance = epsilon, int(fast_variance)
-    a.out = _tensor(ctx, "out", out, x.shape, x.dtype)
+    a = capi.lf_layer_norm_args(rows, c, act_code(x), _tensor(ctx, "x", x), _tensor(ctx, "scale", scale, (c,), torch.float32),
+                                _tensor(ctx, "offset", offset, (c,), torch.float32), epsilon, int(fast_variance),
+                                _tensor(ctx, "out", out, x.shape, x.dtype))
     if stats is not None:
         a.mean = _tensor(ctx, "stats", stats, (2, rows), torch.float32)
         a.rstd = a.mean + 4 * rows
@@ -880,13 +881,16 @@ class Fp8Weight:
         for name, t, shape in (("codes", codes, want[0]), ("scales", scales, want[1])):
             if tuple(t.shape) != shape or t.dtype != torch.uint8 or not t.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous uint8 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
-        self.outputs, self.inputs, self.codes, self.scales = outputs, inputs, codes, scales
+        if codes.device != scales.device:
+            raise ValueError(f"codes are on {codes.device}, scales on {scales.device}")
+        self.outputs, self.inputs, self.codes, self.scales, self.device = outputs, inputs, codes, scales, codes.device
         self.struct = capi.lf_fp8_weight(outputs, inputs, codes.data_ptr(), scales.data_ptr())
+        self._pointer = C.pointer(self.struct)
 
     def _ref(self, ctx: Context, name: str):
-        if self.codes.device != ctx.device or self.scales.device != ctx.device:
-            raise ValueError(f"{name} is on {self.codes.device}; the context is on {ctx.device}")
-        return C.pointer(self.struct)
+        if self.device != ctx.device:
+            raise ValueError(f"{name} is on {self.device}; the context is on {ctx.device}")
+        return self._pointer
 
 
 def _live_weight(name: str, t: torch.Tensor, layout: int) -> capi.lf_weight:
@@ -919,10 +923,8 @@ def fp8_linear(ctx: Context, x: Checkpoint, w: Fp8Weight, bias: torch.Tensor = N
     kept output of a ReLU, whose gradient this is; `residual` is added last and may be `out`."""
     if out is None:
         out = torch.empty((x.rows, w.outputs), dtype=dtype, device=ctx.device)
-    a = capi.lf_fp8_linear_args()
-    a.act, a.w = x._ref(ctx, "x", (x.rows, w.inputs)), w._ref(ctx, "w")
-    a.bias = _tensor(ctx, "bias", bias, (w.outputs,), torch.float32)
-    a.relu = int(relu)
+    a = capi.lf_fp8_linear_args(x._ref(ctx, "x", (x.rows, w.inputs)), w._ref(ctx, "w"),
+                                _tensor(ctx, "bias", bias, (w.outputs,), torch.float32), int(relu))
     if relu_of is not None:
         a.relu_of = relu_of._ref(ctx, "relu_of", (x.rows, w.outputs))
     if isinstance(out, Checkpoint):
