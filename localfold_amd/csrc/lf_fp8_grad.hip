@@ -32,6 +32,13 @@ struct GradParams {
   int dt, swapped;                        // out is [b.cols][a.cols]
 };
 
+// Products of the same rows that share a launch, blocks dealt out in order.
+struct GradBatch {
+  GradParams w[2];
+  unsigned first[2];                      // of the products' blocks
+  unsigned join[2];                       // of the blocks that join them
+};
+
 constexpr int PITCH = GN * 2 + 32;        // LDS bytes of a row of bf16: 4 rows apart by 32 bytes mod 128
 constexpr int BUF = 2 * GSTEP * PITCH;    // one team's buffer: rows of a, then of b
 constexpr size_t GRAD_SMEM = TEAMS * 2 * BUF;
@@ -63,11 +70,13 @@ __device__ __forceinline__ b8 tr_frag(const uint8_t* p) {
   return o;
 }
 
-// SUM: 0 no column sums, 1 of a, 2 of b.
-template <int SUM>
-__global__ __launch_bounds__(GWAVES * 64) void weight_grad_kernel(GradParams p) {
+template <bool SUMS>
+__global__ __launch_bounds__(GWAVES * 64) void weight_grad_kernel(GradBatch batch) {
   extern __shared__ __attribute__((aligned(16))) uint8_t grad_smem[];
-  const int slot = blockIdx.x >> 3, tile = slot % p.tiles, split = slot / p.tiles * 8 + (blockIdx.x & 7);
+  const int op = blockIdx.x >= batch.first[1] ? 1 : 0;
+  const GradParams& p = batch.w[op];
+  const unsigned block = blockIdx.x - batch.first[op];
+  const int slot = block >> 3, tile = slot % p.tiles, split = slot / p.tiles * 8 + (block & 7);
   if (split >= p.splits) return;
   const int i0 = tile / p.tiles_j * GN, j0 = tile % p.tiles_j * GN;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -121,11 +130,12 @@ __global__ __launch_bounds__(GWAVES * 64) void weight_grad_kernel(GradParams p) 
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
   sums[0] = sums[1] = f4{0.f, 0.f, 0.f, 0.f};
-  const bool sum = SUM == 1 ? j0 == 0 : SUM == 2 ? i0 == 0 : false;   // blocks at the other operand's first tile
+  const int of = SUMS ? p.sum_of : 0;
+  const bool sum_a = of == 1 && j0 == 0, sum_b = of == 2 && i0 == 0;     // blocks at the other operand's first tile
   b8 ones;
 #pragma unroll
   for (int k = 0; k < 8; ++k) ones[k] = (__bf16)1.0f;
-  const int xi = SUM == 1 ? wj : 0, xj = SUM == 2 ? wi : 0;
+  const int xi = of == 1 ? wj : 0, xj = of == 2 ? wi : 0;
   const int g = lane >> 4, l16 = lane & 15;
   const uint8_t* const from = mine + (4 * g + (l16 >> 2)) * PITCH;
   const uint8_t* const from_a = from + wi * 128 + ((l16 & 3) * 8 ^ wi * 16) + xi * 32;
@@ -157,11 +167,14 @@ __global__ __launch_bounds__(GWAVES * 64) void weight_grad_kernel(GradParams p) 
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (sum) {
+    if constexpr (SUMS) {
+      if (sum_a) {
 #pragma unroll
-      for (int f = 0; f < 2; ++f)
-        sums[f] = SUM == 1 ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[2 * f], ones, sums[f], 0, 0, 0)
-                           : __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fb[2 * f], sums[f], 0, 0, 0);
+        for (int f = 0; f < 2; ++f) sums[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[2 * f], ones, sums[f], 0, 0, 0);
+      } else if (sum_b) {
+#pragma unroll
+        for (int f = 0; f < 2; ++f) sums[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fb[2 * f], sums[f], 0, 0, 0);
+      }
     }
   }
 
@@ -183,7 +196,7 @@ __global__ __launch_bounds__(GWAVES * 64) void weight_grad_kernel(GradParams p) 
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] += at[(i * 4 + j) * 256];
     }
-    if (sum) {     // uniform in the block
+    if (SUMS && (sum_a || sum_b)) {     // uniform in the block
       __syncthreads();
       if (team >= to && team < 2 * to) {
         at[0] = sums[0];
@@ -211,15 +224,15 @@ __global__ __launch_bounds__(GWAVES * 64) void weight_grad_kernel(GradParams p) 
           else store_act(p.out, p.dt, p.swapped ? (size_t)cj * ca + ci + k : (size_t)(ci + k) * cb + cj, acc[i][j][k]);
         }
     }
-  if (!sum) return;
+  if (!sum_a && !sum_b) return;
   // of a: lane group g has columns 4g .. 4g + 3 of a fragment, in every lane; of b: lane l16 column l16
-  const int cn = SUM == 1 ? ca : cb;
+  const int cn = sum_a ? ca : cb;
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int k = 0; k < (SUM == 1 ? 4 : 1); ++k) {
-      const int c = SUM == 1 ? i0 + wi * 64 + (2 * h + xi) * 16 + 4 * g + k : j0 + wj * 64 + (2 * h + xj) * 16 + l16;
-      if ((SUM == 1 ? l16 : g) == 0 && c < cn) {
+    for (int k = 0; k < 4; ++k) {
+      const int c = sum_a ? i0 + wi * 64 + (2 * h + xi) * 16 + 4 * g + k : j0 + wj * 64 + (2 * h + xj) * 16 + l16;
+      if ((sum_a ? l16 == 0 : g == 0 && k == 0) && c < cn) {
         if (part) p.colsum[(size_t)split * cn + c] = sums[h][k];
         else store_act(p.bias, p.dt, c, sums[h][k]);
       }
@@ -227,12 +240,17 @@ __global__ __launch_bounds__(GWAVES * 64) void weight_grad_kernel(GradParams p) 
 }
 
 // Partial sums added in order: 64 outputs a block, 16 runs of the splits at a time.
-__global__ __launch_bounds__(256) void weight_grad_join_kernel(GradParams p, long long n, int cn) {
+__global__ __launch_bounds__(256) void weight_grad_join_kernel(GradBatch batch) {
+  const int op = blockIdx.x >= batch.join[1] ? 1 : 0;
+  const GradParams& p = batch.w[op];
+  const unsigned block = blockIdx.x - batch.join[op];
+  const long long n = (long long)p.a.cols * p.b.cols;
+  const int cn = p.sum_of == 1 ? p.a.cols : p.b.cols;     // blocks for it are there only if it is summed
   __shared__ f4 sm[16][16];
   const int c = threadIdx.x & 15, run = threadIdx.x >> 4;
   const long long blocks_n = (n + 63) / 64;
-  const bool main = blockIdx.x < blocks_n;
-  const long long len = main ? n : cn, i = ((long long)blockIdx.x - (main ? 0 : blocks_n)) * 64 + c * 4;
+  const bool main = block < blocks_n;
+  const long long len = main ? n : cn, i = ((long long)block - (main ? 0 : blocks_n)) * 64 + c * 4;
   const float* src = main ? p.partial : p.colsum;
   const int per = (p.splits + 15) / 16, s0 = run * per, s1 = min(p.splits, s0 + per);
   f4 t = {0.f, 0.f, 0.f, 0.f};
@@ -264,65 +282,85 @@ struct GradPlan {
   int tiles, tiles_j, splits;
   long long rows_per;
 };
-GradPlan grad_plan(long long rows, int ci, int cj) {
+int tiles_of(int n, int k) { return (n + GN - 1) / GN * ((k + GN - 1) / GN); }
+// A block a CU, over all products of the launch.
+GradPlan grad_plan(long long rows, int ci, int cj, int all_tiles) {
   GradPlan q{};
   q.tiles_j = (cj + GN - 1) / GN;
-  q.tiles = (ci + GN - 1) / GN * q.tiles_j;
-  const long long want = std::max<long long>(1, 256 / q.tiles);      // a block a CU
+  q.tiles = tiles_of(ci, cj);
+  const long long want = std::max<long long>(1, 256 / all_tiles);
   const long long turns = (rows + TEAMS * GSTEP - 1) / (TEAMS * GSTEP);
   q.rows_per = (turns + want - 1) / want * (TEAMS * GSTEP);
   q.splits = (int)((rows + q.rows_per - 1) / q.rows_per);
   return q;
 }
 
-template <int SUM>
-int go(lf_context* ctx, const GradParams& p) {
-  static const bool lds = hipFuncSetAttribute(reinterpret_cast<const void*>(&weight_grad_kernel<SUM>),
+template <bool SUMS>
+int go(lf_context* ctx, const GradBatch& b, unsigned grid) {
+  static const bool lds = hipFuncSetAttribute(reinterpret_cast<const void*>(&weight_grad_kernel<SUMS>),
                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)GRAD_SMEM) == hipSuccess;
   if (!lds) return set_error(LF_ERR_DEVICE, "weight gradient: the device refuses the LDS it needs");
-  const unsigned grid = (unsigned)((p.splits + 7) / 8 * p.tiles * 8);
-  hipLaunchKernelGGL((weight_grad_kernel<SUM>), dim3(grid), dim3(GWAVES * 64), GRAD_SMEM, ctx->stream, p);
+  hipLaunchKernelGGL((weight_grad_kernel<SUMS>), dim3(grid), dim3(GWAVES * 64), GRAD_SMEM, ctx->stream, b);
   return check_hip(hipGetLastError(), "weight gradient launch");
 }
 
 size_t up16(size_t n) { return (n + 15) & ~size_t(15); }
 
-}  // namespace
-
-size_t weight_grad_partials(int rows, int outputs, int inputs) {
-  const GradPlan q = grad_plan(rows, std::max(outputs, inputs), std::min(outputs, inputs));
-  return up16((size_t)q.splits * outputs * inputs * sizeof(float)) + (size_t)q.splits * std::max(outputs, inputs) * sizeof(float);
+size_t partial_bytes(int rows, int outputs, int inputs, int all_tiles) {
+  const GradPlan q = grad_plan(rows, std::max(outputs, inputs), std::min(outputs, inputs), all_tiles);
+  return up16((size_t)q.splits * outputs * inputs * sizeof(float)) +
+         up16((size_t)q.splits * std::max(outputs, inputs) * sizeof(float));
 }
 
-int run_weight_grad(lf_context* ctx, const Kept& a, const Kept& b, void* out, void* bias, bool bias_of_b, int dt,
-                    void* scratch, const char* label) {
-  GradParams p{};
-  p.swapped = a.cols < b.cols;
-  p.a = p.swapped ? b : a;
-  p.b = p.swapped ? a : b;
-  const GradPlan q = grad_plan(a.rows, p.a.cols, p.b.cols);
-  const long long n = (long long)a.cols * b.cols;
-  p.sum_of = !bias ? 0 : bias_of_b == (p.swapped != 0) ? 1 : 2;
-  p.splits = q.splits;
-  p.tiles = q.tiles;
-  p.tiles_j = q.tiles_j;
-  p.rows_per = q.rows_per;
-  p.out = out;
-  p.bias = bias;
-  p.dt = dt;
-  if (q.splits > 1) {
-    p.partial = static_cast<float*>(scratch);
-    p.colsum = reinterpret_cast<float*>(static_cast<char*>(scratch) + up16((size_t)q.splits * n * sizeof(float)));
+}  // namespace
+
+size_t weight_grad_partials(int rows, int outputs, int inputs, int products) {
+  return products * partial_bytes(rows, outputs, inputs, products * tiles_of(outputs, inputs));
+}
+
+int run_weight_grads(lf_context* ctx, const WeightGrad* w, int count, int dt, void* scratch, const char* label) {
+  GradBatch batch{};
+  int all = 0;
+  for (int k = 0; k < count; ++k) all += tiles_of(w[k].a.cols, w[k].b.cols);
+  unsigned grid = 0, joins = 0;
+  bool sums = false;
+  char* at = static_cast<char*>(scratch);
+  for (int k = 0; k < 2; ++k) {
+    batch.first[k] = grid;
+    batch.join[k] = joins;
+    if (k >= count) break;
+    GradParams& p = batch.w[k];
+    p.swapped = w[k].a.cols < w[k].b.cols;
+    p.a = p.swapped ? w[k].b : w[k].a;
+    p.b = p.swapped ? w[k].a : w[k].b;
+    const GradPlan q = grad_plan(p.a.rows, p.a.cols, p.b.cols, all);
+    p.sum_of = !w[k].bias ? 0 : w[k].bias_of_b == (p.swapped != 0) ? 1 : 2;
+    p.splits = q.splits;
+    p.tiles = q.tiles;
+    p.tiles_j = q.tiles_j;
+    p.rows_per = q.rows_per;
+    p.out = w[k].out;
+    p.bias = w[k].bias;
+    p.dt = dt;
+    sums = sums || p.sum_of != 0;
+    grid += (unsigned)((q.splits + 7) / 8 * q.tiles * 8);
+    if (q.splits == 1) continue;
+    const size_t n = (size_t)p.a.cols * p.b.cols;
+    const int cn = p.sum_of == 0 ? 0 : p.sum_of == 1 ? p.a.cols : p.b.cols;
+    p.partial = reinterpret_cast<float*>(at);
+    at += up16(q.splits * n * sizeof(float));
+    p.colsum = reinterpret_cast<float*>(at);
+    at += up16((size_t)q.splits * cn * sizeof(float));
+    joins += (unsigned)((n + 63) / 64 + (cn + 63) / 64);
   }
+  if (count == 1) batch.first[1] = batch.join[1] = ~0u;
   {
     LaunchScope ls(ctx, label);
-    LF_TRY(p.sum_of == 0 ? go<0>(ctx, p) : p.sum_of == 1 ? go<1>(ctx, p) : go<2>(ctx, p));
+    LF_TRY(sums ? go<true>(ctx, batch, grid) : go<false>(ctx, batch, grid));
   }
-  if (q.splits == 1) return LF_OK;
-  const int cn = p.sum_of == 0 ? 0 : p.sum_of == 1 ? p.a.cols : p.b.cols;
+  if (joins == 0) return LF_OK;
   LaunchScope ls(ctx, "fp8.weight_grad_join");
-  hipLaunchKernelGGL(weight_grad_join_kernel, dim3((unsigned)((n + 63) / 64 + (cn + 63) / 64)), dim3(256), 0, ctx->stream, p,
-                     n, cn);
+  hipLaunchKernelGGL(weight_grad_join_kernel, dim3(joins), dim3(256), 0, ctx->stream, batch);
   return check_hip(hipGetLastError(), "weight gradient join launch");
 }
 

@@ -215,8 +215,8 @@ int fp8_weight_grad(lf_context* ctx, const lf_fp8_weight_grad_args& a) {
   LF_TRY(take_scratch(ctx, fn, a.scratch, a.scratch_bytes, weight_grad_partials(a.grad->rows, a.grad->cols, a.act->cols),
                       &scratch));
   const bool in_out = a.layout == LF_IN_OUT;
-  return run_weight_grad(ctx, kept_view(in_out ? *a.act : *a.grad), kept_view(in_out ? *a.grad : *a.act), a.out, a.bias,
-                         in_out, a.grad_dtype, scratch, "fp8.weight_grad");
+  const WeightGrad w{kept_view(in_out ? *a.act : *a.grad), kept_view(in_out ? *a.grad : *a.act), a.out, a.bias, in_out};
+  return run_weight_grads(ctx, &w, 1, a.grad_dtype, scratch, "fp8.weight_grad");
 }
 
 // ---- the transition's training step ------------------------------------------------------------
@@ -253,8 +253,7 @@ struct Carve {
 
 size_t train_bytes(int, int c, int h) { return packed_bytes(h, c) + packed_bytes(c, h); }
 size_t backward_bytes(int rows, int c, int h) {
-  const size_t partials = std::max(std::max(weight_grad_partials(rows, c, h), weight_grad_partials(rows, h, c)),
-                                   std::max(layer_norm_partials(rows, c), train_partials(c)));
+  const size_t partials = std::max(weight_grad_partials(rows, h, c, 2), std::max(layer_norm_partials(rows, c), train_partials(c)));
   return packed_bytes(h, c) + packed_bytes(c, h) + kept_bytes(rows, c) + kept_bytes(rows, h) +
          up((size_t)rows * c * 4) + up(partials);
 }
@@ -357,24 +356,22 @@ int transition_backward(lf_context* ctx, const lf_transition_backward_args& a) {
   const PackWeight packs[2] = {pack_of(w.w2, true, w2.codes, w2.scales), pack_of(w.w1, true, w1.codes, w1.scales)};
   LF_TRY(run_pack_weights(ctx, packs, 2));
   const bool t2 = w.w2.layout == LF_IN_OUT, t1 = w.w1.layout == LF_IN_OUT;
+  // half the blocks each: half the partial sums of two launches, and one start and end
+  const WeightGrad grads[2] = {
+      {kept_view(t2 ? s.hidden : d), kept_view(t2 ? d : s.hidden), a.grad_w2, a.grad_b2, t2},
+      {kept_view(t1 ? s.normed : e), kept_view(t1 ? e : s.normed), a.grad_w1, a.grad_b1, t1}};
   if (train_fused(c, h, a.grad, a.out)) {
     LF_TRY(run_train_backward(ctx, a, w2, w1, kept_view(d), kept_view(e), static_cast<float*>(partials)));
-    LF_TRY(run_weight_grad(ctx, kept_view(t2 ? s.hidden : d), kept_view(t2 ? d : s.hidden), a.grad_w2, a.grad_b2, t2,
-                           a.grad_dtype, partials, "fp8.weight_grad2"));
-    return run_weight_grad(ctx, kept_view(t1 ? s.normed : e), kept_view(t1 ? e : s.normed), a.grad_w1, a.grad_b1, t1,
-                           a.grad_dtype, partials, "fp8.weight_grad1");
+    return run_weight_grads(ctx, grads, 2, a.grad_dtype, partials, "fp8.weight_grads");
   }
   LF_TRY(run_checkpoint_pack(ctx, a.grad, a.act_dtype, kept_view(d)));
-  LF_TRY(run_weight_grad(ctx, kept_view(t2 ? s.hidden : d), kept_view(t2 ? d : s.hidden), a.grad_w2, a.grad_b2, t2,
-                         a.grad_dtype, partials, "fp8.weight_grad2"));
   lf_fp8_linear_args l{};
   l.act = &d;
   l.w = &w2;
   l.relu_of = &s.hidden;
   l.out_kept = &e;
   LF_TRY(fp8_linear(ctx, l));
-  LF_TRY(run_weight_grad(ctx, kept_view(t1 ? s.normed : e), kept_view(t1 ? e : s.normed), a.grad_w1, a.grad_b1, t1,
-                         a.grad_dtype, partials, "fp8.weight_grad1"));
+  LF_TRY(run_weight_grads(ctx, grads, 2, a.grad_dtype, partials, "fp8.weight_grads"));
   lf_fp8_linear_args o{};
   o.act = &e;
   o.w = &w1;

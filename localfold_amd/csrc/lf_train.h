@@ -47,10 +47,15 @@ size_t layer_norm_partials(int rows, int channels);
 int run_layer_norm_backward(lf_context* ctx, const lf_layer_norm_backward_args& a, void* scratch, bool wide = false);
 // fast: f32 outputs by the 8-bit instruction too, for a caller whose results are of 16 bits.
 int run_fp8_linear(lf_context* ctx, const LinearParams& p, int out_dtype, const char* label, bool fast = false);
-size_t weight_grad_partials(int rows, int outputs, int inputs);
-// out = [a.cols, b.cols] = sum over rows of a^T b; bias = sum of a's rows, or of b's when bias_of_b
-int run_weight_grad(lf_context* ctx, const Kept& a, const Kept& b, void* out, void* bias, bool bias_of_b, int dt,
-                    void* scratch, const char* label);
+// One of up to two products of the same rows in a launch: out = [a.cols, b.cols] = sum over rows of a^T b;
+// bias = sum of a's rows, or of b's when bias_of_b.
+struct WeightGrad {
+  Kept a, b;
+  void *out, *bias;
+  bool bias_of_b;
+};
+size_t weight_grad_partials(int rows, int outputs, int inputs, int products = 1);   // of products of one size
+int run_weight_grads(lf_context* ctx, const WeightGrad* w, int count, int dt, void* scratch, const char* label);
 
 // Adds [blocks][2 channels] partial sums of scale and offset gradients.
 int run_norm_join(lf_context* ctx, const float* partial, int blocks, int channels, void* grad_scale, void* grad_offset,
