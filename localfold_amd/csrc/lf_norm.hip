@@ -5,9 +5,10 @@
 //
 // Both are bound by memory: a row is read once into registers, 8 consecutive channels a lane and
 // vector, and its sums go over a team of L lanes (L * NV * 8 >= channels) by permutes.  The team is
-// the smallest that leaves a lane at most 3 vectors, so narrow rows share a wave; rows past 1024
-// channels take the whole block, whose four waves join their sums in LDS.
+// small, so that narrow rows share a wave (team_of); rows past 1024 channels take the whole block, whose four
+// waves join their sums in LDS.
 #include <algorithm>
+#include <type_traits>
 
 #include "lf_train.h"
 
@@ -253,15 +254,18 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(const float* partial, i
 
 namespace {
 
-// A team and vectors a lane for a width: see the head of this file.
+// A team and vectors a lane for a width: see the head of this file.  bf16, us: 147456 rows of 64 forward and
+// backward 9 and 16, where a wave of two vectors a row takes 81 and 113; of 128 16 and 24 for 79 and 113; 100000 rows of
+// 384 29 and 51 for 57 and 81.  Three vectors a lane are faster forward (29 us, two of a team of 32 36) and
+// slower backward (55 us for 51), which holds three times as many.
 struct Team {
   int lanes, vectors;
 };
-Team team_of(int C) {
+Team team_of(int C, bool backward) {
   if (C <= 64) return {8, 1};
   if (C <= 128) return {16, 1};
   if (C <= 256) return {16, 2};
-  if (C <= 384) return {16, 3};
+  if (C <= 384 && !backward) return {16, 3};
   if (C <= 512) return {32, 2};
   if (C <= 1024) return {64, 2};
   if (C <= 2048) return {256, 1};
@@ -271,16 +275,17 @@ Team team_of(int C) {
 constexpr int GRAD_BLOCKS = 1024;   // at most; four a CU
 
 int grad_blocks(int rows, int C) {
-  const int slots = 256 / team_of(C).lanes;
+  const int slots = 256 / team_of(C, true).lanes;
   return (int)std::min<long long>(((long long)rows + slots - 1) / slots, GRAD_BLOCKS);
 }
 
 template <template <int, int, int> class F, int ACT, class P>
 void by_team(const Team& t, const P& p, dim3 grid, hipStream_t s) {
+  if constexpr (std::is_same<P, NormParams>::value)
+    if (t.vectors == 3) return F<ACT, 16, 3>::go(p, grid, s);
   if (t.lanes == 8) F<ACT, 8, 1>::go(p, grid, s);
   else if (t.lanes == 16 && t.vectors == 1) F<ACT, 16, 1>::go(p, grid, s);
   else if (t.lanes == 16 && t.vectors == 2) F<ACT, 16, 2>::go(p, grid, s);
-  else if (t.lanes == 16) F<ACT, 16, 3>::go(p, grid, s);
   else if (t.lanes == 32) F<ACT, 32, 2>::go(p, grid, s);
   else if (t.lanes == 64) F<ACT, 64, 2>::go(p, grid, s);
   else if (t.vectors == 1) F<ACT, 256, 1>::go(p, grid, s);
@@ -327,7 +332,7 @@ int run_layer_norm(lf_context* ctx, const lf_layer_norm_args& a) {
   p.C = a.channels;
   p.eps = a.epsilon;
   p.fast_var = a.fast_variance;
-  const Team t = team_of(a.channels);
+  const Team t = team_of(a.channels, false);
   const int slots = 256 / t.lanes;
   LaunchScope ls(ctx, "layer_norm");
   by_type<GoNorm>(a.act_dtype, t, p, dim3((unsigned)(((long long)a.rows + slots - 1) / slots)), ctx->stream);
@@ -354,7 +359,7 @@ int run_layer_norm_backward(lf_context* ctx, const lf_layer_norm_backward_args& 
   const int blocks = grad_blocks(a.rows, a.channels);
   {
     LaunchScope ls(ctx, "layer_norm.backward");
-    const Team t = team_of(a.channels);
+    const Team t = team_of(a.channels, true);
     if (wide) by_type<GoNormGradWide>(a.act_dtype, t, p, dim3(blocks), ctx->stream);
     else by_type<GoNormGrad>(a.act_dtype, t, p, dim3(blocks), ctx->stream);
   }

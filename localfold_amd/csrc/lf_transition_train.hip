@@ -10,8 +10,11 @@
 //   backward: d8 = q(dout); per 128 hidden units e8 = q(d8 W2^T where h8 > 0), acc += e8 W1^T = dy;
 //             dx = LN's gradient of dy (+ dout), ds and do summed over the block's rows
 //
-// Bound by memory where nothing else stalls: the forward pass moves 2 b c + 2 c + h bytes a row, the
-// backward 2 b c + 2 c + 2 h.
+// The forward pass moves 2 b c + 2 c + h bytes a row, the backward 2 b c + 2 c + 2 h: at 5.1 TB/s 37 us and 52 us for
+// 147456 rows of 128 x 512 in bf16, which take 64 us and 76 us.  The vector instructions (decoding the first
+// product's weights, rounding to codes, the norm) are about half of the time, the matrix instructions a quarter.
+// Run as single operators the passes take 96 us and 122 us.  Tiles of 16 rows for the last, partly filled
+// turn gained 4 % for this shape, lost 3 % for 207872 rows of 64 x 256, and are not there.
 #include <algorithm>
 
 #include "lf_fp8.h"
