@@ -270,7 +270,8 @@ __global__ __launch_bounds__(SW * 64, 2) void fp8_linear_stream_kernel(LinearPar
 // its waves a group of columns each, in turn, fragments straight from memory, sums joined in LDS.  59 rows of
 // 384 x 1536 in bf16: 3.5 us, where a block that stages its weights first takes 8.
 //
-// Every block reads its weights and its rows from L2 again, so larger products take the other kernels.  In
+// Every block reads its weights and its rows from L2 again, so products of more than one block of rows and many
+// outputs take the other kernels.  In
 // tiles of 32 x 32 outputs the times cross between 1000 (1024 x 256) and 2600 (64 x 256) for resident
 // weights (f32: 1350 and 3500), and at 3000 for streamed ones (f32: 4200).  bf16, us, small and other:
 // 384 x 1536: 1024 rows 8.2 and 8.1, 4096 rows 22 and 11; 128 x 512: 2048 rows 3.8 and 6.3, 16384 rows 17 and
@@ -354,7 +355,7 @@ int go(lf_context* ctx, const LinearParams& p) {
   LinearGrid q{};
   if constexpr (OUT != OUT_KEPT) {
     const long long mt = ((long long)p.rows + 16 * FM - 1) / (16 * FM), tiles = mt * ((p.outputs + 31) / 32);
-    if (tiles <= (kbs <= RESIDENT_TILES ? FEW_TILES : FEW_TILES_LONG)) {
+    if (mt == 1 || tiles <= (kbs <= RESIDENT_TILES ? FEW_TILES : FEW_TILES_LONG)) {
       const dim3 grid((p.outputs + 16 * Run<OUT>::PER - 1) / (16 * Run<OUT>::PER), (unsigned)mt);
       hipLaunchKernelGGL((fp8_linear_few_kernel<OUT, FAST>), grid, dim3(std::min(kbs, FW) * 64), 0, ctx->stream, p);
       return check_hip(hipGetLastError(), "fp8 linear launch");

@@ -31,7 +31,7 @@ struct GradParams {
   float* partial;                         // [splits][a.cols][b.cols]; null: one split, straight to out
   float* colsum;                          // [splits][cols of the summed one], or null
   int sum_of;                             // 0: no column sums, 1: of a, 2: of b
-  int splits, tiles, tiles_j;
+  int splits, tiles, tiles_j, per_xcd;
   long long rows_per;                     // rows of a split, a multiple of TEAMS GSTEP
   void *out, *bias;
   int dt, swapped;                        // out is [b.cols][a.cols]
@@ -81,7 +81,8 @@ __global__ __launch_bounds__(GWAVES * 64) void weight_grad_kernel(GradBatch batc
   const int op = blockIdx.x >= batch.first[1] ? 1 : 0;
   const GradParams& p = batch.w[op];
   const unsigned block = blockIdx.x - batch.first[op];
-  const int slot = block >> 3, tile = slot % p.tiles, split = slot / p.tiles * 8 + (block & 7);
+  // tiles of the same rows share an XCD (blocks are dealt out to 8 in turn, and products begin at multiples of 8)
+  const int index = (block & 7) * p.per_xcd + (block >> 3), tile = index % p.tiles, split = index / p.tiles;
   if (split >= p.splits) return;
   const int i0 = tile / p.tiles_j * GN, j0 = tile % p.tiles_j * GN;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -288,14 +289,22 @@ struct GradPlan {
   long long rows_per;
 };
 int tiles_of(int n, int k) { return (n + GN - 1) / GN * ((k + GN - 1) / GN); }
-// A block a CU, over all products of the launch.
+// How many ways the rows are split: the blocks' turns, at 1.25 us a step of the four teams, against the partial
+// sums, 64 KB a block written and read, and the join's launch (5 us).
 GradPlan grad_plan(long long rows, int ci, int cj, int all_tiles) {
   GradPlan q{};
   q.tiles_j = (cj + GN - 1) / GN;
   q.tiles = tiles_of(ci, cj);
-  const long long want = std::max<long long>(1, 256 / all_tiles);
   const long long turns = (rows + TEAMS * GSTEP - 1) / (TEAMS * GSTEP);
-  q.rows_per = (turns + want - 1) / want * (TEAMS * GSTEP);
+  double least = 1e300;
+  for (int w = 1; w <= 256 && w <= turns; ++w) {
+    const long long per = (turns + w - 1) / w, blocks = (long long)all_tiles * w;
+    const double cost = 1.25 * per * ((blocks + 255) / 256) + (w > 1 ? 5 + 0.033 * blocks : 0);
+    if (cost < least) {
+      least = cost;
+      q.rows_per = per * (TEAMS * GSTEP);
+    }
+  }
   q.splits = (int)((rows + q.rows_per - 1) / q.rows_per);
   return q;
 }
@@ -348,7 +357,8 @@ int run_weight_grads(lf_context* ctx, const WeightGrad* w, int count, int dt, vo
     p.bias = w[k].bias;
     p.dt = dt;
     sums = sums || p.sum_of != 0;
-    grid += (unsigned)((q.splits + 7) / 8 * q.tiles * 8);
+    p.per_xcd = (q.splits * q.tiles + 7) / 8;
+    grid += 8u * p.per_xcd;
     if (q.splits == 1) continue;
     const size_t n = (size_t)p.a.cols * p.b.cols;
     const int cn = p.sum_of == 0 ? 0 : p.sum_of == 1 ? p.a.cols : p.b.cols;

@@ -740,6 +740,9 @@ def af2_recycle(ctx: Context, f: dict, state: dict, masks: dict, embed_ws, extra
 # transition's training step.  Tensors are contiguous and on the context's device.
 # ---------------------------------------------------------------------------------------
 
+_MOST = 2 ** 31 - 1      # of a dimension: the C side has them as int
+
+
 def _tensor(ctx: Context, name: str, t: torch.Tensor, shape=None, dtype=None) -> int:
     """Address of a tensor argument after its checks (None for None)."""
     if t is None:
@@ -765,7 +768,10 @@ def _rows(t: torch.Tensor):
     shape = t.shape
     if len(shape) < 1 or shape[-1] == 0:
         raise ValueError(f"activations need a last dimension, got shape {tuple(shape)}")
-    return t.numel() // shape[-1], shape[-1]
+    rows = t.numel() // shape[-1]
+    if rows > _MOST:
+        raise ValueError(f"{rows} rows; at most {_MOST}")
+    return rows, shape[-1]
 
 
 class Checkpoint:
@@ -773,6 +779,8 @@ class Checkpoint:
     `scales` uint8 [groups of 128 columns, rows rounded up to 16], a byte b standing for 2^(b - 127)."""
 
     def __init__(self, rows: int, cols: int, codes: torch.Tensor, scales: torch.Tensor):
+        if max(rows, cols) > _MOST:
+            raise ValueError(f"a checkpoint of {rows} x {cols}; dimensions are at most {_MOST}")
         want = (rows, -(-cols // 64) * 64), (-(-cols // 128), -(-rows // 16) * 16)
         for name, t, shape in (("codes", codes, want[0]), ("scales", scales, want[1])):
             if tuple(t.shape) != shape or t.dtype != torch.uint8 or not t.is_contiguous():
@@ -877,6 +885,8 @@ class Fp8Weight:
     up to 64] (e4m3), `scales` uint8 [tiles of outputs, tiles of inputs], one per 128 x 128."""
 
     def __init__(self, outputs: int, inputs: int, codes: torch.Tensor, scales: torch.Tensor):
+        if max(outputs, inputs) > _MOST:
+            raise ValueError(f"a weight of {outputs} x {inputs}; dimensions are at most {_MOST}")
         want = (outputs, -(-inputs // 64) * 64), (-(-outputs // 128), -(-inputs // 128))
         for name, t, shape in (("codes", codes, want[0]), ("scales", scales, want[1])):
             if tuple(t.shape) != shape or t.dtype != torch.uint8 or not t.is_contiguous():
@@ -895,7 +905,7 @@ class Fp8Weight:
 
 def _live_weight(name: str, t: torch.Tensor, layout: int) -> capi.lf_weight:
     """lf_weight over a CUDA tensor as it is (read at the time of each call)."""
-    if t.dim() != 2 or not t.is_contiguous() or not t.is_cuda:
+    if t.dim() != 2 or not t.is_contiguous() or not t.is_cuda or max(t.shape) > _MOST:
         raise ValueError(f"{name} must be a contiguous 2-D CUDA tensor, got shape {tuple(t.shape)} on {t.device}")
     return capi.lf_weight(act_code(t), layout, t.shape[0], t.shape[1], 0, t.data_ptr(), None, None)
 

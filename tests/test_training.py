@@ -118,6 +118,19 @@ def test_checkpoint_layout_is_checked():
         D.Fp8Weight(130, 70, torch.zeros(130, 128, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.uint8))
 
 
+def test_dimensions_past_32_bits_are_refused():
+    """They would arrive in C as other numbers."""
+    from localfold_amd import device as D
+    x = torch.empty((2 ** 32 + 5, 1), device="meta")
+    with pytest.raises(ValueError, match="rows"):
+        D._rows(x)
+    codes, scales = (torch.empty(s, dtype=torch.uint8, device="meta") for s in ((2 ** 32 + 5, 64), (1, 2 ** 32 + 16)))
+    with pytest.raises(ValueError, match="at most"):
+        D.Checkpoint(2 ** 32 + 5, 1, codes, scales)
+    with pytest.raises(ValueError, match="at most"):
+        D.Fp8Weight(2 ** 32 + 5, 1, codes, scales)
+
+
 def test_struct_layouts(tmp_path):
     """sizeof of the training structs in C and in Python."""
     import ctypes as C
@@ -546,6 +559,18 @@ def test_weight_grad(ctx, rows, n, k):
         close(out, turn(want), depth * 2 * U * turn(size), dt, f"dw {layout} {dt}")
         close(bias, gv.sum(0), depth * 2 * U * np.abs(gv).sum(0), dt, "db")
         assert torch.equal(out, alone)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,k", [(300, 1536, 1500), (1000, 2100, 260), (40, 3000, 2000), (3000, 700, 700)])
+def test_weight_grad_many_tiles(ctx, rows, n, k):
+    test_weight_grad(ctx, rows, n, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,n", [(1, 64, 50001), (32, 200, 49000), (1, 1300, 65536)])
+def test_linear_one_tile_of_rows(ctx, rows, k, n):
+    test_linear(ctx, torch.bfloat16, rows, k, n)
 
 
 @pytest.mark.gpu
