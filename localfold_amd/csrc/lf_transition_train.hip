@@ -180,13 +180,19 @@ __global__ __launch_bounds__(TW * 64, 2) void train_forward_kernel(TrainParams p
         for (int a = 0; a < NH; ++a)
 #pragma unroll
           for (int e = 0; e < 16; ++e) var += v[a][e] * v[a][e];
+      }
+#pragma unroll
+      for (int a = 0; a < NH; ++a)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[a][e] -= mean[q];
+      if (p.fast_var) {
         var = lanes4_sum(var) / C - mean[q] * mean[q];
         var = var < 0.f ? 0.f : var;
       } else {
 #pragma unroll
         for (int a = 0; a < NH; ++a)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) var += (v[a][e] - mean[q]) * (v[a][e] - mean[q]);
+          for (int e = 0; e < 16; ++e) var += v[a][e] * v[a][e];
         var = lanes4_sum(var) / C;
       }
       rstd[q] = 1.0f / sqrtf(var + p.eps);
@@ -197,7 +203,7 @@ __global__ __launch_bounds__(TW * 64, 2) void train_forward_kernel(TrainParams p
           const f4 sc = *reinterpret_cast<const f4*>(vec + 64 * a + 16 * g + 4 * b);
           const f4 of = *reinterpret_cast<const f4*>(vec + C + 64 * a + 16 * g + 4 * b);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[a][4 * b + j] = (v[a][4 * b + j] - mean[q]) * rstd[q] * sc[j] + of[j];
+          for (int j = 0; j < 4; ++j) v[a][4 * b + j] = v[a][4 * b + j] * rstd[q] * sc[j] + of[j];
         }
       keep_row<NH>(y8, q, v);
     }
