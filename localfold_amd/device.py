@@ -1019,9 +1019,11 @@ def _transition_args(ctx: Context, a, x: torch.Tensor, out: torch.Tensor, wstruc
     a.rows, a.channels, a.hidden, a.act_dtype = rows, c, saved.hidden_size, act_code(x)
     a.out = _tensor(ctx, "out", out, x.shape, x.dtype)
     a.accumulate = int(accumulate)
-    for name, t in wstruct._owner.items():
-        if t is not None and t.device != ctx.device:
-            raise ValueError(f"{name} is on {t.device}; the context is on {ctx.device}")
+    owner = getattr(wstruct, "_owner", None)     # the tensors by name, or the DeviceWeights that holds them
+    for name, t in owner.items() if isinstance(owner, dict) else [("weights", owner)]:
+        device = None if t is None else torch.device(t.device)
+        if device is not None and (device.type != "cuda" or device.index not in (None, ctx.device.index)):
+            raise ValueError(f"{name} is on {device}; the context is on {ctx.device}")
     a.w, a.saved = C.pointer(wstruct), C.pointer(saved.struct)
     _scratch(ctx, a, scratch)
 
@@ -1059,6 +1061,8 @@ def transition_backward(ctx: Context, grad: torch.Tensor, wstruct: capi.lf_trans
         del shapes["firstBias"]
     if not wstruct.b2:
         del shapes["secondBias"]
+    if grad_dtype not in _TORCH_ACT:
+        raise TypeError(f"gradient dtype {grad_dtype} is not float32/float16/bfloat16")
     if grads is None:
         grads = {k: torch.empty(s, dtype=grad_dtype, device=ctx.device) for k, s in shapes.items()}
     at = {k: _tensor(ctx, f"grads[{k!r}]", grads[k], s, grad_dtype) for k, s in shapes.items()}

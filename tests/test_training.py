@@ -801,6 +801,24 @@ def test_training_step_in_a_graph(ctx):
 
 
 @pytest.mark.gpu
+def test_training_from_inference_weights(ctx):
+    """The struct that transition_weights builds for lf_transition works here too."""
+    from localfold_amd import device as D
+    rng = np.random.default_rng(8)
+    w = transition_case(ctx, rng, 128, 256, torch.float32)
+    x, grad = rows_of(rng, 100, 128, torch.float32).to(ctx.device), rows_of(rng, 100, 128, torch.float32).to(ctx.device)
+    got = []
+    for ws in (D.transition_train_weights(w),
+               D.transition_weights(D.DeviceWeights(ctx.device), {k: t.cpu().numpy() for k, t in w.items()})):
+        saved = D.transition_saved(100, 128, 256, ctx.device)
+        out = D.transition_train(ctx, x, ws, saved)
+        dx, grads = D.transition_backward(ctx, grad, ws, saved)
+        torch.cuda.synchronize()
+        got.append([out, dx, *grads.values()])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.gpu
 def test_refusals(ctx):
     import ctypes as C
     from localfold_amd import capi, device as D
