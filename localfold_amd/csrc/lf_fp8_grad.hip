@@ -3,14 +3,16 @@
 //
 // The reduction runs over the rows, along which each value has a scale of its own, so the codes are turned
 // into bf16 (exactly) as they are staged into LDS, and the fragments, whose lanes need 8 rows of a column,
-// are read from there by transposing reads.  A block of four teams of four waves computes a tile of
+// are read from there by transposing reads.  A block of three teams of four waves computes a tile of
 // 128 x 128 outputs over its share of the rows, the teams on steps of 32 rows in turn, joined in LDS; the
 // blocks' partial sums are added in order by a second kernel.  Column sums are a product with ones.
 //
-// 196608 rows, 1024 x 256: 128 to 143 us (720 to 800 TFLOP/s; its bytes alone are 49 us).  Nothing is
-// full: of the time the matrix pipes are busy 40 to 45 %, LDS 40 to 60 %, issue 20 %, and they overlap only as far as waves
-// differ, which is why 16 waves of 128 registers beat 8 that fetch fragments a step ahead (140 us) and 12 that
-// do (129).  Codes in LDS and converted after the read halve its traffic but double the conversions: 166 us.
+// 196608 rows, 1024 x 256: 126 to 136 us (760 to 820 TFLOP/s; its bytes alone are 49 us); 147456 rows, 512 x 128 and
+// 128 x 512 in one launch: 56 us.  Nothing is full: matrix pipes, LDS and issue are each busy about 40 % of
+// the time, and overlap only as far as waves differ.  12 waves that load three steps ahead beat 16 of 128
+// registers that load two ahead (134 to 153 us and 59 us), 8 (140 us and 78 us in two launches), and any that
+// fetch fragments a step ahead (149 to 164 us and 63 us).  Codes in LDS, converted after the read, halve
+// its traffic but double the conversions: 166 us.
 #include <algorithm>
 
 #include "lf_train.h"
@@ -23,7 +25,7 @@ typedef short s4v __attribute__((ext_vector_type(4)));
 
 constexpr int GN = GROUP;                 // outputs of a block, either way: one group of both operands
 constexpr int GSTEP = 32;                 // rows of a step: one matrix instruction's
-constexpr int TEAMS = 4;                  // of four waves, on steps in turn
+constexpr int TEAMS = 3;                  // of four waves, on steps in turn
 constexpr int GWAVES = 4 * TEAMS;
 
 struct GradParams {
@@ -47,7 +49,7 @@ struct GradBatch {
 constexpr int PITCH = GN * 2 + 32;        // LDS bytes of a row of bf16: 4 rows apart by 32 bytes mod 128
 constexpr int BUF = 2 * GSTEP * PITCH;    // one team's buffer: rows of a, then of b
 constexpr size_t GRAD_SMEM = TEAMS * 2 * BUF;
-static_assert(GRAD_SMEM >= (size_t)2 * GN * GN * 4 && GRAD_SMEM <= 160 * 1024, "the join of two teams at a time; LDS");
+static_assert(GRAD_SMEM >= 18 * 256 * 16 && GRAD_SMEM <= 160 * 1024, "the join of two teams at a time; LDS");
 
 // The transposing read: of each 16 lanes, lanes 4k .. 4k+3 address row k's 16 columns, 4 each; lane i
 // receives column i of the 4 rows.
@@ -101,25 +103,25 @@ __global__ __launch_bounds__(GWAVES * 64) void weight_grad_kernel(GradBatch batc
   const uint8_t* const scale[2] = {p.a.scales + (size_t)(i0 / GROUP) * p.a.sp + m0, p.b.scales + (size_t)(j0 / GROUP) * p.b.sp + m0};
   const int pitch[2] = {p.a.pitch, p.b.pitch};
   const int col[2] = {min(i0 + pc * 16, pitch[0] - 16), min(j0 + pc * 16, pitch[1] - 16)};
-  u32x4 raw[2];        // a, b
-  int sc[2];
+  u32x4 raw[2][2];        // [step][a, b]
+  int sc[2][2];
   // 24-bit products: the 64-bit multiply-add that the compiler would take reads a register pair whose other
   // half may be a load in flight, and waits for it
-  auto load = [&](int s, int k) __attribute__((always_inline)) {
+  auto load = [&](int s, int ring, int k) __attribute__((always_inline)) {
     const int m = (int)min(((uint32_t)s * TEAMS + team) * GSTEP, (uint32_t)n - 1), r = min(row, n - 1 - m);
-    raw[k] = *reinterpret_cast<const u32x4*>(code[k] + (size_t)m * pitch[k] + (__umul24(r, pitch[k]) + col[k]));
-    sc[k] = (scale[k] + m)[(uint32_t)r];
+    raw[ring][k] = *reinterpret_cast<const u32x4*>(code[k] + (size_t)m * pitch[k] + (__umul24(r, pitch[k]) + col[k]));
+    sc[ring][k] = (scale[k] + m)[(uint32_t)r];
   };
   // A lane's 16 values are two 16-byte pieces; in the upper half of a row they lie the other way round, so
   // that the 8 lanes of a row store to all banks at once.
   const int dst = row * PITCH + pc * 32 + (pc & 4 ? 16 : 0);
-  auto store = [&](int s, int k) __attribute__((always_inline)) {
+  auto store = [&](int s, int ring, int k) __attribute__((always_inline)) {
     const bool ok = row < (int)(n - ((uint32_t)s * TEAMS + team) * GSTEP);
-    const float f = scale_value(sc[k]);
+    const float f = scale_value(sc[ring][k]);
     uint32_t w[8];
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
-      const int c = ok ? (int)raw[k][d] : 0;
+      const int c = ok ? (int)raw[ring][k][d] : 0;
       w[2 * d] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, f, false));
       w[2 * d + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, f, true));
     }
@@ -148,71 +150,70 @@ __global__ __launch_bounds__(GWAVES * 64) void weight_grad_kernel(GradBatch batc
   const uint8_t* const from_b = from + GSTEP * PITCH + wj * 128 + ((l16 & 3) * 8 ^ wj * 16) + xj * 32;
   const int odd_a = (1 - 2 * xi) * 32, odd_b = (1 - 2 * xj) * 32;
 
-  // Step s is multiplied while step s + 1 is converted and stored and step s + 2 is loaded.
+  // Step s is multiplied while step s + 1 is converted and stored; steps s + 2 and s + 3 are under way.
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    load(0, k);
-    store(0, k);
-    load(1, k);
+    load(0, 0, k);
+    load(1, 1, k);
   }
-  for (int s = 0; s < steps; ++s) {
-    __syncthreads();
-    const int at = (s & 1) * BUF;
-    b8 fa[4], fb[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) fb[j] = tr_frag(from_b + (j & 1 ? at + (j - 1) * 32 + odd_b : at + j * 32));
+  for (int k = 0; k < 2; ++k) {
+    store(0, 0, k);
+    load(2, 0, k);
+  }
+  for (int s0 = 0; s0 < steps; s0 += 2) {     // past the last step: zeros
 #pragma unroll
-    for (int i = 0; i < 4; ++i) fa[i] = tr_frag(from_a + (i & 1 ? at + (i - 1) * 32 + odd_a : at + i * 32));
+    for (int u = 0; u < 2; ++u) {
+      __syncthreads();
+      const int at = u * BUF;
+      b8 fa[4], fb[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+      for (int j = 0; j < 4; ++j) fb[j] = tr_frag(from_b + (j & 1 ? at + (j - 1) * 32 + odd_b : at + j * 32));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
-      if (i & 1) {
-        store(s + 1, i >> 1);
-        load(s + 2, i >> 1);
+      for (int i = 0; i < 4; ++i) fa[i] = tr_frag(from_a + (i & 1 ? at + (i - 1) * 32 + odd_a : at + i * 32));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+        if (i & 1) {
+          store(s0 + u + 1, 1 - u, i >> 1);
+          load(s0 + u + 3, 1 - u, i >> 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if constexpr (SUMS) {
-      if (sum_a) {
+      if constexpr (SUMS) {
+        if (sum_a) {
 #pragma unroll
-        for (int f = 0; f < 2; ++f) sums[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[2 * f], ones, sums[f], 0, 0, 0);
-      } else if (sum_b) {
+          for (int f = 0; f < 2; ++f) sums[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[2 * f], ones, sums[f], 0, 0, 0);
+        } else if (sum_b) {
 #pragma unroll
-        for (int f = 0; f < 2; ++f) sums[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fb[2 * f], sums[f], 0, 0, 0);
+          for (int f = 0; f < 2; ++f) sums[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fb[2 * f], sums[f], 0, 0, 0);
+        }
       }
     }
   }
 
-  // the teams' sums, joined in halves: 2 and 3 to 0 and 1, then 1 to 0
-#pragma unroll
-  for (int to = TEAMS / 2; to > 0; to >>= 1) {
-    f4* const at = reinterpret_cast<f4*>(grad_smem) + ((team & (to - 1)) * 16 * 4 + (wi * 2 + wj)) * 64 + lane;   // [to][16][4 waves][64]
+  // the other teams' sums are added to the first's, in order
+  f4* const join = reinterpret_cast<f4*>(grad_smem) + (wi * 2 + wj) * 64 + lane;   // [18][4 waves][64]
+#pragma unroll 1
+  for (int t = 1; t < TEAMS; ++t) {
     __syncthreads();
-    if (team >= to && team < 2 * to) {
+    if (team == t) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) at[(i * 4 + j) * 256] = acc[i][j];
+        for (int j = 0; j < 4; ++j) join[(i * 4 + j) * 256] = acc[i][j];
+      join[16 * 256] = sums[0];
+      join[17 * 256] = sums[1];
     }
     __syncthreads();
-    if (team < to) {
+    if (team == 0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += at[(i * 4 + j) * 256];
-    }
-    if (SUMS && (sum_a || sum_b)) {     // uniform in the block
-      __syncthreads();
-      if (team >= to && team < 2 * to) {
-        at[0] = sums[0];
-        at[256] = sums[1];
-      }
-      __syncthreads();
-      if (team < to) {
-        sums[0] += at[0];
-        sums[1] += at[256];
-      }
+        for (int j = 0; j < 4; ++j) acc[i][j] += join[(i * 4 + j) * 256];
+      sums[0] += join[16 * 256];
+      sums[1] += join[17 * 256];
     }
   }
   if (team != 0) return;
@@ -289,8 +290,8 @@ struct GradPlan {
   long long rows_per;
 };
 int tiles_of(int n, int k) { return (n + GN - 1) / GN * ((k + GN - 1) / GN); }
-// How many ways the rows are split: the blocks' turns, at 1.25 us a step of the four teams, against the partial
-// sums, 64 KB a block written and read, and the join's launch (5 us).
+// How many ways the rows are split: the blocks' turns, at 0.95 us a step of the three teams, steps in twos, against the
+// partial sums, 64 KB a block written and read, and the join's launch (5 us).
 GradPlan grad_plan(long long rows, int ci, int cj, int all_tiles) {
   GradPlan q{};
   q.tiles_j = (cj + GN - 1) / GN;
@@ -299,7 +300,7 @@ GradPlan grad_plan(long long rows, int ci, int cj, int all_tiles) {
   double least = 1e300;
   for (int w = 1; w <= 256 && w <= turns; ++w) {
     const long long per = (turns + w - 1) / w, blocks = (long long)all_tiles * w;
-    const double cost = 1.25 * per * ((blocks + 255) / 256) + (w > 1 ? 5 + 0.033 * blocks : 0);
+    const double cost = 0.95 * ((per + 1) & ~1ll) * ((blocks + 255) / 256) + (w > 1 ? 5 + 0.033 * blocks : 0);
     if (cost < least) {
       least = cost;
       q.rows_per = per * (TEAMS * GSTEP);
