@@ -20,7 +20,6 @@
 namespace lf {
 
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 typedef short s4v __attribute__((ext_vector_type(4)));
 
 constexpr int GN = GROUP;                 // outputs of a block, either way: one group of both operands

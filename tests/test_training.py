@@ -690,6 +690,13 @@ def test_transition_step_composed(ctx, rows, c, h, dt, shift):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,c,h,dt", [(8100, 384, 1200, torch.bfloat16), (6200, 256, 512, torch.float16)])
+def test_transition_step_many(ctx, rows, c, h, dt):
+    """Composed, with products large enough for the kernels that stage weights, streamed and resident."""
+    transition_step(ctx, rows, c, h, dt, torch.float32, True, False)
+
+
+@pytest.mark.gpu
 def test_transition_gradients_by_differences(ctx):
     """The step's gradients against differences of its own float32 forward pass along random
     directions.  The codes' roundings (2^-4 each, unbiased, over rows x hidden of them) leave a few
