@@ -494,12 +494,12 @@ int lf_msa_module_block(lf_context* ctx, const lf_msa_block_args* args);
  * same way with one scale per tile of 128 x 128: codes [outputs][LF_CHECKPOINT_PITCH(inputs)],
  * scales [LF_CHECKPOINT_GROUPS(outputs)][LF_CHECKPOINT_GROUPS(inputs)].
  *
- * Products of two kept matrices: their values are exact in bfloat16, and with f32 or kept outputs
- * they are multiplied in it, products exact and sums in f32.  16-bit outputs of lf_fp8_linear take
- * the 8-bit matrix instruction, whose sums are f32 too but which drops, of 8 products added at a
- * time, what lies 2^-13 below the largest: about 2e-5 of the result for inputs of like size, far
- * under the output's own rounding.  So do the inner products of the transition's step whose results
- * are not kept, when act_dtype is of 16 bits.
+ * Products of two kept matrices are multiplied in bfloat16, where their values are exact (but for codes
+ * below 2^-6 under scale bytes 1 and 2, which become multiples of 2^-133, and values of 2^128 and
+ * beyond, which become infinities), and added in f32, whatever the output's type.  The inner products
+ * of the transition's step whose results are not kept take the 8-bit matrix instruction when act_dtype is
+ * of 16 bits, whose sums are f32 too but which drops, of 8 products added at a time, what lies 2^-13 below
+ * the largest.
  *
  * Matrices are row-major and contiguous.  Inputs and outputs do not overlap except where it says
  * so.  Sums over rows (gradients of weights, biases, scales and offsets) are added in a fixed

@@ -8,8 +8,11 @@
 namespace lf {
 
 // 144 KB of LDS, which leaves room for the biases.  Longer reductions stream both operands.  bf16, us, resident and
-// streamed: 147456 rows of 128 x 512 32 and 42, of 512 x 512 51 and 64, of 640 x 640 117 and 105, of
-// 1024 x 1024 207 and 204, 16384 rows of 1024 x 256 13 and 17.
+// streamed: 147456 rows of 128 x 512 35 and 46, of 512 x 512 73 and 88, of 640 x 640 129 and 141, of 640 x 128 31
+// and 53, of 1024 x 1024 269 and 282, 16384 rows of 1024 x 256 20 and 27; the other way 256 x 1024, 130 and 114.
+// f32: 35 and 60 for 640 x 128, 95 and 104 for 1024 x 256, but 190 and 176 for 640 x 640, 337 and 282 for 384 x 1536:
+// where outputs are many times the inputs, streaming gains up to 16 %.  The rule stays with what fits: neither
+// outputs nor rows tell those shapes from 1152 x 1152, which is faster resident at any number of rows.
 constexpr int RESIDENT_TILES = 9;
 
 // No load has a condition, or the compiler could not count those in flight and would wait for all: rows past
@@ -88,7 +91,7 @@ struct LinearGrid {
 // then run through (32 rows, output group) units with no barrier, x straight from memory to registers.
 // These shapes are bound by memory: 16 waves of 128 registers hide its latency better than 8 of 256 with
 // 64 rows, at twice the LDS reads, of which there are enough.  Units of the same rows run in
-// neighbouring waves.  147456 rows of 128 x 512 in bf16: 32 us, 5.3 TB/s.
+// neighbouring waves.  147456 rows of 128 x 512 in bf16: 35 us, 4.9 TB/s.
 constexpr int RW = 16, RM = 2;            // waves of a block, tiles of 16 rows of a wave
 
 template <int OUT, bool FAST>
@@ -159,8 +162,7 @@ constexpr int SW = 8, SM = 4, MROWS = 16 * SM;   // the streaming kernel's waves
 // Long reductions: a block of 256 rows and two output groups walks the columns 128 at a time, tiles of both
 // operands in two LDS buffers in turn.  One barrier a step; the next step's tiles are under way during this
 // one's products.  Blocks on one XCD run through 4 row tiles and then the outputs, so its L2 serves both.  8192 rows of
-// 4096 x 4096 in bf16: 113 to 117 us, 2.4 PFLOP/s; LDS (192 KB read and 64 KB written a step of 2048 matrix
-// clocks) is as busy as the matrix pipes.
+// 4096 x 4096 in bf16: 199 us, 1.38 PFLOP/s, where a large bf16 library product has 1.2.
 template <int OUT, bool FAST>
 __global__ __launch_bounds__(SW * 64, 2) void fp8_linear_stream_kernel(LinearParams p, LinearGrid q) {
   // Two weight tiles and 4 tiles of 64 rows each.  Separate objects: reads of one are then known not to wait
@@ -267,15 +269,15 @@ __global__ __launch_bounds__(SW * 64, 2) void fp8_linear_stream_kernel(LinearPar
 }
 
 // Small products: what counts is the time to the last byte.  A block computes 32 rows by one run of outputs,
-// its waves a group of columns each, in turn, fragments straight from memory, sums joined in LDS.  59 rows of
-// 384 x 1536 in bf16: 3.5 us, where a block that stages its weights first takes 8.
+// its waves a group of columns each, in turn, fragments straight from memory, sums joined in LDS.  256 rows of
+// 384 x 1536 in bf16: 4.3 us, where a block that stages its weights first takes 10.
 //
 // Every block reads its weights and its rows from L2 again, so products of more than one block of rows and many
 // outputs take the other kernels.  In
-// tiles of 32 x 32 outputs the times cross between 1000 (1024 x 256) and 2600 (64 x 256) for resident
-// weights (f32: 1350 and 3500), and at 3000 for streamed ones (f32: 4200).  bf16, us, small and other:
-// 384 x 1536: 1024 rows 8.2 and 8.1, 4096 rows 22 and 11; 128 x 512: 2048 rows 3.8 and 6.3, 16384 rows 17 and
-// 9.8; 4096 x 4096: 512 rows 60 and 89, 1024 rows 117 and 89.
+// tiles of 32 x 32 outputs the times cross between 1600 (1024 x 256) and 3500 (64 x 256) for resident
+// weights (f32: 1300 and 3500), and for streamed ones between 3000 (1536 x 1536) and 6300 (4096 x 4096) (f32: 2300 and
+// 4300).  bf16, us, small and other: 384 x 1536: 1024 rows 7.4 and 10.5, 4096 rows 22 and 13; 128 x 512: 2048 rows
+// 3.9 and 7.1, 16384 rows 16 and 10; 4096 x 4096: 512 rows 60 and 174, 2048 rows 230 and 178.
 constexpr int FW = 8, FM = 2;             // most waves of a block, tiles of 16 rows
 constexpr int FEW_TILES = 1500, FEW_TILES_LONG = 3000;
 
@@ -348,7 +350,7 @@ __global__ __launch_bounds__(FW * 64) void fp8_linear_few_kernel(LinearParams p)
 
 namespace {
 
-template <int OUT, bool FAST = OUT == DT_F16 || OUT == DT_BF16>
+template <int OUT, bool FAST = false>
 int go(lf_context* ctx, const LinearParams& p) {
   const int nbs = (p.outputs + GROUP - 1) / GROUP, kbs = (p.inputs + GROUP - 1) / GROUP;
   const int cus = ctx->num_cus;
@@ -368,7 +370,7 @@ int go(lf_context* ctx, const LinearParams& p) {
     const long long busy = std::max<long long>(1, mt * nbs / ((long long)cus * RW));
     q.per = (int)std::min<long long>(std::min(fit, nbs), busy);
     q.subsets = (nbs + q.per - 1) / q.per;
-    // a unit for every SIMD before a second one: 2048 rows of 128 x 512 in 6.3 us, in blocks of 16 units 10
+    // a unit for every SIMD before a second one: 2048 rows of 128 x 512 in 7.1 us
     q.blocks = (int)std::min<long long>((mt * q.per + 3) / 4, std::max(1, cus / q.subsets));
     static const bool lds = hipFuncSetAttribute(reinterpret_cast<const void*>(&fp8_linear_resident_kernel<OUT, FAST>),
                                                 hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) == hipSuccess;

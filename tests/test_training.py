@@ -879,3 +879,26 @@ def test_refusals(ctx):
         D.transition_train(ctx, x, ws, D.transition_saved(10, 128, 64, dev))
     before = torch.cuda.current_device()
     assert before == 0
+
+
+def dominated(rng, rows, k, n):
+    """Operands whose first two products are a thousand times the others and cancel: what an instruction
+    that drops the small ones beside them leaves out is all there is."""
+    x, w = rng.normal(size=(rows, k)), rng.normal(size=(n, k)) / 4
+    x[:, :2], w[:, 0], w[:, 1] = 32, 32, -32
+    return torch.as_tensor(x).float(), torch.as_tensor(w).float()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rows,k,n", [(59, 384, 1536), (3, 22, 49), (9000, 128, 257), (6001, 192, 300), (3100, 1000, 512),
+                                      (59, 4096, 64), (25000, 1153, 130)])
+def test_linear_sums_are_of_32_bits(ctx, dt, rows, k, n):
+    """The small, resident and streamed products, whole and half groups of columns: whatever the output's
+    type, sums are float32's."""
+    from localfold_amd import capi, device as D
+    x, w = dominated(np.random.default_rng(rows + k), rows, k, n)
+    x8, w8 = D.checkpoint_pack(ctx, x.to(ctx.device)), D.fp8_weight(ctx, w.to(ctx.device), capi.LF_OUT_IN)
+    xv, wv = values_of(x8), weight_values(w8)
+    assert (xv[:, 0] * wv[:, :1] + xv[:, 1] * wv[:, 1:2]).max() == 0
+    close(D.fp8_linear(ctx, x8, w8, dtype=dt), xv @ wv.T, linear_slack(xv, wv, k, True), dt)
