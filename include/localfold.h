@@ -496,10 +496,8 @@ int lf_msa_module_block(lf_context* ctx, const lf_msa_block_args* args);
  *
  * Products of two kept matrices are multiplied in bfloat16, where their values are exact (but for codes
  * below 2^-6 under scale bytes 1 and 2, which become multiples of 2^-133, and values of 2^128 and
- * beyond, which become infinities), and added in f32, whatever the output's type.  The inner products
- * of the transition's step whose results are not kept take the 8-bit matrix instruction when act_dtype is
- * of 16 bits, whose sums are f32 too but which drops, of 8 products added at a time, what lies 2^-13 below
- * the largest.
+ * beyond, which become infinities), and added in f32, whatever the output's type; so are the products
+ * inside the transition's step.
  *
  * Matrices are row-major and contiguous.  Inputs and outputs do not overlap except where it says
  * so.  Sums over rows (gradients of weights, biases, scales and offsets) are added in a fixed

@@ -9,8 +9,7 @@
 // Operands are converted in registers for the bf16 instruction: codes times a power of two fit bfloat16, products
 // are exact and sums are f32's.  The 8-bit instructions, with and without scales, drop what lies 2^-13 below
 // the largest of 8 products that they add at a time (measured: 1.6e-5 of the result for normal inputs; where large
-// ones cancel, up to 1e-3 of those), always downwards.  Only the inner products of the transition's step whose
-// results are not kept take the scaled one, when activations are of 16 bits.
+// ones cancel, up to 1e-3 of those), always downwards.
 #pragma once
 #include "lf_train.h"
 
@@ -18,7 +17,6 @@ namespace lf {
 
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-typedef int i8v __attribute__((ext_vector_type(8)));
 
 constexpr int OUT_KEPT = 3;               // beside DT_F32, DT_F16, DT_BF16
 constexpr int WTILE = GROUP * GROUP;      // bytes of a weight tile
@@ -73,32 +71,19 @@ __device__ __forceinline__ void w_stage(uint8_t* dst, const uint8_t* w, int pitc
 }
 
 // acc[q] += 16 outputs x 16 MT rows x 128 columns, w a lane's two pieces of its output's codes.
-template <bool FAST, int MT>
+template <int MT>
 __device__ __forceinline__ void mma_frag(f4 (&acc)[MT], const u32x4 (&w)[2], const XFrag<MT>& x, int wscale) {
 #if __HIP_DEVICE_COMPILE__
-  if constexpr (FAST) {
-    const i8v a = {(int)w[0].x, (int)w[0].y, (int)w[0].z, (int)w[0].w, (int)w[1].x, (int)w[1].y, (int)w[1].z, (int)w[1].w};
-#define LF_MM(q)                                                                                                           \
-  {                                                                                                                        \
-    const i8v b = {(int)x.v[q][0].x, (int)x.v[q][0].y, (int)x.v[q][0].z, (int)x.v[q][0].w,                                 \
-                   (int)x.v[q][1].x, (int)x.v[q][1].y, (int)x.v[q][1].z, (int)x.v[q][1].w};                                \
-    acc[q] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[q], 0, 0, 0, wscale, q, (int)x.scale);             \
-  }
-    static_assert(MT == 2, "");
-    LF_MM(0) LF_MM(1)
-#undef LF_MM
-  } else {
-    const float sw = scale_value(wscale);
+  const float sw = scale_value(wscale);
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const b8 a0 = codes_bf16(w[half].x, w[half].y, sw), a1 = codes_bf16(w[half].z, w[half].w, sw);
+  for (int half = 0; half < 2; ++half) {
+    const b8 a0 = codes_bf16(w[half].x, w[half].y, sw), a1 = codes_bf16(w[half].z, w[half].w, sw);
 #pragma unroll
-      for (int q = 0; q < MT; ++q) {
-        const float sx = scale_value((x.scale >> (8 * q)) & 255);
-        const u32x4 v = x.v[q][half];
-        acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, codes_bf16(v.x, v.y, sx), acc[q], 0, 0, 0);
-        acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, codes_bf16(v.z, v.w, sx), acc[q], 0, 0, 0);
-      }
+    for (int q = 0; q < MT; ++q) {
+      const float sx = scale_value((x.scale >> (8 * q)) & 255);
+      const u32x4 v = x.v[q][half];
+      acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, codes_bf16(v.x, v.y, sx), acc[q], 0, 0, 0);
+      acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, codes_bf16(v.z, v.w, sx), acc[q], 0, 0, 0);
     }
   }
 #else
@@ -110,73 +95,42 @@ __device__ __forceinline__ void mma_frag(f4 (&acc)[MT], const u32x4 (&w)[2], con
 }
 
 // acc += one step: 16 NT outputs x 16 MT rows x 128 columns (HALF: 64, the others are zeros); FIRST: acc =
-// bias + the step, bias 16 NT floats in LDS.  FAST: the scaled 8-bit instruction, else bf16.  w: the
-// lane's place in an LDS tile, wx the same with the other half of the columns.  A tile's fragment is read
-// while the one before it is multiplied; the barriers keep the compiler from reading all eight at once,
-// which would spill.  next() may load over x: it is called once x is no longer read.
-template <int OUT, bool FAST, bool FIRST, bool HALF, int NT, int MT, class NEXT>
+// bias + the step, bias 16 NT floats in LDS.  w: the lane's place in an LDS tile, wx the same with the other
+// half of the columns.  A tile's fragment is read while the one before it is multiplied; the barriers keep the
+// compiler from reading all eight at once, which would spill.  next() may load over x: it is called once x is
+// no longer read.
+template <int OUT, bool FIRST, bool HALF, int NT, int MT, class NEXT>
 __device__ __forceinline__ void mma(f4 (&acc)[NT][MT], const uint8_t* w, const uint8_t* wx, const XFrag<MT>& x, int wscale,
                                     const float* bias, int g, NEXT next) {
 #if __HIP_DEVICE_COMPILE__
   f4 c;
-  if constexpr (FAST) {
-    u32x4 a0[2], a1[2];
-    a1[0] = a1[1] = u32x4{0, 0, 0, 0};
-    a0[0] = *reinterpret_cast<const u32x4*>(w);
-    if constexpr (!HALF) a1[0] = *reinterpret_cast<const u32x4*>(wx);
+  const float sw = scale_value(wscale);
+#pragma unroll
+  for (int half = 0; half < (HALF ? 1 : 2); ++half) {
+    const uint8_t* wh = half ? wx : w;
+    b8 b[MT][2];
+    u32x4 a[2];
+    a[0] = *reinterpret_cast<const u32x4*>(wh);
+#pragma unroll
+    for (int q = 0; q < MT; ++q) {
+      const float sx = scale_value((x.scale >> (8 * q)) & 255);
+      const u32x4 v = x.v[q][half];
+      b[q][0] = codes_bf16(v.x, v.y, sx);
+      b[q][1] = codes_bf16(v.z, v.w, sx);
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      if (t < NT - 1) {
-        const int at = n_of<OUT>(t + 1, 0) * GROUP;
-        a0[(t + 1) & 1] = *reinterpret_cast<const u32x4*>(w + at);
-        if constexpr (!HALF) a1[(t + 1) & 1] = *reinterpret_cast<const u32x4*>(wx + at);
-      }
-      if constexpr (FIRST) c = *reinterpret_cast<const f4*>(bias + n_of<OUT>(t, 4 * g));
-      const u32x4 c0 = a0[t & 1], c1 = a1[t & 1];
-      const i8v a = {(int)c0.x, (int)c0.y, (int)c0.z, (int)c0.w, (int)c1.x, (int)c1.y, (int)c1.z, (int)c1.w};
-#define LF_MM(q)                                                                                                  \
-  if constexpr (q < MT) {                                                                                         \
-    const i8v b = {(int)x.v[q][0].x, (int)x.v[q][0].y, (int)x.v[q][0].z, (int)x.v[q][0].w,                        \
-                   (int)x.v[q][1].x, (int)x.v[q][1].y, (int)x.v[q][1].z, (int)x.v[q][1].w};                       \
-    acc[t][q] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, FIRST ? c : acc[t][q], 0, 0, 0, wscale, q, \
-                                                                 (int)x.scale);                                   \
-  }
-      LF_MM(0) LF_MM(1)
-      if constexpr (MT == 4) {
-        LF_MM(MT - 2) LF_MM(MT - 1)
-      }
-#undef LF_MM
+      if (t < NT - 1) a[(t + 1) & 1] = *reinterpret_cast<const u32x4*>(wh + n_of<OUT>(t + 1, 0) * GROUP);
+      if constexpr (FIRST)
+        if (half == 0) c = *reinterpret_cast<const f4*>(bias + n_of<OUT>(t, 4 * g));
+      const u32x4 v = a[t & 1];
+      const b8 a0 = codes_bf16(v.x, v.y, sw), a1 = codes_bf16(v.z, v.w, sw);
+#pragma unroll
+      for (int q = 0; q < MT; ++q)
+        acc[t][q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, b[q][0], FIRST && half == 0 ? c : acc[t][q], 0, 0, 0);
+#pragma unroll
+      for (int q = 0; q < MT; ++q) acc[t][q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, b[q][1], acc[t][q], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
-    }
-  } else {
-    const float sw = scale_value(wscale);
-#pragma unroll
-    for (int half = 0; half < (HALF ? 1 : 2); ++half) {
-      const uint8_t* wh = half ? wx : w;
-      b8 b[MT][2];
-      u32x4 a[2];
-      a[0] = *reinterpret_cast<const u32x4*>(wh);
-#pragma unroll
-      for (int q = 0; q < MT; ++q) {
-        const float sx = scale_value((x.scale >> (8 * q)) & 255);
-        const u32x4 v = x.v[q][half];
-        b[q][0] = codes_bf16(v.x, v.y, sx);
-        b[q][1] = codes_bf16(v.z, v.w, sx);
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if (t < NT - 1) a[(t + 1) & 1] = *reinterpret_cast<const u32x4*>(wh + n_of<OUT>(t + 1, 0) * GROUP);
-        if constexpr (FIRST)
-          if (half == 0) c = *reinterpret_cast<const f4*>(bias + n_of<OUT>(t, 4 * g));
-        const u32x4 v = a[t & 1];
-        const b8 a0 = codes_bf16(v.x, v.y, sw), a1 = codes_bf16(v.z, v.w, sw);
-#pragma unroll
-        for (int q = 0; q < MT; ++q)
-          acc[t][q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, b[q][0], FIRST && half == 0 ? c : acc[t][q], 0, 0, 0);
-#pragma unroll
-        for (int q = 0; q < MT; ++q) acc[t][q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, b[q][1], acc[t][q], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-      }
     }
   }
 #endif

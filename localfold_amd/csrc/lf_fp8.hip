@@ -94,7 +94,7 @@ struct LinearGrid {
 // neighbouring waves.  147456 rows of 128 x 512 in bf16: 35 us, 4.9 TB/s.
 constexpr int RW = 16, RM = 2;            // waves of a block, tiles of 16 rows of a wave
 
-template <int OUT, bool FAST>
+template <int OUT>
 __global__ __launch_bounds__(RW * 64) void fp8_linear_resident_kernel(LinearParams p, LinearGrid q) {
   extern __shared__ __attribute__((aligned(16))) uint8_t fp8_smem[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
@@ -140,14 +140,14 @@ __global__ __launch_bounds__(RW * 64) void fp8_linear_resident_kernel(LinearPara
     const float* const bn = bias + nb_now * GROUP;
     int at = nb_now * kbs * WTILE + wl;
     x_zero(x, p, 0);
-    mma<OUT, FAST, true, false>(acc, fp8_smem + at, fp8_smem + (at ^ 64), x, ws[0], bn, g, [&]() __attribute__((always_inline)) {
+    mma<OUT, true, false>(acc, fp8_smem + at, fp8_smem + (at ^ 64), x, ws[0], bn, g, [&]() __attribute__((always_inline)) {
       x_load(x, p, (long long)(kbs == 1 ? mt : mt_now) * 16 * RM, kbs == 1 ? 0 : 1, r, g);
     });
     for (int kb = 1; kb < kbs; ++kb) {
       at += WTILE;
       const bool last = kb + 1 == kbs;
       x_zero(x, p, kb);
-      mma<OUT, FAST, false, false>(acc, fp8_smem + at, fp8_smem + (at ^ 64), x, ws[kb], bn, g, [&]() __attribute__((always_inline)) {
+      mma<OUT, false, false>(acc, fp8_smem + at, fp8_smem + (at ^ 64), x, ws[kb], bn, g, [&]() __attribute__((always_inline)) {
         x_load(x, p, (long long)(last ? mt : mt_now) * 16 * RM, last ? 0 : kb + 1, r, g);
       });
     }
@@ -162,8 +162,9 @@ constexpr int SW = 8, SM = 4, MROWS = 16 * SM;   // the streaming kernel's waves
 // Long reductions: a block of 256 rows and two output groups walks the columns 128 at a time, tiles of both
 // operands in two LDS buffers in turn.  One barrier a step; the next step's tiles are under way during this
 // one's products.  Blocks on one XCD run through 4 row tiles and then the outputs, so its L2 serves both.  8192 rows of
-// 4096 x 4096 in bf16: 199 us, 1.38 PFLOP/s, where a large bf16 library product has 1.2.
-template <int OUT, bool FAST>
+// 4096 x 4096 in bf16: 199 to 219 us, 1.26 to 1.38 PFLOP/s (a large bf16 library product has 1.2): matrix pipes busy 63 %,
+// vector instructions, most of them conversions, 45 %, LDS reads 16 %.
+template <int OUT>
 __global__ __launch_bounds__(SW * 64, 2) void fp8_linear_stream_kernel(LinearParams p, LinearGrid q) {
   // Two weight tiles and 4 tiles of 64 rows each.  Separate objects: reads of one are then known not to wait
   // for copies into the other.
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(SW * 64, 2) void fp8_linear_stream_kernel(LinearPar
     __builtin_amdgcn_sched_barrier(0);
     stage(other, kn);
     __builtin_amdgcn_sched_barrier(0);     // the copies are under way first, the fragments come one by one
-    mma<OUT, FAST, false, false>(acc, buf + wl, buf + wlx, x, wnow, bias, g, []() {});
+    mma<OUT, false, false>(acc, buf + wl, buf + wlx, x, wnow, bias, g, []() {});
     // products touch no memory: without this they would be moved past the next step's barrier
 #pragma unroll
     for (int t = 0; t < 8; ++t)
@@ -281,7 +282,7 @@ __global__ __launch_bounds__(SW * 64, 2) void fp8_linear_stream_kernel(LinearPar
 constexpr int FW = 8, FM = 2;             // most waves of a block, tiles of 16 rows
 constexpr int FEW_TILES = 1500, FEW_TILES_LONG = 3000;
 
-template <int OUT, bool FAST>
+template <int OUT>
 __global__ __launch_bounds__(FW * 64) void fp8_linear_few_kernel(LinearParams p) {
   constexpr int NT = Run<OUT>::PER;
   __shared__ f4 part[FW - 1][NT][FM][64];
@@ -319,7 +320,7 @@ __global__ __launch_bounds__(FW * 64) void fp8_linear_few_kernel(LinearParams p)
   auto multiply = [&](Step& s, int kb) __attribute__((always_inline)) {
     x_zero(s.x, p, kb);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) mma_frag<FAST>(acc[t], s.w[t], s.x, s.ws);
+    for (int t = 0; t < NT; ++t) mma_frag(acc[t], s.w[t], s.x, s.ws);
   };
   for (int kb = wave; kb < kbs; kb += 2 * waves) {
     Step a, b;
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(FW * 64) void fp8_linear_few_kernel(LinearParams p)
 
 namespace {
 
-template <int OUT, bool FAST = false>
+template <int OUT>
 int go(lf_context* ctx, const LinearParams& p) {
   const int nbs = (p.outputs + GROUP - 1) / GROUP, kbs = (p.inputs + GROUP - 1) / GROUP;
   const int cus = ctx->num_cus;
@@ -359,7 +360,7 @@ int go(lf_context* ctx, const LinearParams& p) {
     const long long mt = ((long long)p.rows + 16 * FM - 1) / (16 * FM), tiles = mt * ((p.outputs + 31) / 32);
     if (mt == 1 || tiles <= (kbs <= RESIDENT_TILES ? FEW_TILES : FEW_TILES_LONG)) {
       const dim3 grid((p.outputs + 16 * Run<OUT>::PER - 1) / (16 * Run<OUT>::PER), (unsigned)mt);
-      hipLaunchKernelGGL((fp8_linear_few_kernel<OUT, FAST>), grid, dim3(std::min(kbs, FW) * 64), 0, ctx->stream, p);
+      hipLaunchKernelGGL((fp8_linear_few_kernel<OUT>), grid, dim3(std::min(kbs, FW) * 64), 0, ctx->stream, p);
       return check_hip(hipGetLastError(), "fp8 linear launch");
     }
   }
@@ -370,30 +371,30 @@ int go(lf_context* ctx, const LinearParams& p) {
     const long long busy = std::max<long long>(1, mt * nbs / ((long long)cus * RW));
     q.per = (int)std::min<long long>(std::min(fit, nbs), busy);
     q.subsets = (nbs + q.per - 1) / q.per;
-    // a unit for every SIMD before a second one: 2048 rows of 128 x 512 in 7.1 us
+    // a unit for every SIMD before a second one: 8192 rows of 128 x 512 in 8.2 us, in blocks of 16 units 11.4
     q.blocks = (int)std::min<long long>((mt * q.per + 3) / 4, std::max(1, cus / q.subsets));
-    static const bool lds = hipFuncSetAttribute(reinterpret_cast<const void*>(&fp8_linear_resident_kernel<OUT, FAST>),
+    static const bool lds = hipFuncSetAttribute(reinterpret_cast<const void*>(&fp8_linear_resident_kernel<OUT>),
                                                 hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) == hipSuccess;
     if (!lds) return set_error(LF_ERR_DEVICE, "fp8 linear: the device refuses the LDS it needs");
     const size_t smem = (size_t)q.per * (kbs * WTILE + GROUP * 4 + kbs);
     const unsigned grid = (unsigned)((q.blocks * q.subsets + 7) / 8 * 8);
-    hipLaunchKernelGGL((fp8_linear_resident_kernel<OUT, FAST>), dim3(grid), dim3(RW * 64), smem, ctx->stream, p, q);
+    hipLaunchKernelGGL((fp8_linear_resident_kernel<OUT>), dim3(grid), dim3(RW * 64), smem, ctx->stream, p, q);
     return check_hip(hipGetLastError(), "fp8 linear launch");
   }
   const long long mt = ((long long)p.rows + MROWS - 1) / MROWS;
   q.subsets = (nbs + 1) / 2;
   q.blocks = (int)((mt + 3) / 4);
   const unsigned grid = (unsigned)(((long long)q.blocks + 31) / 32 * 32 * q.subsets);
-  hipLaunchKernelGGL((fp8_linear_stream_kernel<OUT, FAST>), dim3(grid), dim3(SW * 64), 0, ctx->stream, p, q);
+  hipLaunchKernelGGL((fp8_linear_stream_kernel<OUT>), dim3(grid), dim3(SW * 64), 0, ctx->stream, p, q);
   return check_hip(hipGetLastError(), "fp8 linear launch");
 }
 
 }  // namespace
 
-int run_fp8_linear(lf_context* ctx, const LinearParams& p, int out_dtype, const char* label, bool fast) {
+int run_fp8_linear(lf_context* ctx, const LinearParams& p, int out_dtype, const char* label) {
   LaunchScope ls(ctx, label);
   if (!p.out) return go<OUT_KEPT>(ctx, p);
-  if (out_dtype == LF_F32) return fast ? go<DT_F32, true>(ctx, p) : go<DT_F32>(ctx, p);
+  if (out_dtype == LF_F32) return go<DT_F32>(ctx, p);
   if (out_dtype == LF_F16) return go<DT_F16>(ctx, p);
   return go<DT_BF16>(ctx, p);
 }

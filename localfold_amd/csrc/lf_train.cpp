@@ -165,7 +165,7 @@ int fp8_pack_weight(lf_context* ctx, const lf_fp8_weight_args& a) {
   return run_pack_weights(ctx, &p, 1);
 }
 
-int fp8_linear(lf_context* ctx, const lf_fp8_linear_args& a, bool fast = false) {
+int fp8_linear(lf_context* ctx, const lf_fp8_linear_args& a) {
   static const char fn[] = "lf_fp8_linear";
   LF_REQUIRE(a.act && a.w, "lf_fp8_linear: act or w is NULL");
   const lf_fp8_weight& w = *a.w;
@@ -198,7 +198,7 @@ int fp8_linear(lf_context* ctx, const lf_fp8_linear_args& a, bool fast = false) 
   p.out = a.out;
   if (a.out_kept) p.q = kept_view(*a.out_kept);
   p.q.pitch = (int)LF_CHECKPOINT_PITCH(w.outputs);
-  return run_fp8_linear(ctx, p, a.out ? a.out_dtype : LF_BF16, "fp8.linear", fast);
+  return run_fp8_linear(ctx, p, a.out ? a.out_dtype : LF_BF16, "fp8.linear");
 }
 
 int fp8_weight_grad(lf_context* ctx, const lf_fp8_weight_grad_args& a) {
@@ -377,7 +377,7 @@ int transition_backward(lf_context* ctx, const lf_transition_backward_args& a) {
   o.w = &w1;
   o.out_dtype = LF_F32;      // as the fused pass has it: rounded to 16 bits, the norm's gradients were twice as far off
   o.out = dy;
-  LF_TRY(fp8_linear(ctx, o, a.act_dtype != LF_F32));
+  LF_TRY(fp8_linear(ctx, o));
 
   lf_layer_norm_backward_args n{};
   n.rows = a.rows;

@@ -45,8 +45,7 @@ int run_layer_norm(lf_context* ctx, const lf_layer_norm_args& a);
 size_t layer_norm_partials(int rows, int channels);
 // wide: a.grad is f32, whatever act_dtype is.
 int run_layer_norm_backward(lf_context* ctx, const lf_layer_norm_backward_args& a, void* scratch, bool wide = false);
-// fast: f32 outputs by the 8-bit instruction, for a caller whose results are of 16 bits.
-int run_fp8_linear(lf_context* ctx, const LinearParams& p, int out_dtype, const char* label, bool fast = false);
+int run_fp8_linear(lf_context* ctx, const LinearParams& p, int out_dtype, const char* label);
 // One of up to two products of the same rows in a launch: out = [a.cols, b.cols] = sum over rows of a^T b;
 // bias = sum of a's rows, or of b's when bias_of_b.
 struct WeightGrad {

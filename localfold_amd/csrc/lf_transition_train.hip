@@ -11,10 +11,10 @@
 //             dx = LN's gradient of dy (+ dout), ds and do summed over the block's rows
 //
 // The forward pass moves 2 b c + 2 c + h bytes a row, the backward 2 b c + 2 c + 2 h: at 5.1 TB/s 37 us and 52 us for
-// 147456 rows of 128 x 512 in bf16, which take 64 us and 76 us.  The vector instructions (decoding the first
-// product's weights, rounding to codes, the norm) are about half of the time, the matrix instructions a quarter.
-// Run as single operators the passes take 96 us and 122 us.  Tiles of 16 rows for the last, partly filled
-// turn gained 4 % for this shape, lost 3 % for 207872 rows of 64 x 256, and are not there.
+// 147456 rows of 128 x 512 in bf16, which take 70 us and 80 us.  The vector instructions (decoding the weights
+// of both products, rounding to codes, the norm) are more than half of the time, the matrix instructions a quarter.
+// Run as single operators the two calls take 97 us for 69 and 196 us for 144.  Tiles of 16 rows for the last, partly
+// filled turn gained 4 % for this shape, lost 3 % for 207872 rows of 64 x 256, and are not there.
 #include <algorithm>
 
 #include "lf_fp8.h"
@@ -121,7 +121,6 @@ __device__ __forceinline__ Tiles block_tiles(int rows, int wave) {
 template <int ACT, int C>
 __global__ __launch_bounds__(TW * 64, 2) void train_forward_kernel(TrainParams p) {
   constexpr int NH = C / 64, NT2 = C / 16;
-  constexpr bool FAST = ACT != DT_F32;
   extern __shared__ __attribute__((aligned(16))) uint8_t train_smem[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int groups = p.hidden / GROUP;
@@ -226,7 +225,7 @@ __global__ __launch_bounds__(TW * 64, 2) void train_forward_kernel(TrainParams p
       for (int q = 0; q < TM; ++q) acc[t][q] = *reinterpret_cast<const f4*>(vec + 2 * C + n_of<ACT>(t, 4 * g));
     for (int hb = 0; hb < groups; ++hb) {
       f4 hid[8][TM];
-      mma<OUT_KEPT, false, true, C == 64>(hid, wa + hb * WTILE, wax + hb * WTILE, y8, s1 >> (8 * hb) & 255, vec + 3 * C + hb * GROUP, g,
+      mma<OUT_KEPT, true, C == 64>(hid, wa + hb * WTILE, wax + hb * WTILE, y8, s1 >> (8 * hb) & 255, vec + 3 * C + hb * GROUP, g,
                                           [] {});
 #pragma unroll
       for (int t = 0; t < 8; ++t)
@@ -238,7 +237,7 @@ __global__ __launch_bounds__(TW * 64, 2) void train_forward_kernel(TrainParams p
       keep_tile(hid, h8);
       store_kept(h8, p.kh.codes + (size_t)m0 * p.hidden + hb * GROUP, p.kh.scales + (size_t)hb * p.kh.sp + m0, p.hidden,
                  left, GROUP, r, g);
-      mma<ACT, FAST, false, false>(acc, wb + hb * WTILE, wbx + hb * WTILE, h8, s2 >> (8 * hb) & 255, vec, g, [] {});
+      mma<ACT, false, false>(acc, wb + hb * WTILE, wbx + hb * WTILE, h8, s2 >> (8 * hb) & 255, vec, g, [] {});
     }
     finish<ACT>(acc, fin, m0, 0, r, g);
     if constexpr (ACT == DT_F32) load(min(tile + TW, tiles.end - 1));
@@ -259,7 +258,6 @@ __device__ __forceinline__ void halve(float (&v)[M], bool upper) {
 template <int ACT, int C>
 __global__ __launch_bounds__(TW * 64, 2) void train_backward_kernel(TrainParams p) {
   constexpr int NH = C / 64, NT2 = C / 16;
-  constexpr bool FAST = ACT != DT_F32;
   extern __shared__ __attribute__((aligned(16))) uint8_t train_smem[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int groups = p.hidden / GROUP;
@@ -319,7 +317,7 @@ __global__ __launch_bounds__(TW * 64, 2) void train_backward_kernel(TrainParams 
     load_gate(0);
     for (int hb = 0; hb < groups; ++hb) {
       f4 e[8][TM];
-      mma<OUT_KEPT, false, true, C == 64>(e, wa + hb * WTILE, wax + hb * WTILE, d8, s1 >> (8 * hb) & 255, vec + C, g, [] {});
+      mma<OUT_KEPT, true, C == 64>(e, wa + hb * WTILE, wax + hb * WTILE, d8, s1 >> (8 * hb) & 255, vec + C, g, [] {});
 #pragma unroll
       for (int t = 0; t < 8; ++t)
 #pragma unroll
@@ -330,7 +328,7 @@ __global__ __launch_bounds__(TW * 64, 2) void train_backward_kernel(TrainParams 
       store_kept(e8, p.k2.codes + (size_t)m0 * p.hidden + hb * GROUP, p.k2.scales + (size_t)hb * p.k2.sp + m0, p.hidden,
                  left, GROUP, r, g);
       const int at = (groups + hb) * WTILE;
-      mma<OUT_KEPT, FAST, false, false>(dy, wa + at, wax + at, e8, s2 >> (8 * hb) & 255, vec, g, [] {});
+      mma<OUT_KEPT, false, false>(dy, wa + at, wax + at, e8, s2 >> (8 * hb) & 255, vec, g, [] {});
     }
 
     // LayerNorm's gradient: a lane has columns 64 a + 16 g + 4 b + j of its rows in dy[4 a + b][q][j]

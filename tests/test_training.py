@@ -902,3 +902,142 @@ def test_linear_sums_are_of_32_bits(ctx, dt, rows, k, n):
     xv, wv = values_of(x8), weight_values(w8)
     assert (xv[:, 0] * wv[:, :1] + xv[:, 1] * wv[:, 1:2]).max() == 0
     close(D.fp8_linear(ctx, x8, w8, dtype=dt), xv @ wv.T, linear_slack(xv, wv, k, True), dt)
+
+
+# ---- the transition's step, each stage from what the stage before it kept ---------------------------
+#
+# Hidden gradients are not at hand.  A code is that of a number within its sum's float32 error (code_range),
+# so all but those next to a border between two codes, a few in 10^4, are known, and what follows from them
+# is held to float32's errors.
+
+def code_range(lo, hi):
+    """The smallest and the largest that a number within [lo, hi] may stand for once it is kept."""
+    least, most = np.empty_like(lo), np.empty_like(hi)
+    for g in range(0, lo.shape[1], 128):
+        l, h = lo[:, g:g + 128], hi[:, g:g + 128]
+        inner = np.where((l <= 0) & (h >= 0), 0.0, np.minimum(np.abs(l), np.abs(h)))
+        fs = [scale_of(m.max(1, keepdims=True)) for m in (inner, np.maximum(np.abs(l), np.abs(h)))]
+        least[:, g:g + 128] = np.minimum(*(np.maximum(round_e4m3(l / f), -448) * f for f in fs))
+        most[:, g:g + 128] = np.maximum(*(np.minimum(round_e4m3(h / f), 448) * f for f in fs))
+    return least, most
+
+
+def sum_depth(k):
+    return 32 + k / 32 + 4      # products of an instruction, instructions, waves that are joined
+
+
+def check_step(dt, x, grad, p, residual, fast, saved, got):
+    """A step's results against float64.  p: parameters by name; saved: the values of act, normed and
+    hidden, and stats; got: out, dx and grads, as stored."""
+    rows, c = x.shape
+    h = saved["hidden"].shape[1]
+    w1, w2, s, o = kept_weight64(p["firstWeight"]), kept_weight64(p["secondWeight"]), p["layerNormScale"], p["layerNormOffset"]
+    y8, h8, x8 = saved["normed"], saved["hidden"], saved["act"]
+    d1, d2 = sum_depth(c) * 2 * U, sum_depth(h) * 2 * U
+
+    def within(v, lo, hi, label):
+        lo, hi = code_range(lo, hi)
+        bad = ~((v >= lo) & (v <= hi))
+        assert not bad.any(), (label, int(bad.sum()), np.argwhere(bad)[:4].tolist())
+
+    assert np.array_equal(x8, kept64(x)), "act"
+    y, m, r = norm64(x, s, o, float(np.float32(1e-5)), fast)
+    slack = norm_slack(x, s, o, m, r, c)
+    within(y8, y - slack, y + slack, "normed")
+    depth = 2 * (min(c, 64) + 8) * U
+    size = (x * x).mean(1)
+    close(saved["stats"][0], m[:, 0], depth * np.abs(x).mean(1), torch.float32, "mean")
+    close(saved["stats"][1], r[:, 0], r[:, 0] * (depth * (1 + r[:, 0] ** 2 * size) + 4 * U), torch.float32, "rstd")
+    pre = y8 @ w1 + p["firstBias"]
+    slack = (np.abs(y8) @ np.abs(w1) + np.abs(p["firstBias"])) * d1
+    within(h8, np.maximum(pre - slack, 0), np.maximum(pre + slack, 0), "hidden")
+    total = h8 @ w2 + p["secondBias"]
+    slack = (np.abs(h8) @ np.abs(w2) + np.abs(p["secondBias"])) * d2
+    if residual:
+        total = total + x
+    close(got["out"], total, slack + 2 * U * np.abs(total), dt, "out")
+
+    # gradients: of the weights over the rows (32 an instruction, three teams in turn, 256 splits joined in runs)
+    d8, over = kept64(grad), (32 + rows / 96 + 51) * 2 * U
+    close(got["grads"]["secondWeight"], h8.T @ d8, over * (np.abs(h8).T @ np.abs(d8)), torch.float32, "dw2")
+    gate = h8 > 0
+    pre = d8 @ w2.T
+    slack = (np.abs(d8) @ np.abs(w2.T)) * d1
+    lo, hi = code_range(np.where(gate, pre - slack, 0), np.where(gate, pre + slack, 0))
+    e, off = (lo + hi) / 2, (hi - lo) / 2
+    assert (off > 0).mean() < 0.01
+    close(got["grads"]["firstWeight"], y8.T @ e, np.abs(y8).T @ (off + over * (np.abs(e) + off)), torch.float32, "dw1")
+    if "firstBias" in got["grads"]:
+        close(got["grads"]["firstBias"], e.sum(0), (off + over * (np.abs(e) + off)).sum(0), torch.float32, "db1")
+        close(got["grads"]["secondBias"], d8.sum(0), over * np.abs(d8).sum(0), torch.float32, "db2")
+    dy, off = e @ w1.T, (off + d2 * (np.abs(e) + off)) @ np.abs(w1.T)
+    m, r = saved["stats"][0][:, None], saved["stats"][1][:, None]
+    dx, ds, do = norm_backward64(dy, x8, s, m, r)
+    hh, g, go = (x8 - m) * r, dy * s, off * np.abs(s)
+    dh = 2 * U * (np.abs(x8) + np.abs(m)) * r
+    b = np.abs(g * hh).mean(1, keepdims=True)
+    slack = r * (4 * U * np.abs(g) + depth * np.abs(g).mean(1, keepdims=True) + dh * b
+                 + np.abs(hh) * (depth * b + (np.abs(g) * dh).mean(1, keepdims=True)))
+    slack = slack + r * (go + go.mean(1, keepdims=True) + np.abs(hh) * (go * np.abs(hh)).mean(1, keepdims=True)) + 4 * U * np.abs(dx)
+    if residual:
+        dx = dx + grad
+        slack = slack + 2 * U * np.abs(dx)
+    close(got["dx"], dx, slack, dt, "dx")
+    # a lane's rows, a block's lanes, the blocks
+    over = (rows / 256 + 128) * 2 * U
+    close(got["grads"]["layerNormScale"], ds, (off * np.abs(hh) + over * np.abs(dy * hh) + np.abs(dy) * dh).sum(0), torch.float32, "ds")
+    close(got["grads"]["layerNormOffset"], do, (off + over * np.abs(dy)).sum(0), torch.float32, "do")
+
+
+def params64(w, c, h):
+    zero = {"firstBias": np.zeros(h), "secondBias": np.zeros(c)}
+    return {k: f64(w[k]) if k in w else zero[k] for k in ("layerNormScale", "layerNormOffset", "firstWeight", "firstBias",
+                                                          "secondWeight", "secondBias")}
+
+
+def checked_step(ctx, rows, c, h, dt, wdt, residual, fast, shift=0, spike=None, layouts=None):
+    """Runs a step and checks it.  shift: everything that many elements behind an aligned address; layouts:
+    of the two matrices as they are stored; spike: two hidden units a thousand times the others that cancel
+    in the output, or whose gradients cancel in the first channel of the norm's output."""
+    from localfold_amd import capi, device as D
+    rng = np.random.default_rng(rows + 5 * c + h)
+    w = transition_case(ctx, rng, c, h, wdt, bias=rows != 45)
+    if spike == "out":
+        w["firstWeight"][:, :2], w["firstBias"][:2] = 0, 20
+        w["secondWeight"][0] = torch.as_tensor(rng.normal(size=c)).to(wdt)
+        w["secondWeight"][1] = -w["secondWeight"][0]
+    elif spike == "dy":
+        w["firstWeight"][:, :2], w["firstBias"][:2] = 0, 40
+        w["firstWeight"][0, 0], w["firstWeight"][0, 1] = 4, -4
+        w["secondWeight"][0] = torch.as_tensor(rng.normal(size=c)).to(wdt)
+        w["secondWeight"][1] = w["secondWeight"][0]
+    ws, saved = D.transition_train_weights(w), D.transition_saved(rows, c, h, ctx.device)
+    turned = [l == capi.LF_OUT_IN for l in layouts] if layouts else [False, False]
+    if layouts:
+        stored = [w[n].t().contiguous() if t else w[n] for n, t in zip(("firstWeight", "secondWeight"), turned)]
+        ws.w1, ws.w2 = (D._live_weight("w", t, l) for t, l in zip(stored, layouts))
+    x, grad = rows_of(rng, rows, c, dt, 0.3).to(ctx.device), (rows_of(rng, rows, c, dt) * 0.01).to(dt).to(ctx.device)
+    if rows > 2:
+        grad[rows // 2] = 0      # a padded row
+    out, dx = torch.empty_like(x), torch.empty_like(grad)
+    if shift:
+        x, grad, out, dx = (torch.cat([t.new_zeros(shift), t.flatten()])[shift:].view(rows, c) for t in (x, grad, out, dx))
+    D.transition_train(ctx, x, ws, saved, out=out, accumulate=residual, fast_variance=fast)
+    _, grads = D.transition_backward(ctx, grad, ws, saved, out=dx, accumulate=residual)
+    torch.cuda.synchronize()
+    got = {"out": f64(out), "dx": f64(dx), "grads": {k: f64(t) for k, t in grads.items()}}
+    for n, t in zip(("firstWeight", "secondWeight"), turned):
+        if t:
+            got["grads"][n] = got["grads"][n].T
+    kept = {"act": values_of(saved.act), "normed": values_of(saved.normed), "hidden": values_of(saved.hidden),
+            "stats": f64(saved.stats)}
+    check_step(dt, f64(x), f64(grad), params64(w, c, h), residual, fast, kept, got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,c,h", [(300, 128, 512), (300, 64, 256), (150, 256, 320), (8100, 384, 1200)])
+@pytest.mark.parametrize("spike", ["out", "dy"])
+def test_transition_sums_are_of_32_bits(ctx, rows, c, h, dt, spike):
+    """The step's products too, fused and composed: the float32 gradients of the norm's vectors come from them."""
+    checked_step(ctx, rows, c, h, dt, torch.float32, False, False, spike=spike)
