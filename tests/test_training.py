@@ -1041,3 +1041,96 @@ def checked_step(ctx, rows, c, h, dt, wdt, residual, fast, shift=0, spike=None, 
 def test_transition_sums_are_of_32_bits(ctx, rows, c, h, dt, spike):
     """The step's products too, fused and composed: the float32 gradients of the norm's vectors come from them."""
     checked_step(ctx, rows, c, h, dt, torch.float32, False, False, spike=spike)
+
+
+STEP_SHAPES = [(1, 128, 512, torch.float32, torch.float32, True, False), (37, 64, 256, torch.float16, torch.float32, True, True),
+               (300, 128, 512, torch.bfloat16, torch.bfloat16, True, False), (33, 64, 128, torch.bfloat16, torch.float32, True, False),
+               (31, 128, 128, torch.float16, torch.float16, False, True), (257, 64, 512, torch.float32, torch.float32, False, False),
+               (1000, 128, 384, torch.float32, torch.bfloat16, True, True), (45, 128, 256, torch.float32, torch.float32, True, False),
+               (66001, 64, 128, torch.bfloat16, torch.float32, True, False), (33003, 128, 128, torch.float16, torch.float32, False, False),
+               # widths that run as single operators
+               (150, 256, 1024, torch.float32, torch.float16, False, False), (90, 384, 100, torch.bfloat16, torch.float32, False, True),
+               (45, 22, 70, torch.float32, torch.float32, True, False), (600, 49, 130, torch.float16, torch.bfloat16, False, False),
+               (131, 64, 640, torch.bfloat16, torch.float32, True, False), (8100, 384, 1200, torch.bfloat16, torch.float32, True, False),
+               (6200, 256, 512, torch.float16, torch.float32, True, False)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,c,h,dt,wdt,residual,fast", STEP_SHAPES)
+def test_transition_step_to_f32(ctx, rows, c, h, dt, wdt, residual, fast):
+    checked_step(ctx, rows, c, h, dt, wdt, residual, fast)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,c,h,dt,shift", [(70, 128, 256, torch.bfloat16, 1), (70, 64, 128, torch.float16, 4),
+                                               (70, 128, 128, torch.float32, 1)])
+def test_transition_step_off_alignment_to_f32(ctx, rows, c, h, dt, shift):
+    checked_step(ctx, rows, c, h, dt, torch.float32, True, False, shift)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first,second", [(0, 1), (1, 0), (1, 1)])
+@pytest.mark.parametrize("rows,c,h,wdt", [(70, 128, 256, torch.float32), (50, 64, 128, torch.bfloat16), (90, 49, 130, torch.float16)])
+def test_transition_step_layouts(ctx, rows, c, h, wdt, first, second):
+    """Matrices stored [outputs, inputs], whose gradients come in that layout."""
+    from localfold_amd import capi
+    kinds = (capi.LF_IN_OUT, capi.LF_OUT_IN)
+    checked_step(ctx, rows, c, h, torch.float32, wdt, True, False, layouts=(kinds[first], kinds[second]))
+
+
+def test_transition_checks_see_mistakes():
+    """check_step passes a step computed here, and none with a mistake in one of its results: zeros, another
+    sign, columns in another order, a column's values off by a twentieth, a tile of rows left out of a sum."""
+    rng = np.random.default_rng(1)
+    for rows, c, h, dt, residual in ((300, 128, 256, torch.bfloat16, True), (700, 64, 128, torch.float32, False)):
+        p = {"layerNormScale": 1 + 0.2 * rng.uniform(-1, 1, c), "layerNormOffset": 0.1 * rng.uniform(-1, 1, c),
+             "firstWeight": rng.normal(size=(c, h)) / math.sqrt(c), "firstBias": 0.1 * rng.uniform(-1, 1, h),
+             "secondWeight": rng.normal(size=(h, c)) / math.sqrt(h), "secondBias": 0.1 * rng.uniform(-1, 1, c)}
+        x, grad = f64(rows_of(rng, rows, c, dt, 0.3)), f64((rows_of(rng, rows, c, dt) * 0.01).to(dt))
+
+        def stored(v, t=torch.float32):
+            return f64(torch.as_tensor(v).to(t))
+
+        y, m, r = norm64(x, p["layerNormScale"], p["layerNormOffset"], float(np.float32(1e-5)))
+        w1, w2 = kept_weight64(p["firstWeight"]), kept_weight64(p["secondWeight"])
+        x8, y8, d8 = kept64(x), kept64(y), kept64(grad)
+        h8 = kept64(np.maximum(y8 @ w1 + p["firstBias"], 0))
+        e8 = kept64(np.where(h8 > 0, d8 @ w2.T, 0))
+        stats = stored(np.concatenate([m, r], 1).T)
+        dy = e8 @ w1.T
+        dx, ds, do = norm_backward64(dy, x8, p["layerNormScale"], stats[0][:, None], stats[1][:, None])
+        out = h8 @ w2 + p["secondBias"]
+        got = {"out": stored(out + x if residual else out, dt), "dx": stored(dx + grad if residual else dx, dt),
+               "grads": {k: stored(v) for k, v in (("firstWeight", y8.T @ e8), ("firstBias", e8.sum(0)),
+                                                   ("secondWeight", h8.T @ d8), ("secondBias", d8.sum(0)),
+                                                   ("layerNormScale", ds), ("layerNormOffset", do))}}
+        saved = {"act": x8, "normed": y8, "hidden": h8, "stats": stats}
+        check_step(dt, x, grad, p, residual, False, saved, got)
+
+        def refused(saved, got):
+            with pytest.raises(AssertionError):
+                check_step(dt, x, grad, p, residual, False, saved, got)
+
+        def one_column(v):
+            v = v.copy()
+            v[..., 5] *= 1.05
+            return v
+
+        wrong = {"zeros": np.zeros_like, "sign": np.negative, "order": lambda v: np.roll(v, 4, -1), "column": one_column}
+        for how, f in wrong.items():
+            for k in ("out", "dx"):
+                refused(saved, {**got, k: f(got[k])})
+            for k in got["grads"]:
+                refused(saved, {**got, "grads": {**got["grads"], k: f(got["grads"][k])}})
+        tail = slice(0, rows - 32)       # a tile of rows
+        for k, v in (("layerNormScale", norm_backward64(dy[tail], x8[tail], p["layerNormScale"], stats[0][tail, None],
+                                                        stats[1][tail, None])[1]), ("layerNormOffset", dy[tail].sum(0)),
+                     ("firstWeight", y8[tail].T @ e8[tail]), ("firstBias", e8[tail].sum(0))):
+            refused(saved, {**got, "grads": {**got["grads"], k: stored(v)}})
+        for k in ("normed", "hidden"):
+            refused({**saved, k: np.roll(saved[k], 1, 1)}, got)
+        # the norm's incoming gradient rounded to 16 bits on its way
+        if dt != torch.float32:
+            _, ds, do = norm_backward64(stored(dy, dt), x8, p["layerNormScale"], stats[0][:, None], stats[1][:, None])
+            refused(saved, {**got, "grads": {**got["grads"], "layerNormScale": stored(ds)}})
+            refused(saved, {**got, "grads": {**got["grads"], "layerNormOffset": stored(do)}})
