@@ -1134,3 +1134,54 @@ def test_transition_checks_see_mistakes():
             _, ds, do = norm_backward64(stored(dy, dt), x8, p["layerNormScale"], stats[0][:, None], stats[1][:, None])
             refused(saved, {**got, "grads": {**got["grads"], "layerNormScale": stored(ds)}})
             refused(saved, {**got, "grads": {**got["grads"], "layerNormOffset": stored(do)}})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,n", LINEAR_SHAPES + LONG_SHAPES + [(9000, 128, 257), (6001, 192, 300), (2500, 1216, 400)])
+def test_linear_kept_sums_are_of_32_bits(ctx, rows, k, n):
+    """A kept product is the code of a number within float32's error of the product, also where its
+    largest terms cancel."""
+    from localfold_amd import capi, device as D
+    rng = np.random.default_rng(rows + 7 * k + n)
+    plain = rows_of(rng, rows, k, torch.float32), torch.as_tensor(rng.normal(size=(n, k)) / math.sqrt(k)).float()
+    for x, w in (plain, dominated(rng, rows, k, n)) if k > 2 else (plain,):
+        x8, w8 = D.checkpoint_pack(ctx, x.to(ctx.device)), D.fp8_weight(ctx, w.to(ctx.device), capi.LF_OUT_IN)
+        bias = vec(rng, ctx, n, 1.0)
+        got = D.checkpoint_empty(rows, n, ctx.device)
+        D.fp8_linear(ctx, x8, w8, bias, out=got)
+        xv, wv = values_of(x8), weight_values(w8)
+        want = xv @ wv.T + f64(bias)
+        slack = linear_slack(xv, wv, k, True) + 2 * U * (np.abs(want) + np.abs(f64(bias)))
+        lo, hi = code_range(want - slack, want + slack)
+        v = values_of(got)
+        assert ((v >= lo) & (v <= hi)).all()
+
+
+# A half group of columns at the end: the small, resident and streamed products.
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,n", [(40, 192, 200), (40, 64, 200), (9000, 192, 200), (40, 1344, 200), (13000, 1344, 260)])
+def test_linear_weight_specials(ctx, rows, k, n):
+    """A NaN or an infinity in a weight's row stays in that output, wherever it lies in the row."""
+    from localfold_amd import capi, device as D
+    rng = np.random.default_rng(rows + k)
+    w = (rng.normal(size=(n, k)) / math.sqrt(k)).astype(np.float32).astype(np.float64)
+    w[17, 5], w[41, k - 1], w[n - 1, k // 2], w[130, 0] = np.nan, np.inf, -np.inf, np.nan
+    bad = np.zeros(n, bool)
+    bad[[17, 41, n - 1, 130]] = True
+    x8 = D.checkpoint_pack(ctx, torch.as_tensor(rng.normal(size=(rows, k))).float().to(ctx.device))
+    wt = torch.as_tensor(w).float().to(ctx.device)
+    w8 = D.fp8_weight(ctx, wt, capi.LF_OUT_IN)
+    turned = D.fp8_weight(ctx, wt.t().contiguous(), capi.LF_IN_OUT)
+    assert torch.equal(w8.codes & 127, turned.codes & 127) and torch.equal(w8.scales, turned.scales)
+    xv, wv = values_of(x8), weight_values(w8)
+    assert np.array_equal(np.isnan(wv), ~np.isfinite(w))
+    assert np.array_equal(wv[~bad], kept_weight64(np.where(np.isfinite(w), w, 0))[~bad])
+    want, slack = xv @ wv[~bad].T, linear_slack(xv, wv[~bad], k, True)
+    for dt in TYPES:
+        out = f64(D.fp8_linear(ctx, x8, w8, relu=True, dtype=dt))
+        assert np.isnan(out[:, bad]).all()
+        close(out[:, ~bad], np.maximum(want, 0), slack, dt)
+    kept = D.checkpoint_empty(rows, n, ctx.device)
+    D.fp8_linear(ctx, x8, w8, out=kept)
+    v = values_of(kept)
+    assert np.isnan(v[:, bad]).all() and np.isfinite(v[:, ~bad]).all()
