@@ -507,7 +507,7 @@ int lf_msa_module_block(lf_context* ctx, const lf_msa_block_args* args);
  * for the call's partial sums, at least what the entry point's _scratch function says, 16-byte
  * aligned.  NULL: the context's workspace, which another call may replace: a call that is captured
  * into a HIP graph has to bring its own (LF_ERR_INVALID otherwise), one for each graph that may
- * run at the same time. */
+ * run at the same time.  lf_fp8_weight_grad over few rows, which it does not split, uses neither. */
 typedef struct {
   int rows, cols;
   void* codes;

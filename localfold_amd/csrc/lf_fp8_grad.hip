@@ -320,16 +320,19 @@ int go(lf_context* ctx, const GradBatch& b, unsigned grid) {
 
 size_t up16(size_t n) { return (n + 15) & ~size_t(15); }
 
-size_t partial_bytes(int rows, int outputs, int inputs, int all_tiles) {
-  const GradPlan q = grad_plan(rows, std::max(outputs, inputs), std::min(outputs, inputs), all_tiles);
-  return up16((size_t)q.splits * outputs * inputs * sizeof(float)) +
-         up16((size_t)q.splits * std::max(outputs, inputs) * sizeof(float));
+size_t partial_bytes(int splits, int outputs, int inputs) {
+  return up16((size_t)splits * outputs * inputs * sizeof(float)) + up16((size_t)splits * std::max(outputs, inputs) * sizeof(float));
 }
 
 }  // namespace
 
 size_t weight_grad_partials(int rows, int outputs, int inputs, int products) {
-  return products * partial_bytes(rows, outputs, inputs, products * tiles_of(outputs, inputs));
+  const int splits =
+      grad_plan(rows, std::max(outputs, inputs), std::min(outputs, inputs), products * tiles_of(outputs, inputs)).splits;
+  return splits == 1 ? 0 : products * partial_bytes(splits, outputs, inputs);
+}
+size_t weight_grad_scratch(int rows, int outputs, int inputs) {
+  return std::max(weight_grad_partials(rows, outputs, inputs), partial_bytes(1, outputs, inputs));
 }
 
 int run_weight_grads(lf_context* ctx, const WeightGrad* w, int count, int dt, void* scratch, const char* label) {

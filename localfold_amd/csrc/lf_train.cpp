@@ -212,8 +212,10 @@ int fp8_weight_grad(lf_context* ctx, const lf_fp8_weight_grad_args& a) {
   LF_TRY(check_act(fn, "out", a.out, a.grad_dtype));
   LF_TRY(check_act(fn, "bias", a.bias, a.grad_dtype));
   void* scratch = nullptr;
-  LF_TRY(take_scratch(ctx, fn, a.scratch, a.scratch_bytes, weight_grad_partials(a.grad->rows, a.grad->cols, a.act->cols),
-                      &scratch));
+  const size_t need = weight_grad_partials(a.grad->rows, a.grad->cols, a.act->cols);
+  if (a.scratch || need)     // rows that are not split leave no partial sums
+    LF_TRY(take_scratch(ctx, fn, a.scratch, a.scratch_bytes,
+                        a.scratch ? weight_grad_scratch(a.grad->rows, a.grad->cols, a.act->cols) : need, &scratch));
   const bool in_out = a.layout == LF_IN_OUT;
   const WeightGrad w{kept_view(in_out ? *a.act : *a.grad), kept_view(in_out ? *a.grad : *a.act), a.out, a.bias, in_out};
   return run_weight_grads(ctx, &w, 1, a.grad_dtype, scratch, "fp8.weight_grad");
@@ -448,7 +450,7 @@ size_t lf_layer_norm_backward_scratch(int rows, int channels) {
   return positive(rows, channels) ? lf::layer_norm_partials(rows, channels) : 0;
 }
 size_t lf_fp8_weight_grad_scratch(int rows, int outputs, int inputs) {
-  return positive(rows, outputs, inputs) ? lf::weight_grad_partials(rows, outputs, inputs) : 0;
+  return positive(rows, outputs, inputs) ? lf::weight_grad_scratch(rows, outputs, inputs) : 0;
 }
 size_t lf_transition_train_scratch(int rows, int channels, int hidden) {
   return positive(rows, channels, hidden) ? lf::train_bytes(rows, channels, hidden) : 0;

@@ -53,7 +53,8 @@ struct WeightGrad {
   void *out, *bias;
   bool bias_of_b;
 };
-size_t weight_grad_partials(int rows, int outputs, int inputs, int products = 1);   // of products of one size
+size_t weight_grad_partials(int rows, int outputs, int inputs, int products = 1);   // of products of one size; 0: not split
+size_t weight_grad_scratch(int rows, int outputs, int inputs);   // what a caller's buffer has: one split's sums at least
 int run_weight_grads(lf_context* ctx, const WeightGrad* w, int count, int dt, void* scratch, const char* label);
 
 // Adds [blocks][2 channels] partial sums of scale and offset gradients.

@@ -1185,3 +1185,36 @@ def test_linear_weight_specials(ctx, rows, k, n):
     D.fp8_linear(ctx, x8, w8, out=kept)
     v = values_of(kept)
     assert np.isnan(v[:, bad]).all() and np.isfinite(v[:, ~bad]).all()
+
+
+@pytest.mark.gpu
+def test_weight_grad_of_one_split_takes_no_workspace(ctx):
+    """Few rows are not split: their sums go straight to the result."""
+    from localfold_amd import device as D
+    rng = np.random.default_rng(0)
+    rows, n, k = 40, 3000, 2000
+    own = D.Context(0)
+    try:
+        g8, x8 = (D.checkpoint_pack(own, rows_of(rng, rows, c, torch.float32).to(own.device)) for c in (n, k))
+        before = own.memory_stats()
+        bias = torch.empty(n, device=own.device)
+        out = D.fp8_weight_grad(own, g8, x8, bias_out=bias)
+        torch.cuda.synchronize()
+        assert own.memory_stats() == before
+        given = torch.empty(own.lib.lf_fp8_weight_grad_scratch(rows, n, k), dtype=torch.uint8, device=own.device)
+        assert torch.equal(out, D.fp8_weight_grad(own, g8, x8, scratch=given))
+        many = D.checkpoint_pack(own, rows_of(rng, 5000, 64, torch.float32).to(own.device))
+        D.fp8_weight_grad(own, many, many)
+        torch.cuda.synchronize()
+        assert own.memory_stats()["currentBytes"] > before["currentBytes"]
+    finally:
+        own.close()
+
+
+def test_scratch_of_a_step_of_few_rows():
+    """A step whose weight gradients are not split asks for no partial sums of them."""
+    from localfold_amd import capi
+    lib = capi.load()
+    rows, c, h = 59, 384, 1536
+    operands = 2 * 2 * h * c + rows * (3 * (c + h) + 4 * c)     # packed weights, kept gradients, the norm's gradient
+    assert lib.lf_transition_backward_scratch(rows, c, h) < operands + 2 * c * 4 * 600
