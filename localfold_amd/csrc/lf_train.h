@@ -134,11 +134,11 @@ __device__ __forceinline__ void store8(typename Act<ACT>::T* p, int n, const flo
   }
 }
 
-// Largest magnitude of eight values; NaN is passed over, an infinity is not.
+// Largest magnitude of eight values, 0 where all are NaN; NaN is passed over, an infinity is not.
 __device__ __forceinline__ float amax8(const float (&v)[8]) {
-  float m = fmaxf(fabsf(v[0]), fabsf(v[1]));
+  float m = 0.f;
 #pragma unroll
-  for (int k = 2; k < 8; ++k) m = fmaxf(m, fabsf(v[k]));
+  for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(v[k]));
   return m;
 }
 __device__ __forceinline__ float amax8_finite(const float (&v)[8]) {

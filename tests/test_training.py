@@ -1218,3 +1218,21 @@ def test_scratch_of_a_step_of_few_rows():
     rows, c, h = 59, 384, 1536
     operands = 2 * 2 * h * c + rows * (3 * (c + h) + 4 * c)     # packed weights, kept gradients, the norm's gradient
     assert lib.lf_transition_backward_scratch(rows, c, h) < operands + 2 * c * 4 * 600
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+def test_checkpoint_scale_of_a_group_with_nothing_finite(ctx, dt):
+    """It has no largest finite value, so its scale is that of zeros, whether infinities or NaN are what it holds."""
+    from localfold_amd import device as D
+    for c in (64, 128, 200):
+        x = torch.ones(4, c, dtype=dt)
+        x[0], x[1], x[2, :] = float("nan"), float("inf"), float("nan")
+        x[2, 0] = -float("inf")
+        kept = D.checkpoint_pack(ctx, x.to(ctx.device))
+        ys = D.checkpoint_empty(4, c, ctx.device)      # a row with a NaN is normalised to NaN
+        D.layer_norm(ctx, x.to(ctx.device), torch.ones(c, device=ctx.device), torch.zeros(c, device=ctx.device), y_saved=ys)
+        torch.cuda.synchronize()
+        assert np.isnan(values_of(kept)[:3]).all() and np.isnan(values_of(ys)[:3]).all()
+        assert (kept.scales[:, :3] == 1).all() and (kept.scales[:, 3] == 119).all()
+        assert (ys.scales[:, :3] == 1).all()
