@@ -499,8 +499,9 @@ int lf_msa_module_block(lf_context* ctx, const lf_msa_block_args* args);
  * beyond, which become infinities), and added in f32, whatever the output's type; so are the products
  * inside the transition's step.
  *
- * Matrices are row-major and contiguous.  Inputs and outputs do not overlap except where it says
- * so.  Sums over rows (gradients of weights, biases, scales and offsets) are added in a fixed
+ * Matrices are row-major and contiguous, at most 65536 wide (a LayerNorm's rows 4096, weights 65536
+ * either way) and of at most 2^34 elements with their columns rounded up to 64.  Inputs and outputs do
+ * not overlap except where it says so.  Sums over rows (gradients of weights, biases, scales and offsets) are added in a fixed
  * order: the same call gives the same bits.
  *
  * scratch (lf_layer_norm_backward, lf_fp8_weight_grad, lf_transition_train and _backward): memory

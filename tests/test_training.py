@@ -1236,3 +1236,42 @@ def test_checkpoint_scale_of_a_group_with_nothing_finite(ctx, dt):
         assert np.isnan(values_of(kept)[:3]).all() and np.isnan(values_of(ys)[:3]).all()
         assert (kept.scales[:, :3] == 1).all() and (kept.scales[:, 3] == 119).all()
         assert (ys.scales[:, :3] == 1).all()
+
+
+@pytest.mark.gpu
+def test_products_at_the_ends_of_the_scales(ctx):
+    """Kept values are exact operands at scale bytes 3 to 246; below, multiples of 2^-133; from 2^128 on, infinities."""
+    from localfold_amd import capi, device as D
+    rows = 254
+    scales = torch.full((1, 256), 127, dtype=torch.uint8)
+    scales[0, :rows] = torch.arange(1, rows + 1)
+    w8 = D.fp8_weight(ctx, torch.eye(16, 128, device=ctx.device), capi.LF_OUT_IN)
+    for first, n in ((0x01, 126), (0x81, 126)):
+        for start in range(0, n, 16):
+            codes = torch.zeros(rows, 128, dtype=torch.uint8)
+            codes[:, :16] = torch.arange(first + start, first + start + 16).clamp(max=first + n - 1)
+            x8 = D.Checkpoint(rows, 128, codes.to(ctx.device), scales.to(ctx.device))
+            out, v = f64(D.fp8_linear(ctx, x8, w8, dtype=torch.float32)), values_of(x8)[:, :16]
+            assert np.array_equal(out[2:246], v[2:246])
+            assert (out[:2] % 2.0 ** -133 == 0).all() and (np.abs(out[:2] - v[:2]) <= 2.0 ** -134).all()
+            small = np.abs(v).max(1) < 2.0 ** 128     # beyond, an infinity times the other weights' zeros
+            assert np.array_equal(out[2:][small[2:]], v[2:][small[2:]]) and not np.isfinite(out[~small]).any()
+
+
+@pytest.mark.gpu
+def test_size_limits(ctx):
+    """Refused by the host, which launches nothing."""
+    import ctypes as C
+    from localfold_amd import capi
+    x = torch.zeros(1024, device=ctx.device)
+    for rows, cols, word in ((2 ** 28 + 1, 64, b"2^34"), (2 ** 28 + 1, 1, b"2^34"), (1, 65537, b"wide"), (0, 64, b"positive")):
+        kept = capi.lf_checkpoint(rows, cols, x.data_ptr(), x.data_ptr())
+        for entry in ("lf_checkpoint_pack", "lf_checkpoint_unpack"):
+            a = capi.lf_checkpoint_args(capi.LF_F32, x.data_ptr(), C.pointer(kept))
+            assert getattr(ctx.lib, entry)(ctx.handle, C.byref(a)) == capi.LF_ERR_INVALID
+            assert word in ctx.lib.lf_last_error()
+    w = capi.lf_fp8_weight_args()
+    out = capi.lf_fp8_weight(65537, 8, x.data_ptr(), x.data_ptr())
+    w.w = capi.lf_weight(capi.LF_F32, capi.LF_OUT_IN, 65537, 8, 0, x.data_ptr(), None, None)
+    w.out = C.pointer(out)
+    assert ctx.lib.lf_fp8_pack_weight(ctx.handle, C.byref(w)) == capi.LF_ERR_INVALID and b"65536" in ctx.lib.lf_last_error()
