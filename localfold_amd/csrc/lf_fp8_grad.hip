@@ -7,10 +7,10 @@
 // 128 x 128 outputs over its share of the rows, the teams on steps of 32 rows in turn, joined in LDS; the
 // blocks' partial sums are added in order by a second kernel.  Column sums are a product with ones.
 //
-// 196608 rows, 1024 x 256: 126 to 154 us from box to box (670 to 820 TFLOP/s; its bytes alone are 49 us); 147456 rows,
+// 196608 rows, 1024 x 256: 126 to 154 us from card to card (670 to 820 TFLOP/s; its bytes alone are 49 us); 147456 rows,
 // 512 x 128 and 128 x 512 in one launch: 56 us.  Nothing is full: matrix pipes, LDS and issue are each busy about 40 % of
 // the time, and overlap only as far as waves differ.  12 waves that load three steps ahead beat 16 of 128
-// registers that load two ahead: in turn on one box, medians with the join, 131 us and 137, 147456 rows of 512 x 128
+// registers that load two ahead: in turn on one card, medians with the join, 131 us and 137, 147456 rows of 512 x 128
 // 36.5 us and 38.1, 90601 rows of 128 x 128 22.3 us and 22.9.  Before those, 8 waves took 140 us and 78 us in two
 // launches, and forms that fetch fragments a step ahead 149 to 164 us and 63 us.  Codes in LDS, converted after the
 // read, halve its traffic but double the conversions: 166 us.
