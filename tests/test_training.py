@@ -1275,3 +1275,34 @@ def test_size_limits(ctx):
     w.w = capi.lf_weight(capi.LF_F32, capi.LF_OUT_IN, 65537, 8, 0, x.data_ptr(), None, None)
     w.out = C.pointer(out)
     assert ctx.lib.lf_fp8_pack_weight(ctx.handle, C.byref(w)) == capi.LF_ERR_INVALID and b"65536" in ctx.lib.lf_last_error()
+
+
+@pytest.mark.gpu
+def test_weight_grad_of_one_split_in_a_graph(ctx):
+    """It needs no scratch, so a captured call may come without; rows that are split are refused."""
+    from localfold_amd import capi, device as D
+    rng = np.random.default_rng(9)
+    g8, x8 = (D.checkpoint_pack(ctx, rows_of(rng, 50, c, torch.float32).to(ctx.device)) for c in (130, 70))
+    many = D.checkpoint_pack(ctx, rows_of(rng, 5000, 64, torch.float32).to(ctx.device))
+    out, bias = torch.empty(130, 70, device=ctx.device), torch.empty(130, device=ctx.device)
+    big = torch.empty(64, 64, device=ctx.device)
+    D.fp8_weight_grad(ctx, g8, x8, out=out, bias_out=bias)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph):
+            ctx.bind_stream()
+            with pytest.raises(capi.LocalfoldError, match="scratch"):
+                D.fp8_weight_grad(ctx, many, many, out=big)
+            D.fp8_weight_grad(ctx, g8, x8, out=out, bias_out=bias)
+    finally:
+        ctx.bind_stream()
+    for turn in range(3):
+        D.checkpoint_pack(ctx, rows_of(rng, 50, 130, torch.float32).to(ctx.device), out=g8)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone(), bias.clone()
+        D.fp8_weight_grad(ctx, many, many, out=big)      # eager, with the workspace
+        D.fp8_weight_grad(ctx, g8, x8, out=out, bias_out=bias)
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], out) and torch.equal(got[1], bias), turn
