@@ -657,6 +657,167 @@ typedef struct {
 int lf_transition_backward(lf_context* ctx, const lf_transition_backward_args* args);
 size_t lf_transition_backward_scratch(int rows, int channels, int hidden);
 
+/* ---- training: relative positions, products of 4 bits, orthogonalised updates ------------------ */
+
+/* Beside the section above and under its rules for sums, alignment, overlap and scratch.
+ *
+ * A learned row per relative position, added to every pair: the embedder's relpos_w and relpos_b
+ * (lf_input_embedder: boundaries -31..32, 65 rows) with any buckets, chains and lengths, and its
+ * gradient.  The bucket of query i and key j is the number of boundaries, ascending, that are at most
+ * query_positions[i] - key_positions[j].  With segments (chains), pairs of different segments take the
+ * table's last row, and a negative segment is padding: nothing is added to its pairs, and their
+ * gradient, whatever it holds, is left out. */
+typedef struct {
+  int queries, keys;
+  const int *query_positions, *key_positions;   /* [queries], [keys] */
+  const int *query_segments, *key_segments;     /* [queries], [keys], or both NULL */
+  int boundary_count;                           /* 0..4095 */
+  const int* boundaries;                        /* [boundary_count] */
+} lf_relative_pairs;
+/* Rows of the table: a bucket each, and one for pairs of different segments. */
+#define LF_RELATIVE_ROWS(pairs) ((pairs)->boundary_count + 1 + ((pairs)->query_segments ? 1 : 0))
+
+typedef struct {
+  const lf_relative_pairs* pairs;
+  int channels;                /* 1..4096 */
+  int table_dtype;
+  const void* table;           /* [rows, channels] */
+  const float* bias;           /* [channels], added to every row of the table, or NULL */
+  int act_dtype;
+  const void* act;             /* [queries, keys, channels], added last, or NULL */
+  void* out;                   /* [queries, keys, channels], may alias act */
+} lf_relative_position_args;
+
+int lf_relative_position(lf_context* ctx, const lf_relative_position_args* args);
+
+typedef struct {
+  const lf_relative_pairs* pairs;
+  int channels;
+  int act_dtype;
+  const void* grad;            /* [queries, keys, channels]: of lf_relative_position's out */
+  int grad_dtype;              /* of the gradients below */
+  void* grad_table;            /* [rows, channels]: the sum over a row's pairs, 0 where it has none */
+  void* grad_bias;             /* [channels]: the sum over all pairs, or NULL */
+  void* scratch;
+  size_t scratch_bytes;
+} lf_relative_position_backward_args;
+
+int lf_relative_position_backward(lf_context* ctx, const lf_relative_position_backward_args* args);
+size_t lf_relative_position_backward_scratch(const lf_relative_pairs* pairs, int channels);   /* reads no tensor */
+
+/* A [rows, cols] matrix in 4 bits: e2m1 codes (0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives) with
+ * one scale per row and group of 32 columns, a power of two 2^(b - 127) with b in 1..254 as stored, the
+ * smallest that puts the group's largest magnitude within 6 (b = 1 for a group of zeros).  The
+ * division by it is exact, so the code's rounding (to nearest, ties to even; half the step of 1/2, 1 or
+ * 2 scales) is the only one.  There is no code for an infinity or a NaN: a group that holds one gets b
+ * = 255 and reads back as NaN, all 32 of it.  A value within 2^-3 of the largest of its type may round up to
+ * a power of two beyond it, which reads back as an infinity of that type.
+ *
+ *   codes   [rows][LF_MX4_PITCH(cols) / 2], two a byte, the lower column in the lower half; columns
+ *           from cols to the pitch hold zeros
+ *   scales  [LF_MX4_GROUPS(cols)][LF_MX4_SCALE_PITCH(rows)], one byte b each (not 255 for groups
+ *           behind the last column); bytes of rows >= rows may hold anything
+ *
+ * codes and scales are 16-byte aligned.  At most 2^34 elements, columns rounded up to 128 and rows to 16. */
+typedef struct {
+  int rows, cols;
+  void* codes;
+  void* scales;
+} lf_mx4;
+#define LF_MX4_PITCH(cols) (((size_t)(cols) + 127) / 128 * 128)
+#define LF_MX4_GROUPS(cols) (LF_MX4_PITCH(cols) / 32)
+#define LF_MX4_SCALE_PITCH(rows) (((size_t)(rows) + 15) / 16 * 16)
+
+typedef struct {
+  int rows, cols;
+  int act_dtype;
+  const void* act;             /* [rows, cols] */
+  const lf_mx4* out;           /* [rows, cols], groups along the columns, or NULL */
+  const lf_mx4* transposed;    /* [cols, rows], groups along the rows, or NULL */
+  int sums_dtype;
+  void* sums;                  /* [cols]: the sum of act's rows (not of its codes), or NULL */
+  void* scratch;
+  size_t scratch_bytes;
+} lf_mx4_pack_args;
+
+/* Activations, gradients or weights to 4 bits: `out` is the operand of products along the columns (an
+ * [outputs, inputs] weight, activations), `transposed` of products along the rows (the weight of the
+ * input's gradient; gradient and activations of the weight's).  At least one output is given. */
+int lf_mx4_pack(lf_context* ctx, const lf_mx4_pack_args* args);
+size_t lf_mx4_pack_scratch(int rows, int cols);   /* for sums; 0 is needed without */
+
+typedef struct {
+  int act_dtype;
+  void* act;                   /* [rows, cols] of `kept`, written */
+  const lf_mx4* kept;
+} lf_mx4_unpack_args;
+
+/* The values that codes and scales stand for, rounded to act_dtype. */
+int lf_mx4_unpack(lf_context* ctx, const lf_mx4_unpack_args* args);
+
+typedef struct {
+  int rows;
+  const lf_mx4* kept;          /* [rows, inputs], or NULL: act */
+  int act_dtype;
+  const void* act;             /* [rows, inputs], quantised as lf_mx4_pack does; or NULL: kept */
+  const lf_mx4* w;             /* [outputs, inputs] */
+  const float* bias;           /* [outputs] or NULL */
+  int relu;                    /* values below zero become zero, after the bias */
+  int out_dtype;
+  const void* residual;        /* [rows, outputs], out_dtype, added last, or NULL */
+  void* out;                   /* [rows, outputs], may alias residual */
+  void* scratch;
+  size_t scratch_bytes;
+} lf_mx4_linear_args;
+
+/* out = act w^T + bias.  Products are exact, sums are f32's.  The weight's gradient is the same product
+ * of transposed packs: kept = the gradient's [outputs, rows], w = the activations' [inputs, rows]. */
+int lf_mx4_linear(lf_context* ctx, const lf_mx4_linear_args* args);
+size_t lf_mx4_linear_scratch(int rows, int inputs, int outputs, int from_act);   /* from_act: act is given */
+
+/* Matrices made orthogonal by Newton-Schulz products: with X = act / (|act| + epsilon), |.| the
+ * Frobenius norm, and (a, b, c) a step's coefficients, X <- a X + (b G + c G^2) X, G = X X^T, `steps`
+ * times (for matrices taller than wide the same of the transpose).  Singular values go through
+ * a s + b s^3 + c s^5 each time, vectors stay.  Products are of f32 precision (two f16 parts each, sums in
+ * f32).  Coefficients whose polynomials leave 2^24 on what [0, 1] can become are refused. */
+typedef struct {
+  int batch, rows, cols;       /* rows, cols 1..16384, batch 1..65535 */
+  int act_dtype;
+  const void* act;             /* [batch, rows, cols] */
+  void* out;                   /* [batch, rows, cols], may alias act */
+  int steps;                   /* 1..32 */
+  const float* coefficients;   /* HOST memory: [steps][3], read before the call returns */
+  float epsilon;               /* >= 0; a matrix of zeros with 0 becomes NaN */
+  void* scratch;
+  size_t scratch_bytes;
+} lf_orthogonalize_args;
+
+int lf_orthogonalize(lf_context* ctx, const lf_orthogonalize_args* args);
+
+/* An optimiser's step for a batch of weight matrices: m' = momentum_factor m + grad, u = grad +
+ * momentum_factor m' (nesterov) or m', weight' = (1 - rate decay) weight - rate scale O(u), O as above. */
+typedef struct {
+  int batch, rows, cols;
+  int grad_dtype;
+  const void* grad;            /* [batch, rows, cols] */
+  const float* momentum;       /* [batch, rows, cols]: m, or NULL with momentum_out: u = grad */
+  float* momentum_out;         /* m', may alias momentum */
+  float momentum_factor;
+  int nesterov;
+  int weight_dtype;
+  const void* weight;          /* [batch, rows, cols] */
+  void* weight_out;            /* may alias weight */
+  float rate, decay, scale;
+  int steps;
+  const float* coefficients;   /* as above */
+  float epsilon;
+  void* scratch;
+  size_t scratch_bytes;
+} lf_muon_step_args;
+
+int lf_muon_step(lf_context* ctx, const lf_muon_step_args* args);
+size_t lf_muon_scratch(int batch, int rows, int cols);   /* for both */
+
 #ifdef __cplusplus
 }
 #endif

@@ -251,6 +251,57 @@ class lf_transition_backward_args(C.Structure):
                 ("scratch", P), ("scratch_bytes", C.c_size_t)]
 
 
+class lf_relative_pairs(C.Structure):
+    _fields_ = [("queries", C.c_int), ("keys", C.c_int), ("query_positions", P), ("key_positions", P),
+                ("query_segments", P), ("key_segments", P), ("boundary_count", C.c_int), ("boundaries", P)]
+
+
+class lf_relative_position_args(C.Structure):
+    _fields_ = [("pairs", C.POINTER(lf_relative_pairs)), ("channels", C.c_int), ("table_dtype", C.c_int), ("table", P),
+                ("bias", P), ("act_dtype", C.c_int), ("act", P), ("out", P)]
+
+
+class lf_relative_position_backward_args(C.Structure):
+    _fields_ = [("pairs", C.POINTER(lf_relative_pairs)), ("channels", C.c_int), ("act_dtype", C.c_int), ("grad", P),
+                ("grad_dtype", C.c_int), ("grad_table", P), ("grad_bias", P), ("scratch", P), ("scratch_bytes", C.c_size_t)]
+
+
+class lf_mx4(C.Structure):
+    _fields_ = [("rows", C.c_int), ("cols", C.c_int), ("codes", P), ("scales", P)]
+
+
+MX4 = C.POINTER(lf_mx4)
+
+
+class lf_mx4_pack_args(C.Structure):
+    _fields_ = [("rows", C.c_int), ("cols", C.c_int), ("act_dtype", C.c_int), ("act", P), ("out", MX4),
+                ("transposed", MX4), ("sums_dtype", C.c_int), ("sums", P), ("scratch", P), ("scratch_bytes", C.c_size_t)]
+
+
+class lf_mx4_unpack_args(C.Structure):
+    _fields_ = [("act_dtype", C.c_int), ("act", P), ("kept", MX4)]
+
+
+class lf_mx4_linear_args(C.Structure):
+    _fields_ = [("rows", C.c_int), ("kept", MX4), ("act_dtype", C.c_int), ("act", P), ("w", MX4), ("bias", P),
+                ("relu", C.c_int), ("out_dtype", C.c_int), ("residual", P), ("out", P), ("scratch", P),
+                ("scratch_bytes", C.c_size_t)]
+
+
+class lf_orthogonalize_args(C.Structure):
+    _fields_ = [("batch", C.c_int), ("rows", C.c_int), ("cols", C.c_int), ("act_dtype", C.c_int), ("act", P), ("out", P),
+                ("steps", C.c_int), ("coefficients", C.POINTER(C.c_float)), ("epsilon", C.c_float), ("scratch", P),
+                ("scratch_bytes", C.c_size_t)]
+
+
+class lf_muon_step_args(C.Structure):
+    _fields_ = [("batch", C.c_int), ("rows", C.c_int), ("cols", C.c_int), ("grad_dtype", C.c_int), ("grad", P),
+                ("momentum", P), ("momentum_out", P), ("momentum_factor", C.c_float), ("nesterov", C.c_int),
+                ("weight_dtype", C.c_int), ("weight", P), ("weight_out", P), ("rate", C.c_float), ("decay", C.c_float),
+                ("scale", C.c_float), ("steps", C.c_int), ("coefficients", C.POINTER(C.c_float)),
+                ("epsilon", C.c_float), ("scratch", P), ("scratch_bytes", C.c_size_t)]
+
+
 PROTOTYPES = [
     ("lf_context_create", P, [C.c_int]),
     ("lf_context_destroy", None, [P]),
@@ -295,6 +346,17 @@ PROTOTYPES = [
     ("lf_transition_train_scratch", C.c_size_t, [C.c_int, C.c_int, C.c_int]),
     ("lf_transition_backward", C.c_int, [P, C.POINTER(lf_transition_backward_args)]),
     ("lf_transition_backward_scratch", C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    ("lf_relative_position", C.c_int, [P, C.POINTER(lf_relative_position_args)]),
+    ("lf_relative_position_backward", C.c_int, [P, C.POINTER(lf_relative_position_backward_args)]),
+    ("lf_relative_position_backward_scratch", C.c_size_t, [C.POINTER(lf_relative_pairs), C.c_int]),
+    ("lf_mx4_pack", C.c_int, [P, C.POINTER(lf_mx4_pack_args)]),
+    ("lf_mx4_pack_scratch", C.c_size_t, [C.c_int, C.c_int]),
+    ("lf_mx4_unpack", C.c_int, [P, C.POINTER(lf_mx4_unpack_args)]),
+    ("lf_mx4_linear", C.c_int, [P, C.POINTER(lf_mx4_linear_args)]),
+    ("lf_mx4_linear_scratch", C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int]),
+    ("lf_orthogonalize", C.c_int, [P, C.POINTER(lf_orthogonalize_args)]),
+    ("lf_muon_step", C.c_int, [P, C.POINTER(lf_muon_step_args)]),
+    ("lf_muon_scratch", C.c_size_t, [C.c_int, C.c_int, C.c_int]),
 ]
 
 _lib = None

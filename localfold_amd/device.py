@@ -1075,3 +1075,257 @@ def transition_backward(ctx: Context, grad: torch.Tensor, wstruct: capi.lf_trans
     a.grad_w2, a.grad_b2 = at["secondWeight"], at.get("secondBias")
     check(ctx.lib.lf_transition_backward(ctx.handle, C.byref(a)))
     return out, grads
+
+
+# ---------------------------------------------------------------------------------------
+# Training: relative positions, products of 4 bits, orthogonalised updates.  Tensors are contiguous and
+# on the context's device.
+# ---------------------------------------------------------------------------------------
+
+def clipped_boundaries(max_relative: int, device="cpu") -> torch.Tensor:
+    """Boundaries of one bucket per difference, those beyond +-max_relative sharing the outer two
+    (2 max_relative + 1 buckets; the embedder's are of 32)."""
+    if max_relative < 1:
+        raise ValueError(f"max_relative must be positive, got {max_relative}")
+    return torch.arange(1 - max_relative, max_relative + 1, dtype=torch.int32, device=device)
+
+
+def log_boundaries(buckets: int, max_distance: int, device="cpu") -> torch.Tensor:
+    """Boundaries of an even number of buckets, half of them for positive differences: single distances up
+    to buckets / 4, then ratios that stay the same up to max_distance, where the last bucket begins."""
+    half = buckets // 2
+    near = max(1, half // 2)
+    if buckets < 4 or buckets % 2 or max_distance < near:
+        raise ValueError(f"buckets must be even and 4 at least, max_distance {near} at least; got {buckets}, {max_distance}")
+    steps = list(range(1, near + 1))
+    n = near
+    for j in range(1, half - near + 1):     # the first n >= near (max_distance / near)^(j / (half - near)), in whole numbers
+        while n ** (half - near) < near ** (half - near - j) * max_distance ** j:
+            n += 1
+        steps.append(n)
+    return torch.tensor([1 - s for s in reversed(steps[1:])] + steps, dtype=torch.int32, device=device)
+
+
+def _relative_pairs(ctx: Context, boundaries, positions, key_positions, segments, key_segments) -> capi.lf_relative_pairs:
+    if key_positions is None:
+        if key_segments is not None:
+            raise ValueError("key_segments without key_positions")
+        key_positions, key_segments = positions, segments
+    if (segments is None) != (key_segments is None):
+        raise ValueError("segments and key_segments are given together")
+    for name, t in (("positions", positions), ("key_positions", key_positions), ("boundaries", boundaries)):
+        if t.dim() != 1 or t.shape[0] > _MOST:
+            raise ValueError(f"{name} must have one dimension, got shape {tuple(t.shape)}")
+    q, k, i32 = positions.shape[0], key_positions.shape[0], torch.int32
+    return capi.lf_relative_pairs(q, k, _tensor(ctx, "positions", positions, None, i32),
+                                  _tensor(ctx, "key_positions", key_positions, None, i32),
+                                  _tensor(ctx, "segments", segments, (q,), i32),
+                                  _tensor(ctx, "key_segments", key_segments, (k,), i32), boundaries.shape[0],
+                                  _tensor(ctx, "boundaries", boundaries, None, i32) or None)
+
+
+def _relative_rows(p: capi.lf_relative_pairs) -> int:
+    return p.boundary_count + 1 + (p.query_segments is not None)
+
+
+def relative_position(ctx: Context, table: torch.Tensor, boundaries: torch.Tensor, positions: torch.Tensor,
+                      key_positions: torch.Tensor = None, segments: torch.Tensor = None, key_segments: torch.Tensor = None,
+                      bias: torch.Tensor = None, pair: torch.Tensor = None, out: torch.Tensor = None,
+                      dtype=None) -> torch.Tensor:
+    """table[bucket] + bias, added to `pair` where it is given, for every query and key (lf_relative_position):
+    [queries, keys, channels].  The bucket is the number of `boundaries` (int32, ascending) that are at most
+    positions[i] - key_positions[j]; keys are the queries where key_positions is None.  With `segments`,
+    pairs of different segments take the table's last row and pairs with a negative one get nothing.
+    `out` may be `pair`; its dtype is pair's, `dtype` or table's."""
+    p = _relative_pairs(ctx, boundaries, positions, key_positions, segments, key_segments)
+    if table.dim() != 2 or table.shape[0] != _relative_rows(p):
+        raise ValueError(f"table has shape {tuple(table.shape)}; expected {_relative_rows(p)} rows")
+    c = table.shape[1]
+    shape = (p.queries, p.keys, c)
+    if out is None:
+        out = torch.empty(shape, dtype=pair.dtype if pair is not None else dtype or table.dtype, device=ctx.device)
+    a = capi.lf_relative_position_args(C.pointer(p), c, act_code(table), _tensor(ctx, "table", table),
+                                       _tensor(ctx, "bias", bias, (c,), torch.float32), act_code(out),
+                                       _tensor(ctx, "pair", pair, shape, out.dtype), _tensor(ctx, "out", out, shape))
+    check(ctx.lib.lf_relative_position(ctx.handle, C.byref(a)))
+    return out
+
+
+def relative_position_backward(ctx: Context, grad: torch.Tensor, boundaries: torch.Tensor, positions: torch.Tensor,
+                               key_positions: torch.Tensor = None, segments: torch.Tensor = None,
+                               key_segments: torch.Tensor = None, table_grad: torch.Tensor = None,
+                               bias_grad: torch.Tensor = None, grad_dtype=torch.float32, scratch: torch.Tensor = None):
+    """The table's gradient (lf_relative_position_backward), and in `bias_grad` [channels], where it is given,
+    the bias's; pair's is `grad` itself."""
+    p = _relative_pairs(ctx, boundaries, positions, key_positions, segments, key_segments)
+    if grad.dim() != 3:
+        raise ValueError(f"grad has shape {tuple(grad.shape)}; expected [queries, keys, channels]")
+    c = grad.shape[2]
+    if table_grad is None:
+        table_grad = torch.empty((_relative_rows(p), c), dtype=grad_dtype, device=ctx.device)
+    a = capi.lf_relative_position_backward_args(C.pointer(p), c, act_code(grad),
+                                                _tensor(ctx, "grad", grad, (p.queries, p.keys, c)), act_code(table_grad),
+                                                _tensor(ctx, "table_grad", table_grad, (_relative_rows(p), c)),
+                                                _tensor(ctx, "bias_grad", bias_grad, (c,), table_grad.dtype))
+    _scratch(ctx, a, scratch)
+    check(ctx.lib.lf_relative_position_backward(ctx.handle, C.byref(a)))
+    return table_grad
+
+
+class Mx4:
+    """A [rows, cols] matrix in 4 bits: `codes` uint8 [rows, half of cols rounded up to 128] (two e2m1 codes, the
+    lower column in the lower half), `scales` uint8 [groups of 32 columns, rows rounded up to 16], a byte b standing
+    for 2^(b - 127)."""
+
+    def __init__(self, rows: int, cols: int, codes: torch.Tensor, scales: torch.Tensor):
+        if max(rows, cols) > _MOST:
+            raise ValueError(f"a 4-bit matrix of {rows} x {cols}; dimensions are at most {_MOST}")
+        want = (rows, -(-cols // 128) * 64), (-(-cols // 128) * 4, -(-rows // 16) * 16)
+        for name, t, shape in (("codes", codes, want[0]), ("scales", scales, want[1])):
+            if tuple(t.shape) != shape or t.dtype != torch.uint8 or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous uint8 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+        if codes.device != scales.device:
+            raise ValueError(f"codes are on {codes.device}, scales on {scales.device}")
+        self.rows, self.cols, self.codes, self.scales, self.device = rows, cols, codes, scales, codes.device
+        self.struct = capi.lf_mx4(rows, cols, codes.data_ptr(), scales.data_ptr())
+        self._pointer = C.pointer(self.struct)
+
+    def _ref(self, ctx: Context, name: str, shape=None):
+        if self.device != ctx.device:
+            raise ValueError(f"{name} is on {self.device}; the context is on {ctx.device}")
+        if shape is not None and (self.rows, self.cols) != shape:
+            raise ValueError(f"{name} is {self.rows} x {self.cols}; expected {shape[0]} x {shape[1]}")
+        return self._pointer
+
+
+def mx4_empty(rows: int, cols: int, device) -> Mx4:
+    codes = torch.empty((rows, -(-cols // 128) * 64), dtype=torch.uint8, device=device)
+    scales = torch.empty((-(-cols // 128) * 4, -(-rows // 16) * 16), dtype=torch.uint8, device=device)
+    return Mx4(rows, cols, codes, scales)
+
+
+def mx4_pack(ctx: Context, x: torch.Tensor, out: Mx4 = None, transposed: Mx4 = None, sums: torch.Tensor = None,
+             scratch: torch.Tensor = None) -> Mx4:
+    """x [..., cols] in 4 bits (lf_mx4_pack) with groups along the columns, in `out`, and along the rows, in
+    `transposed` [cols, rows]; `sums` [cols] receives the sum of the rows.  Writes whichever are given; `out`
+    is made when none is."""
+    rows, cols = _rows(x)
+    if out is None and transposed is None and sums is None:
+        out = mx4_empty(rows, cols, ctx.device)
+    a = capi.lf_mx4_pack_args()
+    a.rows, a.cols, a.act_dtype, a.act = rows, cols, act_code(x), _tensor(ctx, "x", x)
+    if out is not None:
+        a.out = out._ref(ctx, "out", (rows, cols))
+    if transposed is not None:
+        a.transposed = transposed._ref(ctx, "transposed", (cols, rows))
+    if sums is not None:
+        a.sums_dtype, a.sums = act_code(sums), _tensor(ctx, "sums", sums, (cols,))
+    _scratch(ctx, a, scratch)
+    check(ctx.lib.lf_mx4_pack(ctx.handle, C.byref(a)))
+    return out
+
+
+def mx4_unpack(ctx: Context, kept: Mx4, dtype=torch.float32, out: torch.Tensor = None) -> torch.Tensor:
+    """The values that a 4-bit matrix stands for (lf_mx4_unpack)."""
+    if out is None:
+        out = torch.empty((kept.rows, kept.cols), dtype=dtype, device=ctx.device)
+    if _rows(out) != (kept.rows, kept.cols):
+        raise ValueError(f"out has shape {tuple(out.shape)}; expected {kept.rows} x {kept.cols}")
+    a = capi.lf_mx4_unpack_args(act_code(out), _tensor(ctx, "out", out), kept._ref(ctx, "kept"))
+    check(ctx.lib.lf_mx4_unpack(ctx.handle, C.byref(a)))
+    return out
+
+
+def mx4_linear(ctx: Context, x, w: Mx4, bias: torch.Tensor = None, relu: bool = False, residual: torch.Tensor = None,
+               out: torch.Tensor = None, dtype=torch.bfloat16, scratch: torch.Tensor = None) -> torch.Tensor:
+    """x w^T + bias (lf_mx4_linear).  x: an Mx4, or a tensor [..., inputs] that is quantised as mx4_pack does;
+    `residual` is added last and may be `out`.  The weight's gradient is the product of the gradient's and the
+    activations' transposed packs."""
+    a = capi.lf_mx4_linear_args()
+    if isinstance(x, Mx4):
+        rows, lead = x.rows, (x.rows,)
+        a.kept = x._ref(ctx, "x", (x.rows, w.cols))
+    else:
+        rows, cols = _rows(x)
+        if cols != w.cols:
+            raise ValueError(f"x has shape {tuple(x.shape)}; expected rows of {w.cols}")
+        lead = x.shape[:-1]
+        a.act_dtype, a.act = act_code(x), _tensor(ctx, "x", x)
+    if out is None:
+        out = torch.empty((*lead, w.rows), dtype=residual.dtype if residual is not None else dtype, device=ctx.device)
+    if _rows(out) != (rows, w.rows):
+        raise ValueError(f"out has shape {tuple(out.shape)}; expected {rows} x {w.rows}")
+    a.rows, a.w, a.relu = rows, w._ref(ctx, "w"), int(relu)
+    a.bias = _tensor(ctx, "bias", bias, (w.rows,), torch.float32)
+    a.out_dtype, a.out = act_code(out), _tensor(ctx, "out", out)
+    a.residual = _tensor(ctx, "residual", residual, out.shape, out.dtype)
+    _scratch(ctx, a, scratch)
+    check(ctx.lib.lf_mx4_linear(ctx.handle, C.byref(a)))
+    return out
+
+
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)     # steep at zero: five steps bring singular values from 1e-3 up into 0.7 .. 1.2
+
+
+def _matrices(name: str, t: torch.Tensor):
+    if t.dim() < 2:
+        raise ValueError(f"{name} must be matrices [..., rows, cols], got shape {tuple(t.shape)}")
+    rows, cols = t.shape[-2:]
+    if rows == 0 or cols == 0 or max(rows, cols, t.numel() // (rows * cols)) > _MOST:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}")
+    return t.numel() // (rows * cols), rows, cols
+
+
+def _coefficients(coefficients, steps: int):
+    """[steps][3] floats for a call: one triple for every step, or one for each."""
+    if not 1 <= steps <= 32:
+        raise ValueError(f"steps must be in 1..32, got {steps}")
+    if not hasattr(coefficients[0], "__len__"):
+        coefficients = [coefficients] * steps
+    if len(coefficients) != steps or any(len(c) != 3 for c in coefficients):
+        raise ValueError(f"coefficients are three numbers, or three for each of {steps} steps")
+    return (C.c_float * (3 * steps))(*(float(v) for c in coefficients for v in c))
+
+
+def orthogonalize(ctx: Context, x: torch.Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ, epsilon: float = 1e-7,
+                  out: torch.Tensor = None, scratch: torch.Tensor = None) -> torch.Tensor:
+    """Each matrix of x [..., rows, cols] made orthogonal by `steps` Newton-Schulz products (lf_orthogonalize);
+    `coefficients`: (a, b, c), or one such triple a step.  `out` may be x."""
+    if out is None:
+        out = torch.empty_like(x)
+    a = capi.lf_orthogonalize_args()
+    a.batch, a.rows, a.cols = _matrices("x", x)
+    a.act_dtype, a.act, a.out = act_code(x), _tensor(ctx, "x", x), _tensor(ctx, "out", out, x.shape, x.dtype)
+    a.steps, a.coefficients, a.epsilon = steps, _coefficients(coefficients, steps), epsilon
+    _scratch(ctx, a, scratch)
+    check(ctx.lib.lf_orthogonalize(ctx.handle, C.byref(a)))
+    return out
+
+
+def muon_step(ctx: Context, weight: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor = None, rate: float = 0.02,
+              decay: float = 0.0, momentum_factor: float = 0.95, nesterov: bool = True, scale: float = None,
+              steps: int = 5, coefficients=NEWTON_SCHULZ, epsilon: float = 1e-7, out: torch.Tensor = None,
+              momentum_out: torch.Tensor = None, scratch: torch.Tensor = None) -> torch.Tensor:
+    """An optimiser's step of weight matrices [..., rows, cols] (lf_muon_step): m' = momentum_factor m + grad,
+    u = grad + momentum_factor m' (or m' without nesterov), weight' = (1 - rate decay) weight - rate scale O(u), O as
+    orthogonalize.  In place unless `out` and `momentum_out` are given; momentum is float32, None for u = grad;
+    `scale` is max(1, rows / cols)^(1/2) unless given."""
+    a = capi.lf_muon_step_args()
+    a.batch, a.rows, a.cols = _matrices("weight", weight)
+    out = weight if out is None else out
+    a.grad_dtype, a.grad = act_code(grad), _tensor(ctx, "grad", grad, weight.shape)
+    if momentum is not None:
+        a.momentum = _tensor(ctx, "momentum", momentum, weight.shape, torch.float32)
+        a.momentum_out = _tensor(ctx, "momentum_out", momentum if momentum_out is None else momentum_out, weight.shape,
+                                 torch.float32)
+    elif momentum_out is not None:
+        raise ValueError("momentum_out without momentum")
+    a.momentum_factor, a.nesterov = momentum_factor, int(nesterov)
+    a.weight_dtype, a.weight = act_code(weight), _tensor(ctx, "weight", weight)
+    a.weight_out = _tensor(ctx, "out", out, weight.shape, weight.dtype)
+    a.rate, a.decay = rate, decay
+    a.scale = max(1.0, a.rows / a.cols) ** 0.5 if scale is None else scale
+    a.steps, a.coefficients, a.epsilon = steps, _coefficients(coefficients, steps), epsilon
+    _scratch(ctx, a, scratch)
+    check(ctx.lib.lf_muon_step(ctx.handle, C.byref(a)))
+    return out
