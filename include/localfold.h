@@ -718,7 +718,7 @@ size_t lf_relative_position_backward_scratch(const lf_relative_pairs* pairs, int
  *   scales  [LF_MX4_GROUPS(cols)][LF_MX4_SCALE_PITCH(rows)], one byte b each (not 255 for groups
  *           behind the last column); bytes of rows >= rows may hold anything
  *
- * codes and scales are 16-byte aligned.  At most 2^34 elements, columns rounded up to 128 and rows to 16. */
+ * codes and scales are 16-byte aligned.  At most 2^26 columns and 2^34 elements, columns rounded up to 128 and rows to 16. */
 typedef struct {
   int rows, cols;
   void* codes;

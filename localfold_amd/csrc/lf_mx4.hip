@@ -1,4 +1,4 @@
-// Matrices of 4 bits: pack, unpack and products (lf_mx4_pack, lf_mx4_unpack, lf_mx4_linear).
+// Matrices of 4 bits: pack and unpack (lf_mx4_pack, lf_mx4_unpack).
 #include <algorithm>
 
 #include "lf_mx4.h"
@@ -138,123 +138,6 @@ int run_mx4_unpack(lf_context* ctx, const lf_mx4_unpack_args& a) {
   else if (a.act_dtype == LF_F16) go_unpack<DT_F16>(a, ctx->stream);
   else go_unpack<DT_BF16>(a, ctx->stream);
   return check_hip(hipGetLastError(), "4-bit unpack launch");
-}
-
-// ---- products ------------------------------------------------------------------------------------
-
-struct MxLinear {
-  Mx x, w;
-  int rows, outputs, steps;      // steps of 128 columns
-  const float* bias;
-  int relu;
-  const void* residual;
-  void* out;
-};
-
-// w is the instruction's first operand, so a lane's sums are 4 outputs of one row.  Row i of tile t (of 4) of the
-// first operand is output 4 f(i) + t: the scale bytes of a lane's four tiles are one word.  f puts the 16 outputs
-// that a lane holds in runs of 16 bytes, four lanes' runs side by side.
-template <int OUT>
-__device__ __forceinline__ int mx_f(int i) {
-  return OUT == DT_F32 ? (i & 3) * 4 + (i >> 2) : (i & 2) * 4 + (i >> 2) * 2 + (i & 1);
-}
-
-// A wave computes 64 rows by 64 outputs, operands straight from memory.
-template <int OUT>
-__global__ __launch_bounds__(256) void mx4_linear_kernel(MxLinear p, int out_tiles, long long tiles) {
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const long long tile = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (tile >= tiles) return;
-  const long long m0 = tile / out_tiles * 64;
-  const int n0 = (int)(tile % out_tiles) * 64;
-  const uint8_t *wrow[4], *xrow[4];
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {     // rows past the end repeat the last one
-    wrow[t] = p.w.codes + (size_t)min(n0 + 4 * mx_f<OUT>(r) + t, p.outputs - 1) * p.w.pitch + 16 * g;
-    xrow[t] = p.x.codes + (size_t)min(m0 + 4 * r + t, (long long)p.rows - 1) * p.x.pitch + 16 * g;
-  }
-  // scale rows are whole sixteens: a word of four is in bounds where its first byte's row exists
-  const uint8_t* ws = p.w.scales + (size_t)g * p.w.sp + min(n0 + 4 * mx_f<OUT>(r), (p.outputs - 1) & ~3);
-  const uint8_t* xs = p.x.scales + (size_t)g * p.x.sp + min(m0 + 4 * r, ((long long)p.rows - 1) & ~3LL);
-  f4 acc[4][4];
-#pragma unroll
-  for (int t = 0; t < 4; ++t)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) acc[t][q] = f4{0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < p.steps; ++s) {
-    u32x4 a[4], b[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      a[t] = *reinterpret_cast<const u32x4*>(wrow[t] + (size_t)s * 64);
-      b[t] = *reinterpret_cast<const u32x4*>(xrow[t] + (size_t)s * 64);
-    }
-    const uint32_t sa = *reinterpret_cast<const uint32_t*>(ws + (size_t)4 * s * p.w.sp);
-    const uint32_t sb = *reinterpret_cast<const uint32_t*>(xs + (size_t)4 * s * p.x.sp);
-#define MX_ROW(T)                                     \
-  acc[T][0] = mx_mma<T, 0>(a[T], b[0], acc[T][0], sa, sb); \
-  acc[T][1] = mx_mma<T, 1>(a[T], b[1], acc[T][1], sa, sb); \
-  acc[T][2] = mx_mma<T, 2>(a[T], b[2], acc[T][2], sa, sb); \
-  acc[T][3] = mx_mma<T, 3>(a[T], b[3], acc[T][3], sa, sb);
-    MX_ROW(0) MX_ROW(1) MX_ROW(2) MX_ROW(3)
-#undef MX_ROW
-  }
-  typedef typename Act<OUT>::T T;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const long long m = m0 + 4 * r + q;
-    if (m >= p.rows) continue;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int n = n0 + 4 * mx_f<OUT>(4 * g + j) + t;
-        if (n >= p.outputs) continue;
-        float v = acc[t][q][j];
-        if (p.bias) v += p.bias[n];
-        if (p.relu) v = __builtin_elementwise_maximum(v, 0.f);   // keeps NaN
-        const size_t at = (size_t)m * p.outputs + n;
-        if (p.residual) v += Act<OUT>::ld(static_cast<const T*>(p.residual) + at);
-        Act<OUT>::st(static_cast<T*>(p.out) + at, v);
-      }
-  }
-}
-
-size_t mx4_linear_bytes(int rows, int inputs, int, bool from_act) {
-  if (!from_act) return 0;
-  return ((size_t)rows * LF_MX4_PITCH(inputs) / 2 + 255) / 256 * 256 + LF_MX4_GROUPS(inputs) * LF_MX4_SCALE_PITCH(rows);
-}
-
-int run_mx4_linear(lf_context* ctx, const lf_mx4_linear_args& a, void* scratch) {
-  MxLinear p{};
-  lf_mx4 packed{};
-  if (a.act) {
-    packed = {a.rows, a.w->cols, scratch,
-              static_cast<char*>(scratch) + ((size_t)a.rows * LF_MX4_PITCH(a.w->cols) / 2 + 255) / 256 * 256};
-    lf_mx4_pack_args k{};
-    k.rows = a.rows;
-    k.cols = a.w->cols;
-    k.act_dtype = a.act_dtype;
-    k.act = a.act;
-    k.out = &packed;
-    LF_TRY(run_mx4_pack(ctx, k, nullptr));
-  }
-  p.x = mx_view(a.act ? packed : *a.kept);
-  p.w = mx_view(*a.w);
-  p.rows = a.rows;
-  p.outputs = a.w->rows;
-  p.steps = (int)(LF_MX4_PITCH(a.w->cols) / 128);
-  p.bias = a.bias;
-  p.relu = a.relu;
-  p.residual = a.residual;
-  p.out = a.out;
-  const int out_tiles = (p.outputs + 63) / 64;
-  const long long tiles = ((long long)p.rows + 63) / 64 * out_tiles;
-  LaunchScope ls(ctx, "mx4.linear");
-  const dim3 grid((unsigned)((tiles + 3) / 4)), block(256);
-  if (a.out_dtype == LF_F32) hipLaunchKernelGGL((mx4_linear_kernel<DT_F32>), grid, block, 0, ctx->stream, p, out_tiles, tiles);
-  else if (a.out_dtype == LF_F16) hipLaunchKernelGGL((mx4_linear_kernel<DT_F16>), grid, block, 0, ctx->stream, p, out_tiles, tiles);
-  else hipLaunchKernelGGL((mx4_linear_kernel<DT_BF16>), grid, block, 0, ctx->stream, p, out_tiles, tiles);
-  return check_hip(hipGetLastError(), "4-bit product launch");
 }
 
 }  // namespace lf

@@ -8,6 +8,7 @@ namespace lf {
 namespace {
 
 constexpr int MOST_BOUNDARIES = 4095;
+constexpr int MOST_MX_COLS = 1 << 26;     // offsets of 64 rows of codes are 32 bits
 constexpr int MOST_SIDE = 16384;         // of a matrix that is made orthogonal
 constexpr int MOST_BATCH = 65535;        // a grid's third dimension
 
@@ -54,6 +55,7 @@ int relative_position_backward(lf_context* ctx, const lf_relative_position_backw
 int check_size(const char* fn, long long rows, long long cols) {
   const Name f{fn, nullptr};
   LF_REQUIRE(rows > 0 && cols > 0, f + ": dimensions must be positive");
+  LF_REQUIRE(cols <= MOST_MX_COLS, f + ": 4-bit matrices are at most 2^26 wide");
   LF_REQUIRE((long long)LF_MX4_SCALE_PITCH(rows) <= MOST_ELEMENTS / (long long)LF_MX4_PITCH(cols), f + ": more than 2^34 elements");
   return LF_OK;
 }
@@ -102,7 +104,7 @@ int mx4_linear(lf_context* ctx, const lf_mx4_linear_args& a) {
   const long long inputs = a.w->cols, outputs = a.w->rows;
   LF_TRY(check_size(fn, outputs, inputs));
   LF_TRY(check_size(fn, a.rows, inputs));
-  LF_TRY(check_size(fn, a.rows, outputs));
+  LF_REQUIRE((long long)a.rows * outputs <= MOST_ELEMENTS, "lf_mx4_linear: more than 2^34 elements");
   LF_TRY(check_mx(fn, "w", *a.w, outputs, inputs));
   if (a.kept) LF_TRY(check_mx(fn, "kept", *a.kept, a.rows, inputs));
   else LF_TRY(check_act(fn, "act", a.act, a.act_dtype));
