@@ -129,27 +129,27 @@ __device__ __forceinline__ f4 mx_mma(u32x4 a, u32x4 b, f4 acc, uint32_t sa, uint
 #endif
 }
 
-// acc[t][q] += tile t of a times tile q of b; the scale bytes of the tiles are those of one word.
+// acc[t][q] += tile q of x times tile t of w; the scale bytes of an operand's tiles are those of one word.
 template <int MT>
-__device__ __forceinline__ void mx_mma_set(f4 (&acc)[4][MT], const u32x4 (&a)[4], const u32x4 (&b)[MT], uint32_t sa, uint32_t sb) {
+__device__ __forceinline__ void mx_mma_set(f4 (&acc)[4][MT], const u32x4 (&x)[MT], const u32x4 (&w)[4], uint32_t sx, uint32_t sw) {
   static_assert(MT == 2 || MT == 4, "rows of a lane");
-  acc[0][0] = mx_mma<0, 0>(a[0], b[0], acc[0][0], sa, sb);
-  acc[1][0] = mx_mma<1, 0>(a[1], b[0], acc[1][0], sa, sb);
-  acc[2][0] = mx_mma<2, 0>(a[2], b[0], acc[2][0], sa, sb);
-  acc[3][0] = mx_mma<3, 0>(a[3], b[0], acc[3][0], sa, sb);
-  acc[0][1] = mx_mma<0, 1>(a[0], b[1], acc[0][1], sa, sb);
-  acc[1][1] = mx_mma<1, 1>(a[1], b[1], acc[1][1], sa, sb);
-  acc[2][1] = mx_mma<2, 1>(a[2], b[1], acc[2][1], sa, sb);
-  acc[3][1] = mx_mma<3, 1>(a[3], b[1], acc[3][1], sa, sb);
+  acc[0][0] = mx_mma<0, 0>(x[0], w[0], acc[0][0], sx, sw);
+  acc[1][0] = mx_mma<0, 1>(x[0], w[1], acc[1][0], sx, sw);
+  acc[2][0] = mx_mma<0, 2>(x[0], w[2], acc[2][0], sx, sw);
+  acc[3][0] = mx_mma<0, 3>(x[0], w[3], acc[3][0], sx, sw);
+  acc[0][1] = mx_mma<1, 0>(x[1], w[0], acc[0][1], sx, sw);
+  acc[1][1] = mx_mma<1, 1>(x[1], w[1], acc[1][1], sx, sw);
+  acc[2][1] = mx_mma<1, 2>(x[1], w[2], acc[2][1], sx, sw);
+  acc[3][1] = mx_mma<1, 3>(x[1], w[3], acc[3][1], sx, sw);
   if constexpr (MT == 4) {
-    acc[0][2] = mx_mma<0, 2>(a[0], b[2], acc[0][2], sa, sb);
-    acc[1][2] = mx_mma<1, 2>(a[1], b[2], acc[1][2], sa, sb);
-    acc[2][2] = mx_mma<2, 2>(a[2], b[2], acc[2][2], sa, sb);
-    acc[3][2] = mx_mma<3, 2>(a[3], b[2], acc[3][2], sa, sb);
-    acc[0][3] = mx_mma<0, 3>(a[0], b[3], acc[0][3], sa, sb);
-    acc[1][3] = mx_mma<1, 3>(a[1], b[3], acc[1][3], sa, sb);
-    acc[2][3] = mx_mma<2, 3>(a[2], b[3], acc[2][3], sa, sb);
-    acc[3][3] = mx_mma<3, 3>(a[3], b[3], acc[3][3], sa, sb);
+    acc[0][2] = mx_mma<2, 0>(x[2], w[0], acc[0][2], sx, sw);
+    acc[1][2] = mx_mma<2, 1>(x[2], w[1], acc[1][2], sx, sw);
+    acc[2][2] = mx_mma<2, 2>(x[2], w[2], acc[2][2], sx, sw);
+    acc[3][2] = mx_mma<2, 3>(x[2], w[3], acc[3][2], sx, sw);
+    acc[0][3] = mx_mma<3, 0>(x[3], w[0], acc[0][3], sx, sw);
+    acc[1][3] = mx_mma<3, 1>(x[3], w[1], acc[1][3], sx, sw);
+    acc[2][3] = mx_mma<3, 2>(x[3], w[2], acc[2][3], sx, sw);
+    acc[3][3] = mx_mma<3, 3>(x[3], w[3], acc[3][3], sx, sw);
   }
 }
 

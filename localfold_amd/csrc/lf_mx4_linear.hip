@@ -1,9 +1,11 @@
 // Products of 4-bit operands (lf_mx4_linear): out[m][n] = sum_k x[m][k] w[n][k], with bias, ReLU and residual.
 //
-// w is the instruction's first operand, so a lane's sums are outputs of one row.  Operands go by sets of 64
-// rows, four tiles of 16: row i of tile t is row 4 f(i) + t of the set, so that the scale bytes of a lane's four tiles are
-// one word of memory.
+// x is the instruction's first operand, w its second: a lane's sums are outputs of the column that it has of w.  w goes by
+// sets of 64 rows, four tiles of 16, row i of tile t being row 4 i + t of the set: a lane then holds four
+// neighbouring outputs, 16 lanes a run of 64 (one line of 16-bit outputs), and the scale bytes of its tiles are one word of
+// memory.  x goes the same way, by 64 or 32 rows.
 #include <algorithm>
+#include <climits>
 
 #include "lf_mx4.h"
 
@@ -26,96 +28,101 @@ struct MxLinear {
   float* partial;                // split: [parts][rows][outputs]
 };
 
-// Which row of a set row i of the first operand's tiles belongs to: f puts the 16 outputs of a lane in runs of 16 bytes
-// (PER_RUN outputs), four lanes' runs side by side.
-template <int OUT>
-__device__ __forceinline__ int mx_f(int i) {
-  return OUT == DT_F32 ? (i & 3) * 4 + (i >> 2) : (i & 2) * 4 + (i >> 2) * 2 + (i & 1);
-}
-
-// One set of outputs from n0 on, rows m0 + MT r + q, stored.
+// One set of outputs from n0 on, rows m0 + MT i + q, stored.
 template <int OUT, int MT>
 __device__ __forceinline__ void mx_finish(const f4 (&acc)[4][MT], const MxLinear& p, long long m0, int n0, int r, int g) {
   typedef typename Act<OUT>::T T;
-  constexpr int L = OUT == DT_F32 ? 4 : 8, RUNS = 16 / L;
+  struct Four {
+    T v[4];
+  };
+  const int n = n0 + 4 * r, left = p.outputs - n;
 #pragma unroll
-  for (int q = 0; q < MT; ++q) {
-    const long long m = m0 + MT * r + q;
-    if (m >= p.rows) continue;
+  for (int q = 0; q < MT; ++q)
 #pragma unroll
-    for (int a = 0; a < RUNS; ++a) {
-      const int n = n0 + (OUT == DT_F32 ? 16 * a + 4 * g : 32 * a + 8 * g), left = p.outputs - n;
+    for (int j = 0; j < 4; ++j) {
+      const long long m = m0 + MT * (4 * g + j) + q;
+      if (m >= p.rows) continue;
       const size_t at = (size_t)m * p.outputs + n;
       T* const out = static_cast<T*>(p.out) + at;
       const T* const res = static_cast<const T*>(p.residual) + at;
-      float v[8];
+      float v[4];
 #pragma unroll
-      for (int e = 0; e < L; ++e) {
-        v[e] = OUT == DT_F32 ? acc[e][q][a] : acc[e & 3][q][2 * a + (e >> 2)];
-        if (p.relu) v[e] = __builtin_elementwise_maximum(v[e], 0.f);   // keeps NaN
+      for (int t = 0; t < 4; ++t) {
+        v[t] = acc[t][q][j];
+        if (p.relu) v[t] = __builtin_elementwise_maximum(v[t], 0.f);   // keeps NaN
       }
-      if constexpr (L == 8) {
+      Four o;
+      if (left >= 4) {
         if (p.residual) {
-          float w[8];
-          load8<OUT>(res, left, w);
+          __builtin_memcpy(&o, res, sizeof(o));
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] += w[e];
+          for (int t = 0; t < 4; ++t) v[t] += Act<OUT>::ld(o.v + t);
         }
-        store8<OUT>(out, left, v);
-      } else if (left >= 4) {
-        float4 w = make_float4(v[0], v[1], v[2], v[3]);
-        if (p.residual) {
-          float4 s;
-          __builtin_memcpy(&s, res, 16);
-          w = make_float4(w.x + s.x, w.y + s.y, w.z + s.z, w.w + s.w);
-        }
-        __builtin_memcpy(out, &w, 16);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) Act<OUT>::st(o.v + t, v[t]);
+        __builtin_memcpy(out, &o, sizeof(o));
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (e < left) out[e] = p.residual ? v[e] + res[e] : v[e];
+        for (int t = 0; t < 4; ++t)
+          if (t < left) Act<OUT>::st(out + t, p.residual ? v[t] + Act<OUT>::ld(res + t) : v[t]);
       }
     }
-  }
 }
 
 // ---- weights resident: short reductions ------------------------------------------------------------
 
 // A block copies its sets of outputs, all their columns, to LDS once, in the order in which a wave reads them: a tile's 64
-// lanes side by side.  Its 16 waves then take 32 rows each in turn with no barrier, quantise them in registers (a lane
-// holds whole groups) and run through the sets.
-constexpr int RW = 16, RM = 2, MOST_STEPS = 4;
+// lanes side by side.  Its waves then take 32 rows each in turn with no barrier, quantise them in registers (a lane holds
+// whole groups; the next rows are under way meanwhile, where registers allow) and run through the sets.
+constexpr int RM = 2;            // tiles of 16 rows of a wave
 struct MxResident {
   int per, subsets, blocks;      // sets of a block, blocks that share the outputs, blocks of a subset
 };
 
-// Rows 2 r + q of m0 on, columns 32 g on of every step; rows past the end repeat the last one.
+// One step's rows 2 r + q of m0 on, columns 32 g on; rows past the end repeat the last one.
 template <int SRC>
-__device__ __forceinline__ void mx_rows_load(u32x4 (&v)[RM], uint32_t& scale, const MxLinear& p, long long m0, int kb, int r, int g) {
-  if constexpr (SRC == KEPT) {
+struct MxRows {
+  MxRaw<SRC> raw[RM];
+  __device__ __forceinline__ void load(const MxLinear& p, long long m0, int kb, int r, int g) {
+    const int c = kb * 128 + 32 * g;
 #pragma unroll
     for (int q = 0; q < RM; ++q)
-      v[q] = *reinterpret_cast<const u32x4*>(p.x.codes + (size_t)min(m0 + RM * r + q, (long long)p.rows - 1) * p.x.pitch + kb * 64 + 16 * g);
-    scale = *reinterpret_cast<const uint16_t*>(p.x.scales + (size_t)(4 * kb + g) * p.x.sp + min(m0 + RM * r, ((long long)p.rows - 1) & ~1LL));
-  } else {
-    typedef typename Act<SRC>::T T;
-    MxRaw<SRC> raw[RM];
-#pragma unroll
-    for (int q = 0; q < RM; ++q) {
-      const int c = kb * 128 + 32 * g;
-      raw[q].load(static_cast<const T*>(p.act) + (size_t)min(m0 + RM * r + q, (long long)p.rows - 1) * p.inputs + c, p.inputs - c);
-    }
+      raw[q].load(static_cast<const typename Act<SRC>::T*>(p.act) + (size_t)min(m0 + RM * r + q, (long long)p.rows - 1) * p.inputs + c,
+                  p.inputs - c);
+  }
+  __device__ __forceinline__ void take(u32x4 (&v)[RM], uint32_t& scale) const {
     scale = 0;
 #pragma unroll
     for (int q = 0; q < RM; ++q) scale |= (uint32_t)raw[q].quantise(v[q]) << (8 * q);
   }
-}
+};
+template <>
+struct MxRows<KEPT> {
+  u32x4 codes[RM];
+  uint32_t scales;
+  __device__ __forceinline__ void load(const MxLinear& p, long long m0, int kb, int r, int g) {
+#pragma unroll
+    for (int q = 0; q < RM; ++q)
+      codes[q] = *reinterpret_cast<const u32x4*>(p.x.codes + (size_t)min(m0 + RM * r + q, (long long)p.rows - 1) * p.x.pitch + kb * 64 + 16 * g);
+    scales = *reinterpret_cast<const uint16_t*>(p.x.scales + (size_t)(4 * kb + g) * p.x.sp + min(m0 + RM * r, ((long long)p.rows - 1) & ~1LL));
+  }
+  __device__ __forceinline__ void take(u32x4 (&v)[RM], uint32_t& scale) const {
+#pragma unroll
+    for (int q = 0; q < RM; ++q) v[q] = codes[q];
+    scale = scales;
+  }
+};
 
-template <int SRC, int OUT>
-__global__ __launch_bounds__(RW * 64) void mx4_resident_kernel(MxLinear p, MxResident q) {
+constexpr int resident_waves(int steps) { return steps > 4 ? 8 : 16; }
+
+// STEPS: 1, 2, 4 or 8, at least p.steps.
+template <int SRC, int OUT, int STEPS>
+__global__ __launch_bounds__(resident_waves(STEPS) * 64) void mx4_resident_kernel(MxLinear p, MxResident q) {
+  constexpr int RW = resident_waves(STEPS);
+  constexpr bool EARLY = STEPS == 1 && SRC != DT_F32;
   extern __shared__ __attribute__((aligned(16))) uint8_t mx_smem[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int kbs = p.steps, sets = (p.outputs + 63) / 64;
+  const int kbs = STEPS <= 2 ? STEPS : p.steps, sets = (p.outputs + 63) / 64;
   // blocks of the same rows and other subsets share an XCD (blocks are dealt out to 8 in turn)
   const int index = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3), subset = index % q.subsets, blk = index / q.subsets;
   if (blk >= q.blocks) return;
@@ -124,7 +131,7 @@ __global__ __launch_bounds__(RW * 64) void mx4_resident_kernel(MxLinear p, MxRes
   float* const bias = reinterpret_cast<float*>(ws + q.per * kbs * 64);
   for (int i = wave; i < per * kbs * 4; i += RW) {
     const int set = (i >> 2) / kbs, kb = (i >> 2) % kbs;
-    const int n = min((set0 + set) * 64 + 4 * mx_f<OUT>(r) + (i & 3), p.outputs - 1);
+    const int n = min((set0 + set) * 64 + 4 * r + (i & 3), p.outputs - 1);
     const uint8_t* src = p.w.codes + (size_t)n * p.w.pitch + kb * 64 + 16 * g;
 #if __HIP_DEVICE_COMPILE__
     __builtin_amdgcn_global_load_lds(src, mx_smem + i * 1024, 16, 0, 0);
@@ -133,39 +140,51 @@ __global__ __launch_bounds__(RW * 64) void mx4_resident_kernel(MxLinear p, MxRes
 #endif
   }
   for (int i = wave; i < per * kbs; i += RW) {     // scale rows are whole sixteens
-    const int set = i / kbs, kb = i % kbs, n = min((set0 + set) * 64 + 4 * mx_f<OUT>(r), (p.outputs - 1) & ~3);
+    const int set = i / kbs, kb = i % kbs, n = min((set0 + set) * 64 + 4 * r, (p.outputs - 1) & ~3);
     ws[i * 64 + lane] = *reinterpret_cast<const uint32_t*>(p.w.scales + (size_t)(4 * kb + g) * p.w.sp + n);
   }
-  for (int i = threadIdx.x; i < per * 64; i += RW * 64) {     // [set][tile][row of a tile]
-    const int n = (set0 + (i >> 6)) * 64 + 4 * mx_f<OUT>(i & 15) + ((i >> 4) & 3);
-    bias[i] = p.bias && n < p.outputs ? p.bias[n] : 0.f;
+  for (int i = threadIdx.x; i < per * 64; i += RW * 64) bias[i] = p.bias && set0 * 64 + i < p.outputs ? p.bias[set0 * 64 + i] : 0.f;
+  const long long units = ((long long)p.rows + 16 * RM - 1) / (16 * RM), stride = (long long)q.blocks * RW;
+  long long u = (long long)blk * RW + wave;
+  MxRows<SRC> rows[EARLY ? STEPS : 1];
+  if constexpr (EARLY) {
+#pragma unroll
+    for (int kb = 0; kb < STEPS; ++kb) rows[kb].load(p, min(u, units - 1) * 16 * RM, kb, r, g);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  const long long units = ((long long)p.rows + 16 * RM - 1) / (16 * RM);
-  for (long long u = (long long)blk * RW + wave; u < units; u += (long long)q.blocks * RW) {
+  for (; u < units; u += stride) {
     const long long m0 = u * 16 * RM;
-    u32x4 x[MOST_STEPS][RM];
-    uint32_t xs[MOST_STEPS];
+    u32x4 x[STEPS][RM];
+    uint32_t xs[STEPS];
+    if constexpr (EARLY) {
 #pragma unroll
-    for (int kb = 0; kb < MOST_STEPS; ++kb)
-      if (kb < kbs) mx_rows_load<SRC>(x[kb], xs[kb], p, m0, kb, r, g);
+      for (int kb = 0; kb < STEPS; ++kb) rows[kb].take(x[kb], xs[kb]);
+#pragma unroll
+      for (int kb = 0; kb < STEPS; ++kb) rows[kb].load(p, min(u + stride, units - 1) * 16 * RM, kb, r, g);
+    } else {
+#pragma unroll
+      for (int kb = 0; kb < STEPS; ++kb)
+        if (kb < kbs) {
+          rows[0].load(p, m0, kb, r, g);
+          rows[0].take(x[kb], xs[kb]);
+        }
+    }
     for (int set = 0; set < per; ++set) {
       f4 acc[4][RM];
+      const f4 b = *reinterpret_cast<const f4*>(bias + set * 64 + 4 * r);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const f4 b = *reinterpret_cast<const f4*>(bias + set * 64 + t * 16 + 4 * g);
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int k = 0; k < RM; ++k) acc[t][k] = b;
-      }
+        for (int k = 0; k < RM; ++k) acc[t][k] = f4{b[t], b[t], b[t], b[t]};
 #pragma unroll
-      for (int kb = 0; kb < MOST_STEPS; ++kb) {
+      for (int kb = 0; kb < STEPS; ++kb) {
         if (kb >= kbs) break;
         const uint8_t* at = mx_smem + (size_t)(set * kbs + kb) * 4096 + lane * 16;
         u32x4 a[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) a[t] = *reinterpret_cast<const u32x4*>(at + t * 1024);
-        mx_mma_set<RM>(acc, a, x[kb], ws[(set * kbs + kb) * 64 + lane], xs[kb]);
+        mx_mma_set<RM>(acc, x[kb], a, xs[kb], ws[(set * kbs + kb) * 64 + lane]);
       }
       mx_finish<OUT, RM>(acc, p, m0, (set0 + set) * 64, r, g);
     }
@@ -174,21 +193,24 @@ __global__ __launch_bounds__(RW * 64) void mx4_resident_kernel(MxLinear p, MxRes
 
 // ---- streamed: long reductions ---------------------------------------------------------------------
 
-// A block of WN WM waves computes WN NT 16 outputs by WM 64 rows, 128 columns a step.  Each wave copies one set of 64 rows
-// of an operand, its codes in the order in which the waves read them (a tile's 64 lanes side by side) and its
-// scale words, to one of four LDS buffers, three steps ahead; one barrier a step.
+// A block of 2 by WM waves of NT by 4 tiles of 16, 256 columns a step: whole lines of memory.  Each wave copies
+// sets of 64 rows of an operand to one of two LDS buffers a step ahead, its instructions 8 rows of 128 bytes: four
+// neighbouring lanes read 64 bytes (lanes in the order of the fragments, 16 bytes of a row each, made the copies what
+// the kernel waited for: 98 us instead of 63 for 8192 rows of 4096 x 4096).  Tile t's rows lie side by side in LDS, their
+// 16-byte chunks c at c ^ (row & 7): no conflicts.  Fragments of 128 columns are read half a step ahead, so that the products
+// do not wait for LDS.
 // Split: a block takes part of the steps and stores f32 sums to p.partial, joined by mx4_join_kernel.
 struct MxStream {
   int mtiles, ntiles, parts;
 };
 
-template <int OUT, int NT, int WN, int WM, bool PART>
-__global__ __launch_bounds__(WN * WM * 64, 2) void mx4_stream_kernel(MxLinear p, MxStream q) {
-  constexpr int BN = WN * NT * 16, BM = WM * 64, SETS = WN * WM, AHEAD = 3, LOADS = 5;
-  static_assert(SETS * 64 == BN + BM, "a wave copies a set");
-  constexpr int STAGE = SETS * (4096 + 256);
-  // Separate objects: reads of one are then known not to wait for copies into another.
-  __shared__ __attribute__((aligned(16))) uint8_t S0[STAGE], S1[STAGE], S2[STAGE], S3[STAGE];
+template <int OUT, int NT, int WM, bool PART>
+__global__ __launch_bounds__(128 * WM, 2) void mx4_stream_kernel(MxLinear p, MxStream q) {
+  constexpr int BN = 2 * NT * 16, BM = WM * 64, SETS = (BN + BM) / 64, MINE = SETS / (2 * WM);
+  constexpr int CODES = 64 * 128, STAGE = SETS * (CODES + 2 * 256);
+  static_assert(MINE * 2 * WM == SETS && BN / 64 % MINE == 0, "a wave copies whole sets of one operand");
+  // Separate objects: reads of one are then known not to wait for copies into the other.
+  __shared__ __attribute__((aligned(16))) uint8_t S0[STAGE], S1[STAGE];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   int mt, nt, part;
   if constexpr (PART) {      // the tiles of a part on one XCD, whose L2 then reads that part once
@@ -204,93 +226,117 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_stream_kernel(MxLinear p,
     part = 0;
     if (mt >= q.mtiles) return;
   }
-  const int s0 = (int)((long long)p.steps * part / q.parts), s1 = (int)((long long)p.steps * (part + 1) / q.parts);
+  const int all = p.steps / 2;             // steps of 256 columns; a last 128 come at the end
+  const int s0 = (int)((long long)all * part / q.parts), s1 = (int)((long long)all * (part + 1) / q.parts);
   const long long m0 = (long long)mt * BM;
   const int n0 = nt * BN;
-  // what this wave copies
-  const bool of_w = wave < BN / 64;
+  // what this wave copies: MINE sets of one operand; rows past the end repeat the last one
+  const bool of_w = wave * MINE < BN / 64;
   const Mx& src = of_w ? p.w : p.x;
-  const long long first = of_w ? n0 + wave * 64 : m0 + (wave - BN / 64) * 64, last = (of_w ? p.outputs : p.rows) - 1;
+  const long long first = of_w ? n0 + wave * MINE * 64 : m0 + (wave * MINE - BN / 64) * 64, last = (of_w ? p.outputs : p.rows) - 1;
   const long long base = min(first, last);
   const uint8_t* const codes = src.codes + (size_t)base * src.pitch;
-  const int i0 = of_w ? 4 * mx_f<OUT>(r) : 4 * r;
-  uint32_t off[4];
+  const uint32_t pitch = (uint32_t)src.pitch, sstep = (uint32_t)(4 * src.sp), chunk = 16 * ((lane & 7) ^ (lane >> 3));
+  const int lane_row = (int)(first - base) + 4 * (lane >> 3), last_row = (int)min(last - base, (long long)INT_MAX);
+  uint32_t soff[MINE];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) off[t] = (uint32_t)(min(first + i0 + t, last) - base) * (uint32_t)src.pitch + 16 * g;
-  const uint32_t soff = (uint32_t)(g * src.sp + min(first + i0, last & ~3LL));
-  const uint32_t sstep = (uint32_t)(4 * src.sp);
+  for (int i = 0; i < MINE; ++i) soff[i] = (uint32_t)(g * src.sp + min(first + i * 64 + 4 * r, last & ~3LL));
   auto stage = [&](uint8_t* dst, int s) __attribute__((always_inline)) {
 #if __HIP_DEVICE_COMPILE__
     const __amdgpu_buffer_rsrc_t cr = __builtin_amdgcn_make_buffer_rsrc((void*)codes, 0, 0xffffffffu, 0x27000);
     const __amdgpu_buffer_rsrc_t sr = __builtin_amdgcn_make_buffer_rsrc((void*)src.scales, 0, 0xffffffffu, 0x27000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(sr, dst + SETS * 4096 + wave * 256, 4, soff, s * sstep, 0, 0);
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(cr, dst + wave * 4096 + t * 1024, 16, off[t], s * 64, 0, 0);
+    for (int l = 0; l < 10 * MINE; ++l) {
+      const int i = l / 10, k = l % 10 - 2;
+      if (k < 0) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(sr, dst + SETS * CODES + (wave * MINE + i) * 512 + (k + 2) * 256, 4, soff[i],
+                                                 (2 * s + k + 2) * sstep, 0, 0);
+      } else {       // LDS row 8 k + lane / 8: tile k / 2, its row 8 (k % 2) + lane / 8
+        const uint32_t row = (uint32_t)min(lane_row + i * 64 + 32 * (k & 1) + (k >> 1), last_row);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(cr, dst + (wave * MINE + i) * CODES + k * 1024, 16, row * pitch + chunk, s * 128, 0, 0);
+      }
+    }
 #else
-    (void)codes, (void)dst, (void)s, (void)soff, (void)sstep;
+    (void)codes, (void)dst, (void)s, (void)soff, (void)sstep, (void)pitch, (void)chunk, (void)lane_row, (void)last_row;
 #endif
   };
-  const int wn = wave % WN, wm = wave / WN;
-  f4 acc[NT / 4][4][4];
+  const int wn = wave & 1, wm = wave >> 1;
+  constexpr int H = NT / 4, UNITS = 2 * H;     // units of a step: a half of its columns times a set of outputs
+  f4 acc[H][4][4];
 #pragma unroll
-  for (int h = 0; h < NT / 4; ++h)
+  for (int h = 0; h < H; ++h)
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      f4 b = {0.f, 0.f, 0.f, 0.f};
-      if (!PART && p.bias) {
+      const float b = !PART && p.bias ? p.bias[min(n0 + (wn * H + h) * 64 + 4 * r + t, p.outputs - 1)] : 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) b[j] = p.bias[min(n0 + (wn * NT / 4 + h) * 64 + 4 * mx_f<OUT>(4 * g + j) + t, p.outputs - 1)];
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) acc[h][t][k] = b;
+      for (int k = 0; k < 4; ++k) acc[h][t][k] = f4{b, b, b, b};
     }
+  u32x4 x[2][4], w[2][4];
+  uint32_t sx[2], sw[2];
+  const int at0 = r * 128 + ((g ^ (r & 7)) << 4), at1 = at0 ^ 64;
+  auto read_set = [&](u32x4 (&v)[4], uint32_t& scale, const uint8_t* buf, int set, int half) __attribute__((always_inline)) {
+    scale = *reinterpret_cast<const uint32_t*>(buf + SETS * CODES + set * 512 + half * 256 + lane * 4);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const u32x4*>(buf + set * CODES + k * 2048 + (half ? at1 : at0));
+  };
+  auto read = [&](const uint8_t* buf, int unit) __attribute__((always_inline)) {
+    const int half = unit / H, h = unit % H;
+    if (h == 0) read_set(x[half], sx[half], buf, BN / 64 + wm, half);
+    read_set(w[unit & 1], sw[unit & 1], buf, wn * H + h, half);
+  };
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  stage(S0, s0);
-  stage(S1, min(s0 + 1, s1 - 1));
-  stage(S2, min(s0 + 2, s1 - 1));
-  auto step = [&](int s, const uint8_t* buf, uint8_t* next) __attribute__((always_inline)) {
-    // step s in LDS for every wave; every wave done with `next`, which held step s - 1
-    static_assert((AHEAD - 1) * LOADS == 10, "the wait below");
-    asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+  if (s0 < s1) {
+    stage(S0, s0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    stage(next, min(s + AHEAD, s1 - 1));      // past the end the last step again, which nothing reads
-    __builtin_amdgcn_sched_barrier(0);
-    u32x4 b[4];
+    stage(S1, min(s0 + 1, s1 - 1));
+    read(S0, 0);
+  }
+  // Step s: its first unit is read, it is in `buf`, and step s + 1 on its way to `other`.
+  auto step = [&](int s, uint8_t* buf, uint8_t* other) __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) b[k] = *reinterpret_cast<const u32x4*>(buf + (BN / 16 + wm * 4 + k) * 1024 + lane * 16);
-    const uint32_t sb = *reinterpret_cast<const uint32_t*>(buf + SETS * 4096 + (BN / 64 + wm) * 256 + lane * 4);
-#pragma unroll
-    for (int h = 0; h < NT / 4; ++h) {
-      u32x4 a[4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) a[t] = *reinterpret_cast<const u32x4*>(buf + (wn * NT + h * 4 + t) * 1024 + lane * 16);
-      const uint32_t sa = *reinterpret_cast<const uint32_t*>(buf + SETS * 4096 + (wn * NT / 4 + h) * 256 + lane * 4);
-      mx_mma_set<4>(acc[h], a, b, sa, sb);
+    for (int u = 0; u < UNITS; ++u) {
+      if (u + 1 < UNITS) {
+        read(buf, u + 1);
+      } else {
+        // every wave's copies of s + 1 are there, and every wave has read s
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        read(other, 0);
+        stage(buf, min(s + 2, s1 - 1));      // past the end the last step again, which nothing uses
+      }
+      mx_mma_set<4>(acc[u % H], x[u / H], w[u & 1], sx[u / H], sw[u & 1]);
+      __builtin_amdgcn_sched_barrier(0);   // products touch no memory: they would be moved past the next barrier
     }
-    // products touch no memory: without this they would be moved past the next step's barrier
-#pragma unroll
-    for (int h = 0; h < NT / 4; ++h)
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) asm volatile("" : "+v"(acc[h][t][k]));
   };
   int s = s0;
-  for (; s + 3 < s1; s += 4) {
-    step(s, S0, S3);
+  for (; s + 1 < s1; s += 2) {
+    step(s, S0, S1);
     step(s + 1, S1, S0);
-    step(s + 2, S2, S1);
-    step(s + 3, S3, S2);
   }
-  if (s < s1) step(s, S0, S3);
-  if (s + 1 < s1) step(s + 1, S1, S0);
-  if (s + 2 < s1) step(s + 2, S2, S1);
+  if (s < s1) step(s, S0, S1);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last copies, which nothing reads
+  if ((p.steps & 1) && part == q.parts - 1) {         // the last 128 columns, straight from memory
+    const int kb = p.steps - 1;
+    const long long m = m0 + wm * 64 + 4 * r;
 #pragma unroll
-  for (int h = 0; h < NT / 4; ++h) {
-    const int n = n0 + (wn * NT / 4 + h) * 64;
+    for (int k = 0; k < 4; ++k)
+      x[0][k] = *reinterpret_cast<const u32x4*>(p.x.codes + (size_t)min(m + k, p.rows - 1LL) * p.x.pitch + kb * 64 + 16 * g);
+    sx[0] = *reinterpret_cast<const uint32_t*>(p.x.scales + (size_t)(4 * kb + g) * p.x.sp + min(m, (p.rows - 1LL) & ~3LL));
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      const int n = n0 + (wn * H + h) * 64 + 4 * r;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        w[0][t] = *reinterpret_cast<const u32x4*>(p.w.codes + (size_t)min(n + t, p.outputs - 1) * p.w.pitch + kb * 64 + 16 * g);
+      sw[0] = *reinterpret_cast<const uint32_t*>(p.w.scales + (size_t)(4 * kb + g) * p.w.sp + min(n, (p.outputs - 1) & ~3));
+      mx_mma_set<4>(acc[h], x[0], w[0], sx[0], sw[0]);
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    const int n = n0 + (wn * H + h) * 64;
     if (n >= p.outputs) continue;
     MxLinear o = p;
     if constexpr (PART) {
@@ -302,15 +348,26 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_stream_kernel(MxLinear p,
   }
 }
 
-// The parts' sums, bias, ReLU, residual.
-template <int OUT>
+// The parts' sums in a fixed order, bias, ReLU, residual: P threads share an element.
+template <int OUT, int P>
 __global__ __launch_bounds__(256) void mx4_join_kernel(MxLinear p, int parts) {
   typedef typename Act<OUT>::T T;
+  __shared__ float sm[P][256 / P];
   const size_t count = (size_t)p.rows * p.outputs;
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  const int e = threadIdx.x % (256 / P), k0 = threadIdx.x / (256 / P);
+  const size_t i = (size_t)blockIdx.x * (256 / P) + e;
+  float v = 0.f;
+  if (i < count)
+    for (int k = parts * k0 / P; k < parts * (k0 + 1) / P; ++k) v += p.partial[k * count + i];
+  if constexpr (P > 1) {
+    sm[k0][e] = v;
+    __syncthreads();
+    if (k0 > 0) return;
+#pragma unroll
+    for (int k = 1; k < P; ++k) v += sm[k][e];
+  }
   if (i >= count) return;
-  float v = p.bias ? p.bias[i % p.outputs] : 0.f;
-  for (int k = 0; k < parts; ++k) v += p.partial[k * count + i];
+  if (p.bias) v += p.bias[i % p.outputs];
   if (p.relu) v = __builtin_elementwise_maximum(v, 0.f);
   if (p.residual) v += Act<OUT>::ld(static_cast<const T*>(p.residual) + i);
   Act<OUT>::st(static_cast<T*>(p.out) + i, v);
@@ -319,8 +376,8 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(MxLinear p, int parts) {
 // ---- few rows or outputs -----------------------------------------------------------------------------
 
 // What counts is the time to the last byte: a block computes 32 rows by 16 outputs, its waves steps of the columns in
-// turn, operands straight from memory, sums joined in LDS.
-constexpr int FW = 8;
+// turn, two at a time, operands straight from memory, sums joined in LDS.
+constexpr int FW = 16;
 
 template <int SRC, int OUT>
 __global__ __launch_bounds__(FW * 64) void mx4_few_kernel(MxLinear p) {
@@ -334,14 +391,29 @@ __global__ __launch_bounds__(FW * 64) void mx4_few_kernel(MxLinear p) {
   f4 acc[RM];
 #pragma unroll
   for (int q = 0; q < RM; ++q) acc[q] = f4{0.f, 0.f, 0.f, 0.f};
-  for (int kb = wave; kb < p.steps; kb += waves) {
-    const u32x4 a = *reinterpret_cast<const u32x4*>(wrow + (size_t)kb * 64);
-    const uint32_t sa = wscale[(size_t)4 * kb * p.w.sp];
+  struct Step {
+    u32x4 w;
+    uint32_t ws;
+    MxRows<SRC> x;
+  };
+  auto load = [&](Step& s, int kb) __attribute__((always_inline)) {
+    s.w = *reinterpret_cast<const u32x4*>(wrow + (size_t)kb * 64);
+    s.ws = wscale[(size_t)4 * kb * p.w.sp];
+    s.x.load(p, m0, kb, r, g);
+  };
+  auto multiply = [&](const Step& s) __attribute__((always_inline)) {
     u32x4 b[RM];
     uint32_t sb;
-    mx_rows_load<SRC>(b, sb, p, m0, kb, r, g);
-    acc[0] = mx_mma<0, 0>(a, b[0], acc[0], sa, sb);
-    acc[1] = mx_mma<0, 1>(a, b[1], acc[1], sa, sb);
+    s.x.take(b, sb);
+    acc[0] = mx_mma<0, 0>(b[0], s.w, acc[0], sb, s.ws);
+    acc[1] = mx_mma<1, 0>(b[1], s.w, acc[1], sb, s.ws);
+  };
+  for (int kb = wave; kb < p.steps; kb += 2 * waves) {
+    Step a, b;
+    load(a, kb);
+    load(b, min(kb + waves, p.steps - 1));
+    multiply(a);
+    if (kb + waves < p.steps) multiply(b);
   }
   if (wave > 0) {
 #pragma unroll
@@ -353,13 +425,14 @@ __global__ __launch_bounds__(FW * 64) void mx4_few_kernel(MxLinear p) {
 #pragma unroll
   for (int q = 0; q < RM; ++q) {
     for (int k = 1; k < waves; ++k) acc[q] += part[k - 1][q][lane];
-    const long long m = m0 + RM * r + q;
-    if (m >= p.rows) continue;
+    const int o = n0 + r;
+    if (o >= p.outputs) continue;
+    const float bias = p.bias ? p.bias[o] : 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int o = n0 + 4 * g + j;
-      if (o >= p.outputs) continue;
-      float v = acc[q][j] + (p.bias ? p.bias[o] : 0.f);
+      const long long m = m0 + RM * (4 * g + j) + q;
+      if (m >= p.rows) continue;
+      float v = acc[q][j] + bias;
       if (p.relu) v = __builtin_elementwise_maximum(v, 0.f);
       const size_t at = (size_t)m * p.outputs + o;
       if (p.residual) v += Act<OUT>::ld(static_cast<const T*>(p.residual) + at);
@@ -378,48 +451,63 @@ struct MxPlan {
 };
 constexpr int CUS = 256, FEW_TILES = 1500, FEW_STEPS = 64;
 
+constexpr int set_bytes(int steps) { return steps * (4096 + 256) + 256; }
+
 MxPlan mx_plan(long long rows, int steps, long long outputs) {
   const long long few = (rows + 31) / 32 * ((outputs + 15) / 16);
   if (few <= FEW_TILES && steps <= FEW_STEPS) return {FEW, false, 1};
-  if (steps <= MOST_STEPS) return {RESIDENT, false, 1};
+  if (steps <= 4 || (steps <= 8 && (outputs + 63) / 64 * set_bytes(steps) <= LDS_BYTES)) return {RESIDENT, false, 1};
   const long long wide = (rows + 255) / 256 * ((outputs + 255) / 256);
   if (wide >= CUS / 2) return {STREAM, true, 1};
   const long long tiles = (rows + 127) / 128 * ((outputs + 127) / 128);
-  // a part of 8 steps at least
+  // a part of 1024 columns at least
   const int parts = (int)std::max<long long>(1, std::min<long long>(2 * CUS / tiles, steps / 8));
   return {STREAM, false, parts};
 }
 
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
-template <int OUT, int NT, int WN, int WM, bool PART>
+template <int OUT, int NT, int WM, bool PART>
 void go_stream(lf_context* ctx, const MxLinear& p, int parts) {
-  MxStream q{(p.rows + WM * 64 - 1) / (WM * 64), (p.outputs + WN * NT * 16 - 1) / (WN * NT * 16), parts};
+  constexpr int BM = WM * 64, BN = 2 * NT * 16;
+  MxStream q{(int)(((long long)p.rows + BM - 1) / BM), (p.outputs + BN - 1) / BN, parts};
   const long long blocks = PART ? (parts + 7LL) / 8 * 8 * q.mtiles * q.ntiles : (q.mtiles + 31LL) / 32 * 32 * q.ntiles;
-  hipLaunchKernelGGL((mx4_stream_kernel<OUT, NT, WN, WM, PART>), dim3((unsigned)blocks), dim3(WN * WM * 64), 0, ctx->stream, p, q);
+  hipLaunchKernelGGL((mx4_stream_kernel<OUT, NT, WM, PART>), dim3((unsigned)blocks), dim3(128 * WM), 0, ctx->stream, p, q);
 }
 
-template <int SRC, int OUT>
+template <int OUT, int P>
+void go_join(lf_context* ctx, const MxLinear& p, int parts) {
+  const size_t count = (size_t)p.rows * p.outputs, each = 256 / P;
+  hipLaunchKernelGGL((mx4_join_kernel<OUT, P>), dim3((unsigned)((count + each - 1) / each)), dim3(256), 0, ctx->stream, p, parts);
+}
+
+template <int SRC, int OUT, int STEPS>
 int go_resident(lf_context* ctx, const MxLinear& p) {
-  const int sets = (p.outputs + 63) / 64, set_bytes = p.steps * (4096 + 256) + 256;
+  constexpr int RW = resident_waves(STEPS);
+  const int sets = (p.outputs + 63) / 64, each = set_bytes(p.steps);
   const long long units = ((long long)p.rows + 16 * RM - 1) / (16 * RM);
   MxResident q;
   // as many sets a block as fit, but no more than keep every wave of the chip busy
   const long long busy = std::max<long long>(1, units * sets / (CUS * RW));
-  q.per = (int)std::min<long long>(std::min(LDS_BYTES / set_bytes, sets), busy);
+  q.per = (int)std::min<long long>(std::min(LDS_BYTES / each, sets), busy);
   q.subsets = (sets + q.per - 1) / q.per;
   q.blocks = (int)std::min<long long>((units + 3) / 4, std::max(1, CUS / q.subsets));
-  static const hipError_t lds = hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_resident_kernel<SRC, OUT>),
+  static const hipError_t lds = hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_resident_kernel<SRC, OUT, STEPS>),
                                                     hipFuncAttributeMaxDynamicSharedMemorySize, LDS_BYTES);
   LF_TRY(check_hip(lds, "4-bit product LDS"));
   const unsigned grid = (unsigned)((q.blocks * q.subsets + 7) / 8 * 8);
-  hipLaunchKernelGGL((mx4_resident_kernel<SRC, OUT>), dim3(grid), dim3(RW * 64), (size_t)q.per * set_bytes, ctx->stream, p, q);
+  hipLaunchKernelGGL((mx4_resident_kernel<SRC, OUT, STEPS>), dim3(grid), dim3(RW * 64), (size_t)q.per * each, ctx->stream, p, q);
   return LF_OK;
 }
 
 template <int SRC, int OUT>
 int go_small(lf_context* ctx, const MxLinear& p, const MxPlan& plan) {
-  if (plan.kind == RESIDENT) return go_resident<SRC, OUT>(ctx, p);
+  if (plan.kind == RESIDENT) {
+    if (p.steps == 1) return go_resident<SRC, OUT, 1>(ctx, p);
+    if (p.steps == 2) return go_resident<SRC, OUT, 2>(ctx, p);
+    if (p.steps <= 4) return go_resident<SRC, OUT, 4>(ctx, p);
+    return go_resident<SRC, OUT, 8>(ctx, p);
+  }
   hipLaunchKernelGGL((mx4_few_kernel<SRC, OUT>), dim3((p.outputs + 15) / 16, (p.rows + 31) / 32), dim3(std::min(p.steps, FW) * 64), 0,
                      ctx->stream, p);
   return LF_OK;
@@ -437,15 +525,15 @@ int go(lf_context* ctx, const MxLinear& p, const MxPlan& plan, int act_dtype) {
   }
   {
     LaunchScope ls(ctx, "mx4.linear");
-    if (plan.wide) go_stream<OUT, 8, 2, 4, false>(ctx, p, 1);
-    else if (plan.parts == 1) go_stream<OUT, 4, 2, 2, false>(ctx, p, 1);
-    else go_stream<DT_F32, 4, 2, 2, true>(ctx, p, plan.parts);
+    if (plan.wide) go_stream<OUT, 8, 4, false>(ctx, p, 1);
+    else if (plan.parts == 1) go_stream<OUT, 4, 2, false>(ctx, p, 1);
+    else go_stream<DT_F32, 4, 2, true>(ctx, p, plan.parts);
     LF_TRY(check_hip(hipGetLastError(), "4-bit product launch"));
   }
   if (plan.parts == 1) return LF_OK;
   LaunchScope ls(ctx, "mx4.join");
-  const size_t count = (size_t)p.rows * p.outputs;
-  hipLaunchKernelGGL((mx4_join_kernel<OUT>), dim3((unsigned)((count + 255) / 256)), dim3(256), 0, ctx->stream, p, plan.parts);
+  if (plan.parts > 16) go_join<OUT, 16>(ctx, p, plan.parts);
+  else go_join<OUT, 4>(ctx, p, plan.parts);
   return check_hip(hipGetLastError(), "4-bit join launch");
 }
 

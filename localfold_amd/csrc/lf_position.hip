@@ -169,23 +169,25 @@ __global__ __launch_bounds__(256) void position_grad_kernel(lf_relative_pairs p,
   }
 }
 
-// out[e] = sum over p of partial[p][e]: 64 sums a block, 8 parts of each, joined in order; elements from `split`
+// out[e] = sum over p of partial[p][e]: 16 sums a block, 16 parts of each, joined in order; elements from `split`
 // on go to out2.
 template <int DT>
-__global__ __launch_bounds__(512) void join_kernel(const float* partial, int count, long long width, long long split, void* out,
+__global__ __launch_bounds__(256) void join_kernel(const float* partial, int count, long long width, long long split, void* out,
                                                    void* out2) {
-  __shared__ double sm[8][64];
-  const int part = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const long long e = (long long)blockIdx.x * 64 + lane;
+  __shared__ double sm[16][16];
+  const int part = threadIdx.x >> 4, lane = threadIdx.x & 15;
+  const long long e = (long long)blockIdx.x * 16 + lane;
   double t = 0;
   if (e < width) {
-    const int p1 = (int)((long long)count * (part + 1) / 8);
-    for (int i = (int)((long long)count * part / 8); i < p1; ++i) t += partial[(size_t)i * width + e];
+    const int p1 = (int)((long long)count * (part + 1) / 16);
+#pragma unroll 4
+    for (int i = (int)((long long)count * part / 16); i < p1; ++i) t += partial[(size_t)i * width + e];
   }
   sm[part][lane] = t;
   __syncthreads();
   if (part == 0 && e < width) {
-    for (int i = 1; i < 8; ++i) t += sm[i][lane];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) t += sm[i][lane];
     typedef typename Act<DT>::T T;
     if (e < split) Act<DT>::st(static_cast<T*>(out) + e, (float)t);
     else if (out2) Act<DT>::st(static_cast<T*>(out2) + (e - split), (float)t);
@@ -195,7 +197,7 @@ __global__ __launch_bounds__(512) void join_kernel(const float* partial, int cou
 int run_join(lf_context* ctx, const float* partial, int count, long long width, long long split, void* out, void* out2, int dt,
              const char* label) {
   LaunchScope ls(ctx, label);
-  const dim3 grid((unsigned)((width + 63) / 64)), block(512);
+  const dim3 grid((unsigned)((width + 15) / 16)), block(256);
   if (dt == LF_F32) hipLaunchKernelGGL((join_kernel<DT_F32>), grid, block, 0, ctx->stream, partial, count, width, split, out, out2);
   else if (dt == LF_F16) hipLaunchKernelGGL((join_kernel<DT_F16>), grid, block, 0, ctx->stream, partial, count, width, split, out, out2);
   else hipLaunchKernelGGL((join_kernel<DT_BF16>), grid, block, 0, ctx->stream, partial, count, width, split, out, out2);
