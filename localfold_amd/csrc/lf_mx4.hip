@@ -25,69 +25,122 @@ __global__ __launch_bounds__(256) void mx4_pack_kernel(const typename Act<ACT>::
   if (c0 % MX_GROUP == 0) k.scales[(size_t)(c0 / MX_GROUP) * k.sp + row] = (uint8_t)b;
 }
 
-// A block walks down `chunk` tiles of 128 rows by 64 columns, reads each once and packs it along the columns (k.codes, if
-// given), along the rows (t.codes, if given), and adds up its rows (partial [chunks][cols], if given).  Blocks of
-// neighbouring columns share an XCD, and a block keeps its columns: what they write meets in lines of one L2.
+// A block walks down `chunk` tiles of 128 rows by 128 columns, reads each once, a tile ahead, into LDS and packs it along the
+// columns (k.codes, if given) and along the rows (t.codes, if given), a group a thread, and adds up its rows (partial
+// [chunks][cols], if given).  Four neighbouring lanes write 64 bytes (where every lane wrote 16 of another line, what both
+// wrote of 196608 rows of 1024 in bf16 took 120 us beside the 82 of reading).  Blocks of neighbouring columns share an XCD,
+// and a block keeps its columns: halves of lines meet in one L2.
 struct PackBoth {
   int rows, cols, col_tiles, row_tiles, chunk, blocks;
 };
 template <int ACT>
 __global__ __launch_bounds__(256) void mx4_pack_both_kernel(const typename Act<ACT>::T* x, Mx k, Mx t, float* partial, PackBoth q) {
-  __shared__ float tile[128][64];
-  __shared__ float sm[4][64];
+  typedef typename Act<ACT>::T T;
+  constexpr int V = 16 / (int)sizeof(T), LANES = 128 / V, ROWS = 256 / LANES, PASSES = 128 / ROWS;   // as it reads
+  // A row's 16 bytes more put neighbouring rows 4 banks apart; groups of 32 rows start 16 columns apart.
+  constexpr int PITCH = 128 + V, SKEW = 16;
+  __shared__ __attribute__((aligned(16))) T tile[128 * PITCH + 4 * SKEW];
   const int index = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
   if (index >= q.blocks) return;
-  const int rc = index / q.col_tiles, c0 = index % q.col_tiles * 64, last = min((rc + 1) * q.chunk, q.row_tiles);
-  const int lr = threadIdx.x >> 3, lc = (threadIdx.x & 7) * 8;   // as it reads: row of 32, columns
-  const int c = threadIdx.x & 63, g = threadIdx.x >> 6;          // as it packs along the rows: column, group of 32 rows
-  float sum = 0.f;
+  const int rc = index / q.col_tiles, c0 = index % q.col_tiles * 128, last = min((rc + 1) * q.chunk, q.row_tiles);
+  const int lr = threadIdx.x / LANES, lc = threadIdx.x % LANES * V, left = q.cols - c0 - lc;
+  const int item = threadIdx.x >> 2, g = threadIdx.x & 3;        // as it packs: row or column, group
+  u32x4 in[PASSES];
+  auto load = [&](int rt) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int r = rt * 128 + i * ROWS + lr;
+      const T* const at = x + (size_t)r * q.cols + c0 + lc;
+      in[i] = u32x4{0, 0, 0, 0};
+      if (r < q.rows && left >= V) {
+        __builtin_memcpy(&in[i], at, 16);
+      } else if (r < q.rows && left > 0) {
+        T v[V] = {};
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (e < left) v[e] = at[e];
+        __builtin_memcpy(&in[i], v, 16);
+      }
+    }
+  };
+  float sum[2] = {0.f, 0.f};
+  load(rc * q.chunk);
   for (int rt = rc * q.chunk; rt < last; ++rt) {
     const int r0 = rt * 128;
-    float in[4][8];
-#pragma unroll
-    for (int pass = 0; pass < 4; ++pass) {
-      const int r = r0 + pass * 32 + lr;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) in[pass][j] = 0.f;
-      if (r < q.rows && c0 + lc < q.cols) load8<ACT>(x + (size_t)r * q.cols + c0 + lc, q.cols - c0 - lc, in[pass]);
-    }
     __syncthreads();     // the last tile is read
 #pragma unroll
-    for (int pass = 0; pass < 4; ++pass) {
-      const int r = r0 + pass * 32 + lr;
-      *reinterpret_cast<float4*>(&tile[pass * 32 + lr][lc]) = make_float4(in[pass][0], in[pass][1], in[pass][2], in[pass][3]);
-      *reinterpret_cast<float4*>(&tile[pass * 32 + lr][lc + 4]) = make_float4(in[pass][4], in[pass][5], in[pass][6], in[pass][7]);
-      if (k.codes) {
-        const int b = mx_scale_byte(quad_max(amax_bits8(in[pass])));
-        if (r < q.rows) {
-          *reinterpret_cast<uint32_t*>(k.codes + (size_t)r * k.pitch + (c0 + lc) / 2) = mx_encode8(in[pass], mx_scale_value(b));
-          if (lc % MX_GROUP == 0) k.scales[(size_t)((c0 + lc) / MX_GROUP) * k.sp + r] = (uint8_t)b;
+    for (int i = 0; i < PASSES; ++i) {
+      const int r = i * ROWS + lr;
+      *reinterpret_cast<u32x4*>(&tile[r * PITCH + (r >> 5) * SKEW + lc]) = in[i];
+    }
+    __syncthreads();
+    if (rt + 1 < last) load(rt + 1);
+    if (k.codes) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = i * 64 + item;
+        const T* const at = &tile[r * PITCH + (r >> 5) * SKEW + g * 32];
+        MxRaw<ACT> v;
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < MxRaw<ACT>::WORDS / 4; ++e) {
+          const u32x4 four = *reinterpret_cast<const u32x4*>(at + e * V);
+#pragma unroll
+          for (int h = 0; h < 4; ++h) v.w[4 * e + h] = four[h];
+        }
+        const int b = v.quantise(w);
+        if (r0 + r < q.rows) {
+          *reinterpret_cast<u32x4*>(k.codes + (size_t)(r0 + r) * k.pitch + c0 / 2 + g * 16) = w;
+          k.scales[(size_t)(c0 / MX_GROUP + g) * k.sp + r0 + r] = (uint8_t)b;
         }
       }
     }
-    __syncthreads();
-    float v[32];
-    uint32_t m = 0;
-    float s = 0.f;
+    if (t.codes || partial) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      v[j] = tile[g * 32 + j][c];
-      m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
-      s += v[j];
-    }
-    sum += s;
-    if (t.codes && c0 + c < q.cols) {
-      const int b = mx_scale_byte(m);
-      const float f = mx_scale_value(b);
-      const uint4 w = make_uint4(mx_encode8(v, f), mx_encode8(v + 8, f), mx_encode8(v + 16, f), mx_encode8(v + 24, f));
-      *reinterpret_cast<uint4*>(t.codes + (size_t)(c0 + c) * t.pitch + r0 / 2 + g * 16) = w;
-      t.scales[(size_t)(r0 / MX_GROUP + g) * t.sp + c0 + c] = (uint8_t)b;
+      for (int i = 0; i < 2; ++i) {
+        const int c = i * 64 + item;
+        const T* const at = &tile[g * (32 * PITCH + SKEW) + c];
+        MxRaw<ACT> v;
+#pragma unroll
+        for (int j = 0; j < MxRaw<ACT>::WORDS; ++j) {
+          if constexpr (ACT == DT_F32) {
+            v.w[j] = __float_as_uint(at[j * PITCH]);
+          } else {
+            uint16_t lo, hi;
+            __builtin_memcpy(&lo, at + 2 * j * PITCH, 2);
+            __builtin_memcpy(&hi, at + (2 * j + 1) * PITCH, 2);
+            v.w[j] = lo | (uint32_t)hi << 16;
+          }
+        }
+        if (t.codes) {
+          u32x4 w;
+          const int b = v.quantise(w);
+          if (c0 + c < q.cols) {
+            *reinterpret_cast<u32x4*>(t.codes + (size_t)(c0 + c) * t.pitch + r0 / 2 + g * 16) = w;
+            t.scales[(size_t)(r0 / MX_GROUP + g) * t.sp + c0 + c] = (uint8_t)b;
+          }
+        }
+        if (partial) {
+          float s = 0.f;
+#pragma unroll
+          for (int j = 0; j < MxRaw<ACT>::WORDS; ++j) {
+            if constexpr (ACT == DT_F32) s += __uint_as_float(v.w[j]);
+            else if constexpr (ACT == DT_BF16) s += __uint_as_float(v.w[j] << 16) + __uint_as_float(v.w[j] & 0xffff0000u);
+            else s += h2f((uint16_t)v.w[j]) + h2f((uint16_t)(v.w[j] >> 16));
+          }
+          sum[i] += s;
+        }
+      }
     }
   }
   if (partial) {
-    sm[g][c] = sum;
-    __syncthreads();
-    if (g == 0 && c0 + c < q.cols) partial[(size_t)rc * q.cols + c0 + c] = sm[0][c] + sm[1][c] + sm[2][c] + sm[3][c];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int c = c0 + i * 64 + item;
+      float s = sum[i] + dpp_f<0xB1>(sum[i]);     // the four groups of a column, in one order
+      s += dpp_f<0x4E>(s);
+      if (g == 0 && c < q.cols) partial[(size_t)rc * q.cols + c] = s;
+    }
   }
 }
 
@@ -119,7 +172,7 @@ PackBoth pack_both(int rows, int cols) {
   PackBoth q;
   q.rows = rows;
   q.cols = cols;
-  q.col_tiles = (int)(LF_MX4_PITCH(cols) / 64);
+  q.col_tiles = (int)(LF_MX4_PITCH(cols) / 128);
   q.row_tiles = (int)(((long long)rows + 127) / 128);
   const int chunks = std::min(q.row_tiles, std::max(1, 2048 / q.col_tiles));
   q.chunk = (q.row_tiles + chunks - 1) / chunks;

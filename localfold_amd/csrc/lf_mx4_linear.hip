@@ -29,42 +29,61 @@ struct MxLinear {
 };
 
 // One set of outputs from n0 on, rows m0 + MT i + q, stored.
+template <int OUT>
+struct MxFour {
+  typename Act<OUT>::T v[4];
+};
 template <int OUT, int MT>
 __device__ __forceinline__ void mx_finish(const f4 (&acc)[4][MT], const MxLinear& p, long long m0, int n0, int r, int g) {
   typedef typename Act<OUT>::T T;
-  struct Four {
-    T v[4];
-  };
-  const int n = n0 + 4 * r, left = p.outputs - n;
+  const int rows = (int)min((long long)16 * MT, p.rows - m0), outputs = p.outputs - n0;
+  const size_t first = (size_t)m0 * p.outputs + n0;
+  T* const out = static_cast<T*>(p.out) + first;
+  const T* const res = static_cast<const T*>(p.residual) + first;
+  if (rows == 16 * MT && outputs >= 64 && p.outputs <= 1 << 20) {     // uniform; offsets fit 32 bits
+    const uint32_t row = (uint32_t)p.outputs * sizeof(T), at = 4 * MT * g * row + 4 * r * (uint32_t)sizeof(T);
+    char* const ob = reinterpret_cast<char*>(out);
+    const char* const rb = reinterpret_cast<const char*>(res);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      __builtin_amdgcn_sched_barrier(0);   // few registers: some rows of a lane at a time
+      MxFour<OUT> o[MT];
+      if (p.residual) {
+#pragma unroll
+        for (int q = 0; q < MT; ++q) __builtin_memcpy(&o[q], rb + (at + (MT * j + q) * row), sizeof(o[q]));
+#pragma unroll
+        for (int q = 0; q < MT; ++q)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const float v = p.relu ? __builtin_elementwise_maximum(acc[t][q][j], 0.f) : acc[t][q][j];   // keeps NaN
+            Act<OUT>::st(o[q].v + t, v + Act<OUT>::ld(o[q].v + t));
+          }
+      } else {
+#pragma unroll
+        for (int q = 0; q < MT; ++q)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) Act<OUT>::st(o[q].v + t, p.relu ? __builtin_elementwise_maximum(acc[t][q][j], 0.f) : acc[t][q][j]);
+      }
+#pragma unroll
+      for (int q = 0; q < MT; ++q) __builtin_memcpy(ob + (at + (MT * j + q) * row), &o[q], sizeof(o[q]));
+    }
+    return;
+  }
+  asm volatile("" : "+v"(r), "+v"(g));     // or the offsets of this rare path would be kept in registers throughout
 #pragma unroll
   for (int q = 0; q < MT; ++q)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const long long m = m0 + MT * (4 * g + j) + q;
-      if (m >= p.rows) continue;
-      const size_t at = (size_t)m * p.outputs + n;
-      T* const out = static_cast<T*>(p.out) + at;
-      const T* const res = static_cast<const T*>(p.residual) + at;
-      float v[4];
+      __builtin_amdgcn_sched_barrier(0);
+      const int m = MT * (4 * g + j) + q;
+      if (m >= rows) continue;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        v[t] = acc[t][q][j];
-        if (p.relu) v[t] = __builtin_elementwise_maximum(v[t], 0.f);   // keeps NaN
-      }
-      Four o;
-      if (left >= 4) {
-        if (p.residual) {
-          __builtin_memcpy(&o, res, sizeof(o));
-#pragma unroll
-          for (int t = 0; t < 4; ++t) v[t] += Act<OUT>::ld(o.v + t);
-        }
-#pragma unroll
-        for (int t = 0; t < 4; ++t) Act<OUT>::st(o.v + t, v[t]);
-        __builtin_memcpy(out, &o, sizeof(o));
-      } else {
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-          if (t < left) Act<OUT>::st(out + t, p.residual ? v[t] + Act<OUT>::ld(res + t) : v[t]);
+        if (4 * r + t >= outputs) continue;
+        const size_t at = (size_t)m * p.outputs + 4 * r + t;
+        float v = acc[t][q][j];
+        if (p.relu) v = __builtin_elementwise_maximum(v, 0.f);
+        Act<OUT>::st(out + at, p.residual ? v + Act<OUT>::ld(res + at) : v);
       }
     }
 }
@@ -79,46 +98,48 @@ struct MxResident {
   int per, subsets, blocks;      // sets of a block, blocks that share the outputs, blocks of a subset
 };
 
-// One step's rows 2 r + q of m0 on, columns 32 g on; rows past the end repeat the last one.
-template <int SRC>
+// One step's rows MT r + q of m0 on, columns 32 g on; rows past the end repeat the last one.
+template <int SRC, int MT>
 struct MxRows {
-  MxRaw<SRC> raw[RM];
+  MxRaw<SRC> raw[MT];
   __device__ __forceinline__ void load(const MxLinear& p, long long m0, int kb, int r, int g) {
     const int c = kb * 128 + 32 * g;
 #pragma unroll
-    for (int q = 0; q < RM; ++q)
-      raw[q].load(static_cast<const typename Act<SRC>::T*>(p.act) + (size_t)min(m0 + RM * r + q, (long long)p.rows - 1) * p.inputs + c,
+    for (int q = 0; q < MT; ++q)
+      raw[q].load(static_cast<const typename Act<SRC>::T*>(p.act) + (size_t)min(m0 + MT * r + q, (long long)p.rows - 1) * p.inputs + c,
                   p.inputs - c);
   }
-  __device__ __forceinline__ void take(u32x4 (&v)[RM], uint32_t& scale) const {
+  __device__ __forceinline__ void take(u32x4 (&v)[MT], uint32_t& scale) const {
     scale = 0;
 #pragma unroll
-    for (int q = 0; q < RM; ++q) scale |= (uint32_t)raw[q].quantise(v[q]) << (8 * q);
+    for (int q = 0; q < MT; ++q) scale |= (uint32_t)raw[q].quantise(v[q]) << (8 * q);
   }
 };
-template <>
-struct MxRows<KEPT> {
-  u32x4 codes[RM];
+template <int MT>
+struct MxRows<KEPT, MT> {
+  u32x4 codes[MT];
   uint32_t scales;
   __device__ __forceinline__ void load(const MxLinear& p, long long m0, int kb, int r, int g) {
 #pragma unroll
-    for (int q = 0; q < RM; ++q)
-      codes[q] = *reinterpret_cast<const u32x4*>(p.x.codes + (size_t)min(m0 + RM * r + q, (long long)p.rows - 1) * p.x.pitch + kb * 64 + 16 * g);
-    scales = *reinterpret_cast<const uint16_t*>(p.x.scales + (size_t)(4 * kb + g) * p.x.sp + min(m0 + RM * r, ((long long)p.rows - 1) & ~1LL));
+    for (int q = 0; q < MT; ++q)
+      codes[q] = *reinterpret_cast<const u32x4*>(p.x.codes + (size_t)min(m0 + MT * r + q, (long long)p.rows - 1) * p.x.pitch + kb * 64 + 16 * g);
+    const uint8_t* const s = p.x.scales + (size_t)(4 * kb + g) * p.x.sp + min(m0 + MT * r, ((long long)p.rows - 1) & ~(MT - 1LL));
+    scales = MT == 2 ? *reinterpret_cast<const uint16_t*>(s) : *s;
   }
-  __device__ __forceinline__ void take(u32x4 (&v)[RM], uint32_t& scale) const {
+  __device__ __forceinline__ void take(u32x4 (&v)[MT], uint32_t& scale) const {
 #pragma unroll
-    for (int q = 0; q < RM; ++q) v[q] = codes[q];
+    for (int q = 0; q < MT; ++q) v[q] = codes[q];
     scale = scales;
   }
 };
 
-constexpr int resident_waves(int steps) { return steps > 4 ? 8 : 16; }
+// 16 waves of 128 registers hide memory's latency best; where those do not hold the rows, 8 of 256.
+constexpr int resident_waves(int src, int steps) { return steps > 2 || (steps == 2 && src == DT_F32) ? 8 : 16; }
 
 // STEPS: 1, 2, 4 or 8, at least p.steps.
 template <int SRC, int OUT, int STEPS>
-__global__ __launch_bounds__(resident_waves(STEPS) * 64) void mx4_resident_kernel(MxLinear p, MxResident q) {
-  constexpr int RW = resident_waves(STEPS);
+__global__ __launch_bounds__(resident_waves(SRC, STEPS) * 64) void mx4_resident_kernel(MxLinear p, MxResident q) {
+  constexpr int RW = resident_waves(SRC, STEPS);
   constexpr bool EARLY = STEPS == 1 && SRC != DT_F32;
   extern __shared__ __attribute__((aligned(16))) uint8_t mx_smem[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
@@ -146,7 +167,7 @@ __global__ __launch_bounds__(resident_waves(STEPS) * 64) void mx4_resident_kerne
   for (int i = threadIdx.x; i < per * 64; i += RW * 64) bias[i] = p.bias && set0 * 64 + i < p.outputs ? p.bias[set0 * 64 + i] : 0.f;
   const long long units = ((long long)p.rows + 16 * RM - 1) / (16 * RM), stride = (long long)q.blocks * RW;
   long long u = (long long)blk * RW + wave;
-  MxRows<SRC> rows[EARLY ? STEPS : 1];
+  MxRows<SRC, RM> rows[EARLY ? STEPS : 1];
   if constexpr (EARLY) {
 #pragma unroll
     for (int kb = 0; kb < STEPS; ++kb) rows[kb].load(p, min(u, units - 1) * 16 * RM, kb, r, g);
@@ -204,6 +225,13 @@ struct MxStream {
   int mtiles, ntiles, parts;
 };
 
+// A pointer that every lane has, in scalar registers.
+__device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return reinterpret_cast<const uint8_t*>((uint64_t)hi << 32 | lo);
+}
+
 template <int OUT, int NT, int WM, bool PART>
 __global__ __launch_bounds__(128 * WM, 2) void mx4_stream_kernel(MxLinear p, MxStream q) {
   constexpr int BN = 2 * NT * 16, BM = WM * 64, SETS = (BN + BM) / 64, MINE = SETS / (2 * WM);
@@ -211,8 +239,8 @@ __global__ __launch_bounds__(128 * WM, 2) void mx4_stream_kernel(MxLinear p, MxS
   static_assert(MINE * 2 * WM == SETS && BN / 64 % MINE == 0, "a wave copies whole sets of one operand");
   // Separate objects: reads of one are then known not to wait for copies into the other.
   __shared__ __attribute__((aligned(16))) uint8_t S0[STAGE], S1[STAGE];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  int mt, nt, part;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  int r = lane & 15, g = lane >> 4, mt, nt, part;
   if constexpr (PART) {      // the tiles of a part on one XCD, whose L2 then reads that part once
     const int slot = blockIdx.x >> 3, tiles = q.mtiles * q.ntiles, tile = slot % tiles;
     part = slot / tiles * 8 + (blockIdx.x & 7);
@@ -232,10 +260,12 @@ __global__ __launch_bounds__(128 * WM, 2) void mx4_stream_kernel(MxLinear p, MxS
   const int n0 = nt * BN;
   // what this wave copies: MINE sets of one operand; rows past the end repeat the last one
   const bool of_w = wave * MINE < BN / 64;
-  const Mx& src = of_w ? p.w : p.x;
+  const Mx src = {of_w ? p.w.codes : p.x.codes, of_w ? p.w.scales : p.x.scales, 0, 0, of_w ? p.w.pitch : p.x.pitch,
+                  of_w ? p.w.sp : p.x.sp};
   const long long first = of_w ? n0 + wave * MINE * 64 : m0 + (wave * MINE - BN / 64) * 64, last = (of_w ? p.outputs : p.rows) - 1;
   const long long base = min(first, last);
-  const uint8_t* const codes = src.codes + (size_t)base * src.pitch;
+  const uint8_t* const codes = uniform(src.codes + (size_t)base * src.pitch);
+  const uint8_t* const scales = uniform(src.scales);
   const uint32_t pitch = (uint32_t)src.pitch, sstep = (uint32_t)(4 * src.sp), chunk = 16 * ((lane & 7) ^ (lane >> 3));
   const int lane_row = (int)(first - base) + 4 * (lane >> 3), last_row = (int)min(last - base, (long long)INT_MAX);
   uint32_t soff[MINE];
@@ -244,7 +274,7 @@ __global__ __launch_bounds__(128 * WM, 2) void mx4_stream_kernel(MxLinear p, MxS
   auto stage = [&](uint8_t* dst, int s) __attribute__((always_inline)) {
 #if __HIP_DEVICE_COMPILE__
     const __amdgpu_buffer_rsrc_t cr = __builtin_amdgcn_make_buffer_rsrc((void*)codes, 0, 0xffffffffu, 0x27000);
-    const __amdgpu_buffer_rsrc_t sr = __builtin_amdgcn_make_buffer_rsrc((void*)src.scales, 0, 0xffffffffu, 0x27000);
+    const __amdgpu_buffer_rsrc_t sr = __builtin_amdgcn_make_buffer_rsrc((void*)scales, 0, 0xffffffffu, 0x27000);
 #pragma unroll
     for (int l = 0; l < 10 * MINE; ++l) {
       const int i = l / 10, k = l % 10 - 2;
@@ -257,7 +287,7 @@ __global__ __launch_bounds__(128 * WM, 2) void mx4_stream_kernel(MxLinear p, MxS
       }
     }
 #else
-    (void)codes, (void)dst, (void)s, (void)soff, (void)sstep, (void)pitch, (void)chunk, (void)lane_row, (void)last_row;
+    (void)codes, (void)scales, (void)dst, (void)s, (void)soff, (void)sstep, (void)pitch, (void)chunk, (void)lane_row, (void)last_row;
 #endif
   };
   const int wn = wave & 1, wm = wave >> 1;
@@ -317,6 +347,7 @@ __global__ __launch_bounds__(128 * WM, 2) void mx4_stream_kernel(MxLinear p, MxS
   }
   if (s < s1) step(s, S0, S1);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last copies, which nothing reads
+  asm volatile("" : "+v"(r), "+v"(g));     // or the offsets of what follows would be kept in registers throughout
   if ((p.steps & 1) && part == q.parts - 1) {         // the last 128 columns, straight from memory
     const int kb = p.steps - 1;
     const long long m = m0 + wm * 64 + 4 * r;
@@ -375,26 +406,27 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(MxLinear p, int parts) {
 
 // ---- few rows or outputs -----------------------------------------------------------------------------
 
-// What counts is the time to the last byte: a block computes 32 rows by 16 outputs, its waves steps of the columns in
+// What counts is the time to the last byte: a block computes 16 MT rows by 16 outputs, its waves steps of the columns in
 // turn, two at a time, operands straight from memory, sums joined in LDS.
-constexpr int FW = 16;
+constexpr int few_waves(int src, int mt) { return src == DT_F32 && mt == 2 ? 8 : 16; }    // registers
 
-template <int SRC, int OUT>
-__global__ __launch_bounds__(FW * 64) void mx4_few_kernel(MxLinear p) {
-  __shared__ f4 part[FW - 1][RM][64];
+template <int SRC, int OUT, int MT>
+__global__ __launch_bounds__(few_waves(SRC, MT) * 64) void mx4_few_kernel(MxLinear p) {
+  constexpr int FW = few_waves(SRC, MT);
+  __shared__ f4 part[FW][MT][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int waves = blockDim.x >> 6, n0 = blockIdx.x * 16;
-  const long long m0 = (long long)blockIdx.y * 16 * RM;
+  const long long m0 = (long long)blockIdx.y * 16 * MT;
   const int n = min(n0 + r, p.outputs - 1);
   const uint8_t* const wrow = p.w.codes + (size_t)n * p.w.pitch + 16 * g;
   const uint8_t* const wscale = p.w.scales + (size_t)g * p.w.sp + n;
-  f4 acc[RM];
+  f4 acc[MT];
 #pragma unroll
-  for (int q = 0; q < RM; ++q) acc[q] = f4{0.f, 0.f, 0.f, 0.f};
+  for (int q = 0; q < MT; ++q) acc[q] = f4{0.f, 0.f, 0.f, 0.f};
   struct Step {
     u32x4 w;
     uint32_t ws;
-    MxRows<SRC> x;
+    MxRows<SRC, MT> x;
   };
   auto load = [&](Step& s, int kb) __attribute__((always_inline)) {
     s.w = *reinterpret_cast<const u32x4*>(wrow + (size_t)kb * 64);
@@ -402,11 +434,11 @@ __global__ __launch_bounds__(FW * 64) void mx4_few_kernel(MxLinear p) {
     s.x.load(p, m0, kb, r, g);
   };
   auto multiply = [&](const Step& s) __attribute__((always_inline)) {
-    u32x4 b[RM];
-    uint32_t sb;
-    s.x.take(b, sb);
-    acc[0] = mx_mma<0, 0>(b[0], s.w, acc[0], sb, s.ws);
-    acc[1] = mx_mma<1, 0>(b[1], s.w, acc[1], sb, s.ws);
+    u32x4 x[MT];
+    uint32_t sx;
+    s.x.take(x, sx);
+    acc[0] = mx_mma<0, 0>(x[0], s.w, acc[0], sx, s.ws);
+    if constexpr (MT == 2) acc[1] = mx_mma<1, 0>(x[1], s.w, acc[1], sx, s.ws);
   };
   for (int kb = wave; kb < p.steps; kb += 2 * waves) {
     Step a, b;
@@ -415,29 +447,23 @@ __global__ __launch_bounds__(FW * 64) void mx4_few_kernel(MxLinear p) {
     multiply(a);
     if (kb + waves < p.steps) multiply(b);
   }
-  if (wave > 0) {
 #pragma unroll
-    for (int q = 0; q < RM; ++q) part[wave - 1][q][lane] = acc[q];
-  }
+  for (int q = 0; q < MT; ++q) part[wave][q][lane] = acc[q];
   __syncthreads();
-  if (wave > 0) return;
   typedef typename Act<OUT>::T T;
-#pragma unroll
-  for (int q = 0; q < RM; ++q) {
-    for (int k = 1; k < waves; ++k) acc[q] += part[k - 1][q][lane];
-    const int o = n0 + r;
-    if (o >= p.outputs) continue;
-    const float bias = p.bias ? p.bias[o] : 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const long long m = m0 + RM * (4 * g + j) + q;
-      if (m >= p.rows) continue;
-      float v = acc[q][j] + bias;
-      if (p.relu) v = __builtin_elementwise_maximum(v, 0.f);
-      const size_t at = (size_t)m * p.outputs + o;
-      if (p.residual) v += Act<OUT>::ld(static_cast<const T*>(p.residual) + at);
-      Act<OUT>::st(static_cast<T*>(p.out) + at, v);
-    }
+  // thread: output n0 + e % 16 of row MT i + q, i = 4 (lane / 16) + j of the lane that holds it
+  for (int e = threadIdx.x; e < MT * 256; e += blockDim.x) {
+    const int row = e >> 4, q = row % MT, i = row / MT, o = n0 + (e & 15);
+    const float* const at = reinterpret_cast<const float*>(&part[0][q][(i >> 2) * 16 + (e & 15)]) + (i & 3);
+    float v = at[0];
+    for (int k = 1; k < waves; ++k) v += at[k * MT * 256];
+    const long long m = m0 + row;
+    if (m >= p.rows || o >= p.outputs) continue;
+    if (p.bias) v += p.bias[o];
+    if (p.relu) v = __builtin_elementwise_maximum(v, 0.f);
+    const size_t to = (size_t)m * p.outputs + o;
+    if (p.residual) v += Act<OUT>::ld(static_cast<const T*>(p.residual) + to);
+    Act<OUT>::st(static_cast<T*>(p.out) + to, v);
   }
 }
 
@@ -483,7 +509,7 @@ void go_join(lf_context* ctx, const MxLinear& p, int parts) {
 
 template <int SRC, int OUT, int STEPS>
 int go_resident(lf_context* ctx, const MxLinear& p) {
-  constexpr int RW = resident_waves(STEPS);
+  constexpr int RW = resident_waves(SRC, STEPS);
   const int sets = (p.outputs + 63) / 64, each = set_bytes(p.steps);
   const long long units = ((long long)p.rows + 16 * RM - 1) / (16 * RM);
   MxResident q;
@@ -508,8 +534,12 @@ int go_small(lf_context* ctx, const MxLinear& p, const MxPlan& plan) {
     if (p.steps <= 4) return go_resident<SRC, OUT, 4>(ctx, p);
     return go_resident<SRC, OUT, 8>(ctx, p);
   }
-  hipLaunchKernelGGL((mx4_few_kernel<SRC, OUT>), dim3((p.outputs + 15) / 16, (p.rows + 31) / 32), dim3(std::min(p.steps, FW) * 64), 0,
-                     ctx->stream, p);
+  if (p.rows <= 16)
+    hipLaunchKernelGGL((mx4_few_kernel<SRC, OUT, 1>), dim3((p.outputs + 15) / 16), dim3(std::min(p.steps, few_waves(SRC, 1)) * 64), 0,
+                       ctx->stream, p);
+  else
+    hipLaunchKernelGGL((mx4_few_kernel<SRC, OUT, 2>), dim3((p.outputs + 15) / 16, (p.rows + 31) / 32),
+                       dim3(std::min(p.steps, few_waves(SRC, 2)) * 64), 0, ctx->stream, p);
   return LF_OK;
 }
 
