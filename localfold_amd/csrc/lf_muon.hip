@@ -1,11 +1,18 @@
 // Newton-Schulz products (lf_orthogonalize, lf_muon_step): X <- (a I + b G + c G^2) X with G = X X^T, X scaled
-// to a Frobenius norm of one at first, on the orientation that makes G small.
+// to a Frobenius norm of one at first, on the orientation that makes G small (m x m, X m x n).
 //
 // Operands are pairs of f16, v = hi + lo: products hi hi + hi lo + lo hi keep 22 bits of each factor and are summed
 // in f32.  A power of two per step and matrix, known from the coefficients alone (muon_plan), keeps hi
 // within 2^14 and lo's last bit at 2^-38 of the largest value that the matrix can have, so nothing leaves
 // f16's range.  Rounding X to bf16, as is usual, would leave 2^-9 of the largest singular values on the
 // small ones, which a run of five steps makes a few hundred times larger.
+//
+// Fragments.  An operand is kept as fragments of 16 rows by 32 of the contraction, as the instruction takes
+// them: lane (r, g) = (lane % 16, lane / 16) has row r and eight k.  Which eight is free, as long as both
+// operands agree: k = 16 (e / 4) + 4 g + e % 4 for e < 8.  A product's result has, in lane (r, g), rows 4 g + e of
+// column r of a tile of 16 x 16, so two tiles one above the other are, as they lie in registers, a fragment
+// of the result's transpose; for a symmetric result, of the result itself.  The other order, where it is needed,
+// comes from a product with the identity, which is exact.
 #include <algorithm>
 #include <cmath>
 
@@ -15,20 +22,37 @@ namespace lf {
 
 namespace {
 
-// A matrix in scratch: hi and lo, [rows][ld] each, rows and ld multiples of 64, zeros behind the matrix.
-struct Planes {
-  _Float16 *hi, *lo;
-  int ld;
-  size_t stride;               // between matrices of the batch
-};
-
 struct MuonSize {
-  int m, n, mp, np;            // the smaller side, the larger, both rounded up to 64
+  int m, n;                    // the smaller side, the larger
 };
 
-__device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
-  hi = (_Float16)v;
-  lo = (_Float16)(v - (float)hi);
+__device__ __forceinline__ f4 mfma_pair(h8 ah, h8 al, h8 bh, h8 bl, f4 c) {
+  c = mfma16(al, bh, c);
+  c = mfma16(ah, bl, c);
+  return mfma16(ah, bh, c);
+}
+
+// Four values into half `part` of a pair of fragments.
+__device__ __forceinline__ void split4(f4 v, h8& hi, h8& lo, int part) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const _Float16 h = (_Float16)v[e];
+    hi[4 * part + e] = h;
+    lo[4 * part + e] = (_Float16)(v[e] - (float)h);
+  }
+}
+
+// The fragment of the identity that takes half `part` of a fragment's k to columns.
+__device__ __forceinline__ h8 identity(int part, int r, int g) {
+  h8 v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (_Float16)((e >> 2) == part && r == 4 * g + (e & 3) ? 1.f : 0.f);
+  return v;
+}
+// Fragment f (16 rows, 32 k) transposed: half `part` of its k, 16 of them, by its 16 rows, as half of a fragment.
+__device__ __forceinline__ h4 turn(h8 f, h8 eye) {
+  const f4 d = mfma16(f, eye, f4{0.f, 0.f, 0.f, 0.f});
+  return h4{(_Float16)d[0], (_Float16)d[1], (_Float16)d[2], (_Float16)d[3]};
 }
 
 // u of an element, and its momentum stored.
@@ -44,6 +68,236 @@ __device__ __forceinline__ float muon_u(const Muon& a, size_t i, bool write) {
     m = a.momentum_out[i];
   }
   return a.nesterov ? g + a.momentum_factor * m : m;
+}
+
+// The place of X's element (i, j) in the stored matrix.
+__device__ __forceinline__ size_t place(const Muon& a, int i, int j) {
+  return a.rows > a.cols ? (size_t)j * a.cols + i : (size_t)i * a.cols + j;
+}
+
+template <int OUT>
+__device__ __forceinline__ void muon_store(const Muon& m, size_t at, float o) {
+  typedef typename Act<OUT>::T T;
+  float v = -m.rate * o;
+  if (m.weight) v = m.keep * Act<OUT>::ld(static_cast<const T*>(m.weight) + at) + v;
+  Act<OUT>::st(static_cast<T*>(m.out) + at, v);
+}
+
+// ---- one block a matrix --------------------------------------------------------------------------
+
+// m to 128 and n to 512: a block runs all steps.  Each of its 8 waves keeps J tiles of 16 columns of X, all rows, in
+// registers, as fragments of X^T: the operand of P X, whose result is the next X^T in place.  G takes X by rows: J
+// times the waves turn a tile each, 128 columns together, and put it into LDS, and all add to their tiles of G.  G
+// and then P are in LDS.  MB: m in 32s.
+template <int MB>
+struct MuonTiles {               // a wave's tiles of G: A by B of MT by MT
+  static constexpr int MT = 2 * MB, A = MB == 4 ? 2 : 1, B = MB == 4 ? 4 : MB == 2 ? 2 : 1, ACROSS = MT / B;
+};
+
+struct MuonSteps {
+  float gram[MUON_STEPS], square[MUON_STEPS], gb[MUON_STEPS], diagonal[MUON_STEPS], apply[MUON_STEPS];
+  int count, start;            // start: X's first exponent
+};
+
+template <int MB, int J, int DT, int OUT>
+__global__ __launch_bounds__(512, 2) void muon_block_kernel(Muon a, MuonSize z, MuonSteps steps) {
+  typedef MuonTiles<MB> Q;
+  constexpr int MT = Q::MT;
+  extern __shared__ __attribute__((aligned(16))) uint8_t muon_smem[];
+  __shared__ double norm[8];
+  uint8_t* const xs = muon_smem;                         // X by rows, 128 columns: [tile][32 columns][hi, lo]
+  uint8_t* const gs = muon_smem + MT * 4 * 2048;         // G or P: [tile][32 rows][hi, lo]
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  int r = lane & 15, g = lane >> 4;
+  const size_t base = (size_t)blockIdx.x * a.rows * a.cols;
+  h8 xh[J][MB], xl[J][MB];
+  {
+    float u[J][MB][8];
+    double t = 0;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int kb = 0; kb < MB; ++kb) {
+        __builtin_amdgcn_sched_barrier(0);     // the addresses of 8 elements at a time
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int i = 32 * kb + 16 * (e >> 2) + 4 * g + (e & 3), c = 16 * (8 * j + wave) + r;
+          u[j][kb][e] = i < z.m && c < z.n ? muon_u<DT>(a, base + place(a, i, c), true) : 0.f;
+          t += (double)u[j][kb][e] * u[j][kb][e];
+        }
+      }
+    for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+    if (lane == 0) norm[wave] = t;
+    __syncthreads();
+    t = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t += norm[i];
+    const double f = 1.0 / (sqrt(t) + a.epsilon);
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int kb = 0; kb < MB; ++kb)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          __builtin_amdgcn_sched_barrier(0);
+          f4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = ldexpf((float)(u[j][kb][4 * h + e] * f), steps.start);
+          split4(v, xh[j][kb], xl[j][kb], h);
+        }
+  }
+  const h8 eye[2] = {identity(0, r, g), identity(1, r, g)};
+  const int ta = wave / Q::ACROSS * Q::A, tb = wave % Q::ACROSS * Q::B;      // the wave's tiles of G
+  const bool mine = wave / Q::ACROSS * Q::A < MT;
+  for (int s = 0; s < steps.count; ++s) {
+    f4 gram[Q::A][Q::B];
+#pragma unroll
+    for (int i = 0; i < Q::A; ++i)
+#pragma unroll
+      for (int j = 0; j < Q::B; ++j) gram[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (j > 0) __syncthreads();        // the last columns are read
+#pragma unroll
+      for (int kb = 0; kb < MB; ++kb)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          __builtin_amdgcn_sched_barrier(0);
+          uint8_t* const at = xs + ((2 * kb + h) * 4 + (wave >> 1)) * 2048 + lane * 16 + 8 * (wave & 1);
+          *reinterpret_cast<h4*>(at) = turn(xh[j][kb], eye[h]);
+          *reinterpret_cast<h4*>(at + 1024) = turn(xl[j][kb], eye[h]);
+        }
+      __syncthreads();
+      if (mine) {
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+          __builtin_amdgcn_sched_barrier(0);     // or all fragments would be read at once, and spill
+          h8 ah[Q::A], al[Q::A];
+#pragma unroll
+          for (int i = 0; i < Q::A; ++i) {
+            const uint8_t* const at = xs + ((ta + i) * 4 + kb) * 2048 + lane * 16;
+            ah[i] = *reinterpret_cast<const h8*>(at);
+            al[i] = *reinterpret_cast<const h8*>(at + 1024);
+          }
+#pragma unroll
+          for (int k = 0; k < Q::B; ++k) {
+            const uint8_t* const at = xs + ((tb + k) * 4 + kb) * 2048 + lane * 16;
+            const h8 bh = *reinterpret_cast<const h8*>(at), bl = *reinterpret_cast<const h8*>(at + 1024);
+#pragma unroll
+            for (int i = 0; i < Q::A; ++i) gram[i][k] = mfma_pair(ah[i], al[i], bh, bl, gram[i][k]);
+          }
+        }
+      }
+    }
+    // A symmetric tile (ta + i, tb + k) in its place: rows of tile tb + k, k of tile ta + i.
+    auto put = [&](const f4 (&v)[Q::A][Q::B]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int k = 0; k < Q::B; ++k)
+#pragma unroll
+        for (int i = 0; i < Q::A; ++i) {
+          __builtin_amdgcn_sched_barrier(0);
+          h8 hi, lo;
+          split4(v[i][k], hi, lo, 0);
+          uint8_t* const at = gs + ((tb + k) * MB + (ta + i) / 2) * 2048 + lane * 16 + 8 * ((ta + i) & 1);
+          *reinterpret_cast<h4*>(at) = h4{hi[0], hi[1], hi[2], hi[3]};
+          *reinterpret_cast<h4*>(at + 1024) = h4{lo[0], lo[1], lo[2], lo[3]};
+        }
+    };
+    if (mine) {
+#pragma unroll
+      for (int i = 0; i < Q::A; ++i)
+#pragma unroll
+        for (int k = 0; k < Q::B; ++k) gram[i][k] *= steps.gram[s];
+      put(gram);
+    }
+    __syncthreads();
+    f4 p[Q::A][Q::B];
+    if (mine) {
+#pragma unroll
+      for (int i = 0; i < Q::A; ++i)
+#pragma unroll
+        for (int k = 0; k < Q::B; ++k) p[i][k] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kb = 0; kb < MB; ++kb) {
+        __builtin_amdgcn_sched_barrier(0);
+        h8 ah[Q::A], al[Q::A];
+#pragma unroll
+        for (int i = 0; i < Q::A; ++i) {
+          const uint8_t* const at = gs + ((ta + i) * MB + kb) * 2048 + lane * 16;
+          ah[i] = *reinterpret_cast<const h8*>(at);
+          al[i] = *reinterpret_cast<const h8*>(at + 1024);
+        }
+#pragma unroll
+        for (int k = 0; k < Q::B; ++k) {
+          const uint8_t* const at = gs + ((tb + k) * MB + kb) * 2048 + lane * 16;
+          const h8 bh = *reinterpret_cast<const h8*>(at), bl = *reinterpret_cast<const h8*>(at + 1024);
+#pragma unroll
+          for (int i = 0; i < Q::A; ++i) p[i][k] = mfma_pair(ah[i], al[i], bh, bl, p[i][k]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < Q::A; ++i)
+#pragma unroll
+        for (int k = 0; k < Q::B; ++k) {
+          p[i][k] = p[i][k] * steps.square[s] + gram[i][k] * steps.gb[s];
+          if (ta + i == tb + k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[i][k][e] += r == 4 * g + e ? steps.diagonal[s] : 0.f;
+        }
+    }
+    __syncthreads();          // G is read
+    if (mine) put(p);
+    __syncthreads();
+    const bool last = s + 1 == steps.count;
+    constexpr int JP = J > 1 ? 2 : 1;     // column tiles at a time, which share the reads of P
+#pragma unroll
+    for (int j = 0; j < J; j += JP) {
+      f4 y[JP][MT];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < JP; ++q) y[q][t] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kb = 0; kb < MB; ++kb) {
+          const uint8_t* const at = gs + (t * MB + kb) * 2048 + lane * 16;
+          const h8 ph = *reinterpret_cast<const h8*>(at), pl = *reinterpret_cast<const h8*>(at + 1024);
+#pragma unroll
+          for (int q = 0; q < JP; ++q) y[q][t] = mfma_pair(ph, pl, xh[j + q][kb], xl[j + q][kb], y[q][t]);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < JP; ++q)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          __builtin_amdgcn_sched_barrier(0);
+          y[q][t] *= steps.apply[s];
+          split4(y[q][t], xh[j + q][t / 2], xl[j + q][t / 2], t & 1);
+          if (last) {
+            asm volatile("" : "+v"(r), "+v"(g));     // or the places of all elements would be kept in registers throughout
+            const int c = 16 * (8 * (j + q) + wave) + r;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int i = 16 * t + 4 * g + e;
+              if (i < z.m && c < z.n) muon_store<OUT>(a, base + place(a, i, c), y[q][t][e]);
+            }
+          }
+        }
+    }
+  }
+}
+
+// ---- larger matrices: a product a launch ---------------------------------------------------------
+
+// A matrix in scratch, as fragments: [rows / 16][k / 32][hi, lo], 1 KB each; rows and k are multiples of 128, zeros
+// behind the matrix.
+struct Frags {
+  uint8_t* at;
+  int kbs;
+  size_t stride;               // bytes between matrices of the batch
+};
+__device__ __forceinline__ uint8_t* frag(const Frags& f, int tile, int kb) {
+  return f.at + blockIdx.z * f.stride + ((size_t)tile * f.kbs + kb) * 2048;
 }
 
 constexpr int NORM_MOST = 64;  // blocks that share a matrix
@@ -65,122 +319,274 @@ __global__ __launch_bounds__(256) void muon_norm_kernel(Muon a, double* partial)
   if (threadIdx.x == 0) partial[blockIdx.y * NORM_MOST + blockIdx.x] = sm[0] + sm[1] + sm[2] + sm[3];
 }
 
-// X = u / (|u| + epsilon) times 2^e, as X and as its transpose; one block a tile of 64 x 64.
+// Stores a wave's two tiles of 16 columns, 32 rows, of X: fragments of X^T (j tiles jt, jt + 1) and of X (i tiles).
+__device__ __forceinline__ void store_x(const h8 (&hi)[2], const h8 (&lo)[2], const Frags& x, const Frags& xt, int jt, int kb,
+                                        int lane) {
+  const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    uint8_t* const at = frag(xt, jt + q, kb) + lane * 16;
+    *reinterpret_cast<h8*>(at) = hi[q];
+    *reinterpret_cast<h8*>(at + 1024) = lo[q];
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const h8 eye = identity(h, r, g);
+    const h4 a = turn(hi[0], eye), b = turn(hi[1], eye), c = turn(lo[0], eye), d = turn(lo[1], eye);
+    uint8_t* const at = frag(x, 2 * kb + h, jt / 2) + lane * 16;
+    *reinterpret_cast<h8*>(at) = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    *reinterpret_cast<h8*>(at + 1024) = __builtin_shufflevector(c, d, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
+// X = u / (|u| + epsilon) times 2^e; a wave takes 32 rows by 32 columns.
 template <int DT>
-__global__ __launch_bounds__(256) void muon_start_kernel(Muon a, MuonSize z, const double* partial, int parts, int e, Planes x,
-                                                         Planes xt) {
-  __shared__ float tile[64][65];
+__global__ __launch_bounds__(256) void muon_start_kernel(Muon a, MuonSize z, const double* partial, int parts, int e, Frags x,
+                                                         Frags xt) {
   double t = 0;
   for (int i = 0; i < parts; ++i) t += partial[blockIdx.z * NORM_MOST + i];
   const double f = 1.0 / (sqrt(t) + a.epsilon);
   const size_t base = (size_t)blockIdx.z * a.rows * a.cols;
-  const bool tall = a.rows > a.cols;
-  const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;     // of X
-  const int r0 = tall ? j0 : i0, c0 = tall ? i0 : j0;       // of the stored matrix
-  for (int k = threadIdx.x; k < 64 * 64; k += 256) {
-    const int r = r0 + (k >> 6), c = c0 + (k & 63);
-    float v = 0.f;
-    if (r < a.rows && c < a.cols) v = ldexpf((float)(muon_u<DT>(a, base + (size_t)r * a.cols + c, false) * f), e);
-    tile[k >> 6][k & 63] = v;
-  }
-  __syncthreads();
-  for (int k = threadIdx.x; k < 64 * 64; k += 256) {
-    const int p = k >> 6, q = k & 63;
-    // [stored row][stored column] is X's plane where the matrix is wide, its transpose's where it is tall
-    const Planes& same = tall ? xt : x;
-    const Planes& other = tall ? x : xt;
-    const size_t s = blockIdx.z * same.stride + (size_t)(r0 + p) * same.ld + c0 + q;
-    split(tile[p][q], same.hi[s], same.lo[s]);
-    const size_t o = blockIdx.z * other.stride + (size_t)(c0 + p) * other.ld + r0 + q;
-    split(tile[q][p], other.hi[o], other.lo[o]);
-  }
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int kb = blockIdx.y, jt = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 2;
+  h8 hi[2], lo[2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      f4 v;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = 32 * kb + 16 * h + 4 * g + k, j = 16 * (jt + q) + r;
+        v[k] = i < z.m && j < z.n ? ldexpf((float)(muon_u<DT>(a, base + place(a, i, j), false) * f), e) : 0.f;
+      }
+      split4(v, hi[q], lo[q], h);
+    }
+  store_x(hi, lo, x, xt, jt, kb, lane);
 }
 
-enum { GRAM = 0, SQUARE = 1, APPLY = 2, LAST = 3 };
+enum { GRAM = 0, GRAM_PART = 1, SQUARE = 2, APPLY = 3, LAST = 4 };
 
 struct Product {
-  Planes a, b;                 // out[i][j] = sum over k of a[i][k] b[j][k]
-  int k;
-  Planes out, out_t;           // APPLY: X and its transpose; GRAM, SQUARE: a symmetric matrix
+  Frags a, b;                  // out[i][j] = sum over k of a[i][k] b[j][k]
+  int steps, parts;            // of 32 k; GRAM_PART: blocks that share a tile's steps
+  Frags out, out_t;            // APPLY: X and its transpose; GRAM, SQUARE: a symmetric matrix
+  float* partial;              // GRAM_PART: [part][tile of the block][tile][lane][4]
   float f;                     // factor of the sum
   float fb, fa;                // SQUARE: of a's own element, and the diagonal's
 };
 
-template <int OUT>
-__device__ __forceinline__ void muon_store(const Muon& m, size_t at, float o) {
-  typedef typename Act<OUT>::T T;
-  float v = -m.rate * o;
-  if (m.weight) v = m.keep * Act<OUT>::ld(static_cast<const T*>(m.weight) + at) + v;
-  Act<OUT>::st(static_cast<T*>(m.out) + at, v);
+// The t-th of the tiles on and above the diagonal of n x n.
+__device__ __forceinline__ void upper(int t, int n, int& i, int& j) {
+  i = 0;
+  while (t >= n - i) {
+    t -= n - i;
+    ++i;
+  }
+  j = i + t;
 }
 
-// A wave computes 32 x 32, a block 64 x 64, operands straight from memory.
-template <int KIND, int OUT>
-__global__ __launch_bounds__(256) void muon_product_kernel(Product p, Muon m, MuonSize z) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  if ((KIND == GRAM || KIND == SQUARE) && blockIdx.y > blockIdx.x) return;      // symmetric: the upper tiles, mirrored
-  const int i0 = blockIdx.y * 64 + (wave >> 1) * 32, j0 = blockIdx.x * 64 + (wave & 1) * 32;
-  const size_t za = blockIdx.z * p.a.stride, zb = blockIdx.z * p.b.stride;
-  f4 acc[2][2];
+// Symmetric results: two tiles one above the other in their place, and, off the diagonal, turned in the other.
+__device__ __forceinline__ void store_symmetric(const f4 (&v)[2][2], const Frags& out, int ti, int tj, bool both, int lane) {
+  const int r = lane & 15, g = lane >> 4;
+  h8 hi[2], lo[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int q = 0; q < 2; ++q) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < p.k; k += 32) {
-    h8 ah[2], al[2], bh[2], bl[2];
+    for (int h = 0; h < 2; ++h) split4(v[h][q], hi[q], lo[q], h);
+    uint8_t* const at = frag(out, tj + q, ti / 2) + lane * 16;
+    *reinterpret_cast<h8*>(at) = hi[q];
+    *reinterpret_cast<h8*>(at + 1024) = lo[q];
+  }
+  if (!both) return;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const size_t x = za + (size_t)(i0 + 16 * t + r) * p.a.ld + k + 8 * g;
-      const size_t y = zb + (size_t)(j0 + 16 * t + r) * p.b.ld + k + 8 * g;
-      ah[t] = *reinterpret_cast<const h8*>(p.a.hi + x);
-      al[t] = *reinterpret_cast<const h8*>(p.a.lo + x);
-      bh[t] = *reinterpret_cast<const h8*>(p.b.hi + y);
-      bl[t] = *reinterpret_cast<const h8*>(p.b.lo + y);
+  for (int h = 0; h < 2; ++h) {
+    const h8 eye = identity(h, r, g);
+    const h4 a = turn(hi[0], eye), b = turn(hi[1], eye), c = turn(lo[0], eye), d = turn(lo[1], eye);
+    uint8_t* const at = frag(out, ti + h, tj / 2) + lane * 16;
+    *reinterpret_cast<h8*>(at) = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    *reinterpret_cast<h8*>(at + 1024) = __builtin_shufflevector(c, d, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
+// A block of four waves computes 32 W by 32 W, a wave 16 W by 16 W (W 2 or 4), 32 k a step, both operands through two
+// LDS buffers.
+template <int KIND, int W, int OUT>
+__global__ __launch_bounds__(256, 2) void muon_product_kernel(Product p, Muon m, MuonSize z, int across) {
+  constexpr int STAGE = 4 * W * 2048, EACH = STAGE / 4096;      // copies of 1 KB a wave
+  __shared__ __attribute__((aligned(16))) uint8_t S0[STAGE], S1[STAGE];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  int bi, bj, part = 0;
+  if constexpr (KIND == APPLY || KIND == LAST) {
+    bi = blockIdx.x % across;
+    bj = blockIdx.x / across;
+  } else {
+    const int tile = KIND == GRAM_PART ? blockIdx.x / p.parts : blockIdx.x;
+    part = KIND == GRAM_PART ? blockIdx.x % p.parts : 0;
+    upper(tile, across, bi, bj);
+  }
+  const int s0 = KIND == GRAM_PART ? (int)((long long)p.steps * part / p.parts) : 0;
+  const int s1 = KIND == GRAM_PART ? (int)((long long)p.steps * (part + 1) / p.parts) : p.steps;
+  // [2 W tiles of a][2 W tiles of b], hi and lo of each side by side
+  const uint8_t* const src = frag(wave < 2 ? p.a : p.b, (wave < 2 ? bi : bj) * 2 * W + (wave & 1) * W, 0) + lane * 16;
+  const size_t row = (size_t)(wave < 2 ? p.a.kbs : p.b.kbs) * 2048;
+  auto stage = [&](uint8_t* dst, int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const uint8_t* const at = src + (i >> 1) * row + (size_t)s * 2048 + (i & 1) * 1024;
+#if __HIP_DEVICE_COMPILE__
+      __builtin_amdgcn_global_load_lds(at, dst + (wave * EACH + i) * 1024, 16, 0, 0);
+#else
+      (void)at, (void)dst;
+#endif
     }
+  };
+  const int wi = wave >> 1, wj = wave & 1;
+  f4 acc[W][W];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < W; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        acc[i][j] = mfma16(al[i], bh[j], acc[i][j]);
-        acc[i][j] = mfma16(ah[i], bl[j], acc[i][j]);
-        acc[i][j] = mfma16(ah[i], bh[j], acc[i][j]);
-      }
+    for (int j = 0; j < W; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+  stage(S0, s0);
+  auto step = [&](int s, const uint8_t* buf, uint8_t* other) __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();          // step s in LDS for every wave, every wave done with the other buffer
+    h8 ah[W], al[W], bh[W], bl[W];
+#pragma unroll
+    for (int t = 0; t < W; ++t) {
+      const uint8_t* const a = buf + (wi * W + t) * 2048 + lane * 16;
+      const uint8_t* const b = buf + (2 * W + wj * W + t) * 2048 + lane * 16;
+      ah[t] = *reinterpret_cast<const h8*>(a);
+      al[t] = *reinterpret_cast<const h8*>(a + 1024);
+      bh[t] = *reinterpret_cast<const h8*>(b);
+      bl[t] = *reinterpret_cast<const h8*>(b + 1024);
+    }
+    stage(other, min(s + 1, s1 - 1));
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+      for (int j = 0; j < W; ++j) acc[i][j] = mfma_pair(ah[i], al[i], bh[j], bl[j], acc[i][j]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  int s = s0;
+  for (; s + 1 < s1; s += 2) {
+    step(s, S0, S1);
+    step(s + 1, S1, S0);
+  }
+  if (s < s1) step(s, S0, S1);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last copy, which nothing reads
+  const int ti = (bi * 2 + wi) * W, tj = (bj * 2 + wj) * W;
+  if constexpr (KIND == GRAM_PART) {
+    f4* const at = reinterpret_cast<f4*>(p.partial) +
+                   ((((size_t)blockIdx.z * p.parts + part) * (across * (across + 1) / 2) + blockIdx.x / p.parts) * 4 + wave) * W * W * 64 + lane;
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+      for (int j = 0; j < W; ++j) at[(i * W + j) * 64] = acc[i][j];
+    return;
   }
 #pragma unroll
-  for (int ti = 0; ti < 2; ++ti)
+  for (int i = 0; i < W; i += 2)
 #pragma unroll
-    for (int tj = 0; tj < 2; ++tj)
+    for (int j = 0; j < W; j += 2) {
+      f4 v[2][2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = i0 + 16 * ti + 4 * g + e, j = j0 + 16 * tj + r;
-        float v = acc[ti][tj][e] * p.f;
-        if constexpr (KIND == SQUARE) {
-          const size_t at = za + (size_t)i * p.a.ld + j;
-          v += p.fb * ((float)p.a.hi[at] + (float)p.a.lo[at]);
-          if (i == j) v += p.fa;
-        }
-        if constexpr (KIND == LAST) {
-          if (i >= z.m || j >= z.n) continue;
-          const size_t at = m.rows > m.cols ? (size_t)j * m.cols + i : (size_t)i * m.cols + j;
-          muon_store<OUT>(m, (size_t)blockIdx.z * m.rows * m.cols + at, v);
-        } else {
-          const Planes& t = KIND == APPLY ? p.out_t : p.out;
-          const size_t at = blockIdx.z * p.out.stride + (size_t)i * p.out.ld + j;
-          const size_t tt = blockIdx.z * t.stride + (size_t)j * t.ld + i;
-          split(v, p.out.hi[at], p.out.lo[at]);
-          // a tile on the diagonal holds both halves itself
-          if (KIND == APPLY || blockIdx.x != blockIdx.y) split(v, t.hi[tt], t.lo[tt]);
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) v[h][q] = acc[i + h][j + q] * p.f;
+      if constexpr (KIND == SQUARE) {      // + fb of a's element: symmetric, so rows tj, k ti
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const uint8_t* const at = frag(p.a, tj + j + q, (ti + i) / 2) + lane * 16;
+          const h8 hi = *reinterpret_cast<const h8*>(at), lo = *reinterpret_cast<const h8*>(at + 1024);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              v[h][q][e] += p.fb * ((float)hi[4 * h + e] + (float)lo[4 * h + e]);
+              if (ti + i + h == tj + j + q && r == 4 * g + e) v[h][q][e] += p.fa;
+            }
         }
       }
+      if constexpr (KIND == GRAM || KIND == SQUARE) {
+        store_symmetric(v, p.out, ti + i, tj + j, bi != bj, lane);
+      } else if constexpr (KIND == APPLY) {
+        h8 hi[2], lo[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) split4(v[h][q], hi[q], lo[q], h);
+        store_x(hi, lo, p.out, p.out_t, tj + j, (ti + i) / 2, lane);
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int x = (ti + i + h) * 16 + 4 * g + e, y = (tj + j + q) * 16 + r;
+              if (x < z.m && y < z.n) muon_store<OUT>(m, (size_t)blockIdx.z * m.rows * m.cols + place(m, x, y), v[h][q][e]);
+            }
+      }
+    }
 }
 
-MuonSize muon_size(long long rows, long long cols) {
-  const int m = (int)std::min(rows, cols), n = (int)std::max(rows, cols);
-  return MuonSize{m, n, (m + 63) / 64 * 64, (n + 63) / 64 * 64};
+// The parts of G's tiles added up; a wave a pair of tiles by two.
+template <int W>
+__global__ __launch_bounds__(256) void muon_join_kernel(Product p, int across) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, tiles = across * (across + 1) / 2;
+  constexpr int EACH = W * W / 4;          // pairs by two of a wave's tiles
+  const int tile = blockIdx.x / EACH, k = blockIdx.x % EACH, i = k / (W / 2) * 2, j = k % (W / 2) * 2;
+  int bi, bj;
+  upper(tile, across, bi, bj);
+  f4 v[2][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) v[h][q] = f4{0.f, 0.f, 0.f, 0.f};
+  for (int part = 0; part < p.parts; ++part) {
+    const f4* const at = reinterpret_cast<const f4*>(p.partial) +
+                         ((((size_t)blockIdx.z * p.parts + part) * tiles + tile) * 4 + wave) * W * W * 64 + lane;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) v[h][q] += at[((i + h) * W + j + q) * 64];
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) v[h][q] *= p.f;
+  store_symmetric(v, p.out, (bi * 2 + (wave >> 1)) * W + i, (bj * 2 + (wave & 1)) * W + j, bi != bj, lane);
 }
+
+MuonSize muon_size(long long rows, long long cols) { return MuonSize{(int)std::min(rows, cols), (int)std::max(rows, cols)}; }
+
+// ---- which kernels -------------------------------------------------------------------------------
+
+constexpr int CUS = 256;
+
+bool one_block(const MuonSize& z) { return z.m <= 128 && z.n <= 512; }
+
+struct MuonGrid {
+  int mp, np, w, across, gram_parts;   // padded sides, W, blocks along m
+};
+MuonGrid muon_grid(long long batch, const MuonSize& z) {
+  MuonGrid q;
+  q.mp = (z.m + 127) / 128 * 128;
+  q.np = (z.n + 127) / 128 * 128;
+  q.w = batch * (q.mp / 128) * (q.np / 128) >= CUS ? 4 : 2;
+  q.across = q.mp / (32 * q.w);
+  // G's tiles are few: parts of 8 steps at least until they fill the chip
+  const long long tiles = batch * q.across * (q.across + 1) / 2;
+  q.gram_parts = (int)std::max<long long>(1, std::min<long long>(2 * CUS / tiles, q.np / 256));
+  return q;
+}
+
+size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
 template <int DT>
-int start(lf_context* ctx, const Muon& a, const MuonSize& z, double* partial, int e, const Planes& x, const Planes& xt) {
+int start(lf_context* ctx, const Muon& a, const MuonSize& z, const MuonGrid& q, double* partial, int e, const Frags& x,
+          const Frags& xt) {
   const long long count = (long long)a.rows * a.cols;
   const int parts = (int)std::min<long long>(NORM_MOST, (count + 4095) / 4096);
   {
@@ -189,64 +595,125 @@ int start(lf_context* ctx, const Muon& a, const MuonSize& z, double* partial, in
   }
   LF_TRY(check_hip(hipGetLastError(), "muon norm launch"));
   LaunchScope ls(ctx, "muon.start");
-  hipLaunchKernelGGL((muon_start_kernel<DT>), dim3(z.np / 64, z.mp / 64, a.batch), dim3(256), 0, ctx->stream, a, z, partial, parts,
+  hipLaunchKernelGGL((muon_start_kernel<DT>), dim3(q.np / 128, q.mp / 32, a.batch), dim3(256), 0, ctx->stream, a, z, partial, parts,
                      e, x, xt);
   return check_hip(hipGetLastError(), "muon start launch");
 }
 
+template <int KIND, int W, int OUT = DT_F32>
+void go_product(lf_context* ctx, const Product& p, const Muon& m, const MuonSize& z, const MuonGrid& q) {
+  const int tiles = q.across * (q.across + 1) / 2;
+  const int blocks = KIND == GRAM_PART ? tiles * p.parts : KIND == APPLY || KIND == LAST ? q.across * (q.np / (32 * W)) : tiles;
+  hipLaunchKernelGGL((muon_product_kernel<KIND, W, OUT>), dim3(blocks, 1, m.batch), dim3(256), 0, ctx->stream, p, m, z, q.across);
+}
 template <int KIND, int OUT = DT_F32>
-int product(lf_context* ctx, const Product& p, const Muon& m, const MuonSize& z, const char* label) {
-  const int nx = KIND == GRAM || KIND == SQUARE ? z.mp : z.np;
+int product(lf_context* ctx, const Product& p, const Muon& m, const MuonSize& z, const MuonGrid& q, const char* label) {
   LaunchScope ls(ctx, label);
-  hipLaunchKernelGGL((muon_product_kernel<KIND, OUT>), dim3(nx / 64, z.mp / 64, m.batch), dim3(256), 0, ctx->stream, p, m, z);
+  if (q.w == 4) go_product<KIND, 4, OUT>(ctx, p, m, z, q);
+  else go_product<KIND, 2, OUT>(ctx, p, m, z, q);
   return check_hip(hipGetLastError(), "muon product launch");
 }
 
-size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
+template <int MB, int J, int DT, int OUT>
+int go_block(lf_context* ctx, const Muon& m, const MuonSize& z, const MuonSteps& s) {
+  constexpr int LDS = 2 * MB * 4 * 2048 + 2 * MB * MB * 2048;
+  const auto kernel = muon_block_kernel<MB, J, DT, OUT>;
+  static const hipError_t lds = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+  LF_TRY(check_hip(lds, "muon LDS"));
+  LaunchScope ls(ctx, "muon.block");
+  hipLaunchKernelGGL(kernel, dim3(m.batch), dim3(512), LDS, ctx->stream, m, z, s);
+  return check_hip(hipGetLastError(), "muon launch");
+}
+template <int MB, int DT, int OUT>
+int go_block(lf_context* ctx, const Muon& m, const MuonSize& z, const MuonSteps& s) {
+  if (z.n <= 128) return go_block<MB, 1, DT, OUT>(ctx, m, z, s);
+  if (z.n <= 256) return go_block<MB, 2, DT, OUT>(ctx, m, z, s);
+  return go_block<MB, 4, DT, OUT>(ctx, m, z, s);
+}
+template <int DT, int OUT>
+int go_block(lf_context* ctx, const Muon& m, const MuonSize& z, const MuonSteps& s) {
+  if (z.m <= 32) return go_block<1, DT, OUT>(ctx, m, z, s);
+  if (z.m <= 64) return go_block<2, DT, OUT>(ctx, m, z, s);
+  return go_block<4, DT, OUT>(ctx, m, z, s);
+}
+template <int DT>
+int go_block(lf_context* ctx, const Muon& m, const MuonSize& z, const MuonSteps& s) {
+  if (m.out_dtype == LF_F32) return go_block<DT, DT_F32>(ctx, m, z, s);
+  if (m.out_dtype == LF_F16) return go_block<DT, DT_F16>(ctx, m, z, s);
+  return go_block<DT, DT_BF16>(ctx, m, z, s);
+}
 
 }  // namespace
 
 size_t muon_bytes(long long batch, long long rows, long long cols) {
   const MuonSize z = muon_size(rows, cols);
-  const size_t x = up256(batch * (size_t)z.mp * z.np * 2), g = up256(batch * (size_t)z.mp * z.mp * 2);
-  return up256(batch * NORM_MOST * sizeof(double)) + 8 * x + 4 * g;
+  if (one_block(z)) return 0;
+  const MuonGrid q = muon_grid(batch, z);
+  const size_t x = up256(batch * (size_t)q.mp * q.np * 4), g = up256(batch * (size_t)q.mp * q.mp * 4);
+  const size_t parts = q.gram_parts > 1 ? batch * (size_t)q.gram_parts * (q.across * (q.across + 1) / 2) * (32 * q.w) * (32 * q.w) * 4 : 0;
+  return up256(batch * NORM_MOST * sizeof(double)) + 4 * x + 2 * g + up256(parts);
 }
 
 int run_muon(lf_context* ctx, const Muon& m, const MuonPlan& plan, void* scratch) {
   const MuonSize z = muon_size(m.rows, m.cols);
+  MuonSteps f{};
+  f.count = m.steps;
+  f.start = plan.x[0];
+  for (int k = 0; k < m.steps; ++k) {
+    const float* c = m.coefficients + 3 * k;
+    const int ex = plan.x[k], eg = plan.g[k], ep = plan.p[k];
+    f.gram[k] = std::ldexp(1.f, eg - 2 * ex);
+    f.square[k] = std::ldexp(c[2], ep - 2 * eg);
+    f.gb[k] = std::ldexp(c[1], ep - eg);
+    f.diagonal[k] = std::ldexp(c[0], ep);
+    f.apply[k] = std::ldexp(1.f, (k + 1 == m.steps ? 0 : plan.x[k + 1]) - ep - ex);
+  }
+  if (one_block(z)) {
+    if (m.grad_dtype == LF_F32) return go_block<DT_F32>(ctx, m, z, f);
+    if (m.grad_dtype == LF_F16) return go_block<DT_F16>(ctx, m, z, f);
+    return go_block<DT_BF16>(ctx, m, z, f);
+  }
+  const MuonGrid q = muon_grid(m.batch, z);
   char* at = static_cast<char*>(scratch);
   auto take = [&](size_t bytes) {
-    void* p = at;
+    char* p = at;
     at += up256(bytes);
     return p;
   };
-  double* const partial = static_cast<double*>(take((size_t)m.batch * NORM_MOST * sizeof(double)));
-  auto planes = [&](int rows, int ld) {
-    Planes p;
-    p.stride = (size_t)rows * ld;
-    p.ld = ld;
-    p.hi = static_cast<_Float16*>(take(m.batch * p.stride * 2));
-    p.lo = static_cast<_Float16*>(take(m.batch * p.stride * 2));
+  double* const norms = reinterpret_cast<double*>(take((size_t)m.batch * NORM_MOST * sizeof(double)));
+  auto frags = [&](int rows, int k) {
+    Frags p;
+    p.kbs = k / 32;
+    p.stride = (size_t)rows * k * 4;
+    p.at = reinterpret_cast<uint8_t*>(take(m.batch * p.stride));
     return p;
   };
-  Planes x[2] = {planes(z.mp, z.np), planes(z.mp, z.np)}, xt[2] = {planes(z.np, z.mp), planes(z.np, z.mp)};
-  const Planes g = planes(z.mp, z.mp), q = planes(z.mp, z.mp);
-  if (m.grad_dtype == LF_F32) LF_TRY(start<DT_F32>(ctx, m, z, partial, plan.x[0], x[0], xt[0]));
-  else if (m.grad_dtype == LF_F16) LF_TRY(start<DT_F16>(ctx, m, z, partial, plan.x[0], x[0], xt[0]));
-  else LF_TRY(start<DT_BF16>(ctx, m, z, partial, plan.x[0], x[0], xt[0]));
+  const Frags x[2] = {frags(q.mp, q.np), frags(q.mp, q.np)}, xt[2] = {frags(q.np, q.mp), frags(q.np, q.mp)};
+  const Frags g = frags(q.mp, q.mp), pm = frags(q.mp, q.mp);
+  float* const partial = reinterpret_cast<float*>(at);
+  if (m.grad_dtype == LF_F32) LF_TRY(start<DT_F32>(ctx, m, z, q, norms, f.start, x[0], xt[0]));
+  else if (m.grad_dtype == LF_F16) LF_TRY(start<DT_F16>(ctx, m, z, q, norms, f.start, x[0], xt[0]));
+  else LF_TRY(start<DT_BF16>(ctx, m, z, q, norms, f.start, x[0], xt[0]));
   for (int k = 0; k < m.steps; ++k) {
-    const float* c = m.coefficients + 3 * k;
-    const int ex = plan.x[k], eg = plan.g[k], ep = plan.p[k], now = k & 1;
-    Product gram{x[now], x[now], z.np, g, g, std::ldexp(1.f, eg - 2 * ex), 0.f, 0.f};
-    LF_TRY(product<GRAM>(ctx, gram, m, z, "muon.gram"));
-    Product square{g, g, z.mp, q, q, std::ldexp(c[2], ep - 2 * eg), std::ldexp(c[1], ep - eg), std::ldexp(c[0], ep)};
-    LF_TRY(product<SQUARE>(ctx, square, m, z, "muon.square"));
-    const bool last = k + 1 == m.steps;
-    Product apply{q, xt[now], z.mp, x[!now], xt[!now], std::ldexp(1.f, (last ? 0 : plan.x[k + 1]) - ep - ex), 0.f, 0.f};
-    if (!last) LF_TRY(product<APPLY>(ctx, apply, m, z, "muon.apply"));
-    else if (m.out_dtype == LF_F32) LF_TRY((product<LAST, DT_F32>(ctx, apply, m, z, "muon.last")));
-    else if (m.out_dtype == LF_F16) LF_TRY((product<LAST, DT_F16>(ctx, apply, m, z, "muon.last")));
-    else LF_TRY((product<LAST, DT_BF16>(ctx, apply, m, z, "muon.last")));
+    const int now = k & 1;
+    const Product gram{x[now], x[now], q.np / 32, q.gram_parts, g, g, partial, f.gram[k], 0.f, 0.f};
+    if (q.gram_parts > 1) {
+      LF_TRY(product<GRAM_PART>(ctx, gram, m, z, q, "muon.gram"));
+      LaunchScope ls(ctx, "muon.join");
+      const int pairs = q.across * (q.across + 1) / 2 * q.w * q.w / 4;
+      if (q.w == 4) hipLaunchKernelGGL((muon_join_kernel<4>), dim3(pairs, 1, m.batch), dim3(256), 0, ctx->stream, gram, q.across);
+      else hipLaunchKernelGGL((muon_join_kernel<2>), dim3(pairs, 1, m.batch), dim3(256), 0, ctx->stream, gram, q.across);
+      LF_TRY(check_hip(hipGetLastError(), "muon join launch"));
+    } else {
+      LF_TRY(product<GRAM>(ctx, gram, m, z, q, "muon.gram"));
+    }
+    const Product square{g, g, q.mp / 32, 1, pm, pm, nullptr, f.square[k], f.gb[k], f.diagonal[k]};
+    LF_TRY(product<SQUARE>(ctx, square, m, z, q, "muon.square"));
+    const Product apply{pm, xt[now], q.mp / 32, 1, x[!now], xt[!now], nullptr, f.apply[k], 0.f, 0.f};
+    if (k + 1 < m.steps) LF_TRY(product<APPLY>(ctx, apply, m, z, q, "muon.apply"));
+    else if (m.out_dtype == LF_F32) LF_TRY((product<LAST, DT_F32>(ctx, apply, m, z, q, "muon.last")));
+    else if (m.out_dtype == LF_F16) LF_TRY((product<LAST, DT_F16>(ctx, apply, m, z, q, "muon.last")));
+    else LF_TRY((product<LAST, DT_BF16>(ctx, apply, m, z, q, "muon.last")));
   }
   return LF_OK;
 }
