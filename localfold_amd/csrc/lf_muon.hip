@@ -32,14 +32,21 @@ __device__ __forceinline__ f4 mfma_pair(h8 ah, h8 al, h8 bh, h8 bl, f4 c) {
   return mfma16(ah, bh, c);
 }
 
-// Four values into half `part` of a pair of fragments.
+// Four values into half `part` of a pair of fragments.  The empty assembly makes the compiler pack pairs at once: kept
+// apart until they are used, they would take twice the registers.
 __device__ __forceinline__ void split4(f4 v, h8& hi, h8& lo, int part) {
+  u32x4 h = __builtin_bit_cast(u32x4, hi), l = __builtin_bit_cast(u32x4, lo);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const _Float16 h = (_Float16)v[e];
-    hi[4 * part + e] = h;
-    lo[4 * part + e] = (_Float16)(v[e] - (float)h);
+  for (int e = 0; e < 2; ++e) {
+    const h2 p = h2{(_Float16)v[2 * e], (_Float16)v[2 * e + 1]};
+    const h2 q = h2{(_Float16)(v[2 * e] - (float)p[0]), (_Float16)(v[2 * e + 1] - (float)p[1])};
+    uint32_t a = __builtin_bit_cast(uint32_t, p), b = __builtin_bit_cast(uint32_t, q);
+    asm volatile("" : "+v"(a), "+v"(b));
+    h[2 * part + e] = a;
+    l[2 * part + e] = b;
   }
+  hi = __builtin_bit_cast(h8, h);
+  lo = __builtin_bit_cast(h8, l);
 }
 
 // The fragment of the identity that takes half `part` of a fragment's k to columns.
@@ -55,19 +62,12 @@ __device__ __forceinline__ h4 turn(h8 f, h8 eye) {
   return h4{(_Float16)d[0], (_Float16)d[1], (_Float16)d[2], (_Float16)d[3]};
 }
 
-// u of an element, and its momentum stored.
+// u of an element, from the momentum that is already the new one.
 template <int DT>
-__device__ __forceinline__ float muon_u(const Muon& a, size_t i, bool write) {
+__device__ __forceinline__ float muon_u(const Muon& a, size_t i) {
   const float g = Act<DT>::ld(static_cast<const typename Act<DT>::T*>(a.grad) + i);
   if (!a.momentum) return g;
-  float m;
-  if (write) {
-    m = a.momentum_factor * a.momentum[i] + g;
-    a.momentum_out[i] = m;
-  } else {
-    m = a.momentum_out[i];
-  }
-  return a.nesterov ? g + a.momentum_factor * m : m;
+  return a.nesterov ? g + a.momentum_factor * a.momentum_out[i] : a.momentum_out[i];
 }
 
 // The place of X's element (i, j) in the stored matrix.
@@ -96,8 +96,109 @@ struct MuonTiles {               // a wave's tiles of G: A by B of MT by MT
 
 struct MuonSteps {
   float gram[MUON_STEPS], square[MUON_STEPS], gb[MUON_STEPS], diagonal[MUON_STEPS], apply[MUON_STEPS];
-  int count, start;            // start: X's first exponent
+  int count, start, end;       // X's first and last exponent
 };
+
+// The stored matrix passes through LDS, JW tiles a wave at a time, so that memory is read and written in whole lines.
+// Rows of LDS are 4 columns longer than the matrix's: lanes g then start 16 banks apart.
+template <int MB, int J>
+struct MuonRegion {
+  static constexpr int JW = J < 2 ? J : 2, W = 128 * JW;         // columns of X at a time
+  static constexpr int BYTES = 4 * (32 * MB * (W + 4) > W * (32 * MB + 4) ? 32 * MB * (W + 4) : W * (32 * MB + 4));
+  bool tall;
+  int pitch, m, n, ld;
+  int width;                   // columns of X that exist, from the first of these on
+  int rows, cols;              // of the stored matrix
+  uint32_t first;
+  __device__ __forceinline__ MuonRegion(const Muon& a, const MuonSize& z)
+      : tall(a.rows > a.cols), pitch(tall ? 32 * MB + 4 : W + 4), m(z.m), n(z.n), ld(a.cols) {}
+  __device__ __forceinline__ void at(int j0) {
+    width = max(0, min(W, n - 128 * j0));
+    rows = tall ? width : m;
+    cols = tall ? m : width;
+    first = 128 * j0 * (tall ? ld : 1);
+  }
+};
+
+// Reads u, V elements a lane side by side, stores the momentum and puts u into LDS; the sum of squares.
+template <int DT, int V, class R>
+__device__ __forceinline__ double muon_take(const Muon& a, const R& in, size_t base, float* tile) {
+  typedef typename Act<DT>::T T;
+  struct Vec { T v[V]; };
+  struct VecF { float v[V]; };
+  constexpr int BATCH = 8;     // loads under way
+  const int per = in.cols / V, items = in.rows * per;
+  const T* const grad = static_cast<const T*>(a.grad) + base + in.first;
+  const float* const old = a.momentum + base + in.first;
+  float* const now = a.momentum_out + base + in.first;
+  double t = 0;
+  for (int i0 = 0; i0 < items; i0 += 512 * BATCH) {
+    Vec gv[BATCH];
+    VecF mv[BATCH];
+    int row[BATCH], col[BATCH];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int i = min(i0 + k * 512 + (int)threadIdx.x, items - 1);
+      row[k] = i / per;
+      col[k] = (i - row[k] * per) * V;
+      const uint32_t at = row[k] * in.ld + col[k];
+      __builtin_memcpy(&gv[k], grad + at, sizeof(Vec));
+      if (a.momentum) __builtin_memcpy(&mv[k], old + at, sizeof(VecF));
+    }
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      if (i0 + k * 512 + (int)threadIdx.x >= items) continue;
+      VecF u;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        u.v[e] = Act<DT>::ld(gv[k].v + e);
+        if (a.momentum) {
+          mv[k].v[e] = a.momentum_factor * mv[k].v[e] + u.v[e];
+          u.v[e] = a.nesterov ? u.v[e] + a.momentum_factor * mv[k].v[e] : mv[k].v[e];
+        }
+        t += (double)u.v[e] * u.v[e];
+      }
+      if (a.momentum) __builtin_memcpy(now + (row[k] * in.ld + col[k]), &mv[k], sizeof(VecF));
+      __builtin_memcpy(tile + row[k] * in.pitch + col[k], &u, sizeof(VecF));
+    }
+  }
+  return t;
+}
+
+// The output of what LDS holds.
+template <int OUT, int V, class R>
+__device__ __forceinline__ void muon_give(const Muon& a, const R& in, size_t base, const float* tile) {
+  typedef typename Act<OUT>::T T;
+  struct Vec { T v[V]; };
+  struct VecF { float v[V]; };
+  constexpr int BATCH = 8;
+  const int per = in.cols / V, items = in.rows * per;
+  const T* const weight = static_cast<const T*>(a.weight) + base + in.first;
+  T* const out = static_cast<T*>(a.out) + base + in.first;
+  for (int i0 = 0; i0 < items; i0 += 512 * BATCH) {
+    Vec w[BATCH];
+    int row[BATCH], col[BATCH];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int i = min(i0 + k * 512 + (int)threadIdx.x, items - 1);
+      row[k] = i / per;
+      col[k] = (i - row[k] * per) * V;
+      if (a.weight) __builtin_memcpy(&w[k], weight + (row[k] * in.ld + col[k]), sizeof(Vec));
+    }
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      if (i0 + k * 512 + (int)threadIdx.x >= items) continue;
+      VecF o;
+      __builtin_memcpy(&o, tile + row[k] * in.pitch + col[k], sizeof(VecF));
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float v = -a.rate * o.v[e];
+        Act<OUT>::st(w[k].v + e, a.weight ? a.keep * Act<OUT>::ld(w[k].v + e) + v : v);
+      }
+      __builtin_memcpy(out + (row[k] * in.ld + col[k]), &w[k], sizeof(Vec));
+    }
+  }
+}
 
 template <int MB, int J, int DT, int OUT>
 __global__ __launch_bounds__(512, 2) void muon_block_kernel(Muon a, MuonSize z, MuonSteps steps) {
@@ -111,21 +212,31 @@ __global__ __launch_bounds__(512, 2) void muon_block_kernel(Muon a, MuonSize z, 
   int r = lane & 15, g = lane >> 4;
   const size_t base = (size_t)blockIdx.x * a.rows * a.cols;
   h8 xh[J][MB], xl[J][MB];
+  MuonRegion<MB, J> in(a, z);
   {
     float u[J][MB][8];
     double t = 0;
 #pragma unroll
-    for (int j = 0; j < J; ++j)
+    for (int j0 = 0; j0 < J; j0 += in.JW) {
+      if (j0 > 0) __syncthreads();         // the last columns are read
+      in.at(j0);
+      float* const tile = reinterpret_cast<float*>(muon_smem);
+      if (a.cols % 4 == 0) t += muon_take<DT, 4>(a, in, base, tile);
+      else t += muon_take<DT, 1>(a, in, base, tile);
+      __syncthreads();
 #pragma unroll
-      for (int kb = 0; kb < MB; ++kb) {
-        __builtin_amdgcn_sched_barrier(0);     // the addresses of 8 elements at a time
+      for (int j = 0; j < in.JW; ++j) {
+        const int c = 16 * (8 * j + wave) + r;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int i = 32 * kb + 16 * (e >> 2) + 4 * g + (e & 3), c = 16 * (8 * j + wave) + r;
-          u[j][kb][e] = i < z.m && c < z.n ? muon_u<DT>(a, base + place(a, i, c), true) : 0.f;
-          t += (double)u[j][kb][e] * u[j][kb][e];
-        }
+        for (int kb = 0; kb < MB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int i = 32 * kb + 16 * (e >> 2) + 4 * g + (e & 3);
+            const float v = tile[in.tall ? c * in.pitch + i : i * in.pitch + c];
+            u[j0 + j][kb][e] = i < z.m && c < in.width ? v : 0.f;
+          }
       }
+    }
     for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
     if (lane == 0) norm[wave] = t;
     __syncthreads();
@@ -248,7 +359,6 @@ __global__ __launch_bounds__(512, 2) void muon_block_kernel(Muon a, MuonSize z, 
     __syncthreads();          // G is read
     if (mine) put(p);
     __syncthreads();
-    const bool last = s + 1 == steps.count;
     constexpr int JP = J > 1 ? 2 : 1;     // column tiles at a time, which share the reads of P
 #pragma unroll
     for (int j = 0; j < J; j += JP) {
@@ -271,19 +381,32 @@ __global__ __launch_bounds__(512, 2) void muon_block_kernel(Muon a, MuonSize z, 
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
           __builtin_amdgcn_sched_barrier(0);
-          y[q][t] *= steps.apply[s];
-          split4(y[q][t], xh[j + q][t / 2], xl[j + q][t / 2], t & 1);
-          if (last) {
-            asm volatile("" : "+v"(r), "+v"(g));     // or the places of all elements would be kept in registers throughout
-            const int c = 16 * (8 * (j + q) + wave) + r;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int i = 16 * t + 4 * g + e;
-              if (i < z.m && c < z.n) muon_store<OUT>(a, base + place(a, i, c), y[q][t][e]);
-            }
-          }
+          split4(y[q][t] * steps.apply[s], xh[j + q][t / 2], xl[j + q][t / 2], t & 1);
         }
     }
+  }
+  // What is stored is hi + lo, 22 bits at least of the largest values: the products before keep no more.
+  asm volatile("" : "+v"(r), "+v"(g));     // or the places of all elements would be kept in registers throughout
+  const float back = ldexpf(1.f, -steps.end);
+#pragma unroll
+  for (int j0 = 0; j0 < J; j0 += in.JW) {
+    __syncthreads();                       // LDS is read
+    in.at(j0);
+    float* const tile = reinterpret_cast<float*>(muon_smem);
+#pragma unroll
+    for (int j = 0; j < in.JW; ++j) {
+      const int c = 16 * (8 * j + wave) + r;
+#pragma unroll
+      for (int kb = 0; kb < MB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int i = 32 * kb + 16 * (e >> 2) + 4 * g + (e & 3);
+          tile[in.tall ? c * in.pitch + i : i * in.pitch + c] = ((float)xh[j0 + j][kb][e] + (float)xl[j0 + j][kb][e]) * back;
+        }
+    }
+    __syncthreads();
+    if (a.cols % 4 == 0) muon_give<OUT, 4>(a, in, base, tile);
+    else muon_give<OUT, 1>(a, in, base, tile);
   }
 }
 
@@ -300,7 +423,7 @@ __device__ __forceinline__ uint8_t* frag(const Frags& f, int tile, int kb) {
   return f.at + blockIdx.z * f.stride + ((size_t)tile * f.kbs + kb) * 2048;
 }
 
-constexpr int NORM_MOST = 64;  // blocks that share a matrix
+constexpr int NORM_MOST = 256; // blocks that share a matrix
 
 // Sums of squares, in double: f32's largest values do not overflow it.
 template <int DT>
@@ -309,9 +432,26 @@ __global__ __launch_bounds__(256) void muon_norm_kernel(Muon a, double* partial)
   const long long count = (long long)a.rows * a.cols;
   const size_t base = (size_t)blockIdx.y * count;
   double t = 0;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long long)gridDim.x * 256) {
-    const double u = muon_u<DT>(a, base + i, true);
-    t += u * u;
+  constexpr int V = 4;           // elements under way
+  for (long long i0 = (long long)blockIdx.x * 256 * V + threadIdx.x; i0 < count; i0 += (long long)gridDim.x * 256 * V) {
+    float gv[V], mv[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const size_t i = base + min(i0 + k * 256, count - 1);
+      gv[k] = Act<DT>::ld(static_cast<const typename Act<DT>::T*>(a.grad) + i);
+      mv[k] = a.momentum ? a.momentum[i] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      if (i0 + k * 256 >= count) continue;
+      float u = gv[k];
+      if (a.momentum) {
+        const float m = a.momentum_factor * mv[k] + u;
+        a.momentum_out[base + i0 + k * 256] = m;
+        u = a.nesterov ? u + a.momentum_factor * m : m;
+      }
+      t += (double)u * u;
+    }
   }
   for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = t;
@@ -343,11 +483,12 @@ __device__ __forceinline__ void store_x(const h8 (&hi)[2], const h8 (&lo)[2], co
 template <int DT>
 __global__ __launch_bounds__(256) void muon_start_kernel(Muon a, MuonSize z, const double* partial, int parts, int e, Frags x,
                                                          Frags xt) {
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   double t = 0;
-  for (int i = 0; i < parts; ++i) t += partial[blockIdx.z * NORM_MOST + i];
+  for (int i = lane; i < parts; i += 64) t += partial[blockIdx.z * NORM_MOST + i];
+  for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
   const double f = 1.0 / (sqrt(t) + a.epsilon);
   const size_t base = (size_t)blockIdx.z * a.rows * a.cols;
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int kb = blockIdx.y, jt = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 2;
   h8 hi[2], lo[2];
 #pragma unroll
@@ -358,7 +499,7 @@ __global__ __launch_bounds__(256) void muon_start_kernel(Muon a, MuonSize z, con
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int i = 32 * kb + 16 * h + 4 * g + k, j = 16 * (jt + q) + r;
-        v[k] = i < z.m && j < z.n ? ldexpf((float)(muon_u<DT>(a, base + place(a, i, j), false) * f), e) : 0.f;
+        v[k] = i < z.m && j < z.n ? ldexpf((float)(muon_u<DT>(a, base + place(a, i, j)) * f), e) : 0.f;
       }
       split4(v, hi[q], lo[q], h);
     }
@@ -609,14 +750,17 @@ void go_product(lf_context* ctx, const Product& p, const Muon& m, const MuonSize
 template <int KIND, int OUT = DT_F32>
 int product(lf_context* ctx, const Product& p, const Muon& m, const MuonSize& z, const MuonGrid& q, const char* label) {
   LaunchScope ls(ctx, label);
-  if (q.w == 4) go_product<KIND, 4, OUT>(ctx, p, m, z, q);
-  else go_product<KIND, 2, OUT>(ctx, p, m, z, q);
+  MuonGrid g = q;
+  // G^2's tiles are few too, and its sums short: smaller tiles rather than parts
+  if (KIND == SQUARE && q.w == 4 && (long long)m.batch * q.across * (q.across + 1) / 2 < CUS) g.w = 2, g.across = 2 * q.across;
+  if (g.w == 4) go_product<KIND, 4, OUT>(ctx, p, m, z, g);
+  else go_product<KIND, 2, OUT>(ctx, p, m, z, g);
   return check_hip(hipGetLastError(), "muon product launch");
 }
 
 template <int MB, int J, int DT, int OUT>
 int go_block(lf_context* ctx, const Muon& m, const MuonSize& z, const MuonSteps& s) {
-  constexpr int LDS = 2 * MB * 4 * 2048 + 2 * MB * MB * 2048;
+  constexpr int LDS = std::max(2 * MB * 4 * 2048 + 2 * MB * MB * 2048, MuonRegion<MB, J>::BYTES);
   const auto kernel = muon_block_kernel<MB, J, DT, OUT>;
   static const hipError_t lds = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   LF_TRY(check_hip(lds, "muon LDS"));
@@ -659,6 +803,7 @@ int run_muon(lf_context* ctx, const Muon& m, const MuonPlan& plan, void* scratch
   MuonSteps f{};
   f.count = m.steps;
   f.start = plan.x[0];
+  f.end = plan.x[m.steps];
   for (int k = 0; k < m.steps; ++k) {
     const float* c = m.coefficients + 3 * k;
     const int ex = plan.x[k], eg = plan.g[k], ep = plan.p[k];
@@ -666,7 +811,7 @@ int run_muon(lf_context* ctx, const Muon& m, const MuonPlan& plan, void* scratch
     f.square[k] = std::ldexp(c[2], ep - 2 * eg);
     f.gb[k] = std::ldexp(c[1], ep - eg);
     f.diagonal[k] = std::ldexp(c[0], ep);
-    f.apply[k] = std::ldexp(1.f, (k + 1 == m.steps ? 0 : plan.x[k + 1]) - ep - ex);
+    f.apply[k] = std::ldexp(1.f, plan.x[k + 1] - ep - ex);
   }
   if (one_block(z)) {
     if (m.grad_dtype == LF_F32) return go_block<DT_F32>(ctx, m, z, f);
@@ -709,8 +854,9 @@ int run_muon(lf_context* ctx, const Muon& m, const MuonPlan& plan, void* scratch
     }
     const Product square{g, g, q.mp / 32, 1, pm, pm, nullptr, f.square[k], f.gb[k], f.diagonal[k]};
     LF_TRY(product<SQUARE>(ctx, square, m, z, q, "muon.square"));
-    const Product apply{pm, xt[now], q.mp / 32, 1, x[!now], xt[!now], nullptr, f.apply[k], 0.f, 0.f};
-    if (k + 1 < m.steps) LF_TRY(product<APPLY>(ctx, apply, m, z, q, "muon.apply"));
+    const bool last = k + 1 == m.steps;
+    const Product apply{pm, xt[now], q.mp / 32, 1, x[!now], xt[!now], nullptr, last ? std::ldexp(f.apply[k], -f.end) : f.apply[k], 0.f, 0.f};
+    if (!last) LF_TRY(product<APPLY>(ctx, apply, m, z, q, "muon.apply"));
     else if (m.out_dtype == LF_F32) LF_TRY((product<LAST, DT_F32>(ctx, apply, m, z, q, "muon.last")));
     else if (m.out_dtype == LF_F16) LF_TRY((product<LAST, DT_F16>(ctx, apply, m, z, q, "muon.last")));
     else LF_TRY((product<LAST, DT_BF16>(ctx, apply, m, z, q, "muon.last")));
