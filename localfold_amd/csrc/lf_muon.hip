@@ -120,6 +120,23 @@ struct MuonRegion {
   }
 };
 
+// A thread's items of rows of `per`, 512 apart.
+struct MuonWalk {
+  int per, row, col, rows, cols;
+  __device__ __forceinline__ explicit MuonWalk(int n) : per(max(n, 1)), rows(512 / per), cols(512 % per) {
+    row = threadIdx.x / per;
+    col = threadIdx.x % per;
+  }
+  __device__ __forceinline__ void next() {
+    row += rows;
+    col += cols;
+    if (col >= per) {
+      col -= per;
+      ++row;
+    }
+  }
+};
+
 // Reads u, V elements a lane side by side, stores the momentum and puts u into LDS; the sum of squares.
 template <int DT, int V, class R>
 __device__ __forceinline__ double muon_take(const Muon& a, const R& in, size_t base, float* tile) {
@@ -127,7 +144,8 @@ __device__ __forceinline__ double muon_take(const Muon& a, const R& in, size_t b
   struct Vec { T v[V]; };
   struct VecF { float v[V]; };
   constexpr int BATCH = 8;     // loads under way
-  const int per = in.cols / V, items = in.rows * per;
+  const int items = in.rows * (in.cols / V);
+  MuonWalk walk(in.cols / V);
   const T* const grad = static_cast<const T*>(a.grad) + base + in.first;
   const float* const old = a.momentum + base + in.first;
   float* const now = a.momentum_out + base + in.first;
@@ -136,18 +154,20 @@ __device__ __forceinline__ double muon_take(const Muon& a, const R& in, size_t b
     Vec gv[BATCH];
     VecF mv[BATCH];
     int row[BATCH], col[BATCH];
+    bool there[BATCH];
 #pragma unroll
     for (int k = 0; k < BATCH; ++k) {
-      const int i = min(i0 + k * 512 + (int)threadIdx.x, items - 1);
-      row[k] = i / per;
-      col[k] = (i - row[k] * per) * V;
+      there[k] = walk.row < in.rows;
+      row[k] = there[k] ? walk.row : 0;
+      col[k] = walk.col * V;
+      walk.next();
       const uint32_t at = row[k] * in.ld + col[k];
       __builtin_memcpy(&gv[k], grad + at, sizeof(Vec));
       if (a.momentum) __builtin_memcpy(&mv[k], old + at, sizeof(VecF));
     }
 #pragma unroll
     for (int k = 0; k < BATCH; ++k) {
-      if (i0 + k * 512 + (int)threadIdx.x >= items) continue;
+      if (!there[k]) continue;
       VecF u;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
@@ -172,22 +192,25 @@ __device__ __forceinline__ void muon_give(const Muon& a, const R& in, size_t bas
   struct Vec { T v[V]; };
   struct VecF { float v[V]; };
   constexpr int BATCH = 8;
-  const int per = in.cols / V, items = in.rows * per;
+  const int items = in.rows * (in.cols / V);
+  MuonWalk walk(in.cols / V);
   const T* const weight = static_cast<const T*>(a.weight) + base + in.first;
   T* const out = static_cast<T*>(a.out) + base + in.first;
   for (int i0 = 0; i0 < items; i0 += 512 * BATCH) {
     Vec w[BATCH];
     int row[BATCH], col[BATCH];
+    bool there[BATCH];
 #pragma unroll
     for (int k = 0; k < BATCH; ++k) {
-      const int i = min(i0 + k * 512 + (int)threadIdx.x, items - 1);
-      row[k] = i / per;
-      col[k] = (i - row[k] * per) * V;
+      there[k] = walk.row < in.rows;
+      row[k] = there[k] ? walk.row : 0;
+      col[k] = walk.col * V;
+      walk.next();
       if (a.weight) __builtin_memcpy(&w[k], weight + (row[k] * in.ld + col[k]), sizeof(Vec));
     }
 #pragma unroll
     for (int k = 0; k < BATCH; ++k) {
-      if (i0 + k * 512 + (int)threadIdx.x >= items) continue;
+      if (!there[k]) continue;
       VecF o;
       __builtin_memcpy(&o, tile + row[k] * in.pitch + col[k], sizeof(VecF));
 #pragma unroll
