@@ -1,6 +1,7 @@
 // A learned row per relative position added to every pair, and its gradient (lf_relative_position,
 // lf_relative_position_backward).  Bound by memory: one addition a value.
 #include <algorithm>
+#include <climits>
 
 #include "lf_step.h"
 
@@ -27,46 +28,97 @@ __device__ __forceinline__ int row_of(const lf_relative_pairs& p, int qp, int qs
   return bucket_of((long long)qp - p.key_positions[key], boundaries, p.boundary_count);
 }
 
-// A block adds rows to `tile` (at most 256) keys of one query: the rows' numbers once a pair, in LDS, then 8
-// channels a lane.
-template <int ACT, int TAB>
-__global__ __launch_bounds__(256) void position_kernel(lf_relative_pairs p, int channels, const typename Act<TAB>::T* table,
-                                                       const float* bias, const typename Act<ACT>::T* act,
-                                                       typename Act<ACT>::T* out, int tile, int tiles,
-                                                       long long blocks) {
+// A block adds rows to tiles of `tile` (at most 256) keys of one query: the rows' numbers once a pair, in LDS, then 8
+// channels a lane, FLIGHT loads under way.  Many pairs: blocks that stay, with the table and the bias added up in LDS once
+// (TABLE_LDS), so that a pair costs its own bytes alone.
+struct PositionTiles {
+  int tile, tiles;             // keys of a tile, tiles of a query
+  long long count;             // tiles in all
+  int rows;                    // of the table
+};
+
+template <int ACT, int TAB, bool TABLE_LDS>
+__global__ __launch_bounds__(512, 4) void position_kernel(lf_relative_pairs p, int channels, const typename Act<TAB>::T* table,
+                                                          const float* bias, const typename Act<ACT>::T* act,
+                                                          typename Act<ACT>::T* out, PositionTiles q) {
+  constexpr int FLIGHT = 4;
   __shared__ int rows[256];
-  extern __shared__ int boundaries[];
-  for (int i = threadIdx.x; i < p.boundary_count; i += 256) boundaries[i] = p.boundaries[i];
-  const int chunks = (channels + 7) / 8;
-  for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const int query = (int)(b / tiles), k0 = (int)(b % tiles) * tile, keys = min(tile, p.keys - k0);
+  extern __shared__ __attribute__((aligned(16))) float position_smem[];
+  const int chunks = (channels + 7) / 8, wide = chunks * 8, threads = blockDim.x;
+  int* const boundaries = reinterpret_cast<int*>(position_smem + (TABLE_LDS ? q.rows * wide : 0));
+  for (int i = threadIdx.x; i < p.boundary_count; i += threads) boundaries[i] = p.boundaries[i];
+  // a thread's items of a tile: (key, chunk), `threads` apart
+  const int key0 = threadIdx.x / chunks, chunk0 = threadIdx.x % chunks, dkey = threads / chunks, dchunk = threads % chunks;
+  if constexpr (TABLE_LDS) {
+    for (int row = key0, c = chunk0; row < q.rows;) {
+      float v[8], d[8];
+      load8<TAB>(table + (size_t)row * channels + c * 8, channels - c * 8, v);
+      if (bias) {
+        load8<DT_F32>(bias + c * 8, channels - c * 8, d);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] += d[k];
+      }
+      float4* const at = reinterpret_cast<float4*>(position_smem + row * wide + c * 8);
+      at[0] = make_float4(v[0], v[1], v[2], v[3]);
+      at[1] = make_float4(v[4], v[5], v[6], v[7]);
+      row += dkey;
+      c += dchunk;
+      if (c >= chunks) {
+        c -= chunks;
+        ++row;
+      }
+    }
+  }
+  for (long long b = blockIdx.x; b < q.count; b += gridDim.x) {
+    const int query = (int)(b / q.tiles), k0 = (int)(b % q.tiles) * q.tile, keys = min(q.tile, p.keys - k0);
     __syncthreads();
     if ((int)threadIdx.x < keys)
       rows[threadIdx.x] = row_of(p, p.query_positions[query], p.query_segments ? p.query_segments[query] : 0,
                                  k0 + threadIdx.x, boundaries);
     __syncthreads();
     const size_t first = ((size_t)query * p.keys + k0) * channels;
-    for (int i = threadIdx.x; i < keys * chunks; i += 256) {
-      const int key = i / chunks, c = (i - key * chunks) * 8, n = channels - c;
-      const int row = rows[key];
-      const size_t at = first + (size_t)key * channels + c;
-      float v[8] = {};
-      if (row >= 0) {
-        load8<TAB>(table + (size_t)row * channels + c, n, v);
-        if (bias) {
-          float d[8];
-          load8<DT_F32>(bias + c, n, d);
+    int key = key0, chunk = chunk0;
+    for (int i0 = threadIdx.x; i0 < keys * chunks; i0 += FLIGHT * threads) {
+      float a[FLIGHT][8];
+      int ks[FLIGHT], cs[FLIGHT];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] += d[k];
+      for (int f = 0; f < FLIGHT; ++f) {
+        ks[f] = key;
+        cs[f] = chunk * 8;
+        key += dkey;
+        chunk += dchunk;
+        if (chunk >= chunks) {
+          chunk -= chunks;
+          ++key;
         }
-      }
-      if (act) {
-        float d[8];
-        load8<ACT>(act + at, n, d);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = d[k] + v[k];
+        for (int k = 0; k < 8; ++k) a[f][k] = 0.f;
+        if (act && ks[f] < keys) load8<ACT>(act + first + (size_t)ks[f] * channels + cs[f], channels - cs[f], a[f]);
       }
-      store8<ACT>(out + at, n, v);
+#pragma unroll
+      for (int f = 0; f < FLIGHT; ++f) {
+        if (ks[f] >= keys) continue;
+        const int row = rows[ks[f]], c = cs[f];
+        if (row >= 0) {
+          float v[8];
+          if constexpr (TABLE_LDS) {
+            const float4* const at = reinterpret_cast<const float4*>(position_smem + row * wide + c);
+            const float4 x = at[0], y = at[1];
+            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+          } else {
+            load8<TAB>(table + (size_t)row * channels + c, channels - c, v);
+            if (bias) {
+              float d[8];
+              load8<DT_F32>(bias + c, channels - c, d);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) v[k] += d[k];
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) a[f][k] += v[k];
+        }
+        store8<ACT>(out + first + (size_t)ks[f] * channels + c, channels - c, a[f]);
+      }
     }
   }
 }
@@ -75,96 +127,170 @@ __global__ __launch_bounds__(256) void position_kernel(lf_relative_pairs p, int 
 
 // A lane sums two channels of the keys that its team of L lanes takes, in registers while the table's row stays
 // the same (most pairs are beyond the last boundary, where it does) and into the team's own rows in LDS when it
-// changes: no two lanes share an address, so the order of the sums is fixed.
+// changes: no two lanes share an address, so the order of the sums is fixed.  Those rows, 512 bytes of each a wave, leave
+// room for 4 waves a CU where there are 80: a wave has the next 32 loads under way while it adds up the last ones.
+// (LDS's own float additions took twice as long as reading and writing: 39 us instead of 23 for 384 x 384 pairs of 128
+// channels in bf16.)
 struct PositionGrid {
-  int chunks;               // units of 64 keys of a query
+  int chunks;               // units of a query
   long long units;
   int blocks, slices;       // blocks of a slice of 2 L channels
   int row0, rows;           // the table's rows that this launch sums
   int all;                  // rows of the table
 };
+constexpr int STEPS = 32;                                             // loads of a unit
+constexpr int position_keys(int team) { return STEPS * (64 / team); }    // keys of a unit
 
 template <int ACT, int L, bool EVEN>
-__global__ __launch_bounds__(256) void position_grad_kernel(lf_relative_pairs p, int channels, const typename Act<ACT>::T* grad,
+__global__ __launch_bounds__(512) void position_grad_kernel(lf_relative_pairs p, int channels, const typename Act<ACT>::T* grad,
                                                             float* partial, PositionGrid q) {
   typedef typename Act<ACT>::T T;
-  constexpr int TEAMS = 64 / L, WIDE = 2 * L, BATCH = 16;
-  extern __shared__ float sums[];
-  const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, team = lane / L, tl = lane % L;
+  constexpr int TEAMS = 64 / L, WIDE = 2 * L, KEYS = position_keys(L), REGS = (KEYS + 63) / 64;
+  struct Two {
+    T v[2];
+  };
+  extern __shared__ __attribute__((aligned(16))) float position_smem[];
+  float* const sums = position_smem;
+  const int waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int team = lane / L, tl = lane % L;
   const int slice = blockIdx.x / q.blocks, blk = blockIdx.x % q.blocks;
   const int c = slice * WIDE + 2 * tl;
-  const int copies = waves * TEAMS;
-  int* const boundaries = reinterpret_cast<int*>(sums + (size_t)copies * q.rows * WIDE);
+  const int copies = waves * TEAMS, size = q.rows * WIDE;
+  int* const boundaries = reinterpret_cast<int*>(sums + (size_t)copies * size);
   for (int i = threadIdx.x; i < p.boundary_count; i += blockDim.x) boundaries[i] = p.boundaries[i];
-  for (int i = threadIdx.x; i < copies * q.rows * WIDE; i += blockDim.x) sums[i] = 0.f;
+  for (int i = threadIdx.x; i < copies * size / 4; i += blockDim.x) reinterpret_cast<float4*>(sums)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   __syncthreads();
-  float* const mine = sums + (size_t)(wave * TEAMS + team) * q.rows * WIDE + 2 * tl;
+  float* const mine = sums + (size_t)(wave * TEAMS + team) * size + 2 * tl;
   const int c0 = min(c, channels - (EVEN ? 2 : 1)), c1 = min(c + 1, channels - 1);
   const long long w = (long long)blk * waves + wave, all = (long long)q.blocks * waves;
-  const long long u1 = q.units * (w + 1) / all;
-  int cur = -1;
-  float a0 = 0.f, a1 = 0.f;
-  for (long long u = q.units * w / all; u < u1; ++u) {
-    const int query = (int)(u / q.chunks), k0 = (int)(u % q.chunks) * 64, left = min(64, p.keys - k0);
-    int row = -1;
-    if (lane < left) {
-      row = row_of(p, p.query_positions[query], p.query_segments ? p.query_segments[query] : 0, k0 + lane, boundaries) - q.row0;
-      if (row < 0 || row >= q.rows) row = -1;
-    }
-    const T* const g = grad + ((size_t)query * p.keys + k0) * channels;
-    for (int s0 = 0; s0 < L; s0 += BATCH) {
-      if (s0 * TEAMS >= left) break;
-      float v0[BATCH], v1[BATCH];
+  const long long u0 = q.units * w / all, u1 = q.units * (w + 1) / all;
+  const int nb = p.boundary_count, b0 = nb ? boundaries[0] : INT_MIN, b1 = nb ? boundaries[nb - 1] : INT_MIN;
+  const uint32_t row_bytes = (uint32_t)channels * sizeof(T);
+  Two in[STEPS];
+  int kp[REGS], ks[REGS], qp = 0, qs = 0, left = 0;
+  int query = (int)(u0 / q.chunks), chunk = (int)(u0 % q.chunks);      // of the next unit to load
+  // The loads of a unit: gradients, and the positions that its rows come from.
+  auto load = [&]() __attribute__((always_inline)) {
+    qp = p.query_positions[query];
+    qs = p.query_segments ? p.query_segments[query] : 0;
+    const int k0 = chunk * KEYS;
+    left = min(KEYS, p.keys - k0);
 #pragma unroll
-      for (int s = 0; s < BATCH; ++s) {
-        const int key = min((s0 + s) * TEAMS + team, left - 1);
-        const T* const at = g + (size_t)key * channels;
-        if constexpr (EVEN) {
-          T both[2];
-          __builtin_memcpy(both, at + c0, sizeof(both));
-          v0[s] = Act<ACT>::ld(both);
-          v1[s] = Act<ACT>::ld(both + 1);
-        } else {
-          v0[s] = Act<ACT>::ld(at + c0);
-          v1[s] = Act<ACT>::ld(at + c1);
-        }
+    for (int i = 0; i < REGS; ++i) {
+      const int key = k0 + min(i * 64 + lane, left - 1);
+      kp[i] = p.key_positions[key];
+      ks[i] = p.key_segments ? p.key_segments[key] : 0;
+    }
+    const char* const g = reinterpret_cast<const char*>(grad + ((size_t)query * p.keys + k0) * channels);
+    const uint32_t most = (uint32_t)(left - 1) * row_bytes;      // keys past the end repeat the last one
+    uint32_t at = (uint32_t)team * row_bytes;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const uint32_t row = min(at, most);
+      if constexpr (EVEN) {
+        __builtin_memcpy(&in[s], g + (row + c0 * (uint32_t)sizeof(T)), sizeof(Two));
+      } else {
+        in[s].v[0] = *reinterpret_cast<const T*>(g + (row + c0 * (uint32_t)sizeof(T)));
+        in[s].v[1] = *reinterpret_cast<const T*>(g + (row + c1 * (uint32_t)sizeof(T)));
+      }
+      at += TEAMS * row_bytes;
+    }
+    if (++chunk == q.chunks) {
+      chunk = 0;
+      ++query;
+    }
+  };
+  int cur = -1;
+  float a0 = 0.f, a1 = 0.f, all0 = 0.f, all1 = 0.f;      // of the row, of all rows
+  auto flush = [&]() __attribute__((always_inline)) {
+    if (cur >= 0) {
+      float2* const at = reinterpret_cast<float2*>(mine + cur * WIDE);
+      const float2 old = *at;
+      *at = make_float2(old.x + a0, old.y + a1);
+      all0 += a0;
+      all1 += a1;
+    }
+  };
+  if (u0 < u1) load();
+  for (long long u = u0; u < u1; ++u) {
+    int row[REGS];
+    bool same = true;
+#pragma unroll
+    for (int i = 0; i < REGS; ++i) {
+      const long long d = (long long)qp - kp[i];
+      // beyond the boundaries, as most are, there is nothing to search
+      int r = d >= b1 ? nb : 0;
+      if (__any(d >= b0 && d < b1)) r = bucket_of(d, boundaries, nb);
+      if (p.key_segments) r = qs < 0 || ks[i] < 0 ? -1 : qs != ks[i] ? nb + 1 : r;
+      r -= q.row0;
+      row[i] = r < 0 || r >= q.rows || i * 64 + lane >= left ? -1 : r;
+      const int first = __builtin_amdgcn_readfirstlane(row[0]);
+      if (i * 64 + lane < KEYS) same = same && row[i] == first;
+    }
+    float v0[STEPS], v1[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      v0[s] = Act<ACT>::ld(in[s].v);
+      v1[s] = Act<ACT>::ld(in[s].v + 1);
+    }
+    if (u + 1 < u1) load();
+    if (__all(same)) {             // a unit of one row
+      const int r = __builtin_amdgcn_readfirstlane(row[0]);
+      if (r != cur) {
+        flush();
+        cur = r;
+        a0 = a1 = 0.f;
       }
 #pragma unroll
-      for (int s = 0; s < BATCH; ++s) {
-        if (s0 + s >= L) break;
-        const int r = __shfl(row, (s0 + s) * TEAMS + team);    // -1 past the last key
-        if (r != cur) {
-          if (cur >= 0) {
-            mine[cur * WIDE] += a0;
-            mine[cur * WIDE + 1] += a1;
-          }
-          cur = r;
-          a0 = a1 = 0.f;
-        }
+      for (int s = 0; s < STEPS; ++s) {
         a0 += v0[s];
         a1 += v1[s];
       }
+      continue;
+    }
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const int k = s * TEAMS;
+      const int r = TEAMS == 1 ? __builtin_amdgcn_readlane(row[k / 64], k % 64) : __shfl(row[k / 64], k % 64 + team);
+      if (r != cur) {
+        flush();
+        cur = r;
+        a0 = a1 = 0.f;
+      }
+      a0 += v0[s];
+      a1 += v1[s];
     }
   }
-  if (cur >= 0) {
-    mine[cur * WIDE] += a0;
-    mine[cur * WIDE + 1] += a1;
-  }
+  flush();
   __syncthreads();
   // the block's rows [all + 1][channels], the last one the sum of them all (over the launches of a table)
-  float* const dst = partial + (size_t)blk * (q.all + 1) * channels;
+  float* const dst = partial + (size_t)blk * (q.all + 1) * channels + slice * WIDE;
   const int cn = min(WIDE, channels - slice * WIDE);
-  for (int i = threadIdx.x; i < q.rows * WIDE; i += blockDim.x) {
-    float t = 0.f;
-    for (int k = 0; k < copies; ++k) t += sums[(size_t)k * q.rows * WIDE + i];
-    sums[i] = t;      // this thread alone reads and writes the first copy's i
-    if (i % WIDE < cn) dst[(size_t)(q.row0 + i / WIDE) * channels + slice * WIDE + i % WIDE] = t;
+  for (int i = threadIdx.x; i < size / 4; i += blockDim.x) {
+    float4 t = reinterpret_cast<const float4*>(sums)[i];
+#pragma unroll 4
+    for (int k = 1; k < copies; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(sums + (size_t)k * size + 4 * i);
+      t = make_float4(t.x + v.x, t.y + v.y, t.z + v.z, t.w + v.w);
+    }
+    const int row = 4 * i / WIDE, col = 4 * i % WIDE;
+    float* const at = dst + (size_t)(q.row0 + row) * channels + col;
+    if (col + 4 <= cn) {
+      __builtin_memcpy(at, &t, 16);
+    } else {
+      if (col < cn) at[0] = t.x;
+      if (col + 1 < cn) at[1] = t.y;
+      if (col + 2 < cn) at[2] = t.z;
+    }
   }
+  __syncthreads();
+  sums[(wave * TEAMS + team) * WIDE + 2 * tl] = all0;
+  sums[(wave * TEAMS + team) * WIDE + 2 * tl + 1] = all1;
   __syncthreads();
   for (int i = threadIdx.x; i < cn; i += blockDim.x) {
     float t = 0.f;
-    for (int r = 0; r < q.rows; ++r) t += sums[r * WIDE + i];
-    float* const total = dst + (size_t)q.all * channels + slice * WIDE + i;
+    for (int k = 0; k < copies; ++k) t += sums[k * WIDE + i];
+    float* const total = dst + (size_t)q.all * channels + i;
     *total = q.row0 ? *total + t : t;
   }
 }
@@ -206,19 +332,38 @@ int run_join(lf_context* ctx, const float* partial, int count, long long width, 
 
 namespace {
 
+constexpr int TABLE_MOST = 64 * 1024;      // two blocks a CU
+
 template <int ACT, int TAB>
-void go_position(const lf_relative_position_args& a, int tile, int tiles, hipStream_t s) {
-  const long long blocks = (long long)a.pairs->queries * tiles;
-  hipLaunchKernelGGL((position_kernel<ACT, TAB>), dim3((unsigned)std::min(blocks, 1LL << 20)), dim3(256),
-                     a.pairs->boundary_count * sizeof(int), s, *a.pairs, a.channels,
-                     static_cast<const typename Act<TAB>::T*>(a.table), a.bias,
-                     static_cast<const typename Act<ACT>::T*>(a.act), static_cast<typename Act<ACT>::T*>(a.out), tile, tiles, blocks);
+int go_position(const lf_relative_position_args& a, hipStream_t s) {
+  const long long pairs = (long long)a.pairs->queries * a.pairs->keys;
+  PositionTiles q;
+  // few pairs: small tiles, so that they fill the chip
+  q.tile = pairs >= 256 * 512 ? 256 : pairs >= 64 * 512 ? 64 : 16;
+  q.tiles = (a.pairs->keys + q.tile - 1) / q.tile;
+  q.count = (long long)a.pairs->queries * q.tiles;
+  q.rows = LF_RELATIVE_ROWS(a.pairs);
+  const size_t marks = a.pairs->boundary_count * sizeof(int), table = (size_t)q.rows * ((a.channels + 7) / 8 * 8) * sizeof(float);
+  const auto* t = static_cast<const typename Act<TAB>::T*>(a.table);
+  const auto* act = static_cast<const typename Act<ACT>::T*>(a.act);
+  auto* out = static_cast<typename Act<ACT>::T*>(a.out);
+  // what stays has to be read by every block first: worth it where a block adds many times as much
+  if (table + marks <= TABLE_MOST && (size_t)pairs * a.channels >= 2 * 512 * 8 * (size_t)q.rows * a.channels) {
+    const auto kernel = position_kernel<ACT, TAB, true>;
+    static const hipError_t lds = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, TABLE_MOST);
+    LF_TRY(check_hip(lds, "position LDS"));
+    hipLaunchKernelGGL(kernel, dim3(512), dim3(512), table + marks, s, *a.pairs, a.channels, t, a.bias, act, out, q);
+  } else {
+    hipLaunchKernelGGL((position_kernel<ACT, TAB, false>), dim3((unsigned)std::min(q.count, 1LL << 20)), dim3(q.tile > 64 ? 512 : 256),
+                       marks, s, *a.pairs, a.channels, t, a.bias, act, out, q);
+  }
+  return check_hip(hipGetLastError(), "position launch");
 }
 template <int ACT>
-void go_position(const lf_relative_position_args& a, int tile, int tiles, hipStream_t s) {
-  if (a.table_dtype == LF_F32) go_position<ACT, DT_F32>(a, tile, tiles, s);
-  else if (a.table_dtype == LF_F16) go_position<ACT, DT_F16>(a, tile, tiles, s);
-  else go_position<ACT, DT_BF16>(a, tile, tiles, s);
+int go_position(const lf_relative_position_args& a, hipStream_t s) {
+  if (a.table_dtype == LF_F32) return go_position<ACT, DT_F32>(a, s);
+  if (a.table_dtype == LF_F16) return go_position<ACT, DT_F16>(a, s);
+  return go_position<ACT, DT_BF16>(a, s);
 }
 
 constexpr int LDS_BYTES = 160 * 1024;
@@ -231,11 +376,12 @@ PositionPlan position_plan(int queries, int keys, int channels, int rows) {
   PositionPlan p;
   p.team = channels > 64 ? 64 : channels > 32 ? 32 : channels > 16 ? 16 : 8;
   p.slices = (channels + 2 * p.team - 1) / (2 * p.team);
-  p.chunks = (keys + 63) / 64;
+  const int unit = position_keys(p.team);
+  p.chunks = (keys + unit - 1) / unit;
   p.units = (long long)queries * p.chunks;
   // a wave's rows in LDS: 64 lanes of two sums each
   const int budget = (LDS_BYTES - rows * 4) / 512;
-  p.waves = std::min(4, std::max(1, budget / rows));
+  p.waves = std::min(8, std::max(1, budget / rows));
   p.window = std::min(rows, budget / p.waves);
   const long long want = std::max(1, 256 / p.slices);
   p.blocks = (int)std::min(want, (p.units + p.waves - 1) / p.waves);
@@ -273,15 +419,10 @@ int go_grad(lf_context* ctx, const lf_relative_position_backward_args& a, const 
 }  // namespace
 
 int run_relative_position(lf_context* ctx, const lf_relative_position_args& a) {
-  // few pairs: small tiles, so that they fill the chip
-  const long long pairs = (long long)a.pairs->queries * a.pairs->keys;
-  const int tile = pairs >= 256 * 512 ? 256 : pairs >= 64 * 512 ? 64 : 16;
-  const int tiles = (a.pairs->keys + tile - 1) / tile;
   LaunchScope ls(ctx, "position");
-  if (a.act_dtype == LF_F32) go_position<DT_F32>(a, tile, tiles, ctx->stream);
-  else if (a.act_dtype == LF_F16) go_position<DT_F16>(a, tile, tiles, ctx->stream);
-  else go_position<DT_BF16>(a, tile, tiles, ctx->stream);
-  return check_hip(hipGetLastError(), "position launch");
+  if (a.act_dtype == LF_F32) return go_position<DT_F32>(a, ctx->stream);
+  if (a.act_dtype == LF_F16) return go_position<DT_F16>(a, ctx->stream);
+  return go_position<DT_BF16>(a, ctx->stream);
 }
 
 size_t relative_partials(int queries, int keys, int channels, int rows) {
