@@ -773,7 +773,7 @@ typedef struct {
 /* out = act w^T + bias.  Products are exact, sums are f32's.  The weight's gradient is the same product
  * of transposed packs: kept = the gradient's [outputs, rows], w = the activations' [inputs, rows]. */
 int lf_mx4_linear(lf_context* ctx, const lf_mx4_linear_args* args);
-size_t lf_mx4_linear_scratch(int rows, int inputs, int outputs, int from_act);   /* from_act: act is given */
+size_t lf_mx4_linear_scratch(int rows, int inputs, int outputs, int from_act);   /* from_act: act is given; 0: none is used */
 
 /* Matrices made orthogonal by Newton-Schulz products: with X = act / (|act| + epsilon), |.| the
  * Frobenius norm, and (a, b, c) a step's coefficients, X <- a X + (b G + c G^2) X, G = X X^T, `steps`
@@ -816,7 +816,7 @@ typedef struct {
 } lf_muon_step_args;
 
 int lf_muon_step(lf_context* ctx, const lf_muon_step_args* args);
-size_t lf_muon_scratch(int batch, int rows, int cols);   /* for both */
+size_t lf_muon_scratch(int batch, int rows, int cols);   /* for both; 0: none is used */
 
 #ifdef __cplusplus
 }

@@ -151,7 +151,8 @@ int orthogonalize(lf_context* ctx, const lf_orthogonalize_args& a) {
   MuonPlan plan;
   LF_TRY(check_muon(fn, m, &plan));
   void* scratch = nullptr;
-  LF_TRY(take_scratch(ctx, fn, a.scratch, a.scratch_bytes, muon_bytes(a.batch, a.rows, a.cols), &scratch));
+  const size_t need = muon_bytes(a.batch, a.rows, a.cols);
+  if (need) LF_TRY(take_scratch(ctx, fn, a.scratch, a.scratch_bytes, need, &scratch));
   return run_muon(ctx, m, plan, scratch);
 }
 
@@ -185,7 +186,8 @@ int muon_step(lf_context* ctx, const lf_muon_step_args& a) {
   MuonPlan plan;
   LF_TRY(check_muon(fn, m, &plan));
   void* scratch = nullptr;
-  LF_TRY(take_scratch(ctx, fn, a.scratch, a.scratch_bytes, muon_bytes(a.batch, a.rows, a.cols), &scratch));
+  const size_t need = muon_bytes(a.batch, a.rows, a.cols);
+  if (need) LF_TRY(take_scratch(ctx, fn, a.scratch, a.scratch_bytes, need, &scratch));
   return run_muon(ctx, m, plan, scratch);
 }
 

@@ -174,7 +174,7 @@ def test_scratch_sizes_and_null_need_no_device():
     assert lib.lf_relative_position_backward_scratch(None, 128) == lib.lf_relative_position_backward_scratch(C.byref(pairs), 0) == 0
     assert lib.lf_mx4_pack_scratch(5, 30) >= 30 * 4 and lib.lf_mx4_pack_scratch(0, 30) == 0
     assert lib.lf_mx4_linear_scratch(-1, 3, 3, 1) == 0
-    assert lib.lf_muon_scratch(2, 30, 50) >= 2 * 30 * 50 * 4 and lib.lf_muon_scratch(0, 3, 3) == 0
+    assert lib.lf_muon_scratch(2, 300, 500) >= 2 * 300 * 500 * 4 and lib.lf_muon_scratch(0, 3, 3) == 0
     for name in ("lf_relative_position", "lf_relative_position_backward", "lf_mx4_pack", "lf_mx4_unpack", "lf_mx4_linear",
                  "lf_orthogonalize", "lf_muon_step"):
         assert getattr(lib, name)(None, None) == capi.LF_ERR_INVALID and name.encode() in lib.lf_last_error()
@@ -722,6 +722,8 @@ def test_training_step_in_a_graph(ctx):
     from localfold_amd import capi, device as D
     rng = np.random.default_rng(4)
     cases = []
+    large = torch.ones(200, 300, device=ctx.device)
+    large_out = torch.empty_like(large)
     for _ in range(2):
         s = step_state(ctx, rng)
         n = s["positions"].shape[0]
@@ -737,7 +739,7 @@ def test_training_step_in_a_graph(ctx):
             with torch.cuda.graph(g):
                 ctx.bind_stream()
                 with pytest.raises(capi.LocalfoldError, match="scratch"):
-                    D.orthogonalize(ctx, s["w"], out=s["w_new"])
+                    D.orthogonalize(ctx, large, out=large_out)
                 with pytest.raises(capi.LocalfoldError, match="scratch"):
                     D.relative_position_backward(ctx, s["dx"], s["boundaries"], s["positions"], table_grad=s["dt"],
                                                  segments=s["segments"])
@@ -753,7 +755,7 @@ def test_training_step_in_a_graph(ctx):
             g.replay()
             torch.cuda.synchronize()
             got = [s[k].clone() for k in ("pair", "y", "db", "dx", "dw", "dt", "w_new", "m_new")]
-            D.orthogonalize(ctx, torch.randn(4 * (turn + 1), 128, 256, device=ctx.device))      # moves the workspace
+            D.orthogonalize(ctx, torch.randn(4 * (turn + 1), 200, 256, device=ctx.device))      # moves the workspace
             want = training_step(ctx, s)
             torch.cuda.synchronize()
             assert all(torch.equal(p, q) for p, q in zip(got, want)), turn
@@ -850,7 +852,8 @@ def test_refusals(ctx):
     with bad(capi.LocalfoldError):
         D.muon_step(ctx, t, t, rate=math.inf)
     with bad(capi.LocalfoldError):
-        D.muon_step(ctx, t, t, scratch=torch.zeros(16, dtype=torch.uint8, device=dev))
+        D.muon_step(ctx, torch.zeros(200, 300, device=dev), torch.zeros(200, 300, device=dev),
+                    scratch=torch.zeros(16, dtype=torch.uint8, device=dev))
     # what Python does not reach
     lib, h = ctx.lib, ctx.handle
     pairs = capi.lf_relative_pairs(4, 4, pos.data_ptr(), pos.data_ptr(), pos.data_ptr(), None, 4, b.data_ptr())
