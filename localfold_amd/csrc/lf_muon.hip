@@ -137,8 +137,9 @@ struct MuonWalk {
   }
 };
 
-// Reads u, V elements a lane side by side, stores the momentum and puts u into LDS; the sum of squares.
-template <int DT, int V, class R>
+// Reads u, V elements a lane side by side, stores the momentum (AGAIN: it is the new one already) and puts u into LDS; the
+// sum of squares.
+template <int DT, int V, bool AGAIN, class R>
 __device__ __forceinline__ double muon_take(const Muon& a, const R& in, size_t base, float* tile) {
   typedef typename Act<DT>::T T;
   struct Vec { T v[V]; };
@@ -147,7 +148,7 @@ __device__ __forceinline__ double muon_take(const Muon& a, const R& in, size_t b
   const int items = in.rows * (in.cols / V);
   MuonWalk walk(in.cols / V);
   const T* const grad = static_cast<const T*>(a.grad) + base + in.first;
-  const float* const old = a.momentum + base + in.first;
+  const float* const old = (AGAIN ? a.momentum_out : a.momentum) + base + in.first;
   float* const now = a.momentum_out + base + in.first;
   double t = 0;
   for (int i0 = 0; i0 < items; i0 += 512 * BATCH) {
@@ -173,12 +174,12 @@ __device__ __forceinline__ double muon_take(const Muon& a, const R& in, size_t b
       for (int e = 0; e < V; ++e) {
         u.v[e] = Act<DT>::ld(gv[k].v + e);
         if (a.momentum) {
-          mv[k].v[e] = a.momentum_factor * mv[k].v[e] + u.v[e];
+          if (!AGAIN) mv[k].v[e] = a.momentum_factor * mv[k].v[e] + u.v[e];
           u.v[e] = a.nesterov ? u.v[e] + a.momentum_factor * mv[k].v[e] : mv[k].v[e];
         }
         t += (double)u.v[e] * u.v[e];
       }
-      if (a.momentum) __builtin_memcpy(now + (row[k] * in.ld + col[k]), &mv[k], sizeof(VecF));
+      if (!AGAIN && a.momentum) __builtin_memcpy(now + (row[k] * in.ld + col[k]), &mv[k], sizeof(VecF));
       __builtin_memcpy(tile + row[k] * in.pitch + col[k], &u, sizeof(VecF));
     }
   }
@@ -223,14 +224,132 @@ __device__ __forceinline__ void muon_give(const Muon& a, const R& in, size_t bas
   }
 }
 
+// What a wave of a block does in a step; its tiles of G begin at (ta, tb).
+template <int MB>
+struct MuonCore {
+  typedef MuonTiles<MB> Q;
+  typedef f4 Tiles[Q::A][Q::B];
+  uint8_t *xs, *gs;            // X by rows, 128 columns: [tile][32 columns][hi, lo]; G or P: [tile][32 rows][hi, lo]
+  int wave, lane, ta, tb;
+  bool mine;
+  __device__ __forceinline__ MuonCore(uint8_t* smem, int wave_, int lane_)
+      : xs(smem), gs(smem + Q::MT * 4 * 2048), wave(wave_), lane(lane_), ta(wave_ / Q::ACROSS * Q::A), tb(wave_ % Q::ACROSS * Q::B),
+        mine(wave_ / Q::ACROSS * Q::A < Q::MT) {}
+
+  static __device__ __forceinline__ void clear(Tiles& v) {
+#pragma unroll
+    for (int i = 0; i < Q::A; ++i)
+#pragma unroll
+      for (int k = 0; k < Q::B; ++k) v[i][k] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  // The wave's 16 columns by rows into LDS.
+  __device__ __forceinline__ void turn_columns(const h8 (&xh)[MB], const h8 (&xl)[MB], const h8 (&eye)[2]) const {
+#pragma unroll
+    for (int kb = 0; kb < MB; ++kb)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        __builtin_amdgcn_sched_barrier(0);
+        uint8_t* const at = xs + ((2 * kb + h) * 4 + (wave >> 1)) * 2048 + lane * 16 + 8 * (wave & 1);
+        *reinterpret_cast<h4*>(at) = turn(xh[kb], eye[h]);
+        *reinterpret_cast<h4*>(at + 1024) = turn(xl[kb], eye[h]);
+      }
+  }
+  // v += the product of `from`, KBS fragments a row, with its own transpose.
+  template <int KBS>
+  __device__ __forceinline__ void times_itself(Tiles& v, const uint8_t* from) const {
+#pragma unroll
+    for (int kb = 0; kb < KBS; ++kb) {
+      __builtin_amdgcn_sched_barrier(0);     // or all fragments would be read at once, and spill
+      h8 ah[Q::A], al[Q::A];
+#pragma unroll
+      for (int i = 0; i < Q::A; ++i) {
+        const uint8_t* const at = from + ((ta + i) * KBS + kb) * 2048 + lane * 16;
+        ah[i] = *reinterpret_cast<const h8*>(at);
+        al[i] = *reinterpret_cast<const h8*>(at + 1024);
+      }
+#pragma unroll
+      for (int k = 0; k < Q::B; ++k) {
+        const uint8_t* const at = from + ((tb + k) * KBS + kb) * 2048 + lane * 16;
+        const h8 bh = *reinterpret_cast<const h8*>(at), bl = *reinterpret_cast<const h8*>(at + 1024);
+#pragma unroll
+        for (int i = 0; i < Q::A; ++i) v[i][k] = mfma_pair(ah[i], al[i], bh, bl, v[i][k]);
+      }
+    }
+  }
+  // A symmetric tile (ta + i, tb + k) in its place: rows of tile tb + k, k of tile ta + i.
+  __device__ __forceinline__ void put(const Tiles& v) const {
+#pragma unroll
+    for (int k = 0; k < Q::B; ++k)
+#pragma unroll
+      for (int i = 0; i < Q::A; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        h8 hi, lo;
+        split4(v[i][k], hi, lo, 0);
+        uint8_t* const at = gs + ((tb + k) * MB + (ta + i) / 2) * 2048 + lane * 16 + 8 * ((ta + i) & 1);
+        *reinterpret_cast<h4*>(at) = h4{hi[0], hi[1], hi[2], hi[3]};
+        *reinterpret_cast<h4*>(at + 1024) = h4{lo[0], lo[1], lo[2], lo[3]};
+      }
+  }
+  // From G's tiles, as summed, to P in LDS; every wave has read what was in gs.
+  __device__ __forceinline__ void to_p(Tiles& gram, const MuonSteps& steps, int s) const {
+    if (mine) {
+#pragma unroll
+      for (int i = 0; i < Q::A; ++i)
+#pragma unroll
+        for (int k = 0; k < Q::B; ++k) gram[i][k] *= steps.gram[s];
+      put(gram);
+    }
+    __syncthreads();
+    Tiles p;
+    clear(p);
+    if (mine) {
+      times_itself<MB>(p, gs);
+      const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+      for (int i = 0; i < Q::A; ++i)
+#pragma unroll
+        for (int k = 0; k < Q::B; ++k) {
+          p[i][k] = p[i][k] * steps.square[s] + gram[i][k] * steps.gb[s];
+          if (ta + i == tb + k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[i][k][e] += r == 4 * g + e ? steps.diagonal[s] : 0.f;
+        }
+    }
+    __syncthreads();          // G is read
+    if (mine) put(p);
+    __syncthreads();
+  }
+  // J of the wave's column tiles times P, in place; they share the reads of P.
+  template <int J>
+  __device__ __forceinline__ void apply(h8 (*xh)[MB], h8 (*xl)[MB], float factor) const {
+    f4 y[J][Q::MT];
+#pragma unroll
+    for (int t = 0; t < Q::MT; ++t) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int q = 0; q < J; ++q) y[q][t] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kb = 0; kb < MB; ++kb) {
+        const uint8_t* const at = gs + (t * MB + kb) * 2048 + lane * 16;
+        const h8 ph = *reinterpret_cast<const h8*>(at), pl = *reinterpret_cast<const h8*>(at + 1024);
+#pragma unroll
+        for (int q = 0; q < J; ++q) y[q][t] = mfma_pair(ph, pl, xh[q][kb], xl[q][kb], y[q][t]);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < J; ++q)
+#pragma unroll
+      for (int t = 0; t < Q::MT; ++t) {
+        __builtin_amdgcn_sched_barrier(0);
+        split4(y[q][t] * factor, xh[q][t / 2], xl[q][t / 2], t & 1);
+      }
+  }
+};
+
 template <int MB, int J, int DT, int OUT>
 __global__ __launch_bounds__(512, 2) void muon_block_kernel(Muon a, MuonSize z, MuonSteps steps) {
-  typedef MuonTiles<MB> Q;
-  constexpr int MT = Q::MT;
   extern __shared__ __attribute__((aligned(16))) uint8_t muon_smem[];
   __shared__ double norm[8];
-  uint8_t* const xs = muon_smem;                         // X by rows, 128 columns: [tile][32 columns][hi, lo]
-  uint8_t* const gs = muon_smem + MT * 4 * 2048;         // G or P: [tile][32 rows][hi, lo]
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   int r = lane & 15, g = lane >> 4;
   const size_t base = (size_t)blockIdx.x * a.rows * a.cols;
@@ -244,8 +363,8 @@ __global__ __launch_bounds__(512, 2) void muon_block_kernel(Muon a, MuonSize z, 
       if (j0 > 0) __syncthreads();         // the last columns are read
       in.at(j0);
       float* const tile = reinterpret_cast<float*>(muon_smem);
-      if (a.cols % 4 == 0) t += muon_take<DT, 4>(a, in, base, tile);
-      else t += muon_take<DT, 1>(a, in, base, tile);
+      if (a.cols % 4 == 0) t += muon_take<DT, 4, false>(a, in, base, tile);
+      else t += muon_take<DT, 1, false>(a, in, base, tile);
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < in.JW; ++j) {
@@ -281,132 +400,21 @@ __global__ __launch_bounds__(512, 2) void muon_block_kernel(Muon a, MuonSize z, 
         }
   }
   const h8 eye[2] = {identity(0, r, g), identity(1, r, g)};
-  const int ta = wave / Q::ACROSS * Q::A, tb = wave % Q::ACROSS * Q::B;      // the wave's tiles of G
-  const bool mine = wave / Q::ACROSS * Q::A < MT;
+  const MuonCore<MB> core(muon_smem, wave, lane);
   for (int s = 0; s < steps.count; ++s) {
-    f4 gram[Q::A][Q::B];
-#pragma unroll
-    for (int i = 0; i < Q::A; ++i)
-#pragma unroll
-      for (int j = 0; j < Q::B; ++j) gram[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+    typename MuonCore<MB>::Tiles gram;
+    core.clear(gram);
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      if (j > 0) __syncthreads();        // the last columns are read
-#pragma unroll
-      for (int kb = 0; kb < MB; ++kb)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          __builtin_amdgcn_sched_barrier(0);
-          uint8_t* const at = xs + ((2 * kb + h) * 4 + (wave >> 1)) * 2048 + lane * 16 + 8 * (wave & 1);
-          *reinterpret_cast<h4*>(at) = turn(xh[j][kb], eye[h]);
-          *reinterpret_cast<h4*>(at + 1024) = turn(xl[j][kb], eye[h]);
-        }
+      __syncthreads();        // what was there is read
+      core.turn_columns(xh[j], xl[j], eye);
       __syncthreads();
-      if (mine) {
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
-          __builtin_amdgcn_sched_barrier(0);     // or all fragments would be read at once, and spill
-          h8 ah[Q::A], al[Q::A];
-#pragma unroll
-          for (int i = 0; i < Q::A; ++i) {
-            const uint8_t* const at = xs + ((ta + i) * 4 + kb) * 2048 + lane * 16;
-            ah[i] = *reinterpret_cast<const h8*>(at);
-            al[i] = *reinterpret_cast<const h8*>(at + 1024);
-          }
-#pragma unroll
-          for (int k = 0; k < Q::B; ++k) {
-            const uint8_t* const at = xs + ((tb + k) * 4 + kb) * 2048 + lane * 16;
-            const h8 bh = *reinterpret_cast<const h8*>(at), bl = *reinterpret_cast<const h8*>(at + 1024);
-#pragma unroll
-            for (int i = 0; i < Q::A; ++i) gram[i][k] = mfma_pair(ah[i], al[i], bh, bl, gram[i][k]);
-          }
-        }
-      }
+      if (core.mine) core.template times_itself<4>(gram, core.xs);
     }
-    // A symmetric tile (ta + i, tb + k) in its place: rows of tile tb + k, k of tile ta + i.
-    auto put = [&](const f4 (&v)[Q::A][Q::B]) __attribute__((always_inline)) {
+    core.to_p(gram, steps, s);
+    constexpr int JP = J > 1 ? 2 : 1;     // column tiles at a time
 #pragma unroll
-      for (int k = 0; k < Q::B; ++k)
-#pragma unroll
-        for (int i = 0; i < Q::A; ++i) {
-          __builtin_amdgcn_sched_barrier(0);
-          h8 hi, lo;
-          split4(v[i][k], hi, lo, 0);
-          uint8_t* const at = gs + ((tb + k) * MB + (ta + i) / 2) * 2048 + lane * 16 + 8 * ((ta + i) & 1);
-          *reinterpret_cast<h4*>(at) = h4{hi[0], hi[1], hi[2], hi[3]};
-          *reinterpret_cast<h4*>(at + 1024) = h4{lo[0], lo[1], lo[2], lo[3]};
-        }
-    };
-    if (mine) {
-#pragma unroll
-      for (int i = 0; i < Q::A; ++i)
-#pragma unroll
-        for (int k = 0; k < Q::B; ++k) gram[i][k] *= steps.gram[s];
-      put(gram);
-    }
-    __syncthreads();
-    f4 p[Q::A][Q::B];
-    if (mine) {
-#pragma unroll
-      for (int i = 0; i < Q::A; ++i)
-#pragma unroll
-        for (int k = 0; k < Q::B; ++k) p[i][k] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kb = 0; kb < MB; ++kb) {
-        __builtin_amdgcn_sched_barrier(0);
-        h8 ah[Q::A], al[Q::A];
-#pragma unroll
-        for (int i = 0; i < Q::A; ++i) {
-          const uint8_t* const at = gs + ((ta + i) * MB + kb) * 2048 + lane * 16;
-          ah[i] = *reinterpret_cast<const h8*>(at);
-          al[i] = *reinterpret_cast<const h8*>(at + 1024);
-        }
-#pragma unroll
-        for (int k = 0; k < Q::B; ++k) {
-          const uint8_t* const at = gs + ((tb + k) * MB + kb) * 2048 + lane * 16;
-          const h8 bh = *reinterpret_cast<const h8*>(at), bl = *reinterpret_cast<const h8*>(at + 1024);
-#pragma unroll
-          for (int i = 0; i < Q::A; ++i) p[i][k] = mfma_pair(ah[i], al[i], bh, bl, p[i][k]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < Q::A; ++i)
-#pragma unroll
-        for (int k = 0; k < Q::B; ++k) {
-          p[i][k] = p[i][k] * steps.square[s] + gram[i][k] * steps.gb[s];
-          if (ta + i == tb + k)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) p[i][k][e] += r == 4 * g + e ? steps.diagonal[s] : 0.f;
-        }
-    }
-    __syncthreads();          // G is read
-    if (mine) put(p);
-    __syncthreads();
-    constexpr int JP = J > 1 ? 2 : 1;     // column tiles at a time, which share the reads of P
-#pragma unroll
-    for (int j = 0; j < J; j += JP) {
-      f4 y[JP][MT];
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int q = 0; q < JP; ++q) y[q][t] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kb = 0; kb < MB; ++kb) {
-          const uint8_t* const at = gs + (t * MB + kb) * 2048 + lane * 16;
-          const h8 ph = *reinterpret_cast<const h8*>(at), pl = *reinterpret_cast<const h8*>(at + 1024);
-#pragma unroll
-          for (int q = 0; q < JP; ++q) y[q][t] = mfma_pair(ph, pl, xh[j + q][kb], xl[j + q][kb], y[q][t]);
-        }
-      }
-#pragma unroll
-      for (int q = 0; q < JP; ++q)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          __builtin_amdgcn_sched_barrier(0);
-          split4(y[q][t] * steps.apply[s], xh[j + q][t / 2], xl[j + q][t / 2], t & 1);
-        }
-    }
+    for (int j = 0; j < J; j += JP) core.template apply<JP>(xh + j, xl + j, steps.apply[s]);
   }
   // What is stored is hi + lo, 22 bits at least of the largest values: the products before keep no more.
   asm volatile("" : "+v"(r), "+v"(g));     // or the places of all elements would be kept in registers throughout
@@ -433,6 +441,123 @@ __global__ __launch_bounds__(512, 2) void muon_block_kernel(Muon a, MuonSize z, 
   }
 }
 
+constexpr int NORM_MOST = 256; // blocks that share a matrix's norm
+
+// ---- a block 128 columns, a launch a step ------------------------------------------------------------
+
+// Few matrices of 65 to 128 rows: a block each 128 columns of them, whose parts of G go through memory: a launch adds up
+// the parts, makes P (every block of a matrix its own), multiplies its columns and leaves them and their part of the next G.
+struct MuonPanels {
+  int panels, parts;           // blocks of a matrix, of its norm
+  const double* norms;
+  uint8_t* x;                  // [matrix][panel][wave][32 rows][hi, lo][lane]: fragments of X^T
+  const float* in;             // parts of G: [matrix][panel][tile][lane][4]
+  float* out;
+};
+enum { PANEL_FIRST = 0, PANEL_STEP = 1, PANEL_LAST = 2 };
+
+template <int KIND, int DT, int OUT>
+__global__ __launch_bounds__(512, 2) void muon_panel_kernel(Muon a, MuonSize z, MuonSteps steps, int s, MuonPanels q) {
+  constexpr int MB = 4, TILES = 64;
+  extern __shared__ __attribute__((aligned(16))) uint8_t muon_smem[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  // a matrix's blocks on one XCD, whose L2 holds what they leave for each other (blocks are dealt out to 8 in turn)
+  const int slot = blockIdx.x >> 3, panel = slot % q.panels, matrix = slot / q.panels * 8 + (blockIdx.x & 7);
+  if (matrix >= a.batch) return;
+  const size_t place0 = (size_t)matrix * q.panels + panel;
+  const size_t base = (size_t)matrix * a.rows * a.cols;
+  const MuonCore<MB> core(muon_smem, wave, lane);
+  float* const tile = reinterpret_cast<float*>(muon_smem);
+  uint8_t* const saved = q.x + (place0 * 8 + wave) * MB * 2048 + lane * 16;
+  MuonRegion<MB, 1> in(a, z);
+  in.at(panel);
+  const int c = 16 * wave + r;
+  h8 xh[1][MB], xl[1][MB];
+  if constexpr (KIND == PANEL_FIRST) {
+    double t = 0;
+    for (int i = lane; i < q.parts; i += 64) t += q.norms[matrix * NORM_MOST + i];
+    if (a.cols % 4 == 0) muon_take<DT, 4, true>(a, in, base, tile);
+    else muon_take<DT, 1, true>(a, in, base, tile);
+    for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+    const double f = 1.0 / (sqrt(t) + a.epsilon);
+    __syncthreads();
+#pragma unroll
+    for (int kb = 0; kb < MB; ++kb)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        f4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = 32 * kb + 16 * h + 4 * g + e;
+          const float u = tile[in.tall ? c * in.pitch + i : i * in.pitch + c];
+          v[e] = i < z.m && c < in.width ? ldexpf((float)(u * f), steps.start) : 0.f;
+        }
+        split4(v, xh[0][kb], xl[0][kb], h);
+      }
+    __syncthreads();          // u is read
+  } else {
+    typename MuonCore<MB>::Tiles gram;
+    core.clear(gram);
+#pragma unroll
+    for (int kb = 0; kb < MB; ++kb) {
+      xh[0][kb] = *reinterpret_cast<const h8*>(saved + kb * 2048);
+      xl[0][kb] = *reinterpret_cast<const h8*>(saved + kb * 2048 + 1024);
+    }
+    constexpr int A = MuonTiles<MB>::A, B = MuonTiles<MB>::B;
+    for (int k0 = 0; k0 < q.panels; k0 += 4) {       // the loads of four parts under way together
+      f4 v[4][A][B];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const f4* const at = reinterpret_cast<const f4*>(q.in) + ((size_t)matrix * q.panels + min(k0 + k, q.panels - 1)) * TILES * 64 + lane;
+#pragma unroll
+        for (int i = 0; i < A; ++i)
+#pragma unroll
+          for (int j = 0; j < B; ++j) v[k][i][j] = at[((core.ta + i) * 8 + core.tb + j) * 64];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k0 + k < q.panels)
+#pragma unroll
+          for (int i = 0; i < A; ++i)
+#pragma unroll
+            for (int j = 0; j < B; ++j) gram[i][j] += v[k][i][j];
+    }
+    core.to_p(gram, steps, s);
+    core.template apply<1>(xh, xl, steps.apply[s]);
+  }
+  if constexpr (KIND == PANEL_LAST) {
+    const float back = ldexpf(1.f, -steps.end);
+    __syncthreads();          // P is read
+#pragma unroll
+    for (int kb = 0; kb < MB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int i = 32 * kb + 16 * (e >> 2) + 4 * g + (e & 3);
+        tile[in.tall ? c * in.pitch + i : i * in.pitch + c] = ((float)xh[0][kb][e] + (float)xl[0][kb][e]) * back;
+      }
+    __syncthreads();
+    if (a.cols % 4 == 0) muon_give<OUT, 4>(a, in, base, tile);
+    else muon_give<OUT, 1>(a, in, base, tile);
+  } else {
+    const h8 eye[2] = {identity(0, r, g), identity(1, r, g)};
+#pragma unroll
+    for (int kb = 0; kb < MB; ++kb) {
+      *reinterpret_cast<h8*>(saved + kb * 2048) = xh[0][kb];
+      *reinterpret_cast<h8*>(saved + kb * 2048 + 1024) = xl[0][kb];
+    }
+    core.turn_columns(xh[0], xl[0], eye);
+    __syncthreads();
+    typename MuonCore<MB>::Tiles gram;
+    core.clear(gram);
+    core.template times_itself<4>(gram, core.xs);
+    f4* const at = reinterpret_cast<f4*>(q.out) + place0 * TILES * 64 + lane;
+#pragma unroll
+    for (int i = 0; i < MuonTiles<MB>::A; ++i)
+#pragma unroll
+      for (int j = 0; j < MuonTiles<MB>::B; ++j) at[((core.ta + i) * 8 + core.tb + j) * 64] = gram[i][j];
+  }
+}
+
 // ---- larger matrices: a product a launch ---------------------------------------------------------
 
 // A matrix in scratch, as fragments: [rows / 16][k / 32][hi, lo], 1 KB each; rows and k are multiples of 128, zeros
@@ -445,8 +570,6 @@ struct Frags {
 __device__ __forceinline__ uint8_t* frag(const Frags& f, int tile, int kb) {
   return f.at + blockIdx.z * f.stride + ((size_t)tile * f.kbs + kb) * 2048;
 }
-
-constexpr int NORM_MOST = 256; // blocks that share a matrix
 
 // Sums of squares, in double: f32's largest values do not overflow it.
 template <int DT>
@@ -729,7 +852,14 @@ MuonSize muon_size(long long rows, long long cols) { return MuonSize{(int)std::m
 
 constexpr int CUS = 256;
 
-bool one_block(const MuonSize& z) { return z.m <= 128 && z.n <= 512; }
+enum MuonKind { BLOCK, PANELS, PRODUCTS };
+// Panels while they find a CU each: 48 matrices of 128 x 512 take XX us, and 149 in blocks of their own.
+MuonKind muon_kind(long long batch, const MuonSize& z) {
+  const long long panels = (z.n + 127) / 128;
+  if (z.m > 64 && z.m <= 128 && panels > 1 && panels <= 8 && batch * panels <= 3 * CUS / 2) return PANELS;
+  return z.m <= 128 && z.n <= 512 ? BLOCK : PRODUCTS;
+}
+int norm_parts(long long count) { return (int)std::min<long long>(NORM_MOST, (count + 4095) / 4096); }
 
 struct MuonGrid {
   int mp, np, w, across, gram_parts;   // padded sides, W, blocks along m
@@ -748,20 +878,33 @@ MuonGrid muon_grid(long long batch, const MuonSize& z) {
 
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
+int norms(lf_context* ctx, const Muon& a, double* partial) {
+  const dim3 grid(norm_parts((long long)a.rows * a.cols), a.batch), block(256);
+  LaunchScope ls(ctx, "muon.norm");
+  if (a.grad_dtype == LF_F32) hipLaunchKernelGGL((muon_norm_kernel<DT_F32>), grid, block, 0, ctx->stream, a, partial);
+  else if (a.grad_dtype == LF_F16) hipLaunchKernelGGL((muon_norm_kernel<DT_F16>), grid, block, 0, ctx->stream, a, partial);
+  else hipLaunchKernelGGL((muon_norm_kernel<DT_BF16>), grid, block, 0, ctx->stream, a, partial);
+  return check_hip(hipGetLastError(), "muon norm launch");
+}
+
 template <int DT>
-int start(lf_context* ctx, const Muon& a, const MuonSize& z, const MuonGrid& q, double* partial, int e, const Frags& x,
+int start(lf_context* ctx, const Muon& a, const MuonSize& z, const MuonGrid& q, const double* partial, int e, const Frags& x,
           const Frags& xt) {
-  const long long count = (long long)a.rows * a.cols;
-  const int parts = (int)std::min<long long>(NORM_MOST, (count + 4095) / 4096);
-  {
-    LaunchScope ls(ctx, "muon.norm");
-    hipLaunchKernelGGL((muon_norm_kernel<DT>), dim3(parts, a.batch), dim3(256), 0, ctx->stream, a, partial);
-  }
-  LF_TRY(check_hip(hipGetLastError(), "muon norm launch"));
   LaunchScope ls(ctx, "muon.start");
-  hipLaunchKernelGGL((muon_start_kernel<DT>), dim3(q.np / 128, q.mp / 32, a.batch), dim3(256), 0, ctx->stream, a, z, partial, parts,
-                     e, x, xt);
+  hipLaunchKernelGGL((muon_start_kernel<DT>), dim3(q.np / 128, q.mp / 32, a.batch), dim3(256), 0, ctx->stream, a, z, partial,
+                     norm_parts((long long)a.rows * a.cols), e, x, xt);
   return check_hip(hipGetLastError(), "muon start launch");
+}
+
+constexpr int PANEL_LDS = std::max(2 * 4 * 4 * 2048 + 2 * 4 * 4 * 2048, MuonRegion<4, 1>::BYTES);
+template <int KIND, int DT = DT_F32, int OUT = DT_F32>
+int panel(lf_context* ctx, const Muon& m, const MuonSize& z, const MuonSteps& f, int s, const MuonPanels& q, const char* label) {
+  const auto kernel = muon_panel_kernel<KIND, DT, OUT>;
+  static const hipError_t lds = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, PANEL_LDS);
+  LF_TRY(check_hip(lds, "muon LDS"));
+  LaunchScope ls(ctx, label);
+  hipLaunchKernelGGL(kernel, dim3((m.batch + 7) / 8 * 8 * q.panels), dim3(512), PANEL_LDS, ctx->stream, m, z, f, s, q);
+  return check_hip(hipGetLastError(), "muon panel launch");
 }
 
 template <int KIND, int W, int OUT = DT_F32>
@@ -814,7 +957,9 @@ int go_block(lf_context* ctx, const Muon& m, const MuonSize& z, const MuonSteps&
 
 size_t muon_bytes(long long batch, long long rows, long long cols) {
   const MuonSize z = muon_size(rows, cols);
-  if (one_block(z)) return 0;
+  const MuonKind kind = muon_kind(batch, z);
+  if (kind == BLOCK) return 0;
+  if (kind == PANELS) return up256(batch * NORM_MOST * sizeof(double)) + batch * ((z.n + 127) / 128) * (size_t)(3 * 65536);
   const MuonGrid q = muon_grid(batch, z);
   const size_t x = up256(batch * (size_t)q.mp * q.np * 4), g = up256(batch * (size_t)q.mp * q.mp * 4);
   const size_t parts = q.gram_parts > 1 ? batch * (size_t)q.gram_parts * (q.across * (q.across + 1) / 2) * (32 * q.w) * (32 * q.w) * 4 : 0;
@@ -836,10 +981,36 @@ int run_muon(lf_context* ctx, const Muon& m, const MuonPlan& plan, void* scratch
     f.diagonal[k] = std::ldexp(c[0], ep);
     f.apply[k] = std::ldexp(1.f, plan.x[k + 1] - ep - ex);
   }
-  if (one_block(z)) {
+  const MuonKind kind = muon_kind(m.batch, z);
+  if (kind == BLOCK) {
     if (m.grad_dtype == LF_F32) return go_block<DT_F32>(ctx, m, z, f);
     if (m.grad_dtype == LF_F16) return go_block<DT_F16>(ctx, m, z, f);
     return go_block<DT_BF16>(ctx, m, z, f);
+  }
+  if (kind == PANELS) {
+    char* const at = static_cast<char*>(scratch);
+    double* const sums = reinterpret_cast<double*>(at);
+    MuonPanels q{};
+    q.panels = (z.n + 127) / 128;
+    q.parts = norm_parts((long long)m.rows * m.cols);
+    q.norms = sums;
+    const size_t each = (size_t)m.batch * q.panels * 65536;
+    q.x = reinterpret_cast<uint8_t*>(at + up256((size_t)m.batch * NORM_MOST * sizeof(double)));
+    float* const parts[2] = {reinterpret_cast<float*>(q.x + each), reinterpret_cast<float*>(q.x + 2 * each)};
+    LF_TRY(norms(ctx, m, sums));
+    q.out = parts[0];
+    if (m.grad_dtype == LF_F32) LF_TRY((panel<PANEL_FIRST, DT_F32>(ctx, m, z, f, 0, q, "muon.first")));
+    else if (m.grad_dtype == LF_F16) LF_TRY((panel<PANEL_FIRST, DT_F16>(ctx, m, z, f, 0, q, "muon.first")));
+    else LF_TRY((panel<PANEL_FIRST, DT_BF16>(ctx, m, z, f, 0, q, "muon.first")));
+    for (int k = 0; k < m.steps; ++k) {
+      q.in = parts[k & 1];
+      q.out = parts[!(k & 1)];
+      if (k + 1 < m.steps) LF_TRY((panel<PANEL_STEP>(ctx, m, z, f, k, q, "muon.step")));
+      else if (m.out_dtype == LF_F32) LF_TRY((panel<PANEL_LAST, DT_F32, DT_F32>(ctx, m, z, f, k, q, "muon.last")));
+      else if (m.out_dtype == LF_F16) LF_TRY((panel<PANEL_LAST, DT_F32, DT_F16>(ctx, m, z, f, k, q, "muon.last")));
+      else LF_TRY((panel<PANEL_LAST, DT_F32, DT_BF16>(ctx, m, z, f, k, q, "muon.last")));
+    }
+    return LF_OK;
   }
   const MuonGrid q = muon_grid(m.batch, z);
   char* at = static_cast<char*>(scratch);
@@ -848,7 +1019,7 @@ int run_muon(lf_context* ctx, const Muon& m, const MuonPlan& plan, void* scratch
     at += up256(bytes);
     return p;
   };
-  double* const norms = reinterpret_cast<double*>(take((size_t)m.batch * NORM_MOST * sizeof(double)));
+  double* const sums = reinterpret_cast<double*>(take((size_t)m.batch * NORM_MOST * sizeof(double)));
   auto frags = [&](int rows, int k) {
     Frags p;
     p.kbs = k / 32;
@@ -859,9 +1030,10 @@ int run_muon(lf_context* ctx, const Muon& m, const MuonPlan& plan, void* scratch
   const Frags x[2] = {frags(q.mp, q.np), frags(q.mp, q.np)}, xt[2] = {frags(q.np, q.mp), frags(q.np, q.mp)};
   const Frags g = frags(q.mp, q.mp), pm = frags(q.mp, q.mp);
   float* const partial = reinterpret_cast<float*>(at);
-  if (m.grad_dtype == LF_F32) LF_TRY(start<DT_F32>(ctx, m, z, q, norms, f.start, x[0], xt[0]));
-  else if (m.grad_dtype == LF_F16) LF_TRY(start<DT_F16>(ctx, m, z, q, norms, f.start, x[0], xt[0]));
-  else LF_TRY(start<DT_BF16>(ctx, m, z, q, norms, f.start, x[0], xt[0]));
+  LF_TRY(norms(ctx, m, sums));
+  if (m.grad_dtype == LF_F32) LF_TRY(start<DT_F32>(ctx, m, z, q, sums, f.start, x[0], xt[0]));
+  else if (m.grad_dtype == LF_F16) LF_TRY(start<DT_F16>(ctx, m, z, q, sums, f.start, x[0], xt[0]));
+  else LF_TRY(start<DT_BF16>(ctx, m, z, q, sums, f.start, x[0], xt[0]));
   for (int k = 0; k < m.steps; ++k) {
     const int now = k & 1;
     const Product gram{x[now], x[now], q.np / 32, q.gram_parts, g, g, partial, f.gram[k], 0.f, 0.f};
