@@ -75,12 +75,49 @@ __device__ __forceinline__ size_t place(const Muon& a, int i, int j) {
   return a.rows > a.cols ? (size_t)j * a.cols + i : (size_t)i * a.cols + j;
 }
 
+// Rows i to i + 3 of column j of X, in one access where they lie side by side.
+template <int DT>
+__device__ __forceinline__ f4 muon_u4(const Muon& a, const MuonSize& z, size_t base, int i, int j) {
+  typedef typename Act<DT>::T T;
+  f4 v = {0.f, 0.f, 0.f, 0.f};
+  if (j >= z.n) return v;
+  if (a.rows > a.cols && i + 4 <= z.m) {
+    struct Vec { T v[4]; } gv;
+    f4 mv = v;
+    const size_t at = base + place(a, i, j);
+    __builtin_memcpy(&gv, static_cast<const T*>(a.grad) + at, sizeof(gv));
+    if (a.momentum) __builtin_memcpy(&mv, a.momentum_out + at, 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float g = Act<DT>::ld(gv.v + e);
+      v[e] = !a.momentum ? g : a.nesterov ? g + a.momentum_factor * mv[e] : mv[e];
+    }
+    return v;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (i + e < z.m) v[e] = muon_u<DT>(a, base + place(a, i + e, j));
+  return v;
+}
+
 template <int OUT>
-__device__ __forceinline__ void muon_store(const Muon& m, size_t at, float o) {
+__device__ __forceinline__ void muon_store4(const Muon& m, const MuonSize& z, size_t base, int i, int j, f4 o) {
   typedef typename Act<OUT>::T T;
-  float v = -m.rate * o;
-  if (m.weight) v = m.keep * Act<OUT>::ld(static_cast<const T*>(m.weight) + at) + v;
-  Act<OUT>::st(static_cast<T*>(m.out) + at, v);
+  if (j >= z.n) return;
+  struct Vec { T v[4]; } w;
+  const size_t at = base + place(m, i, j), step = m.rows > m.cols ? 1 : m.cols;
+  const T* const weight = static_cast<const T*>(m.weight) + at;
+  T* const out = static_cast<T*>(m.out) + at;
+  const bool whole = m.rows > m.cols && i + 4 <= z.m;
+  if (m.weight && whole) __builtin_memcpy(&w, weight, sizeof(w));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (i + e >= z.m) continue;
+    float v = -m.rate * o[e];
+    if (m.weight) v = m.keep * Act<OUT>::ld(whole ? w.v + e : weight + e * step) + v;
+    Act<OUT>::st(whole ? w.v + e : out + e * step, v);
+  }
+  if (whole) __builtin_memcpy(out, &w, sizeof(w));
 }
 
 // ---- one block a matrix --------------------------------------------------------------------------
@@ -441,7 +478,7 @@ __global__ __launch_bounds__(512, 2) void muon_block_kernel(Muon a, MuonSize z, 
   }
 }
 
-constexpr int NORM_MOST = 256; // blocks that share a matrix's norm
+constexpr int NORM_MOST = 1024;   // blocks that share a matrix's norm
 
 // ---- a block 128 columns, a launch a step ------------------------------------------------------------
 
@@ -641,12 +678,9 @@ __global__ __launch_bounds__(256) void muon_start_kernel(Muon a, MuonSize z, con
   for (int q = 0; q < 2; ++q)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      f4 v;
+      f4 v = muon_u4<DT>(a, z, base, 32 * kb + 16 * h + 4 * g, 16 * (jt + q) + r);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int i = 32 * kb + 16 * h + 4 * g + k, j = 16 * (jt + q) + r;
-        v[k] = i < z.m && j < z.n ? ldexpf((float)(muon_u<DT>(a, base + place(a, i, j)) * f), e) : 0.f;
-      }
+      for (int k = 0; k < 4; ++k) v[k] = ldexpf((float)(v[k] * f), e);
       split4(v, hi[q], lo[q], h);
     }
   store_x(hi, lo, x, xt, jt, kb, lane);
@@ -696,12 +730,20 @@ __device__ __forceinline__ void store_symmetric(const f4 (&v)[2][2], const Frags
   }
 }
 
-// A block of four waves computes 32 W by 32 W, a wave 16 W by 16 W (W 2 or 4), 32 k a step, both operands through two
-// LDS buffers.
-template <int KIND, int W, int OUT>
-__global__ __launch_bounds__(256, 2) void muon_product_kernel(Product p, Muon m, MuonSize z, int across) {
+// A block of four waves computes 32 W by 32 W, a wave 16 W by 16 W (W 2 or 4), 32 k a step, both operands through one of
+// DEPTH LDS buffers, DEPTH - 1 steps ahead; fragments are read a step ahead too, so that the products do not wait for LDS.
+// Four buffers where a CU has one block anyway, two, which leave room for two blocks, where there are more: 1024 x 1024
+// times 1024 x 4096 (256 blocks) takes 34 us and 40, five steps of 96 matrices of 256 x 1024 995 and 854.
+template <int W>
+struct MuonFrags {
+  h8 ah[W], al[W], bh[W], bl[W];
+};
+
+template <int KIND, int W, int DEPTH, int OUT>
+__global__ __launch_bounds__(256, DEPTH == 4 && W == 4 ? 1 : 2) void muon_product_kernel(Product p, Muon m, MuonSize z, int across) {
   constexpr int STAGE = 4 * W * 2048, EACH = STAGE / 4096;      // copies of 1 KB a wave
-  __shared__ __attribute__((aligned(16))) uint8_t S0[STAGE], S1[STAGE];
+  // Separate objects: reads of one are then known not to wait for copies into another.
+  __shared__ __attribute__((aligned(16))) uint8_t S0[STAGE], S1[STAGE], S2[DEPTH == 4 ? STAGE : 16], S3[DEPTH == 4 ? STAGE : 16];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   int bi, bj, part = 0;
   if constexpr (KIND == APPLY || KIND == LAST) {
@@ -715,18 +757,21 @@ __global__ __launch_bounds__(256, 2) void muon_product_kernel(Product p, Muon m,
   const int s0 = KIND == GRAM_PART ? (int)((long long)p.steps * part / p.parts) : 0;
   const int s1 = KIND == GRAM_PART ? (int)((long long)p.steps * (part + 1) / p.parts) : p.steps;
   // [2 W tiles of a][2 W tiles of b], hi and lo of each side by side
-  const uint8_t* const src = frag(wave < 2 ? p.a : p.b, (wave < 2 ? bi : bj) * 2 * W + (wave & 1) * W, 0) + lane * 16;
-  const size_t row = (size_t)(wave < 2 ? p.a.kbs : p.b.kbs) * 2048;
+  const uint8_t* const src = wave < 2 ? frag(p.a, bi * 2 * W + (wave & 1) * W, 0) : frag(p.b, bj * 2 * W + (wave & 1) * W, 0);
+  const uint32_t row = (uint32_t)(wave < 2 ? p.a.kbs : p.b.kbs) * 2048;
   auto stage = [&](uint8_t* dst, int s) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      const uint8_t* const at = src + (i >> 1) * row + (size_t)s * 2048 + (i & 1) * 1024;
 #if __HIP_DEVICE_COMPILE__
-      __builtin_amdgcn_global_load_lds(at, dst + (wave * EACH + i) * 1024, 16, 0, 0);
+    const uint64_t v = reinterpret_cast<uint64_t>(src);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>((uint64_t)hi << 32 | lo), 0, 0xffffffffu, 0x27000);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, dst + (wave * EACH + i) * 1024, 16, lane * 16, (i >> 1) * row + s * 2048 + (i & 1) * 1024,
+                                               0, 0);
 #else
-      (void)at, (void)dst;
+    (void)src, (void)row, (void)dst, (void)s;
 #endif
-    }
   };
   const int wi = wave >> 1, wj = wave & 1;
   f4 acc[W][W];
@@ -734,34 +779,61 @@ __global__ __launch_bounds__(256, 2) void muon_product_kernel(Product p, Muon m,
   for (int i = 0; i < W; ++i)
 #pragma unroll
     for (int j = 0; j < W; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
-  stage(S0, s0);
-  auto step = [&](int s, const uint8_t* buf, uint8_t* other) __attribute__((always_inline)) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();          // step s in LDS for every wave, every wave done with the other buffer
-    h8 ah[W], al[W], bh[W], bl[W];
+  typedef MuonFrags<W> F;
+  auto read = [&](F& f, const uint8_t* buf) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < W; ++t) {
       const uint8_t* const a = buf + (wi * W + t) * 2048 + lane * 16;
       const uint8_t* const b = buf + (2 * W + wj * W + t) * 2048 + lane * 16;
-      ah[t] = *reinterpret_cast<const h8*>(a);
-      al[t] = *reinterpret_cast<const h8*>(a + 1024);
-      bh[t] = *reinterpret_cast<const h8*>(b);
-      bl[t] = *reinterpret_cast<const h8*>(b + 1024);
+      f.ah[t] = *reinterpret_cast<const h8*>(a);
+      f.al[t] = *reinterpret_cast<const h8*>(a + 1024);
+      f.bh[t] = *reinterpret_cast<const h8*>(b);
+      f.bl[t] = *reinterpret_cast<const h8*>(b + 1024);
     }
-    stage(other, min(s + 1, s1 - 1));
+  };
+  // past the end the last step again, which nothing uses
+  stage(S0, s0);
+  stage(S1, min(s0 + 1, s1 - 1));
+  if constexpr (DEPTH == 4) {
+    stage(S2, min(s0 + 2, s1 - 1));
+    stage(S3, min(s0 + 3, s1 - 1));
+  }
+  F f0, f1;
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 1) * EACH) : "memory");
+  __builtin_amdgcn_s_barrier();
+  read(f0, S0);
+  // Step s: its fragments are in `now`, step s + 1 is in `buf`, and `freed` held step s.
+  auto step = [&](int s, const F& now, F& next, const uint8_t* buf, uint8_t* freed) __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((DEPTH - 2) * EACH) : "memory");
+    __builtin_amdgcn_s_barrier();       // every wave's copies of s + 1 are there, every wave has read s
+    __builtin_amdgcn_sched_barrier(0);
+    read(next, buf);
+    stage(freed, min(s + DEPTH, s1 - 1));
 #pragma unroll
     for (int i = 0; i < W; ++i)
 #pragma unroll
-      for (int j = 0; j < W; ++j) acc[i][j] = mfma_pair(ah[i], al[i], bh[j], bl[j], acc[i][j]);
-    __builtin_amdgcn_sched_barrier(0);
+      for (int j = 0; j < W; ++j) acc[i][j] = mfma_pair(now.ah[i], now.al[i], now.bh[j], now.bl[j], acc[i][j]);
+    __builtin_amdgcn_sched_barrier(0);   // products touch no memory: they would be moved past the next barrier
   };
   int s = s0;
-  for (; s + 1 < s1; s += 2) {
-    step(s, S0, S1);
-    step(s + 1, S1, S0);
+  if constexpr (DEPTH == 4) {
+    for (; s + 3 < s1; s += 4) {
+      step(s, f0, f1, S1, S0);
+      step(s + 1, f1, f0, S2, S1);
+      step(s + 2, f0, f1, S3, S2);
+      step(s + 3, f1, f0, S0, S3);
+    }
+    if (s < s1) step(s, f0, f1, S1, S0);
+    if (s + 1 < s1) step(s + 1, f1, f0, S2, S1);
+    if (s + 2 < s1) step(s + 2, f0, f1, S3, S2);
+  } else {
+    for (; s + 1 < s1; s += 2) {
+      step(s, f0, f1, S1, S0);
+      step(s + 1, f1, f0, S0, S1);
+    }
+    if (s < s1) step(s, f0, f1, S1, S0);
   }
-  if (s < s1) step(s, S0, S1);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last copy, which nothing reads
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last copies, which nothing reads
   const int ti = (bi * 2 + wi) * W, tj = (bj * 2 + wj) * W;
   if constexpr (KIND == GRAM_PART) {
     f4* const at = reinterpret_cast<f4*>(p.partial) +
@@ -809,11 +881,7 @@ __global__ __launch_bounds__(256, 2) void muon_product_kernel(Product p, Muon m,
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int q = 0; q < 2; ++q)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int x = (ti + i + h) * 16 + 4 * g + e, y = (tj + j + q) * 16 + r;
-              if (x < z.m && y < z.n) muon_store<OUT>(m, (size_t)blockIdx.z * m.rows * m.cols + place(m, x, y), v[h][q][e]);
-            }
+            muon_store4<OUT>(m, z, (size_t)blockIdx.z * m.rows * m.cols, (ti + i + h) * 16 + 4 * g, (tj + j + q) * 16 + r, v[h][q]);
       }
     }
 }
@@ -853,7 +921,7 @@ MuonSize muon_size(long long rows, long long cols) { return MuonSize{(int)std::m
 constexpr int CUS = 256;
 
 enum MuonKind { BLOCK, PANELS, PRODUCTS };
-// Panels while they find a CU each: 48 matrices of 128 x 512 take XX us, and 149 in blocks of their own.
+// Panels while there are few: 48 matrices of 128 x 512 take 104 us, and 149 in blocks of their own (256: 205 in blocks).
 MuonKind muon_kind(long long batch, const MuonSize& z) {
   const long long panels = (z.n + 127) / 128;
   if (z.m > 64 && z.m <= 128 && panels > 1 && panels <= 8 && batch * panels <= 3 * CUS / 2) return PANELS;
@@ -911,7 +979,11 @@ template <int KIND, int W, int OUT = DT_F32>
 void go_product(lf_context* ctx, const Product& p, const Muon& m, const MuonSize& z, const MuonGrid& q) {
   const int tiles = q.across * (q.across + 1) / 2;
   const int blocks = KIND == GRAM_PART ? tiles * p.parts : KIND == APPLY || KIND == LAST ? q.across * (q.np / (32 * W)) : tiles;
-  hipLaunchKernelGGL((muon_product_kernel<KIND, W, OUT>), dim3(blocks, 1, m.batch), dim3(256), 0, ctx->stream, p, m, z, q.across);
+  const dim3 grid(blocks, 1, m.batch);
+  if ((long long)blocks * m.batch <= CUS)
+    hipLaunchKernelGGL((muon_product_kernel<KIND, W, 4, OUT>), grid, dim3(256), 0, ctx->stream, p, m, z, q.across);
+  else
+    hipLaunchKernelGGL((muon_product_kernel<KIND, W, 2, OUT>), grid, dim3(256), 0, ctx->stream, p, m, z, q.across);
 }
 template <int KIND, int OUT = DT_F32>
 int product(lf_context* ctx, const Product& p, const Muon& m, const MuonSize& z, const MuonGrid& q, const char* label) {

@@ -221,7 +221,8 @@ def on(ctx, a):
 
 
 PAIRS = [(1, 1, 1, 3), (1, 300, 128, 32), (59, 59, 128, 32), (7, 65, 22, 4), (33, 130, 1, 2), (5, 257, 130, 32), (64, 63, 16, 9),
-         (3, 40, 515, 1), (300, 2, 64, 32), (40, 70, 37, 8), (90, 100, 384, 5)]
+         (3, 40, 515, 1), (300, 2, 64, 32), (40, 70, 37, 8), (90, 100, 384, 5), (200, 190, 8, 1), (300, 400, 22, 4),
+         (400, 500, 130, 8)]
 
 
 @pytest.mark.gpu
@@ -465,6 +466,33 @@ def test_mx4_linear(ctx, dt, rows, k, n):
     assert torch.equal(into, got)
 
 
+# Products of more outputs than one block a run of them takes: weights resident for 1, 2, 4 and 8 steps of 128 columns and
+# 8 that do not fit, both sizes of streamed tiles, whole and ragged, odd numbers of steps.
+MANY = [(3001, 100, 300), (3001, 200, 300), (3001, 500, 300), (3001, 1000, 300), (3040, 1024, 320), (2000, 900, 1500),
+        (4000, 1100, 1100), (8200, 1100, 1000), (8192, 640, 1024)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rows,k,n", MANY)
+def test_mx4_linear_many(ctx, dt, rows, k, n):
+    test_mx4_linear(ctx, dt, rows, k, n)
+
+
+@pytest.mark.gpu
+def test_mx4_pack_of_many_rows(ctx):
+    """A block walks down more than one tile of rows."""
+    from localfold_amd import device as D
+    rng = np.random.default_rng(9)
+    x = stream(rng, 300001, 5, torch.bfloat16)
+    m, t = D.mx4_empty(300001, 5, ctx.device), D.mx4_empty(5, 300001, ctx.device)
+    sums = torch.empty(5, device=ctx.device)
+    D.mx4_pack(ctx, x.to(ctx.device), out=m, transposed=t, sums=sums)
+    assert (values_of(m)[0][:, :5] == mx64(f64(x))).all() and (values_of(t)[0][:, :300001] == mx64(f64(x).T)).all()
+    # a thread's sum of at most 2 x 32 rows, four of them, then doubles
+    close(sums, f64(x).sum(0), 2 * U * 70 * np.abs(f64(x)).sum(0), torch.float32)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,n,k", [(1, 1, 1), (300, 128, 128), (1000, 64, 130), (5000, 22, 49), (20000, 128, 64), (9000, 300, 70)])
 def test_mx4_weight_gradient(ctx, rows, n, k):
@@ -540,7 +568,7 @@ def test_mx4_leaves_the_neighbours(ctx):
 # ---- orthogonalised updates ----------------------------------------------------------------------
 
 SIDES = [(1, 1, 1), (1, 64, 256), (2, 5, 9), (3, 22, 70), (2, 130, 64), (1, 128, 128), (2, 128, 512), (1, 300, 129), (1, 257, 1000),
-         (1, 16, 700), (5, 1, 40), (2, 384, 100), (1, 200, 150)]
+         (1, 16, 700), (5, 1, 40), (2, 384, 100), (1, 200, 150), (2, 66, 1001), (9, 700, 100), (1, 1, 2000), (40, 260, 390)]
 
 
 def gradients(rng, shape, dt):
@@ -564,6 +592,29 @@ def test_orthogonalize(ctx, dt, batch, rows, cols):
             assert d <= bound + store, (steps, b, d, bound, store)
         same = x.to(ctx.device)
         assert D.orthogonalize(ctx, same, steps=steps, coefficients=co, out=same) is same and torch.equal(same, got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [(128, 512), (300, 70), (100, 129)])
+def test_orthogonalize_batches(ctx, rows, cols):
+    """Many matrices take other kernels than few; both are within the bound."""
+    from localfold_amd import device as D
+    x = gradients(np.random.default_rng(rows), (200, rows, cols), torch.float32)
+    many, few = D.orthogonalize(ctx, x.to(ctx.device)), D.orthogonalize(ctx, x[:3].to(ctx.device))
+    for b in (0, 1, 2, 100, 199):
+        want, bound = schulz64(f64(x[b]), 5)
+        for got in (many[b], few[b]) if b < 3 else (many[b],):
+            assert np.linalg.norm(f64(got) - want) <= bound + U * np.linalg.norm(want)
+
+
+@pytest.mark.gpu
+def test_orthogonalize_large(ctx):
+    """Sums over parts, in tiles of 128: a step of a matrix whose bound is close."""
+    from localfold_amd import device as D
+    x = gradients(np.random.default_rng(1), (1, 1025, 2300), torch.float32)
+    got = D.orthogonalize(ctx, x.to(ctx.device), steps=2)
+    want, bound = schulz64(f64(x[0]), 2)
+    assert np.linalg.norm(f64(got[0]) - want) <= bound + U * np.linalg.norm(want)
 
 
 @pytest.mark.gpu
@@ -713,6 +764,32 @@ def test_training_step_other_stream(ctx):
     ctx.bind_stream()
     stream.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_two_contexts_at_once(ctx):
+    """Steps of two contexts on two streams, interleaved, each with a workspace of its own."""
+    from localfold_amd import device as D
+    other = D.Context(0)
+    streams = [torch.cuda.Stream(ctx.device) for _ in range(2)]
+    states = [step_state(ctx, np.random.default_rng(k)) for k in range(2)]
+    large = [torch.randn(2, 200, 300, device=ctx.device) for _ in range(2)]
+    want = [[t.clone() for t in training_step(ctx, s)] + [D.orthogonalize(ctx, x)] for s, x in zip(states, large)]
+    torch.cuda.synchronize()
+    got = [None, None]
+    try:
+        for c, s in zip((ctx, other), streams):
+            c.bind_stream(s)
+        for _ in range(5):
+            for k, c in enumerate((ctx, other)):
+                with torch.cuda.stream(streams[k]):
+                    got[k] = training_step(c, states[k]) + [D.orthogonalize(c, large[k])]
+        torch.cuda.synchronize()
+    finally:
+        ctx.bind_stream()
+        other.close()
+    for a, b in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
 @pytest.mark.gpu
