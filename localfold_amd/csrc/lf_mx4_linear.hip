@@ -33,7 +33,8 @@ template <int OUT>
 struct MxFour {
   typename Act<OUT>::T v[4];
 };
-template <int OUT, int MT>
+// SOON: the next kernel reads it.
+template <int OUT, int MT, bool SOON = false>
 __device__ __forceinline__ void mx_finish(const f4 (&acc)[4][MT], const MxLinear& p, long long m0, int n0, int r, int g) {
   typedef typename Act<OUT>::T T;
   const int rows = (int)min((long long)16 * MT, p.rows - m0), outputs = p.outputs - n0;
@@ -65,7 +66,10 @@ __device__ __forceinline__ void mx_finish(const f4 (&acc)[4][MT], const MxLinear
           for (int t = 0; t < 4; ++t) Act<OUT>::st(o[q].v + t, p.relu ? __builtin_elementwise_maximum(acc[t][q][j], 0.f) : acc[t][q][j]);
       }
 #pragma unroll
-      for (int q = 0; q < MT; ++q) __builtin_memcpy(ob + (at + (MT * j + q) * row), &o[q], sizeof(o[q]));
+      for (int q = 0; q < MT; ++q) {
+        if constexpr (SOON) __builtin_memcpy(ob + (at + (MT * j + q) * row), &o[q], sizeof(o[q]));
+        else stream_out(ob + (at + (MT * j + q) * row), o[q]);
+      }
     }
     return;
   }
@@ -375,7 +379,7 @@ __global__ __launch_bounds__(128 * WM, 2) void mx4_stream_kernel(MxLinear p, MxS
       o.residual = nullptr;
       o.out = p.partial + (size_t)part * p.rows * p.outputs;
     }
-    mx_finish<OUT, 4>(acc[h], o, m0 + wm * 64, n, r, g);
+    mx_finish<OUT, 4, PART>(acc[h], o, m0 + wm * 64, n, r, g);
   }
 }
 

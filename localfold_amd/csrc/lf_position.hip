@@ -117,7 +117,15 @@ __global__ __launch_bounds__(512, 4) void position_kernel(lf_relative_pairs p, i
 #pragma unroll
           for (int k = 0; k < 8; ++k) a[f][k] += v[k];
         }
-        store8<ACT>(out + first + (size_t)ks[f] * channels + c, channels - c, a[f]);
+        typename Act<ACT>::T* const at = out + first + (size_t)ks[f] * channels + c;
+        if (channels - c >= 8) {
+          uint4 w[sizeof(*at) / 2];
+          pack8<ACT>(a[f], w);
+#pragma unroll
+          for (int k = 0; k < (int)sizeof(*at) / 2; ++k) stream_out(reinterpret_cast<uint4*>(at) + k, w[k]);
+        } else {
+          store8<ACT>(at, channels - c, a[f]);
+        }
       }
     }
   }
