@@ -33,7 +33,8 @@ __global__ __launch_bounds__(256) void mx4_pack_kernel(const typename Act<ACT>::
 struct PackBoth {
   int rows, cols, col_tiles, row_tiles, chunk, blocks;
 };
-template <int ACT>
+// BEYOND: the cache behind the L2s does not hold x, loads pass by it.
+template <int ACT, bool BEYOND>
 __global__ __launch_bounds__(256) void mx4_pack_both_kernel(const typename Act<ACT>::T* x, Mx k, Mx t, float* partial, PackBoth q) {
   typedef typename Act<ACT>::T T;
   constexpr int V = 16 / (int)sizeof(T), LANES = 128 / V, ROWS = 256 / LANES, PASSES = 128 / ROWS;   // as it reads
@@ -53,7 +54,8 @@ __global__ __launch_bounds__(256) void mx4_pack_both_kernel(const typename Act<A
       const T* const at = x + (size_t)r * q.cols + c0 + lc;
       in[i] = u32x4{0, 0, 0, 0};
       if (r < q.rows && left >= V) {
-        __builtin_memcpy(&in[i], at, 16);
+        if constexpr (BEYOND) stream_in(in[i], at);
+        else __builtin_memcpy(&in[i], at, 16);
       } else if (r < q.rows && left > 0) {
         T v[V] = {};
 #pragma unroll
@@ -169,7 +171,7 @@ namespace {
 
 // About 2048 blocks, twice what the chip holds at a time.
 PackBoth pack_both(int rows, int cols) {
-  PackBoth q;
+  PackBoth q{};
   q.rows = rows;
   q.cols = cols;
   q.col_tiles = (int)(LF_MX4_PITCH(cols) / 128);
@@ -189,8 +191,13 @@ void go_pack(const lf_mx4_pack_args& a, float* partial, hipStream_t s) {
     return;
   }
   const PackBoth q = pack_both(a.rows, a.cols);
-  hipLaunchKernelGGL((mx4_pack_both_kernel<ACT>), dim3((q.blocks + 7) / 8 * 8), dim3(256), 0, s, x,
-                     a.out ? mx_view(*a.out) : Mx{}, a.transposed ? mx_view(*a.transposed) : Mx{}, partial, q);
+  // That cache has 256 MB.  403 MB of 196608 rows of 1024 in bf16 (packs and products of a backward pass): 249 us, and 265
+  // with plain loads; 46 MB of 90601 rows of 128 in f32, which it may still hold from the kernel that wrote them: 48 and 44.
+  const bool beyond = (size_t)a.rows * a.cols * act_bytes(a.act_dtype) > (256u << 20);
+  const dim3 grid((q.blocks + 7) / 8 * 8), block(256);
+  const Mx k = a.out ? mx_view(*a.out) : Mx{}, t = a.transposed ? mx_view(*a.transposed) : Mx{};
+  if (beyond) hipLaunchKernelGGL((mx4_pack_both_kernel<ACT, true>), grid, block, 0, s, x, k, t, partial, q);
+  else hipLaunchKernelGGL((mx4_pack_both_kernel<ACT, false>), grid, block, 0, s, x, k, t, partial, q);
 }
 template <int ACT>
 void go_unpack(const lf_mx4_unpack_args& a, hipStream_t s) {

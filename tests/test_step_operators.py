@@ -494,6 +494,26 @@ def test_mx4_pack_of_many_rows(ctx):
 
 
 @pytest.mark.gpu
+def test_mx4_pack_beyond_the_cache(ctx):
+    """307 MB, whose loads pass by the cache: the same codes and bytes as of a part of it, and exact sums of whole numbers."""
+    from localfold_amd import device as D
+    rows, c, part = 600001, 128, 128 * 41
+    x = torch.randint(-7, 8, (rows, c), device=ctx.device, dtype=torch.int32).float()
+    x *= torch.exp2(torch.randint(-3, 4, (rows, 1), device=ctx.device).float())
+    m, t, sums = D.mx4_empty(rows, c, ctx.device), D.mx4_empty(c, rows, ctx.device), torch.empty(c, device=ctx.device)
+    D.mx4_pack(ctx, x, out=m, transposed=t, sums=sums)
+    for r0 in (0, rows // 128 * 128 - 128 * 40):
+        some = x[r0:r0 + part].contiguous()
+        n = some.shape[0]
+        sm, st = D.mx4_empty(n, c, ctx.device), D.mx4_empty(c, n, ctx.device)
+        D.mx4_pack(ctx, some, out=sm, transposed=st)
+        assert torch.equal(m.codes[r0:r0 + n], sm.codes) and torch.equal(m.scales[:, r0:r0 + n], sm.scales[:, :n])
+        assert torch.equal(t.codes[:, r0 // 2:r0 // 2 + st.codes.shape[1]], st.codes)
+        assert torch.equal(t.scales[r0 // 32:r0 // 32 + st.scales.shape[0], :c], st.scales[:, :c])
+    close(sums, f64(x.double().sum(0)), 2 * U * 400 * f64(x.abs().double().sum(0)), torch.float32)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,n,k", [(1, 1, 1), (300, 128, 128), (1000, 64, 130), (5000, 22, 49), (20000, 128, 64), (9000, 300, 70)])
 def test_mx4_weight_gradient(ctx, rows, n, k):
     """The three products and sums of a linear layer's backward pass."""
