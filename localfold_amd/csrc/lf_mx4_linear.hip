@@ -245,18 +245,15 @@ __global__ __launch_bounds__(128 * WM, 2) void mx4_stream_kernel(MxLinear p, MxS
   __shared__ __attribute__((aligned(16))) uint8_t S0[STAGE], S1[STAGE];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   int r = lane & 15, g = lane >> 4, mt, nt, part;
-  if constexpr (PART) {      // the tiles of a part on one XCD, whose L2 then reads that part once
-    const int slot = blockIdx.x >> 3, tiles = q.mtiles * q.ntiles, tile = slot % tiles;
-    part = slot / tiles * 8 + (blockIdx.x & 7);
-    mt = tile % q.mtiles;
-    nt = tile / q.mtiles;
-    if (part >= q.parts) return;
-  } else {                   // blocks on one XCD run through 4 tiles of rows and then the outputs
-    const int slot = blockIdx.x >> 3, turn = slot / (4 * q.ntiles), in = slot % (4 * q.ntiles);
-    mt = (turn * 4 + in % 4) * 8 + (blockIdx.x & 7);
-    nt = in / 4;
-    part = 0;
-    if (mt >= q.mtiles) return;
+  {      // an XCD takes a run of blocks, parts first, then 4 tiles of rows and all outputs, so that its L2 reads little twice
+    const long long tiles = (long long)q.mtiles * q.ntiles, blocks = tiles * q.parts;
+    const long long id = (blockIdx.x & 7) * ((blocks + 7) / 8) + (blockIdx.x >> 3);
+    if (id >= min(blocks, ((blockIdx.x & 7) + 1) * ((blocks + 7) / 8))) return;
+    part = PART ? (int)(id / tiles) : 0;
+    const int tile = (int)(PART ? id % tiles : id), turn = tile / (4 * q.ntiles), in = tile - turn * 4 * q.ntiles;
+    const int tall = min(4, q.mtiles - turn * 4);
+    mt = turn * 4 + in % tall;
+    nt = in / tall;
   }
   const int all = p.steps / 2;             // steps of 256 columns; a last 128 come at the end
   const int s0 = (int)((long long)all * part / q.parts), s1 = (int)((long long)all * (part + 1) / q.parts);
@@ -383,29 +380,50 @@ __global__ __launch_bounds__(128 * WM, 2) void mx4_stream_kernel(MxLinear p, MxS
   }
 }
 
-// The parts' sums in a fixed order, bias, ReLU, residual: P threads share an element.
-template <int OUT, int P>
+// The parts' sums in a fixed order, bias, ReLU, residual: a thread sums V elements in a row, P threads share them.
+template <int OUT, int P, int V>
 __global__ __launch_bounds__(256) void mx4_join_kernel(MxLinear p, int parts) {
   typedef typename Act<OUT>::T T;
-  __shared__ float sm[P][256 / P];
+  typedef float fv __attribute__((ext_vector_type(V), aligned(4)));      // a part begins at any element
+  constexpr int E = 256 / P;
+  __shared__ float sm[P > 1 ? P : 1][P > 1 ? E * V : 1];
   const size_t count = (size_t)p.rows * p.outputs;
-  const int e = threadIdx.x % (256 / P), k0 = threadIdx.x / (256 / P);
-  const size_t i = (size_t)blockIdx.x * (256 / P) + e;
-  float v = 0.f;
-  if (i < count)
-    for (int k = parts * k0 / P; k < parts * (k0 + 1) / P; ++k) v += p.partial[k * count + i];
+  const int e = threadIdx.x % E, k0 = threadIdx.x / E;
+  const size_t i = ((size_t)blockIdx.x * E + e) * V;
+  float v[V] = {};
+  const int first = parts * k0 / P, end = parts * (k0 + 1) / P;
+  if (i + V <= count) {
+#pragma unroll 4
+    for (int k = first; k < end; ++k) {
+      const fv t = *reinterpret_cast<const fv*>(p.partial + k * count + i);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] += t[j];
+    }
+  } else {
+    for (int k = first; k < end; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (i + j < count) v[j] += p.partial[k * count + i + j];
+  }
   if constexpr (P > 1) {
-    sm[k0][e] = v;
+#pragma unroll
+    for (int j = 0; j < V; ++j) sm[k0][j * E + e] = v[j];
     __syncthreads();
     if (k0 > 0) return;
 #pragma unroll
-    for (int k = 1; k < P; ++k) v += sm[k][e];
+    for (int k = 1; k < P; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] += sm[k][j * E + e];
   }
-  if (i >= count) return;
-  if (p.bias) v += p.bias[i % p.outputs];
-  if (p.relu) v = __builtin_elementwise_maximum(v, 0.f);
-  if (p.residual) v += Act<OUT>::ld(static_cast<const T*>(p.residual) + i);
-  Act<OUT>::st(static_cast<T*>(p.out) + i, v);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (i + j >= count) return;
+    float s = v[j];
+    if (p.bias) s += p.bias[(i + j) % p.outputs];
+    if (p.relu) s = __builtin_elementwise_maximum(s, 0.f);
+    if (p.residual) s += Act<OUT>::ld(static_cast<const T*>(p.residual) + i + j);
+    Act<OUT>::st(static_cast<T*>(p.out) + i + j, s);
+  }
 }
 
 // ---- few rows or outputs -----------------------------------------------------------------------------
@@ -479,19 +497,28 @@ struct MxPlan {
   bool wide;                 // STREAM: 256 x 256 tiles, else 128 x 128
   int parts;
 };
-constexpr int CUS = 256, FEW_TILES = 1500, FEW_STEPS = 64;
+constexpr int CUS = 256;
 
 constexpr int set_bytes(int steps) { return steps * (4096 + 256) + 256; }
 
 MxPlan mx_plan(long long rows, int steps, long long outputs) {
+  // Few: in runs of 32 rows by 16 outputs the times cross at 2300 for one step (128 x 512 in bf16: 1500 runs 8.1 us and 10.5
+  // resident, 3000 12.6 and 11.0), near 1100 for more (512 x 128: 700 9.2 and 12.2, 1500 16.6 and 12.3; 1024 x 256: 700 15
+  // and 22, 1500 28 and 22), and near 400 for streamed ones (1024 x 1024: 300 6.9 and 8.5, 700 15 and 8.7; 4096 x 4096: 300
+  // 11.5 and 12.5, 700 22 and 13.5).  Past 8192 columns the parts of a streamed product share them.
+  const bool resident = steps <= 4 || (steps <= 8 && (outputs + 63) / 64 * set_bytes(steps) <= LDS_BYTES);
   const long long few = (rows + 31) / 32 * ((outputs + 15) / 16);
-  if (few <= FEW_TILES && steps <= FEW_STEPS) return {FEW, false, 1};
-  if (steps <= 4 || (steps <= 8 && (outputs + 63) / 64 * set_bytes(steps) <= LDS_BYTES)) return {RESIDENT, false, 1};
+  if (few <= (steps == 1 ? 2300 : resident ? 1100 : 400) && steps <= 64) return {FEW, false, 1};
+  if (resident) return {RESIDENT, false, 1};
   const long long wide = (rows + 255) / 256 * ((outputs + 255) / 256);
-  if (wide >= CUS / 2) return {STREAM, true, 1};
+  if (wide >= 128) return {STREAM, true, 1};
+  // P parts take 0.34 / P us a step of 128 columns and 0.044 P us a tile for their sums' way through memory, so that
+  // sqrt(8 steps / tiles) is best: 128 x 128 outputs of 147456 columns take 359 us in one part, 23 in 16, 13 in 64, 14 in
+  // 128; 256 x 512 of them 388, 34, 26, 37; 480 x 1024 of 24576 columns 67 in one, 25 in 4, 23 in 8, 24 in 16.  A part has
+  // 1024 columns at least.
   const long long tiles = (rows + 127) / 128 * ((outputs + 127) / 128);
-  // a part of 1024 columns at least
-  const int parts = (int)std::max<long long>(1, std::min<long long>(2 * CUS / tiles, steps / 8));
+  int parts = 1;
+  while (parts < 64 && parts < steps / 8 && (parts + 1LL) * (parts + 1) * tiles <= 8LL * steps) ++parts;
   return {STREAM, false, parts};
 }
 
@@ -501,14 +528,15 @@ template <int OUT, int NT, int WM, bool PART>
 void go_stream(lf_context* ctx, const MxLinear& p, int parts) {
   constexpr int BM = WM * 64, BN = 2 * NT * 16;
   MxStream q{(int)(((long long)p.rows + BM - 1) / BM), (p.outputs + BN - 1) / BN, parts};
-  const long long blocks = PART ? (parts + 7LL) / 8 * 8 * q.mtiles * q.ntiles : (q.mtiles + 31LL) / 32 * 32 * q.ntiles;
+  const long long blocks = ((long long)q.mtiles * q.ntiles * parts + 7) / 8 * 8;
   hipLaunchKernelGGL((mx4_stream_kernel<OUT, NT, WM, PART>), dim3((unsigned)blocks), dim3(128 * WM), 0, ctx->stream, p, q);
 }
 
 template <int OUT, int P>
 void go_join(lf_context* ctx, const MxLinear& p, int parts) {
-  const size_t count = (size_t)p.rows * p.outputs, each = 256 / P;
-  hipLaunchKernelGGL((mx4_join_kernel<OUT, P>), dim3((unsigned)((count + each - 1) / each)), dim3(256), 0, ctx->stream, p, parts);
+  constexpr int V = 4;
+  const size_t count = (size_t)p.rows * p.outputs, each = 256 / P * V;
+  hipLaunchKernelGGL((mx4_join_kernel<OUT, P, V>), dim3((unsigned)((count + each - 1) / each)), dim3(256), 0, ctx->stream, p, parts);
 }
 
 template <int SRC, int OUT, int STEPS>
@@ -567,7 +595,8 @@ int go(lf_context* ctx, const MxLinear& p, const MxPlan& plan, int act_dtype) {
   if (plan.parts == 1) return LF_OK;
   LaunchScope ls(ctx, "mx4.join");
   if (plan.parts > 16) go_join<OUT, 16>(ctx, p, plan.parts);
-  else go_join<OUT, 4>(ctx, p, plan.parts);
+  else if (plan.parts > 4) go_join<OUT, 4>(ctx, p, plan.parts);
+  else go_join<OUT, 1>(ctx, p, plan.parts);
   return check_hip(hipGetLastError(), "4-bit join launch");
 }
 
