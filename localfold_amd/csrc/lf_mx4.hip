@@ -7,7 +7,7 @@ namespace lf {
 
 // ---- pack and unpack: bound by memory ------------------------------------------------------------
 
-// Four lanes pack a group of a row, 8 columns each.
+// Four lanes pack a group of a row, 8 columns each.  8192 rows of 4096 in bf16: 16 us, 5.4 TB/s.
 template <int ACT>
 __global__ __launch_bounds__(256) void mx4_pack_kernel(const typename Act<ACT>::T* x, Mx k) {
   const long long item = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -29,7 +29,7 @@ __global__ __launch_bounds__(256) void mx4_pack_kernel(const typename Act<ACT>::
 // columns (k.codes, if given) and along the rows (t.codes, if given), a group a thread, and adds up its rows (partial
 // [chunks][cols], if given).  Four neighbouring lanes write 64 bytes (where every lane wrote 16 of another line, what both
 // wrote of 196608 rows of 1024 in bf16 took 120 us beside the 82 of reading).  Blocks of neighbouring columns share an XCD,
-// and a block keeps its columns: halves of lines meet in one L2.
+// and a block keeps its columns: halves of lines meet in one L2.  Those packs take 113 us, 5.4 TB/s.
 struct PackBoth {
   int rows, cols, col_tiles, row_tiles, chunk, blocks;
 };
