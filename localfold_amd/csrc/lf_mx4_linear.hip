@@ -250,7 +250,7 @@ __global__ __launch_bounds__(128 * WM, 2) void mx4_stream_kernel(MxLinear p, MxS
   {      // an XCD takes a run of blocks, parts first, then 4 tiles of rows and all outputs, so that its L2 reads little twice
     const long long tiles = (long long)q.mtiles * q.ntiles, blocks = tiles * q.parts;
     const long long id = (blockIdx.x & 7) * ((blocks + 7) / 8) + (blockIdx.x >> 3);
-    if (id >= min(blocks, ((blockIdx.x & 7) + 1) * ((blocks + 7) / 8))) return;
+    if (id >= blocks) return;
     part = PART ? (int)(id / tiles) : 0;
     const int tile = (int)(PART ? id % tiles : id), turn = tile / (4 * q.ntiles), in = tile - turn * 4 * q.ntiles;
     const int tall = min(4, q.mtiles - turn * 4);

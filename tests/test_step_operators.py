@@ -469,12 +469,14 @@ def test_mx4_linear(ctx, dt, rows, k, n):
 # Products of more outputs than one block a run of them takes: weights resident for 1, 2, 4 and 8 steps of 128 columns and
 # 8 that do not fit, both sizes of streamed tiles, whole and ragged, odd numbers of steps.
 MANY = [(3001, 100, 300), (3001, 200, 300), (3001, 500, 300), (3001, 1000, 300), (3040, 1024, 320), (2000, 900, 1500),
-        (4000, 1100, 1100), (8200, 1100, 1000), (8192, 640, 1024)]
+        (4000, 1100, 1100), (8200, 1100, 1000), (8192, 640, 1024), (5001, 100, 300)]
+# Sums over 3, 2, 8, 11 and 19 parts, tiles that do not divide by the XCDs, numbers of outputs that do not divide by 4.
+SPLIT = [(601, 4096, 523), (901, 4000, 701), (200, 9000, 203), (129, 12500, 261), (301, 20000, 71)]
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", TYPES)
-@pytest.mark.parametrize("rows,k,n", MANY)
+@pytest.mark.parametrize("rows,k,n", MANY + SPLIT)
 def test_mx4_linear_many(ctx, dt, rows, k, n):
     test_mx4_linear(ctx, dt, rows, k, n)
 
