@@ -349,7 +349,7 @@ int go_position(const lf_relative_position_args& a, hipStream_t s) {
   PositionTiles q;
   // few pairs: small tiles, so that they fill the chip
   q.tile = pairs >= 256 * 512 ? 256 : pairs >= 64 * 512 ? 64 : 16;
-  q.tiles = (a.pairs->keys + q.tile - 1) / q.tile;
+  q.tiles = (int)(((long long)a.pairs->keys + q.tile - 1) / q.tile);     // 2^31 - 1 keys rounded up are more than an int
   q.count = (long long)a.pairs->queries * q.tiles;
   q.rows = LF_RELATIVE_ROWS(a.pairs);
   const size_t marks = a.pairs->boundary_count * sizeof(int), table = (size_t)q.rows * ((a.channels + 7) / 8 * 8) * sizeof(float);
@@ -386,7 +386,7 @@ PositionPlan position_plan(int queries, int keys, int channels, int rows) {
   p.team = channels > 64 ? 64 : channels > 32 ? 32 : channels > 16 ? 16 : 8;
   p.slices = (channels + 2 * p.team - 1) / (2 * p.team);
   const int unit = position_keys(p.team);
-  p.chunks = (keys + unit - 1) / unit;
+  p.chunks = (int)(((long long)keys + unit - 1) / unit);
   p.units = (long long)queries * p.chunks;
   // a wave's rows in LDS: 64 lanes of two sums each
   const int budget = (LDS_BYTES - rows * 4) / 512;

@@ -180,6 +180,15 @@ def test_scratch_sizes_and_null_need_no_device():
         assert getattr(lib, name)(None, None) == capi.LF_ERR_INVALID and name.encode() in lib.lf_last_error()
 
 
+def test_scratch_of_the_most_keys():
+    """256 blocks at most leave partial sums, also of 2^31 - 1 keys, which rounded up to whole units are more."""
+    from localfold_amd import capi
+    lib = capi.load()
+    for q, k in ((1, 2 ** 31 - 1), (1, 2 ** 31 - 200), (8, 2 ** 31 - 1), (2 ** 31 - 1, 1)):
+        pairs = capi.lf_relative_pairs(q, k, None, None, None, None, 1, None)
+        assert lib.lf_relative_position_backward_scratch(C.byref(pairs), 1) == 256 * 3 * 4, (q, k)
+
+
 def test_coefficients_are_checked():
     from localfold_amd import device as D
     assert list(D._coefficients((1, 2, 3), 2)) == [1, 2, 3, 1, 2, 3]
@@ -301,6 +310,26 @@ def test_position_far_apart_and_odd_boundaries(ctx):
         grad = torch.ones((7, 7, 1), device=ctx.device)
         dt = D.relative_position_backward(ctx, grad, on(ctx, b), on(ctx, p))
         assert (f64(dt)[:, 0] == np.bincount(row.ravel(), minlength=len(b) + 1)).all(), b
+
+
+@pytest.mark.gpu
+def test_position_of_the_most_keys(ctx):
+    """2^31 - 1 keys of a query, one channel: both ends of the keys and of the buckets."""
+    from localfold_amd import device as D
+    k, half = 2 ** 31 - 1, 2 ** 30
+    kp = torch.arange(k, dtype=torch.int32, device=ctx.device)
+    qp = torch.tensor([half], dtype=torch.int32, device=ctx.device)
+    b = torch.tensor([1, half], dtype=torch.int32, device=ctx.device)       # keys past `half`, those before it, key 0
+    table = torch.tensor([[1.0], [2.0], [3.0]], device=ctx.device)
+    out = torch.zeros((1, k, 1), dtype=torch.bfloat16, device=ctx.device)
+    D.relative_position(ctx, table, b, qp, key_positions=kp, out=out)
+    flat = out.view(-1)
+    assert float(flat[0]) == 3 and bool((flat[1:half] == 2).all()) and bool((flat[half:] == 1).all())
+    out.zero_()
+    flat[:5], flat[half - 3:half + 4], flat[k - 6:] = 8, 1, 0.5             # few enough that every sum is exact
+    db = torch.empty(1, device=ctx.device)
+    got = D.relative_position_backward(ctx, out, b, qp, key_positions=kp, bias_grad=db)
+    assert got[:, 0].tolist() == [4 + 3.0, 32 + 3.0, 8.0] and float(db) == 50
 
 
 @pytest.mark.gpu
