@@ -1095,13 +1095,16 @@ def log_boundaries(buckets: int, max_distance: int, device="cpu") -> torch.Tenso
     to buckets / 4, then ratios that stay the same up to max_distance, where the last bucket begins."""
     half = buckets // 2
     near = max(1, half // 2)
-    if buckets < 4 or buckets % 2 or max_distance < near:
-        raise ValueError(f"buckets must be even and 4 at least, max_distance {near} at least; got {buckets}, {max_distance}")
+    if buckets < 4 or buckets % 2 or not near <= max_distance < 2 ** 31:
+        raise ValueError(f"buckets must be even and 4 at least, max_distance {near} to 2^31 - 1; got {buckets}, {max_distance}")
     steps = list(range(1, near + 1))
-    n = near
-    for j in range(1, half - near + 1):     # the first n >= near (max_distance / near)^(j / (half - near)), in whole numbers
-        while n ** (half - near) < near ** (half - near - j) * max_distance ** j:
+    k = half - near
+    for j in range(1, k + 1):     # the first n >= near (max_distance / near)^(j / k): about there, then in whole numbers
+        n, least = round(near * (max_distance / near) ** (j / k)), near ** (k - j) * max_distance ** j
+        while n ** k < least:
             n += 1
+        while (n - 1) ** k >= least:
+            n -= 1
         steps.append(n)
     return torch.tensor([1 - s for s in reversed(steps[1:])] + steps, dtype=torch.int32, device=device)
 

@@ -135,6 +135,22 @@ def test_boundaries():
         D.clipped_boundaries(0)
 
 
+def test_log_boundaries_of_far_distances():
+    """Up to what positions can differ by, at once; past what an int32 holds is refused."""
+    from localfold_amd import device as D
+    for buckets, far in ((32, 10 ** 6), (64, 2 ** 31 - 1), (4096, 2 ** 31 - 1)):
+        b = D.log_boundaries(buckets, far)
+        half, near = buckets // 2, buckets // 4
+        steps = [int(v) for v in b[half - 1:]]
+        assert b.dtype == torch.int32 and len(b) == buckets - 1 and steps[:near] == list(range(1, near + 1)) and steps[-1] == far
+        for j in (1, 2, (half - near) // 2, half - near - 1):        # the first whole number at (far / near)^(j / half - near) near
+            n, k = steps[near - 1 + j], half - near
+            assert (n - 1) ** k < near ** (k - j) * far ** j <= n ** k, (buckets, far, j)
+    for far in (2 ** 31, 10 ** 30):
+        with pytest.raises(ValueError, match="max_distance"):
+            D.log_boundaries(32, far)
+
+
 def test_struct_layouts(tmp_path):
     from localfold_amd import capi
     names = [n for n in dir(capi) if n.startswith(("lf_relative", "lf_mx4", "lf_orthogonalize", "lf_muon"))
