@@ -180,6 +180,7 @@ int muon_step(lf_context* ctx, const lf_muon_step_args& a) {
   m.out = a.weight_out;
   m.keep = (float)(1.0 - (double)a.rate * a.decay);
   m.rate = (float)((double)a.rate * a.scale);
+  LF_REQUIRE(std::isfinite(m.keep) && std::isfinite(m.rate), "lf_muon_step: 1 - rate decay and rate scale must be finite in f32");
   m.steps = a.steps;
   m.coefficients = a.coefficients;
   m.epsilon = a.epsilon;

@@ -1012,3 +1012,17 @@ def test_refusals(ctx):
     o = capi.lf_orthogonalize_args(1, 4, 4, 0, t.data_ptr(), t.data_ptr(), 5, None, 1e-7)
     assert lib.lf_orthogonalize(h, C.byref(o)) == capi.LF_ERR_INVALID and b"coefficients" in lib.lf_last_error()
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_muon_step_refuses_factors_past_f32(ctx):
+    """rate scale and 1 - rate decay are what the kernels multiply with: as infinities they would make NaN of zeros."""
+    from localfold_amd import capi, device as D
+    t = torch.zeros(4, 4, device=ctx.device)
+    w = torch.ones(4, 4, device=ctx.device)
+    for args in (dict(rate=1e30, scale=1e30), dict(rate=-1e20, scale=1e20), dict(rate=1e30, decay=1e30)):
+        with pytest.raises(capi.LocalfoldError, match="finite"):
+            D.muon_step(ctx, w, t, **args)
+    assert (w == 1).all()
+    D.muon_step(ctx, w, t, rate=1e30, decay=-1e-30, scale=1e8)
+    assert (w == 2).all()
