@@ -3,9 +3,13 @@
 Tolerances.  U = 2^-24 is half a step of float32; a sum whose terms pass through at most D additions is off by
 at most D * 2U times the sum of magnitudes (2U: an addition may cut instead of round).  A stored value adds half a
 step of its type, relative to it."""
+import ast
 import ctypes as C
+import glob
+import inspect
 import math
 import os
+import re
 import subprocess
 
 import numpy as np
@@ -149,6 +153,38 @@ def test_log_boundaries_of_far_distances():
     for far in (2 ** 31, 10 ** 30):
         with pytest.raises(ValueError, match="max_distance"):
             D.log_boundaries(32, far)
+
+
+def documented_examples():
+    """The Python examples of the documents beside the package that call its device module, as (document, code)."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    for path in sorted(glob.glob(os.path.join(root, "*.md"))):
+        with open(path, encoding="utf-8") as f:
+            for code in re.findall(r"^```python\n(.*?)^```", f.read(), re.S | re.M):
+                if "device as D" in code:
+                    yield os.path.basename(path), code
+
+
+def test_documented_calls():
+    """Every call of an example has the function's arguments, and what it takes apart is a tuple of as many."""
+    from localfold_amd import device as D
+
+    def returned(f):
+        return [n.value for n in ast.walk(ast.parse(inspect.getsource(f))) if isinstance(n, ast.Return)]
+
+    seen = set()
+    for where, code in documented_examples():
+        tree = ast.parse(code)
+        for call in (n for n in ast.walk(tree) if isinstance(n, ast.Call)):
+            if isinstance(call.func, ast.Attribute) and isinstance(call.func.value, ast.Name) and call.func.value.id == "D":
+                seen.add(call.func.attr)
+                f = getattr(D, call.func.attr)
+                inspect.signature(f).bind(*call.args, **{k.arg: k.value for k in call.keywords})
+        for n in ast.walk(tree):
+            if isinstance(n, ast.Assign) and isinstance(n.targets[0], ast.Tuple) and isinstance(n.value, ast.Call):
+                f = getattr(D, n.value.func.attr)
+                assert all(isinstance(v, ast.Tuple) and len(v.elts) == len(n.targets[0].elts) for v in returned(f)), (where, ast.unparse(n))
+    assert {"relative_position", "relative_position_backward", "mx4_pack", "mx4_linear", "muon_step"} <= seen
 
 
 def test_struct_layouts(tmp_path):
@@ -1026,3 +1062,31 @@ def test_muon_step_refuses_factors_past_f32(ctx):
     assert (w == 1).all()
     D.muon_step(ctx, w, t, rate=1e30, decay=-1e-30, scale=1e8)
     assert (w == 2).all()
+
+@pytest.mark.gpu
+def test_documented_step_runs(ctx):
+    """The example of these operators, as it stands, on tensors of the names that it uses."""
+    rng = np.random.default_rng(11)
+    n, c, outputs = 24, 40, 72
+    rows = n * n
+    t = lambda *shape: torch.as_tensor(rng.normal(size=shape)).float().to(ctx.device)
+    from localfold_amd import device as D
+    chains = (torch.arange(n, device=ctx.device) > 9).to(torch.int32)
+    v = dict(table=t(66, c), positions=torch.arange(n, dtype=torch.int32, device=ctx.device), chains=chains, bias=t(c),
+             weight=t(outputs, c), b=t(outputs), rows=rows, outputs=outputs, dout=t(rows, outputs), db=t(outputs), dpair=t(n, n, c),
+             dbias=t(c), momentum=torch.zeros(outputs, c, device=ctx.device))
+    v["wt"], v["xt"] = D.mx4_empty(c, outputs, ctx.device), D.mx4_empty(c, rows, ctx.device)
+    D.mx4_pack(ctx, v["weight"], transposed=v["wt"])
+    D.mx4_pack(ctx, t(rows, c), transposed=v["xt"])
+    (code,) = [code for _, code in documented_examples() if "muon_step" in code]
+    exec(code, v)
+    torch.cuda.synchronize()
+    v["ctx"].close()
+    p, s = np.arange(n, dtype=np.int32), chains.cpu().numpy()
+    row = rows64(np.arange(-31, 33), p, p, s, s)
+    want, mags = np.zeros((66, c)), np.zeros((66, c))
+    np.add.at(want, row.ravel(), f64(v["dpair"]).reshape(-1, c))
+    np.add.at(mags, row.ravel(), np.abs(f64(v["dpair"])).reshape(-1, c))
+    close(v["dtable"], want, 2 * U * rows * mags, torch.float32)
+    close(v["dbias"], want.sum(0), 2 * U * rows * mags.sum(0), torch.float32)
+    assert v["pair"].shape == (n, n, c) and v["out"].shape == (n, n, outputs) and torch.equal(v["momentum"], v["dw"])
