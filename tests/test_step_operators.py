@@ -1090,3 +1090,104 @@ def test_documented_step_runs(ctx):
     close(v["dtable"], want, 2 * U * rows * mags, torch.float32)
     close(v["dbias"], want.sum(0), 2 * U * rows * mags.sum(0), torch.float32)
     assert v["pair"].shape == (n, n, c) and v["out"].shape == (n, n, outputs) and torch.equal(v["momentum"], v["dw"])
+
+
+# Where a block does not take a whole matrix, momentum and weights pass through other kernels: blocks of 128 columns (smaller
+# side 65 to 128), wide, tall and of odd widths; products of tiles of 64 and of 128 (40 matrices), tall with whole and cut
+# groups of four rows, narrow.
+STEPS = [(2, 128, 512), (3, 300, 70), (1, 101, 257), (2, 1001, 66), (1, 200, 300), (1, 301, 150), (2, 16, 700), (40, 390, 260), (1, 1500, 9)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wdt,gdt", [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float16, torch.float16)])
+@pytest.mark.parametrize("nesterov", [False, True])
+@pytest.mark.parametrize("batch,rows,cols", STEPS)
+def test_muon_step_of_larger_matrices(ctx, batch, rows, cols, wdt, gdt, nesterov):
+    from localfold_amd import device as D
+    rng = np.random.default_rng(rows * 1000 + cols)
+    shape = batch, rows, cols
+    g, w = gradients(rng, shape, gdt).to(ctx.device), torch.as_tensor(rng.normal(size=shape)).to(wdt).to(ctx.device)
+    m = gradients(rng, shape, torch.float32).to(ctx.device)
+    rate, decay, mu, scale = 0.25, 0.125, 0.9375, 3.0                   # exact in every type
+    args = dict(rate=rate, decay=decay, momentum_factor=mu, nesterov=nesterov, scale=scale)
+    for momentum in (m, None):
+        out, mo = torch.empty_like(w), None if momentum is None else torch.empty_like(m)
+        kept = [t.clone() for t in (w, g, m)]
+        D.muon_step(ctx, w, g, momentum, out=out, momentum_out=mo, **args)
+        assert all(torch.equal(a, b) for a, b in zip((w, g, m), kept))  # none of the inputs is written
+        m64 = f64(g) if momentum is None else mu * f64(m) + f64(g)
+        if momentum is not None:
+            close(mo, m64, 4 * U * (np.abs(f64(m)) + np.abs(f64(g))), torch.float32, "momentum")
+        u = m64 if momentum is None or not nesterov else f64(g) + mu * m64
+        for b in sorted({0, batch // 2, batch - 1}):
+            o, bound = schulz64(u[b], 5)
+            want = (1 - rate * decay) * f64(w[b]) - rate * scale * o
+            # u itself is off by a few U, which the steps' growth (4 a step at most) carries on
+            bound += 8 * U * 4.0 ** 5
+            store = (HALF[wdt] + 3 * U) * (np.linalg.norm(f64(w[b])) + rate * scale * (np.linalg.norm(o) + bound))
+            assert np.linalg.norm(f64(out[b]) - want) <= rate * scale * bound + store, b
+        w2, m2 = w.clone(), None if momentum is None else m.clone()
+        assert D.muon_step(ctx, w2, g, m2, **args) is w2
+        assert torch.equal(w2, out) and (momentum is None or torch.equal(m2, mo))
+
+
+@pytest.mark.gpu
+def test_muon_step_in_place_in_graphs(ctx):
+    """Steps in place of both kinds that use scratch, captured with scratch of their own and replayed in turn, with eager
+    ones between that move the context's workspace."""
+    from localfold_amd import device as D
+    rng = np.random.default_rng(12)
+    cases = []
+    for shape in ((3, 128, 512), (2, 300, 200)):
+        w, m = torch.as_tensor(rng.normal(size=shape)).float().to(ctx.device), torch.zeros(shape, device=ctx.device)
+        g = gradients(rng, shape, torch.float32).to(ctx.device)
+        scratch = torch.empty(ctx.lib.lf_muon_scratch(*shape), dtype=torch.uint8, device=ctx.device)
+        D.muon_step(ctx, w, g, m, decay=0.1, scratch=scratch)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        try:
+            with torch.cuda.graph(graph):
+                ctx.bind_stream()
+                D.muon_step(ctx, w, g, m, decay=0.1, scratch=scratch)
+        finally:
+            ctx.bind_stream()
+        cases.append((graph, w, g, m, w.clone(), m.clone(), scratch))
+    for turn in range(4):
+        for graph, w, g, m, w2, m2, _ in cases:
+            g *= -0.75
+            graph.replay()
+            torch.cuda.synchronize()
+            D.orthogonalize(ctx, torch.randn(4 * (turn + 1), 200, 256, device=ctx.device))
+            D.muon_step(ctx, w2, g, m2, decay=0.1)
+            torch.cuda.synchronize()
+            assert torch.equal(w, w2) and torch.equal(m, m2), turn
+
+
+@pytest.mark.gpu
+def test_muon_steps_of_two_contexts_at_once(ctx):
+    from localfold_amd import device as D
+    other = D.Context(0)
+    streams = [torch.cuda.Stream(ctx.device) for _ in range(2)]
+    shapes = ((3, 128, 512), (2, 300, 200))
+    state = [[(torch.as_tensor(rng.normal(size=s)).float().to(ctx.device), gradients(rng, s, torch.float32).to(ctx.device),
+               torch.zeros(s, device=ctx.device)) for s in shapes] for rng in (np.random.default_rng(k) for k in (13, 14))]
+    want = [[[t.clone() for t in part] for part in s] for s in state]
+    for s in want:
+        for _ in range(4):
+            for w, g, m in s:
+                D.muon_step(ctx, w, g, m, decay=0.1)
+    torch.cuda.synchronize()
+    try:
+        for c, s in zip((ctx, other), streams):
+            c.bind_stream(s)
+        for _ in range(4):
+            for k, c in enumerate((ctx, other)):
+                with torch.cuda.stream(streams[k]):
+                    for w, g, m in state[k]:
+                        D.muon_step(c, w, g, m, decay=0.1)
+        torch.cuda.synchronize()
+    finally:
+        ctx.bind_stream()
+        other.close()
+    for a, b in zip(state, want):
+        assert all(torch.equal(p, q) for x, y in zip(a, b) for p, q in zip(x, y))
