@@ -1191,3 +1191,70 @@ def test_muon_steps_of_two_contexts_at_once(ctx):
         other.close()
     for a, b in zip(state, want):
         assert all(torch.equal(p, q) for x, y in zip(a, b) for p, q in zip(x, y))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("q,k,c,reach", [(3, 5, 4096, 2), (2, 40, 2051, 4), (70, 60, 2304, 1)])
+def test_position_of_wide_rows(ctx, q, k, c, reach, dt):
+    """Rows of more chunks of channels than a block has threads, and of 32 slices of channels in the gradient."""
+    for segments in (False, True):
+        test_position(ctx, q, k, c, reach, dt, segments)
+        test_position_backward(ctx, q, k, c, reach, dt, segments)
+
+
+def edges(dt):
+    """Rows of 64 at the edges of a type: ties of every code and their neighbours, subnormals, the largest values."""
+    big, small = torch.finfo(dt).max, torch.finfo(dt).smallest_normal * torch.finfo(dt).eps      # the smallest subnormal
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0], dtype=dt)
+    v = torch.zeros(12, 64, dtype=dt)
+    for r, size in enumerate((1.0, 2.0 ** -10, 2.0 ** 10)):
+        v[r, :8], v[r, 8:16], v[r, 32:40], v[r, 40:48] = (t * size for t in (ties, -ties, torch.nextafter(ties, ties * 0), -torch.nextafter(ties, ties * 0)))
+    k = torch.arange(1, 65).double() * small
+    v[3], v[4], v[5] = k.to(dt), -(k * 7).to(dt), (k.flip(0) * 31).to(dt)
+    v[6, 0], v[6, 1], v[6, 32] = big, -big / 4, -big
+    v[7] = small
+    v[8, ::2] = torch.finfo(dt).smallest_normal
+    v[8, 1::2] = -3 * small
+    v[9, 5], v[9, 40] = math.inf, 1.0
+    v[10, 63], v[10, 0] = math.nan, -1.0
+    v[11] = -0.0
+    return v
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+def test_mx4_edges_of_every_type(ctx, dt):
+    """The same codes and bytes whichever way a matrix is packed, and products of them whether packed before or inside."""
+    from localfold_amd import device as D
+    v = edges(dt)
+    x, want = v.to(ctx.device), mx64(f64(v))
+    out, tr, alone = D.mx4_empty(12, 64, ctx.device), D.mx4_empty(12, 64, ctx.device), D.mx4_pack(ctx, x)
+    D.mx4_pack(ctx, x, out=out, transposed=D.mx4_empty(64, 12, ctx.device))
+    D.mx4_pack(ctx, x.t().contiguous(), transposed=tr)
+    for name, m in (("alone", alone), ("both", out), ("transposed", tr)):
+        got = values_of(m)[0][:, :64]
+        assert np.array_equal(got, want, equal_nan=True), (name, np.argwhere(~((got == want) | np.isnan(want)))[:6].tolist())
+    eye = torch.zeros(64, 64, device=ctx.device).fill_diagonal_(1.0)
+    w = D.mx4_pack(ctx, eye)
+    for rows in (12, 24, 12 * 3000):                 # few rows, two tiles of them, weights resident
+        many = x.repeat(rows // 12, 1)
+        got = f64(D.mx4_linear(ctx, many, w, dtype=torch.float32))
+        with np.errstate(over="ignore"):
+            # 0 times NaN is NaN: a group that holds one makes its whole row so
+            full = np.where(np.isnan(want).any(1, keepdims=True), np.nan, want).astype(np.float32)
+        assert np.array_equal(got[:12], full, equal_nan=True), (rows, np.argwhere(~((got[:12] == full) | np.isnan(full)))[:6].tolist())
+        assert np.array_equal(got, np.tile(got[:12], (rows // 12, 1)), equal_nan=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,n", [(3, 200, 40), (100, 200, 100), (6000, 200, 100), (600, 4096, 530), (8192, 640, 1024)])
+def test_mx4_linear_far_exponents(ctx, rows, k, n):
+    """Operands times powers of two that cancel or carry the product far: the same bits, shifted."""
+    from localfold_amd import device as D
+    rng = np.random.default_rng(rows + k)
+    x, w = stream(rng, rows, k, torch.float32).to(ctx.device), stream(rng, n, k, torch.float32).to(ctx.device)
+    base = D.mx4_linear(ctx, x, D.mx4_pack(ctx, w), dtype=torch.float32)
+    for a, b in ((100, -100), (-100, 100), (110, -20), (-20, 110), (-40, -40), (40, 40), (-110, 120)):
+        got = D.mx4_linear(ctx, x * 2.0 ** a, D.mx4_pack(ctx, w * 2.0 ** b), dtype=torch.float32)
+        assert torch.equal(got, base * 2.0 ** (a + b)), (a, b)
