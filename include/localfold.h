@@ -779,7 +779,9 @@ size_t lf_mx4_linear_scratch(int rows, int inputs, int outputs, int from_act);  
  * Frobenius norm, and (a, b, c) a step's coefficients, X <- a X + (b G + c G^2) X, G = X X^T, `steps`
  * times (for matrices taller than wide the same of the transpose).  Singular values go through
  * a s + b s^3 + c s^5 each time, vectors stay.  Products are of f32 precision (two f16 parts each, sums in
- * f32).  Coefficients whose polynomials leave 2^24 on what [0, 1] can become are refused. */
+ * f32).  The two parts hold an element to 2^-38 of the largest singular value that X can have, so that a
+ * matrix whose norm is far below epsilon keeps fewer bits of its result, which is small then, and at last
+ * none.  Coefficients whose polynomials leave 2^24 on what [0, 1] can become are refused. */
 typedef struct {
   int batch, rows, cols;       /* rows, cols 1..16384, batch 1..65535 */
   int act_dtype;

@@ -1293,7 +1293,8 @@ def _coefficients(coefficients, steps: int):
 def orthogonalize(ctx: Context, x: torch.Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ, epsilon: float = 1e-7,
                   out: torch.Tensor = None, scratch: torch.Tensor = None) -> torch.Tensor:
     """Each matrix of x [..., rows, cols] made orthogonal by `steps` Newton-Schulz products (lf_orthogonalize);
-    `coefficients`: (a, b, c), or one such triple a step.  `out` may be x."""
+    `coefficients`: (a, b, c), or one such triple a step.  `out` may be x.  A matrix whose norm is far below epsilon keeps
+    fewer bits of its small result."""
     if out is None:
         out = torch.empty_like(x)
     a = capi.lf_orthogonalize_args()

@@ -1258,3 +1258,20 @@ def test_mx4_linear_far_exponents(ctx, rows, k, n):
     for a, b in ((100, -100), (-100, 100), (110, -20), (-20, 110), (-40, -40), (40, 40), (-110, 120)):
         got = D.mx4_linear(ctx, x * 2.0 ** a, D.mx4_pack(ctx, w * 2.0 ** b), dtype=torch.float32)
         assert torch.equal(got, base * 2.0 ** (a + b)), (a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,rows,cols", [(2, 40, 70), (2, 128, 512), (1, 300, 200)])
+def test_orthogonalize_far_below_epsilon(ctx, batch, rows, cols):
+    """A norm far below epsilon: elements are kept to 2^-38 at the start and after each step, whatever the norm, and a
+    difference grows by a = 3.4445 a step at most; beside that f32's relative errors, a 2^-20 a step with the roundings of P."""
+    from localfold_amd import device as D
+    u = np.random.default_rng(rows).normal(size=(batch, rows, cols))
+    u /= np.linalg.norm(u, axis=(1, 2), keepdims=True)
+    for size in (2.0 ** -8, 2.0 ** -20, 2.0 ** -45):
+        x = torch.as_tensor(u * EPS * size).float()
+        got = D.orthogonalize(ctx, x.to(ctx.device))
+        for b in range(batch):
+            want, _ = schulz64(f64(x[b]), 5)
+            kept = sum(NS[0] ** k for k in range(6)) * math.sqrt(rows * cols) * 2.0 ** -38
+            assert np.linalg.norm(f64(got[b]) - want) <= kept + 6 * 2.0 ** -20 * np.linalg.norm(want), (size, b)
