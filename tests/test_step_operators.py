@@ -1275,3 +1275,54 @@ def test_orthogonalize_far_below_epsilon(ctx, batch, rows, cols):
             want, _ = schulz64(f64(x[b]), 5)
             kept = sum(NS[0] ** k for k in range(6)) * math.sqrt(rows * cols) * 2.0 ** -38
             assert np.linalg.norm(f64(got[b]) - want) <= kept + 6 * 2.0 ** -20 * np.linalg.norm(want), (size, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("q,k,c,reach", [(30, 33, 12, 2047), (400, 400, 128, 64)])
+def test_position_of_large_tables(ctx, q, k, c, reach, dt):
+    """4094 boundaries, of 4095 that may be given; and a table that LDS does not hold, of many pairs."""
+    for segments in (False, True):
+        test_position(ctx, q, k, c, reach, dt, segments)
+        test_position_backward(ctx, q, k, c, reach, dt, segments)
+
+
+@pytest.mark.gpu
+def test_position_of_the_most_boundaries(ctx):
+    from localfold_amd import device as D
+    p = np.arange(-4200, 4200, 3).astype(np.int32)
+    b = (2 * np.arange(4095) - 4095).astype(np.int32)
+    zero = np.zeros(1, np.int32)
+    row = rows64(b, p, zero)[:, 0]
+    table = torch.arange(4096, dtype=torch.float32, device=ctx.device)[:, None].contiguous()
+    got = D.relative_position(ctx, table, on(ctx, b), on(ctx, p), key_positions=on(ctx, zero))
+    assert (f64(got)[:, 0, 0] == row).all()
+    dt = D.relative_position_backward(ctx, torch.ones_like(got), on(ctx, b), on(ctx, p), key_positions=on(ctx, zero))
+    assert (f64(dt)[:, 0] == np.bincount(row, minlength=4096)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,rows,cols", [(2, 40, 70), (3, 128, 512), (1, 300, 200)])
+def test_orthogonalize_of_the_most_steps(ctx, batch, rows, cols):
+    """32 steps, a triple each, that bring every singular value to one: what is left is the polar factor.
+
+    A step keeps that factor; its rounding E, as schulz64 counts it, changes it by at most 2 |E| over the smallest singular
+    value of the step's result."""
+    from localfold_amd import device as D
+    x = torch.as_tensor(np.random.default_rng(cols).normal(size=(batch, rows, cols))).float()
+    co = [(1.5, -0.5, 0.0), (1.875, -1.25, 0.375)] * 16
+    got = f64(D.orthogonalize(ctx, x.to(ctx.device), steps=32, coefficients=co))
+    m, n = sorted((rows, cols))
+    gamma = lambda k: 2.0 ** -21 + 3 * (k / 32 + 8) * 2 * U
+    for i in range(batch):
+        u, s, vt = np.linalg.svd(f64(x[i]), full_matrices=False)
+        s = s / (np.linalg.norm(s) + EPS)
+        bound = 2 * 4 * U / s.min()
+        for a, b, c in co:
+            f, p = np.linalg.norm(s), a + b * s ** 2 + c * s ** 4
+            dp = (abs(b) + 2 * abs(c) * s.max() ** 2) * gamma(n) * f * f + gamma(m) * abs(c) * np.linalg.norm(s ** 2) ** 2 + 2.0 ** -21 * np.linalg.norm(p)
+            e = s.max() * dp + gamma(m) * np.linalg.norm(p) * f
+            s = p * s
+            bound += 2 * (e + 2.0 ** -21 * np.linalg.norm(s)) / s.min()
+        assert np.abs(s - 1).max() < 1e-12 and bound < 0.1 * math.sqrt(m)
+        assert np.linalg.norm(got[i] - u @ vt) <= bound + U * math.sqrt(m)
