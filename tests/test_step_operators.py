@@ -1326,3 +1326,46 @@ def test_orthogonalize_of_the_most_steps(ctx, batch, rows, cols):
             bound += 2 * (e + 2.0 ** -21 * np.linalg.norm(s)) / s.min()
         assert np.abs(s - 1).max() < 1e-12 and bound < 0.1 * math.sqrt(m)
         assert np.linalg.norm(got[i] - u @ vt) <= bound + U * math.sqrt(m)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,n", [(17000005, 128, 130), (2000001, 1100, 1080)])
+def test_mx4_past_four_gigabytes(ctx, rows, k, n):
+    """Activations and outputs past 2^32 bytes, by weights resident and streamed: rows at the end as in a call of their own."""
+    from localfold_amd import device as D
+    x = torch.empty(rows, k, dtype=torch.bfloat16, device=ctx.device).normal_()
+    w = D.mx4_pack(ctx, torch.randn(n, k, device=ctx.device))
+    out = D.mx4_linear(ctx, x, w)
+    kept, t, sums = D.mx4_empty(rows, k, ctx.device), D.mx4_empty(k, rows, ctx.device), torch.empty(k, device=ctx.device)
+    D.mx4_pack(ctx, x, out=kept, transposed=t, sums=sums)
+    assert torch.equal(D.mx4_linear(ctx, kept, w), out)
+    for r0 in (0, rows // 256 * 256 - 256 * 200):
+        part = x[r0:r0 + 256 * 200 + 100].contiguous()
+        m = part.shape[0]
+        pk, pt = D.mx4_empty(m, k, ctx.device), D.mx4_empty(k, m, ctx.device)
+        D.mx4_pack(ctx, part, out=pk, transposed=pt)
+        assert torch.equal(D.mx4_linear(ctx, part, w), out[r0:r0 + m])
+        assert torch.equal(pk.codes, kept.codes[r0:r0 + m]) and torch.equal(pk.scales[:, :m], kept.scales[:, r0:r0 + m])
+        whole = m // 32 * 32                                # the part's last group of rows may be cut
+        assert torch.equal(pt.codes[:, :whole // 2], t.codes[:, r0 // 2:(r0 + whole) // 2])
+        assert torch.equal(pt.scales[:whole // 32, :k], t.scales[r0 // 32:(r0 + whole) // 32, :k])
+    want, mags = torch.zeros(k, dtype=torch.float64, device=ctx.device), torch.zeros(k, dtype=torch.float64, device=ctx.device)
+    for some in x.split(1000000):
+        want += some.double().sum(0)
+        mags += some.double().abs().sum(0)
+    # 32 rows of a tile, then a run's tiles of 128 rows (2048 runs of all columns, the last one shorter), then doubles
+    depth = 32 + 4 + math.ceil(rows / 128 / (2048 // -(-k // 128)))
+    close(sums, f64(want), 2 * U * depth * f64(mags), torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,rows,cols", [(60000, 128, 300), (2800, 700, 1100)])
+def test_orthogonalize_past_eight_gigabytes(ctx, batch, rows, cols):
+    """More than 2^31 elements, a block a matrix and in products, written in place."""
+    from localfold_amd import device as D
+    x = torch.empty(batch, rows, cols, device=ctx.device).normal_()
+    some = {b: x[b].clone() for b in (0, batch // 2, batch - 1)}
+    D.orthogonalize(ctx, x, steps=2, out=x)
+    for b, u in some.items():
+        want, bound = schulz64(f64(u), 2)
+        assert np.linalg.norm(f64(x[b]) - want) <= bound + U * np.linalg.norm(want), b
