@@ -926,10 +926,12 @@ MuonSize muon_size(long long rows, long long cols) { return MuonSize{(int)std::m
 constexpr int CUS = 256;
 
 enum MuonKind { BLOCK, PANELS, PRODUCTS };
-// Panels while there are few: 48 matrices of 128 x 512 take 104 us, and 149 in blocks of their own (256: 205 in blocks).
+// Panels where a matrix has three or more and the chip holds all of them at once: 64 matrices of 128 x 512 take 112 us, and
+// 137 in blocks of their own, 65 175 and 137; 64 of 128 x 384 97 and 134, 86 176 and 139; 16 of 128 x 256, two panels, 78 and
+// 75, 64 91 and 77.  Beyond 512 columns the others are products: 32 of 128 x 1024 124 and 187, 33 197 and 191.
 MuonKind muon_kind(long long batch, const MuonSize& z) {
   const long long panels = (z.n + 127) / 128;
-  if (z.m > 64 && z.m <= 128 && panels > 1 && panels <= 8 && batch * panels <= 3 * CUS / 2) return PANELS;
+  if (z.m > 64 && z.m <= 128 && panels > 2 && panels <= 8 && batch * panels <= CUS) return PANELS;
   return z.m <= 128 && z.n <= 512 ? BLOCK : PRODUCTS;
 }
 int norm_parts(long long count) { return (int)std::min<long long>(NORM_MOST, (count + 4095) / 4096); }

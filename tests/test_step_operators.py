@@ -1369,3 +1369,26 @@ def test_orthogonalize_past_eight_gigabytes(ctx, batch, rows, cols):
     for b, u in some.items():
         want, bound = schulz64(f64(u), 2)
         assert np.linalg.norm(f64(x[b]) - want) <= bound + U * np.linalg.norm(want), b
+
+
+def test_muon_scratch_of_the_kinds():
+    """Panels keep 192 KB for each 128 columns and 8 KB a matrix, blocks of their own nothing: panels where there are at least
+    three of a matrix, and a CU for each of all of them."""
+    from localfold_amd import capi
+    lib = capi.load()
+    for batch, rows, cols, panels in ((64, 128, 512, 4), (65, 128, 512, 0), (85, 70, 300, 3), (86, 300, 70, 0), (1, 128, 256, 0), (128, 256, 66, 0),
+                                      (32, 128, 1024, 8), (3, 64, 512, 0), (1, 128, 385, 4)):
+        need = lib.lf_muon_scratch(batch, rows, cols)
+        assert need == (batch * (8192 + panels * 196608) if panels else 0), (batch, rows, cols)
+    assert lib.lf_muon_scratch(33, 128, 1024) > 33 * 128 * 1024 * 16       # products: X and its transpose twice
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,rows,cols", [(64, 128, 512), (65, 128, 512), (85, 300, 70), (86, 70, 300), (1, 128, 256), (33, 128, 1024)])
+def test_orthogonalize_on_both_sides_of_the_rule(ctx, batch, rows, cols):
+    from localfold_amd import device as D
+    x = gradients(np.random.default_rng(batch), (batch, rows, cols), torch.bfloat16).to(ctx.device)
+    got = D.orthogonalize(ctx, x)
+    for b in sorted({0, batch // 2, batch - 1}):
+        want, bound = schulz64(f64(x[b]), 5)
+        assert np.linalg.norm(f64(got[b]) - want) <= bound + HALF[torch.bfloat16] * (np.linalg.norm(want) + bound), b
