@@ -702,6 +702,7 @@ typedef struct {
   size_t scratch_bytes;
 } lf_relative_position_backward_args;
 
+/* A table of more than about 300 rows is summed in parts, each a pass over grad. */
 int lf_relative_position_backward(lf_context* ctx, const lf_relative_position_backward_args* args);
 size_t lf_relative_position_backward_scratch(const lf_relative_pairs* pairs, int channels);   /* reads no tensor */
 

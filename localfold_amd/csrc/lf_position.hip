@@ -31,7 +31,7 @@ __device__ __forceinline__ int row_of(const lf_relative_pairs& p, int qp, int qs
 // A block adds rows to tiles of `tile` (at most 256) keys of one query: the rows' numbers once a pair, in LDS, then 8
 // channels a lane, FLIGHT loads under way.  Many pairs: blocks that stay, with the table and the bias added up in LDS once
 // (TABLE_LDS), so that a pair costs its own bytes alone: 825 x 825 pairs of 128 channels in bf16, read and written, 62 us,
-// 5.6 TB/s.
+// 5.6 TB/s.  A table that LDS does not hold comes from the caches at the same rate (130 rows of it 64 us, 66 63.5).
 struct PositionTiles {
   int tile, tiles;             // keys of a tile, tiles of a query
   long long count;             // tiles in all
@@ -137,7 +137,8 @@ __global__ __launch_bounds__(512, 4) void position_kernel(lf_relative_pairs p, i
 // A lane sums two channels of the keys that its team of L lanes takes, in registers while the table's row stays
 // the same (most pairs are beyond the last boundary, where it does) and into the team's own rows in LDS when it
 // changes: no two lanes share an address, so the order of the sums is fixed.  Those rows, 512 bytes of each a wave, leave
-// room for 4 waves a CU where there are 80: a wave has the next 32 loads under way while it adds up the last ones.
+// room for 4 waves a CU where there are 66 (80 for 3, 39 and fewer for all 8, more than about 300 for a part of the table
+// at a time, with a pass over the gradient each): a wave has the next 32 loads under way while it adds up the last ones.
 // (LDS's own float additions took twice as long as reading and writing: 39 us instead of 23 for 384 x 384 pairs of 128
 // channels in bf16.)  Those take 20 now, 1.9 TB/s: bound by the waves that LDS has room for, each waiting for its loads.
 struct PositionGrid {
